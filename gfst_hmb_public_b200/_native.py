@@ -23,6 +23,7 @@ SIGN_R_DIAG_POSITIVE = 1
 DTYPE_F32 = 0
 DTYPE_BF16 = 1
 DTYPE_F64 = 2
+DTYPE_F16 = 3  # paged memory only
 
 _c_void_p = ctypes.c_void_p
 _c_int = ctypes.c_int
@@ -122,6 +123,20 @@ _SIGNATURES: dict[str, list] = {
     "gfst_mpuc_recurrent_scan": [
         _c_void_p, _c_int, _c_int, _c_int, _c_int, _c_int, _c_void_p, _c_void_p, _c_void_p, _c_int64, _c_int,
         _c_void_p, _c_void_p, _c_void_p, _c_void_p, _c_void_p, _c_void_p, ctypes.c_size_t, _c_void_p,
+    ],
+    "gfst_block_tables": [
+        _c_void_p, _c_void_p, _c_void_p, _c_void_p, _c_void_p, _c_int, _c_int, _c_int, _c_int64, _c_int64,
+        _c_void_p, _c_void_p, _c_void_p, _c_void_p, _c_void_p, _c_void_p, _c_void_p,
+    ],
+    "gfst_paged_append": [
+        _c_void_p, _c_int64, _c_int64, _c_void_p, _c_int64, _c_int64, _c_void_p, _c_void_p, _c_void_p, _c_int64,
+        _c_int64, _c_int, _c_int, _c_int, _c_int, _c_int, _c_void_p,
+    ],
+    "gfst_prefix_attention_workspace_bytes": [_c_int64, _c_int, _c_int, _c_int, ctypes.POINTER(ctypes.c_size_t)],
+    "gfst_prefix_attention": [
+        _c_void_p, _c_int64, _c_int64, _c_void_p, _c_void_p, _c_int64, _c_int, _c_int, _c_int, _c_int, _c_int,
+        _c_int, _c_void_p, _c_int64, _c_int, _c_void_p, _c_void_p, _c_int, _c_int64, _c_void_p, _c_int, _c_void_p,
+        _c_float, _c_void_p, _c_void_p, _c_int, _c_void_p, ctypes.c_size_t, _c_void_p,
     ],
 }
 _RESTYPES = {

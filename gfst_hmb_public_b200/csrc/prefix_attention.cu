@@ -1,0 +1,198 @@
+// Shared-prefix attention: argument checks, workspace, kernel choice and the
+// merge of the partial results (prefix_attention.cuh).
+//
+// The merge is one warp per (token, query head): the prefix part, the own part
+// and their continuations, at most a few, weighted by 2^(m_i - max m), divided
+// by the joined sum and rounded once to the output type.  It reads each
+// partial once; what bounds it is their 4 B per value.
+#include <cuda_fp16.h>
+
+#include "prefix_attention.cuh"
+
+namespace gfst {
+
+namespace {
+
+constexpr int kMergeThreads = 128;
+
+template <typename T>
+__device__ __forceinline__ void store4(T* dst, float4 v);
+template <>
+__device__ __forceinline__ void store4<float>(float* dst, float4 v) { *reinterpret_cast<float4*>(dst) = v; }
+template <>
+__device__ __forceinline__ void store4<__nv_bfloat16>(__nv_bfloat16* dst, float4 v) {
+  const __nv_bfloat162 a = __floats2bfloat162_rn(v.x, v.y), b = __floats2bfloat162_rn(v.z, v.w);
+  *reinterpret_cast<uint2*>(dst) = make_uint2(*reinterpret_cast<const uint32_t*>(&a), *reinterpret_cast<const uint32_t*>(&b));
+}
+template <>
+__device__ __forceinline__ void store4<__half>(__half* dst, float4 v) {
+  const __half2 a = __floats2half2_rn(v.x, v.y), b = __floats2half2_rn(v.z, v.w);
+  *reinterpret_cast<uint2*>(dst) = make_uint2(*reinterpret_cast<const uint32_t*>(&a), *reinterpret_cast<const uint32_t*>(&b));
+}
+
+// joins one set (m, l, o) into the running one
+struct Join {
+  float m = -INFINITY, l = 0.f;
+  float4 o[2] = {make_float4(0, 0, 0, 0), make_float4(0, 0, 0, 0)};
+  __device__ __forceinline__ void add(float2 ml, const float* src, int lane, int dv) {
+    if (!(ml.y > 0.f) && ml.y == ml.y) return;  // an empty set (a NaN sum is kept)
+    const float now = fmaxf(m, ml.x);
+    const float wa = m == -INFINITY ? 0.f : exp2f(m - now), wb = ml.x == now ? 1.f : exp2f(ml.x - now);
+    m = now;
+    l = l * wa + ml.y * wb;
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const int c = (i * 32 + lane) * 4;
+      if (c < dv) {
+        const float4 v = *reinterpret_cast<const float4*>(src + c);
+        o[i].x = o[i].x * wa + v.x * wb;
+        o[i].y = o[i].y * wa + v.y * wb;
+        o[i].z = o[i].z * wa + v.z * wb;
+        o[i].w = o[i].w * wa + v.w * wb;
+      }
+    }
+  }
+};
+
+template <typename T>
+__global__ void __launch_bounds__(kMergeThreads) prefix_attention_merge_kernel(const AttnArgs a, int MR, int cont_rows) {
+  const int lane = threadIdx.x & 31;
+  const int64_t row = (int64_t)blockIdx.x * (kMergeThreads / 32) + (threadIdx.x >> 5);
+  const int heads = a.H * a.G;
+  const int64_t tok = row / heads;
+  if (tok >= a.n_tokens) return;
+  const bool live = a.B > 0 && tok < attn_tokens(a) && tok >= a.cu[0];
+  Join j;
+  if (live) {
+#pragma unroll
+    for (int own = 0; own < 2; ++own) {
+      if (!own && attn_prefix_len(a) == 0) continue;
+      j.add(a.part_ml[own][row], a.part_o[own] + row * a.dv, lane, a.dv);
+      const int2 nx = a.part_next[own][row];
+      for (int i = 0; i < nx.y; ++i) {
+        const int64_t c = nx.x + (int64_t)i * MR;
+        if (c < 0 || c >= cont_rows) break;  // offsets that cover no item leave this unset
+        j.add(a.cont_ml[c], a.cont_o + c * a.dv, lane, a.dv);
+      }
+    }
+  } else if (!a.fill_tail) {
+    return;
+  }
+  // a row that sees nothing: zeros and -inf
+  const float inv = j.l == 0.f ? 0.f : 1.f / j.l;
+  T* out = static_cast<T*>(a.out) + row * a.dv;
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const int c = (i * 32 + lane) * 4;
+    if (c < a.dv) store4<T>(out + c, make_float4(j.o[i].x * inv, j.o[i].y * inv, j.o[i].z * inv, j.o[i].w * inv));
+  }
+  if (a.lse != nullptr && lane == 0)
+    a.lse[row] = j.l == 0.f ? -INFINITY : (j.m + log2f(j.l)) * 0.69314718055994531f;
+}
+
+struct Workspace {
+  size_t o, ml, next, cont_o, cont_ml, bytes;  // o, ml, next: two of each (prefix, own)
+  int64_t rows;
+  Workspace(int64_t n_tokens, int heads, int dv) {
+    rows = n_tokens * heads;
+    auto up = [](size_t v) { return (v + 255) & ~size_t(255); };
+    size_t at = 0;
+    o = at, at += 2 * up((size_t)rows * dv * 4);
+    ml = at, at += 2 * up((size_t)rows * 8);
+    next = at, at += 2 * up((size_t)rows * 8);
+    const size_t cont = (size_t)kAttnMaxGrid * kAttnFmaRows;
+    cont_o = at, at += up(cont * dv * 4);
+    cont_ml = at, at += up(cont * 8);
+    bytes = at;
+  }
+};
+
+int check_dims(int64_t n_tokens, int H, int G, int dv) {
+  GFST_REQUIRE(n_tokens >= 0 && H >= 1 && G >= 1 && dv >= 1 && dv <= 256, GFST_ERR_SHAPE,
+               "n_tokens %lld kv heads %d group %d dv %d", (long long)n_tokens, H, G, dv);
+  GFST_REQUIRE(n_tokens * H < (1LL << 31) && n_tokens * H * G < (1LL << 31), GFST_ERR_SHAPE,
+               "%lld tokens of %d heads exceed the int32 row range", (long long)n_tokens, H * G);
+  return GFST_OK;
+}
+
+}  // namespace
+}  // namespace gfst
+
+using namespace gfst;
+
+extern "C" int gfst_prefix_attention_workspace_bytes(int64_t n_tokens, int n_kv_heads, int group, int dv,
+                                                     size_t* bytes) {
+  GFST_REQUIRE(bytes != nullptr, GFST_ERR_ARG, "null pointer");
+  const int st = check_dims(n_tokens, n_kv_heads, group, dv);
+  if (st != GFST_OK) return st;
+  *bytes = Workspace(n_tokens, n_kv_heads * group, dv).bytes;
+  return GFST_OK;
+}
+
+extern "C" int gfst_prefix_attention(const void* Q, int64_t q_stride_t, int64_t q_stride_h, const void* pool_K,
+                                     const void* pool_V, int64_t n_blocks, int L, int n_kv_heads, int group, int d,
+                                     int dv, int dtype, const int32_t* tables, int64_t table_stride, int width,
+                                     const int32_t* lens, const int32_t* cu_new, int n_requests, int64_t n_tokens,
+                                     const int32_t* prefix_table, int prefix_width, const int32_t* prefix_len,
+                                     float scale, void* out, float* lse, int fill_tail, void* workspace,
+                                     size_t workspace_bytes, cudaStream_t stream) {
+  GFST_REQUIRE(dtype == GFST_F32 || dtype == GFST_BF16 || dtype == GFST_F16, GFST_ERR_DTYPE, "dtype %d", dtype);
+  int st = check_dims(n_tokens, n_kv_heads, group, dv);
+  if (st != GFST_OK) return st;
+  const int es = dtype == GFST_F32 ? 4 : 2, pv = 16 / es;
+  GFST_REQUIRE(d >= 1 && d <= 256, GFST_ERR_SHAPE, "d=%d outside [1, 256]", d);
+  GFST_REQUIRE(d % pv == 0 && dv % pv == 0, GFST_ERR_ALIGN, "rows of %d and %d elements are no multiple of 16 bytes", d,
+               dv);
+  GFST_REQUIRE(n_requests >= 1 && n_requests <= 65536 && width >= 1 && L >= 1 && n_blocks >= 1 && prefix_width >= 0,
+               GFST_ERR_SHAPE, "requests %d width %d L %d blocks %lld prefix width %d", n_requests, width, L,
+               (long long)n_blocks, prefix_width);
+  GFST_REQUIRE((int64_t)width * L < (1LL << 31) && (int64_t)prefix_width * L < (1LL << 31), GFST_ERR_SHAPE,
+               "positions exceed the int32 range");
+  if (n_tokens == 0) return GFST_OK;
+  GFST_REQUIRE(Q && pool_K && pool_V && tables && lens && cu_new && out && workspace, GFST_ERR_ARG, "null pointer");
+  GFST_REQUIRE(prefix_width == 0 || (prefix_table && prefix_len), GFST_ERR_ARG, "null prefix table or length");
+  GFST_REQUIRE(aligned16(Q) && aligned16(pool_K) && aligned16(pool_V) && aligned16(out) && q_stride_t % pv == 0 &&
+                   q_stride_h % pv == 0,
+               GFST_ERR_ALIGN, "Q, out and the pools need 16-byte aligned rows");
+  GFST_REQUIRE((reinterpret_cast<uintptr_t>(workspace) & 255) == 0, GFST_ERR_ALIGN, "workspace must be 256-byte aligned");
+  const Workspace ws(n_tokens, n_kv_heads * group, dv);
+  GFST_REQUIRE(workspace_bytes >= ws.bytes, GFST_ERR_SHAPE, "workspace of %zu bytes, %zu needed", workspace_bytes,
+               ws.bytes);
+  int dev = 0, sms = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e == cudaSuccess) e = cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
+  GFST_REQUIRE(e == cudaSuccess, GFST_ERR_DEVICE, "device query: %s", cudaGetErrorString(e));
+
+  uint8_t* w = static_cast<uint8_t*>(workspace);
+  auto half = [&](size_t at, size_t next) { return w + at + (next - at) / 2; };
+  AttnArgs a;
+  a.Q = Q, a.q_st = q_stride_t, a.q_sh = q_stride_h;
+  a.pool_K = pool_K, a.pool_V = pool_V, a.n_blocks = n_blocks;
+  a.L = L, a.H = n_kv_heads, a.G = group, a.d = d, a.dv = dv;
+  a.tables = tables, a.table_st = table_stride, a.width = width, a.lens = lens, a.cu = cu_new, a.B = n_requests;
+  a.n_tokens = (int)n_tokens;
+  a.prefix_table = prefix_table, a.prefix_width = prefix_width, a.prefix_len = prefix_width > 0 ? prefix_len : nullptr;
+  a.scale_log2 = (float)((double)scale * 1.4426950408889634);
+  a.out = out, a.lse = lse, a.fill_tail = fill_tail;
+  a.part_o[0] = reinterpret_cast<float*>(w + ws.o);
+  a.part_o[1] = reinterpret_cast<float*>(half(ws.o, ws.ml));
+  a.part_ml[0] = reinterpret_cast<float2*>(w + ws.ml);
+  a.part_ml[1] = reinterpret_cast<float2*>(half(ws.ml, ws.next));
+  a.part_next[0] = reinterpret_cast<int2*>(w + ws.next);
+  a.part_next[1] = reinterpret_cast<int2*>(half(ws.next, ws.cont_o));
+  a.cont_o = reinterpret_cast<float*>(w + ws.cont_o);
+  a.cont_ml = reinterpret_cast<float2*>(w + ws.cont_ml);
+
+  const int MR = kAttnFmaRows;
+  st = launch_prefix_attention_fma(a, dtype, sms, stream);
+  if (st != GFST_OK) return st;
+  const int64_t blocks = (ws.rows + kMergeThreads / 32 - 1) / (kMergeThreads / 32);
+  const int cont_rows = kAttnMaxGrid * MR;
+  if (dtype == GFST_F32)
+    prefix_attention_merge_kernel<float><<<(unsigned)blocks, kMergeThreads, 0, stream>>>(a, MR, cont_rows);
+  else if (dtype == GFST_BF16)
+    prefix_attention_merge_kernel<__nv_bfloat16><<<(unsigned)blocks, kMergeThreads, 0, stream>>>(a, MR, cont_rows);
+  else
+    prefix_attention_merge_kernel<__half><<<(unsigned)blocks, kMergeThreads, 0, stream>>>(a, MR, cont_rows);
+  return check_launch("prefix_attention_merge_kernel");
+}

@@ -1,0 +1,320 @@
+"""Paged block memory: requests of ragged lengths in one pool of L-token blocks,
+a prefix that all of them share, and the softmax attention that reads both.
+
+``memory.BlockMemory`` gives every stream its own ring and moves all streams in
+step; here a request holds as many blocks of the pool as its length needs,
+takes and returns them on the GPU (no length is read back to the host), and the
+blocks of a prefix that every request of the batch starts with (instructions, a
+document) are stored once and attended for all requests in one product.
+
+* ``block_tables``     one step of the tables: blocks taken and returned, the
+                       slot of every new token, packed offsets
+* ``paged_append``     the new tokens' keys and values to their slots
+* ``prefix_attention`` attention of the new tokens over the prefix and over
+                       each request's own positions, causal within the new ones
+* ``PagedMemory``      pool, tables, lengths and prefix of a batch of requests
+
+Layout: pool_K [n_blocks, heads, L, d], pool_V [n_blocks, heads, L, dv]; a block
+of one head is one contiguous L x d slab, as in ``memory.BlockMemory``.  Slot
+``block * L + offset`` names a token's place in the pool.
+
+Serving operators: nothing here records gradients.  The reference
+(pkhairkh/gfst-hmb-public) keeps one Python list of blocks per sample
+(src/gfst_hmb_mpuc/state.py:651-815) and has no shared prefix.
+"""
+from __future__ import annotations
+
+import ctypes
+import math
+from typing import NamedTuple
+
+import torch
+
+from . import _native as nat
+
+_DTYPES = {torch.float32: nat.DTYPE_F32, torch.bfloat16: nat.DTYPE_BF16, torch.float16: nat.DTYPE_F16}
+
+
+def _dtype_code(what: str, *tensors: torch.Tensor) -> int:
+    dtypes = {t.dtype for t in tensors}
+    if len(dtypes) != 1:
+        raise RuntimeError(f"{what}: mixed dtypes {dtypes}")
+    dtype = dtypes.pop()
+    if dtype not in _DTYPES:
+        raise RuntimeError(f"{what}: unsupported dtype {dtype} (float32, bfloat16 or float16)")
+    return _DTYPES[dtype]
+
+
+def _no_grad(what: str, *tensors: torch.Tensor) -> None:
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
+        raise RuntimeError(f"{what} has no backward pass; call it under torch.no_grad()")
+
+
+def _int32(what: str, name: str, t: torch.Tensor, shape: tuple) -> torch.Tensor:
+    if t.dtype != torch.int32:
+        raise RuntimeError(f"{what}: {name} must be int32 (got {t.dtype})")
+    if tuple(t.shape) != shape:
+        raise ValueError(f"{what}: {name} has shape {tuple(t.shape)}, expected {shape}")
+    return t.contiguous()
+
+
+def _rows(t: torch.Tensor) -> torch.Tensor:
+    """t [n, heads, width] with contiguous 16-byte aligned rows (a copy where it has none)."""
+    per = 16 // t.element_size()
+    if t.stride(2) == 1 and t.stride(0) % per == 0 and t.stride(1) % per == 0 and t.data_ptr() % 16 == 0:
+        return t
+    return t.contiguous().clone() if t.is_contiguous() else t.contiguous()
+
+
+class BlockTables(NamedTuple):
+    """What one step of ``block_tables`` leaves (all int32 on the device)."""
+    tables: torch.Tensor      # [B, W] blocks of each request, -1 behind them
+    lens: torch.Tensor        # [B] tokens of each request, the new ones included
+    cu_new: torch.Tensor      # [B + 1] first packed position of each request's new tokens
+    slot_map: torch.Tensor    # [n_tokens] slot of each new token, -1 behind the last
+    free_state: torch.Tensor  # [2] (head, count) of the free ring
+    n_short: torch.Tensor     # [1] blocks wanted and not had: 0 in a step that may be used
+
+
+def block_tables(lens: torch.Tensor, new_lens: torch.Tensor, tables: torch.Tensor, free_ring: torch.Tensor,
+                 free_state: torch.Tensor, *, block_len: int, n_tokens: int,
+                 tables_out: torch.Tensor | None = None) -> BlockTables:
+    """One step of the block tables, on the GPU.
+
+    lens [B] tokens of each request and tables [B, W] its blocks; new_lens [B]
+    the tokens it appends (0: idle, negative: the request ends and returns its
+    blocks); free_ring [n_blocks] with free_state [2] = (head, count) the free
+    blocks.  Blocks are taken in request order from the ring's head; returned
+    ones go behind its tail and are handed out from the next step on.
+    ``free_ring`` is updated in place (only behind the tail, so a step that is
+    not used can be taken again from the same lens, tables and free_state).
+    ``n_tokens`` is the number of packed new tokens the caller holds, at least
+    the sum of the positive new_lens.  ``tables_out`` (may be ``tables``)
+    receives the new tables in place of a new tensor.  All int32."""
+    what = "block_tables"
+    nat.require_cuda(lens, new_lens, tables, free_ring, free_state, tables_out, what=what)
+    if tables.ndim != 2 or free_ring.ndim != 1:
+        raise ValueError("block_tables expects tables [B, W] and free_ring [n_blocks]")
+    B, W = tables.shape
+    lens, new_lens = _int32(what, "lens", lens, (B,)), _int32(what, "new_lens", new_lens, (B,))
+    free_state = _int32(what, "free_state", free_state, (2,))
+    if free_ring.dtype != torch.int32 or not free_ring.is_contiguous():
+        raise RuntimeError("block_tables: free_ring must be contiguous int32")
+    if tables_out is None:
+        tables = _int32(what, "tables", tables, (B, W))
+        tables_out = torch.empty_like(tables)
+    else:
+        if not (tables.is_contiguous() and tables_out.is_contiguous()):
+            raise ValueError("block_tables: tables and tables_out must be contiguous")
+        _int32(what, "tables", tables, (B, W))
+        _int32(what, "tables_out", tables_out, (B, W))
+        a, b, size = tables.data_ptr(), tables_out.data_ptr(), B * W * 4
+        if a != b and a < b + size and b < a + size:
+            raise ValueError("block_tables: tables_out overlaps tables without being it")
+    new = lambda *shape: torch.empty(shape, dtype=torch.int32, device=lens.device)  # noqa: E731
+    out = BlockTables(tables_out, new(B), new(B + 1), new(int(n_tokens)), new(2), new(1))
+    with torch.cuda.device(lens.device):
+        nat.call("gfst_block_tables", nat.ptr(lens), nat.ptr(new_lens), nat.ptr(tables), nat.ptr(free_ring),
+                 nat.ptr(free_state), B, W, int(block_len), int(free_ring.shape[0]), int(n_tokens),
+                 nat.ptr(out.tables), nat.ptr(out.lens), nat.ptr(out.cu_new), nat.ptr(out.slot_map),
+                 nat.ptr(out.free_state), nat.ptr(out.n_short), nat.stream_of(lens))
+    return out
+
+
+def _check_pools(what: str, pool_K: torch.Tensor, pool_V: torch.Tensor) -> tuple:
+    if pool_K.ndim != 4 or pool_V.ndim != 4 or pool_K.shape[:3] != pool_V.shape[:3]:
+        raise ValueError(f"{what} expects pool_K [n_blocks, heads, L, d] and pool_V [n_blocks, heads, L, dv]")
+    if not (pool_K.is_contiguous() and pool_V.is_contiguous()):
+        raise ValueError(f"{what}: pools must be contiguous")
+    return (*pool_K.shape, pool_V.shape[3])
+
+
+def paged_append(K: torch.Tensor, V: torch.Tensor, pool_K: torch.Tensor, pool_V: torch.Tensor,
+                 slot_map: torch.Tensor) -> None:
+    """Write K [n, heads, d] and V [n, heads, dv] to their slots of the pools:
+    pool[s // L, h, s % L] = row (t, h) with s = slot_map[t] (int32 [n]).  Tokens
+    with a negative slot (padding, or a block that was not had) are left out, and
+    so is a slot outside the pool; nothing else of the pools changes.  K and V
+    may be strided views (a fused projection's output) with 16-byte rows."""
+    what = "paged_append"
+    nat.require_cuda(K, V, pool_K, pool_V, slot_map, what=what)
+    n_blocks, H, L, d, dv = _check_pools(what, pool_K, pool_V)
+    if K.ndim != 3 or V.ndim != 3 or tuple(K.shape[1:]) != (H, d) or tuple(V.shape) != (K.shape[0], H, dv):
+        raise ValueError(f"paged_append: K{tuple(K.shape)} V{tuple(V.shape)} do not match pools of {H} heads, "
+                         f"d={d}, dv={dv}")
+    code = _dtype_code(what, K, V, pool_K, pool_V)
+    _no_grad(what, K, V, pool_K, pool_V)
+    slot_map = _int32(what, "slot_map", slot_map, (K.shape[0],))
+    K, V = _rows(K), _rows(V)
+    with torch.cuda.device(K.device):
+        nat.call("gfst_paged_append", nat.ptr(K), K.stride(0), K.stride(1), nat.ptr(V), V.stride(0), V.stride(1),
+                 nat.ptr(pool_K), nat.ptr(pool_V), nat.ptr(slot_map), K.shape[0], n_blocks, L, H, d, dv, code,
+                 nat.stream_of(K))
+
+
+def prefix_attention(Q: torch.Tensor, pool_K: torch.Tensor, pool_V: torch.Tensor, tables: torch.Tensor,
+                     lens: torch.Tensor, cu_new: torch.Tensor, *, prefix_table: torch.Tensor | None = None,
+                     prefix_len: torch.Tensor | None = None, scale: float | None = None,
+                     out: torch.Tensor | None = None, return_lse: bool = False):
+    """Softmax attention of the new tokens over a shared prefix and over each
+    request's own positions.
+
+    Q [n, heads * group, d] in packed order (query head hq reads KV head hq //
+    group; rows may be strided); pools as ``paged_append`` writes them; tables
+    [B, W], lens [B] and cu_new [B + 1] as ``block_tables`` leaves them (lens
+    counts the new tokens, whose keys are already in the pool); prefix_table
+    [P] int32 and prefix_len [1] int32 (on the device): the blocks and length of
+    the prefix, or None.  The i-th of a request's n_b new tokens sees the whole
+    prefix and its own positions up to lens[b] - n_b + i.  ``scale`` defaults to
+    d ** -0.5.
+
+    Returns (out [n, heads * group, dv], lse float32 [n, heads * group] or
+    None).  A token that sees nothing gets zeros and -inf.  Tokens behind
+    cu_new[B] (a padded batch) get the same; with ``out`` given (contiguous,
+    Q's dtype) their rows of it stay as they were.  A table entry outside the
+    pool within a request's length reads as zero keys and values and is
+    reported by ``_native.check_device_errors``."""
+    what = "prefix_attention"
+    nat.require_cuda(Q, pool_K, pool_V, tables, lens, cu_new, prefix_table, prefix_len, out, what=what)
+    n_blocks, H, L, d, dv = _check_pools(what, pool_K, pool_V)
+    if Q.ndim != 3 or Q.shape[2] != d or Q.shape[1] % H != 0 or Q.shape[1] == 0:
+        raise ValueError(f"prefix_attention: Q{tuple(Q.shape)} does not match pools of {H} heads, d={d}")
+    if tables.ndim != 2:
+        raise ValueError("prefix_attention expects tables [B, W]")
+    n, heads = int(Q.shape[0]), int(Q.shape[1])
+    B, W = tables.shape
+    if tables.dtype != torch.int32:
+        raise RuntimeError("prefix_attention: tables must be int32")
+    if W > 0 and tables.stride(1) != 1:
+        tables = tables.contiguous()
+    lens, cu_new = _int32(what, "lens", lens, (B,)), _int32(what, "cu_new", cu_new, (B + 1,))
+    if (prefix_table is None) != (prefix_len is None):
+        raise ValueError("prefix_attention: prefix_table and prefix_len go together")
+    P = 0
+    if prefix_table is not None:
+        P = int(prefix_table.numel())
+        prefix_table = _int32(what, "prefix_table", prefix_table, (P,))
+        prefix_len = _int32(what, "prefix_len", prefix_len, (1,))
+    code = _dtype_code(what, Q, pool_K, pool_V)
+    _no_grad(what, Q, pool_K, pool_V)
+    scale = 1.0 / math.sqrt(d) if scale is None else float(scale)
+    if not math.isfinite(scale):
+        raise ValueError(f"prefix_attention: scale {scale} is not finite")
+    given = out is not None
+    if given:
+        if tuple(out.shape) != (n, heads, dv) or out.dtype != Q.dtype or not out.is_contiguous():
+            raise ValueError(f"prefix_attention: out must be contiguous {Q.dtype} [{n}, {heads}, {dv}]")
+    else:
+        out = torch.empty((n, heads, dv), dtype=Q.dtype, device=Q.device)
+    lse = torch.empty((n, heads), dtype=torch.float32, device=Q.device) if return_lse else None
+    Q = _rows(Q)
+    nbytes = ctypes.c_size_t(0)
+    lib = nat.load()
+    with torch.cuda.device(Q.device):
+        nat.check(lib.gfst_prefix_attention_workspace_bytes(n, H, heads // H, dv, ctypes.byref(nbytes)),
+                  "gfst_prefix_attention_workspace_bytes")
+        ws = torch.empty((int(nbytes.value),), dtype=torch.uint8, device=Q.device)
+        nat.call("gfst_prefix_attention", nat.ptr(Q), Q.stride(0), Q.stride(1), nat.ptr(pool_K), nat.ptr(pool_V),
+                 n_blocks, L, H, heads // H, d, dv, code, nat.ptr(tables), tables.stride(0), W, nat.ptr(lens),
+                 nat.ptr(cu_new), B, n, nat.ptr(prefix_table), P, nat.ptr(prefix_len), scale, nat.ptr(out),
+                 nat.ptr(lse), 0 if given else 1, nat.ptr(ws), int(ws.numel()), nat.stream_of(Q))
+    return out, lse
+
+
+class PagedMemory:
+    """Pool, block tables, lengths and shared prefix of up to ``max_requests``
+    requests, each of up to ``max_blocks`` blocks (``n_layers`` pools share the
+    tables).  A request is an index in [0, max_requests); every step passes one
+    entry per index (0: idle, negative: ends).
+
+    A step: ``step = mem.extend(new_lens, n_tokens)``; then for every layer
+    ``mem.append(K, V, step, layer)`` and ``mem.attend(Q, step, layer=layer)``.
+    Lengths and tables stay on the GPU; shapes depend on ``n_tokens`` alone, so a
+    step can be captured in a CUDA graph and replayed with new ``new_lens`` in
+    the same tensor (tokens behind the last request are padding)."""
+
+    def __init__(self, n_blocks: int, block_len: int, n_heads: int, d: int, dv: int | None = None, *,
+                 max_requests: int, max_blocks: int, n_layers: int = 1, dtype: torch.dtype = torch.bfloat16,
+                 device="cuda"):
+        if dtype not in _DTYPES:
+            raise RuntimeError(f"PagedMemory: unsupported dtype {dtype} (float32, bfloat16 or float16)")
+        if min(n_blocks, block_len, n_heads, d, max_requests, max_blocks, n_layers) < 1:
+            raise ValueError("PagedMemory: sizes must be positive")
+        dv = d if dv is None else dv
+        self.n_blocks, self.block_len, self.n_heads, self.d, self.dv = n_blocks, block_len, n_heads, d, dv
+        self.max_requests, self.max_blocks, self.n_layers, self.dtype = max_requests, max_blocks, n_layers, dtype
+        i32 = dict(dtype=torch.int32, device=device)
+        self.pool_K = torch.zeros((n_layers, n_blocks, n_heads, block_len, d), dtype=dtype, device=device)
+        self.pool_V = torch.zeros((n_layers, n_blocks, n_heads, block_len, dv), dtype=dtype, device=device)
+        self.tables = torch.full((max_requests, max_blocks), -1, **i32)
+        self.lens = torch.zeros((max_requests,), **i32)
+        self.free_ring = torch.arange(n_blocks, **i32)
+        self.free_state = torch.tensor([0, n_blocks], **i32)
+        self.prefix_table = torch.full((max_blocks,), -1, **i32)
+        self.prefix_len = torch.zeros((1,), **i32)
+
+    @property
+    def device(self) -> torch.device:
+        return self.pool_K.device
+
+    def extend(self, new_lens: torch.Tensor, n_tokens: int) -> BlockTables:
+        """Take and return blocks for one step; updates the memory's tables,
+        lengths and free ring in place and returns the step (whose ``tables`` and
+        ``lens`` are the memory's own).  ``n_short`` of the step says whether the
+        pool was too small; read it when the host waits anyway."""
+        t = block_tables(self.lens, new_lens, self.tables, self.free_ring, self.free_state,
+                         block_len=self.block_len, n_tokens=n_tokens, tables_out=self.tables)
+        self.lens.copy_(t.lens)
+        self.free_state.copy_(t.free_state)
+        return t._replace(lens=self.lens, free_state=self.free_state)
+
+    def append(self, K: torch.Tensor, V: torch.Tensor, step: BlockTables, layer: int = 0) -> None:
+        """Keys and values [n_tokens, heads, d / dv] of the step's new tokens."""
+        paged_append(K, V, self.pool_K[layer], self.pool_V[layer], step.slot_map)
+
+    def attend(self, Q: torch.Tensor, step: BlockTables, *, layer: int = 0, scale: float | None = None,
+               out: torch.Tensor | None = None, return_lse: bool = False):
+        """Attention of the step's new tokens, Q [n_tokens, heads * group, d]
+        (``prefix_attention``); append the step's keys first."""
+        return prefix_attention(Q, self.pool_K[layer], self.pool_V[layer], step.tables, step.lens, step.cu_new,
+                                prefix_table=self.prefix_table, prefix_len=self.prefix_len, scale=scale, out=out,
+                                return_lse=return_lse)
+
+    def share(self, request: int) -> None:
+        """Make request ``request``'s tokens the prefix of all requests: its blocks
+        become the prefix's and the index is free again.  The prefix must be
+        empty (``unshare`` first) and the other requests are then taken to
+        continue it."""
+        r = self._index(request)
+        if int(self.prefix_len.item()) != 0:
+            raise RuntimeError("PagedMemory.share: there is a prefix already; unshare it first")
+        self.prefix_table.copy_(self.tables[r])
+        self.prefix_len.copy_(self.lens[r:r + 1])
+        self.tables[r].fill_(-1)
+        self.lens[r:r + 1].zero_()
+
+    def unshare(self, request: int) -> None:
+        """Give the prefix's blocks and tokens to the idle request index
+        ``request`` (end it to return the blocks)."""
+        r = self._index(request)
+        if int(self.lens[r].item()) != 0:
+            raise RuntimeError(f"PagedMemory.unshare: request {r} holds tokens")
+        self.tables[r].copy_(self.prefix_table)
+        self.lens[r:r + 1].copy_(self.prefix_len)
+        self.prefix_table.fill_(-1)
+        self.prefix_len.zero_()
+
+    def reset(self) -> None:
+        """Forget every request and the prefix (the pools keep their bytes)."""
+        self.tables.fill_(-1)
+        self.prefix_table.fill_(-1)
+        self.lens.zero_()
+        self.prefix_len.zero_()
+        self.free_ring.copy_(torch.arange(self.n_blocks, dtype=torch.int32, device=self.device))
+        self.free_state.copy_(torch.tensor([0, self.n_blocks], dtype=torch.int32))
+
+    def _index(self, request: int) -> int:
+        r = int(request)
+        if not 0 <= r < self.max_requests:
+            raise ValueError(f"PagedMemory: request {r} outside [0, {self.max_requests})")
+        return r

@@ -126,7 +126,7 @@ enum gfst_qr_method {
 };
 
 /* Element types of key / value / query / summary buffers. */
-enum gfst_dtype { GFST_F32 = 0, GFST_BF16 = 1, GFST_F64 = 2 };
+enum gfst_dtype { GFST_F32 = 0, GFST_BF16 = 1, GFST_F64 = 2, GFST_F16 = 3 /* paged memory only */ };
 
 /* Human-readable text of a status code (static storage). */
 GFST_API const char* gfst_status_string(int status);
@@ -595,6 +595,83 @@ GFST_API int gfst_mpuc_recurrent_scan(const gfst_mpuc_weights* weights, int fast
                                       int64_t batch, int T, float* states_out, float* boundary_out,
                                       float* fast_state, float* mid_state, float* slow_state,
                                       void* workspace, size_t workspace_bytes, cudaStream_t stream);
+
+/* ---- paged memory: block tables -------------------------------------------
+ * n_requests requests of ragged lengths share a pool of n_blocks blocks of L
+ * tokens.  Request b has lens[b] tokens, held in the first ceil(lens[b] / L)
+ * blocks of its row of `tables` [n_requests, width]; free_ring [n_blocks] with
+ * free_state = (head, count) lists the free blocks at positions head ..
+ * head + count - 1 (modulo n_blocks).  One step, in request order:
+ *   new_lens[b] >= 0: the request appends that many tokens; blocks it lacks
+ *     are taken at the ring's head;
+ *   new_lens[b] < 0: the request ends; its blocks go behind the ring's tail
+ *     (after all takes: they are not handed out in the same step), its row
+ *     becomes -1, its length 0.
+ * Outputs: tables_out (-1 behind a row's blocks; may be `tables` itself),
+ * lens_out, cu_new [n_requests + 1] (first packed position of each request's
+ * new tokens, and their number), slot_map [n_tokens] (slot block * L + offset
+ * of each new token in packed order; -1 behind the last one), free_state_out,
+ * free_ring (updated in place), n_short [1] = blocks that were wanted and not
+ * had (ring empty, or beyond `width`): their table entries and slots are -1
+ * and lens_out counts their tokens all the same, so a step with n_short > 0 is
+ * not to be used.  lens_out and free_state_out must not alias the inputs.
+ * All int32 on the device; nothing is read back.  Limits: n_requests <= 16384;
+ * n_blocks * L, width * L and n_requests * width below 2^31.
+ * No reference counterpart: its exact store holds one Python list of blocks
+ * per sample (src/gfst_hmb_mpuc/state.py:651-815).                           */
+GFST_API int gfst_block_tables(const int32_t* lens, const int32_t* new_lens, const int32_t* tables,
+                               int32_t* free_ring, const int32_t* free_state, int n_requests, int width,
+                               int L, int64_t n_blocks, int64_t n_tokens, int32_t* tables_out,
+                               int32_t* lens_out, int32_t* cu_new, int32_t* slot_map,
+                               int32_t* free_state_out, int32_t* n_short, cudaStream_t stream);
+
+/* ---- paged memory: append ---------------------------------------------------
+ * pool_K[s / L, h, s % L, :] = K[t, h, :] and the same for V, with s =
+ * slot_map[t]; tokens with s outside [0, n_blocks * L) are left out.  K:
+ * [n_tokens, n_heads, d], V: [n_tokens, n_heads, dv], rows contiguous, token
+ * and head strides in elements; pool_K: [n_blocks, n_heads, L, d], pool_V:
+ * [n_blocks, n_heads, L, dv].  dtype GFST_F32, GFST_BF16 or GFST_F16 for all
+ * four.  Rows, strides and pointers need multiples of 16 bytes.  A slot named
+ * by two tokens holds either one's row.                                      */
+GFST_API int gfst_paged_append(const void* K, int64_t k_stride_t, int64_t k_stride_h, const void* V,
+                               int64_t v_stride_t, int64_t v_stride_h, void* pool_K, void* pool_V,
+                               const int32_t* slot_map, int64_t n_tokens, int64_t n_blocks, int L,
+                               int n_heads, int d, int dv, int dtype, cudaStream_t stream);
+
+/* ---- paged memory: attention behind a shared prefix -------------------------
+ * For token t, the i-th of the n_b = cu_new[b+1] - cu_new[b] new tokens of
+ * request b, and query head hq = h * group + g (h in [0, n_kv_heads)):
+ *   out[t, hq] = sum_j p_j v_j / sum_j p_j,  p_j = exp(scale * q . k_j),
+ *   lse[t, hq] = log(sum_j p_j)  (natural logarithm; lse may be NULL)
+ * over the prefix_len positions of the prefix (blocks prefix_table[0 ..]) and
+ * positions j <= lens[b] - n_b + i of the request's own blocks (tables row b;
+ * lens counts the new tokens, whose keys are in the pool).  A row that sees
+ * nothing gets zeros and -inf.  The prefix is read for all requests at once.
+ * Q: [n_tokens, n_kv_heads * group, d], rows contiguous, strides in elements;
+ * out: [n_tokens, n_kv_heads * group, dv] dense; pools as gfst_paged_append;
+ * tables: rows table_stride apart, width entries; prefix_len: [1] on the
+ * device (prefix_width == 0: no prefix, both may be NULL); cu_new[0] == 0,
+ * ascending.  Tokens behind cu_new[n_requests] get zeros and -inf when
+ * fill_tail != 0 and are left as they were otherwise.  FP32 softmax statistics
+ * and sums, one rounding of out; 16-bit weights p on the tensor cores are
+ * rounded to the pools' type.  Lengths beyond the tables' positions are cut to
+ * them; a table entry outside [0, n_blocks) reads as zero keys and values and
+ * records GFST_ERR_ARG for gfst_check_device_errors().
+ * workspace: gfst_prefix_attention_workspace_bytes bytes, 256-byte aligned,
+ * one per concurrent call.  Limits: d, dv <= 256, rows and pointers multiples
+ * of 16 bytes, n_requests <= 65536, n_tokens * heads below 2^31.
+ * No reference counterpart: the reference attends per sample through torch.  */
+GFST_API int gfst_prefix_attention_workspace_bytes(int64_t n_tokens, int n_kv_heads, int group, int dv,
+                                                   size_t* bytes);
+GFST_API int gfst_prefix_attention(const void* Q, int64_t q_stride_t, int64_t q_stride_h,
+                                   const void* pool_K, const void* pool_V, int64_t n_blocks, int L,
+                                   int n_kv_heads, int group, int d, int dv, int dtype,
+                                   const int32_t* tables, int64_t table_stride, int width,
+                                   const int32_t* lens, const int32_t* cu_new, int n_requests,
+                                   int64_t n_tokens, const int32_t* prefix_table, int prefix_width,
+                                   const int32_t* prefix_len, float scale, void* out, float* lse,
+                                   int fill_tail, void* workspace, size_t workspace_bytes,
+                                   cudaStream_t stream);
 
 #ifdef __cplusplus
 }  /* extern "C" */
