@@ -48,6 +48,9 @@ extern "C" int gfst_check_device_errors(int clear) {
   st = gfst::read_attn_fma_error(clear, &w);
   if (st != GFST_OK) return st;
   v = v != 0 ? v : w;
+  st = gfst::read_attn_tc_error(clear, &w);
+  if (st != GFST_OK) return st;
+  v = v != 0 ? v : w;
   if (v == GFST_ERR_ARG) {
     gfst::set_last_error("a block table entry outside the pool was read (device error word %u)", v);
     return (int)v;

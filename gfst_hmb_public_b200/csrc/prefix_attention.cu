@@ -55,7 +55,7 @@ struct Join {
 };
 
 template <typename T>
-__global__ void __launch_bounds__(kMergeThreads) prefix_attention_merge_kernel(const AttnArgs a, int MR, int cont_rows) {
+__global__ void __launch_bounds__(kMergeThreads) prefix_attention_merge_kernel(const AttnArgs a, int cont_rows) {
   const int lane = threadIdx.x & 31;
   const int64_t row = (int64_t)blockIdx.x * (kMergeThreads / 32) + (threadIdx.x >> 5);
   const int heads = a.H * a.G;
@@ -69,8 +69,9 @@ __global__ void __launch_bounds__(kMergeThreads) prefix_attention_merge_kernel(c
       if (!own && attn_prefix_len(a) == 0) continue;
       j.add(a.part_ml[own][row], a.part_o[own] + row * a.dv, lane, a.dv);
       const int2 nx = a.part_next[own][row];
-      for (int i = 0; i < nx.y; ++i) {
-        const int64_t c = nx.x + (int64_t)i * MR;
+      const int n = nx.y >> 9, stride = nx.y & 511;
+      for (int i = 0; i < n; ++i) {
+        const int64_t c = nx.x + (int64_t)i * stride;
         if (c < 0 || c >= cont_rows) break;  // offsets that cover no item leave this unset
         j.add(a.cont_ml[c], a.cont_o + c * a.dv, lane, a.dv);
       }
@@ -90,6 +91,15 @@ __global__ void __launch_bounds__(kMergeThreads) prefix_attention_merge_kernel(c
     a.lse[row] = j.l == 0.f ? -INFINITY : (j.m + log2f(j.l)) * 0.69314718055994531f;
 }
 
+template <typename T>
+int launch_merge(const AttnArgs& a, cudaStream_t stream) {
+  const int64_t rows = (int64_t)a.n_tokens * a.H * a.G;
+  const int64_t blocks = (rows + kMergeThreads / 32 - 1) / (kMergeThreads / 32);
+  prefix_attention_merge_kernel<T>
+      <<<(unsigned)blocks, kMergeThreads, 0, stream>>>(a, a.dv <= 128 ? kAttnTcContRows : kAttnFmaContRows);
+  return check_launch("prefix_attention_merge_kernel");
+}
+
 struct Workspace {
   size_t o, ml, next, cont_o, cont_ml, bytes;  // o, ml, next: two of each (prefix, own)
   int64_t rows;
@@ -100,7 +110,8 @@ struct Workspace {
     o = at, at += 2 * up((size_t)rows * dv * 4);
     ml = at, at += 2 * up((size_t)rows * 8);
     next = at, at += 2 * up((size_t)rows * 8);
-    const size_t cont = (size_t)kAttnMaxGrid * kAttnFmaRows;
+    // the tensor-core kernel takes dv <= 128
+    const size_t cont = dv <= 128 ? (size_t)kAttnTcContRows : (size_t)kAttnFmaContRows;
     cont_o = at, at += up(cont * dv * 4);
     cont_ml = at, at += up(cont * 8);
     bytes = at;
@@ -183,16 +194,10 @@ extern "C" int gfst_prefix_attention(const void* Q, int64_t q_stride_t, int64_t 
   a.cont_o = reinterpret_cast<float*>(w + ws.cont_o);
   a.cont_ml = reinterpret_cast<float2*>(w + ws.cont_ml);
 
-  const int MR = kAttnFmaRows;
-  st = launch_prefix_attention_fma(a, dtype, sms, stream);
+  st = prefix_attention_tc_takes(a, dtype) ? launch_prefix_attention_tc(a, dtype, sms, stream)
+                                           : launch_prefix_attention_fma(a, dtype, sms, stream);
   if (st != GFST_OK) return st;
-  const int64_t blocks = (ws.rows + kMergeThreads / 32 - 1) / (kMergeThreads / 32);
-  const int cont_rows = kAttnMaxGrid * MR;
-  if (dtype == GFST_F32)
-    prefix_attention_merge_kernel<float><<<(unsigned)blocks, kMergeThreads, 0, stream>>>(a, MR, cont_rows);
-  else if (dtype == GFST_BF16)
-    prefix_attention_merge_kernel<__nv_bfloat16><<<(unsigned)blocks, kMergeThreads, 0, stream>>>(a, MR, cont_rows);
-  else
-    prefix_attention_merge_kernel<__half><<<(unsigned)blocks, kMergeThreads, 0, stream>>>(a, MR, cont_rows);
-  return check_launch("prefix_attention_merge_kernel");
+  if (dtype == GFST_F32) return launch_merge<float>(a, stream);
+  if (dtype == GFST_BF16) return launch_merge<__nv_bfloat16>(a, stream);
+  return launch_merge<__half>(a, stream);
 }

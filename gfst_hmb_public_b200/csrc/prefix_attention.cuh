@@ -17,13 +17,14 @@
 // request's positions, up to the last one its rows see.  An item's cost is
 // c0 + w * (number of KT-key tiles).
 //
-// Shares.  All items in a fixed order make one line of cost U; CTA c of n
-// takes [U c / n, U (c + 1) / n) and computes the tiles that begin there: any
-// mixture of lengths loads all SMs alike, and a long request is split over
-// many CTAs without a plan made on the host.  The part of an item that holds
-// its first tile writes to the row's own place (prefix or own); a later part
-// is the first work of its CTA, so one continuation buffer per CTA is enough.
-// The row records where its continuations lie: CTAs first + 1 .. first + n.
+// Shares.  All items of a cut, in a fixed order, make one line of cost U;
+// worker c of n takes [U c / n, U (c + 1) / n) and computes the tiles that begin
+// there: any mixture of lengths loads all SMs alike, and a long request is
+// split over many workers without a plan made on the host.  The part of an item
+// that holds its first tile writes to the row's own place (prefix or own); a
+// later part is the first work of its worker, so one continuation buffer per
+// worker is enough.  The row records where its continuations lie: workers
+// first + 1 .. first + n.
 #pragma once
 
 #include "gfst_common.cuh"
@@ -54,9 +55,9 @@ struct AttnArgs {
   // partial results
   float* part_o[2];        // [n_tokens * H * G, dv]: prefix, own
   float2* part_ml[2];      // (m, l)
-  int2* part_next[2];      // (row in the continuation buffer, continuations)
-  float* cont_o;           // [grid, MR, dv]
-  float2* cont_ml;         // [grid, MR]
+  int2* part_next[2];      // attn_next()
+  float* cont_o;           // [continuation rows, dv]
+  float2* cont_ml;         // [continuation rows]
 };
 
 __device__ __forceinline__ int attn_tokens(const AttnArgs& a) { return min(max(a.cu[a.B], 0), a.n_tokens); }
@@ -77,7 +78,7 @@ __device__ __forceinline__ AttnRequest attn_request(const AttnArgs& a, int b) {
   return r;
 }
 
-// One CTA's part of an item.
+// One worker's part of an item.
 struct AttnPart {
   int own;        // 0: prefix, 1: a request's own positions
   int b, h;
@@ -87,65 +88,77 @@ struct AttnPart {
   int see0;       // row r sees positions < min(len, see0 + r / G + 1) (own items)
   int t0, t1;     // tiles of this part
   int first;      // holds the item's first tile: writes the row's own place
-  int n_cont;     // continuations of the item (first part only), in CTAs cta + 1 ..
+  int n_cont;     // continuations of the item (first part only), by workers worker + 1 ..
 };
 
-template <int MR_, int KT_, int C0_, int W1_, int W2_, int ROWS1_>
-struct AttnCost {
-  static constexpr int MR = MR_, KT = KT_;
-  // an item's fixed cost, and a tile's for items of up to ROWS1 rows and of more
-  static constexpr int C0 = C0_, W1 = W1_, W2 = W2_, ROWS1 = ROWS1_;
-  static constexpr int WMAX = W1 > W2 ? W1 : W2;
-  __device__ static __forceinline__ int weight(int rows) { return rows <= ROWS1 ? W1 : W2; }
+// How a group of R rows is cut into items, and what an item costs: C0 + W per
+// tile.  MR is the most rows of an item.
+template <int MR_, int KT_, int C0_, int W_>
+struct AttnCutAll {
+  static constexpr int MR = MR_, KT = KT_, C0 = C0_, W = W_;
+  __device__ static __forceinline__ int count(int R) { return (R + MR - 1) / MR; }
+  __device__ static __forceinline__ int row0(int, int m) { return m * MR; }
+  __device__ static __forceinline__ int rows(int R, int m) { return min(MR, R - m * MR); }
+};
+// Items of more than HALF rows, up to two HALF-row tiles that share their keys ...
+template <int HALF, int KT_, int C0_, int W_>
+struct AttnCutPairs {
+  static constexpr int MR = 2 * HALF, KT = KT_, C0 = C0_, W = W_;
+  __device__ static __forceinline__ int count(int R) { return R > HALF ? (R - HALF + MR - 1) / MR : 0; }
+  __device__ static __forceinline__ int row0(int, int m) { return m * MR; }
+  __device__ static __forceinline__ int rows(int R, int m) { return min(MR, R - m * MR); }
+};
+// ... and what they leave: at most one item of up to HALF rows.
+template <int HALF, int KT_, int C0_, int W_>
+struct AttnCutRest {
+  using Pairs = AttnCutPairs<HALF, KT_, C0_, W_>;
+  static constexpr int MR = HALF, KT = KT_, C0 = C0_, W = W_;
+  __device__ static __forceinline__ int row0(int R, int) { return Pairs::count(R) * 2 * HALF; }
+  __device__ static __forceinline__ int rows(int R, int) { return R - row0(R, 0); }
+  __device__ static __forceinline__ int count(int R) { return rows(R, 0) > 0 ? 1 : 0; }
 };
 
-// Walks a CTA's share.  init() is called by every thread of the CTA; next() by
-// any set of threads, each for itself (the state is per thread).
+// The line of all items of one cut, over n shares.
 template <class C>
-struct AttnWalk {
-  int64_t U, u0, u1;           // whole cost, this CTA's share
-  int n_cta;
+struct AttnLine {
+  int64_t U, prefix_all, prefix_cost;
+  int n;
   int prefix_len, prefix_rows, prefix_mt, prefix_nt;
-  int64_t prefix_cost;         // one prefix item
-  // current item
-  int own, b, h, m;
-  int64_t at;                  // cost position where the current item begins
-  AttnRequest req;
+  // this thread's requests [b0, b1): their cost and the cost before them
+  int b0, b1;
+  int64_t before, sum;
 
   __device__ static __forceinline__ int tiles(int len) { return max(1, (len + C::KT - 1) / C::KT); }
-  __device__ static __forceinline__ int row_tiles(int rows) { return (rows + C::MR - 1) / C::MR; }
-  // positions that rows [row0, row0 + rows) of a request see between them
+  // positions that the rows up to `last_row` of a request see between them
   __device__ static __forceinline__ int see(const AttnRequest& r, int last_row, int G) {
     return min(r.len, max(0, r.len - r.n + last_row / G + 1));
   }
-  __device__ static __forceinline__ int64_t own_item_cost(const AttnRequest& r, int m, int G) {
-    const int all = r.n * G, rows = min(C::MR, all - m * C::MR);
-    return C::C0 + (int64_t)C::weight(rows) * tiles(see(r, m * C::MR + rows - 1, G));
+  __device__ static __forceinline__ int own_tiles(const AttnRequest& r, int m, int G) {
+    const int R = r.n * G;
+    return tiles(see(r, C::row0(R, m) + C::rows(R, m) - 1, G));
   }
+  __device__ static __forceinline__ int64_t item_cost(int nt) { return C::C0 + (int64_t)C::W * nt; }
   __device__ static __forceinline__ int64_t head_cost(const AttnRequest& r, int G) {
     int64_t c = 0;
-    const int mt = row_tiles(r.n * G);
-    for (int m = 0; m < mt; ++m) c += own_item_cost(r, m, G);
+    const int mt = C::count(r.n * G);
+    for (int m = 0; m < mt; ++m) c += item_cost(own_tiles(r, m, G));
     return c;
   }
 
-  // Shares over at most `grid` CTAs, none smaller than the costliest tile plus
-  // an item's fixed cost.
-  __device__ void init(const AttnArgs& a, int grid, int cta) {
-    __shared__ int64_t s_sum[32];
-    __shared__ int s_b;
-    __shared__ int64_t s_at;
+  // Called by every thread of the CTA.  No share is smaller than an item's
+  // fixed cost and one tile, so every share between the first and the last of
+  // an item holds one of its tiles.
+  __device__ void init(const AttnArgs& a, int most_shares, int64_t* s_sum) {
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, n_warps = (blockDim.x + 31) >> 5;
     prefix_len = attn_prefix_len(a);
     prefix_rows = prefix_len > 0 ? attn_tokens(a) * a.G : 0;
-    prefix_mt = row_tiles(prefix_rows);
+    prefix_mt = C::count(prefix_rows);
     prefix_nt = tiles(prefix_len);
-    prefix_cost = C::C0 + (int64_t)C::weight(prefix_rows) * prefix_nt;
-    const int64_t prefix_all = prefix_cost * prefix_mt * a.H;
-    // thread t owns requests [t * per, (t + 1) * per)
+    prefix_cost = item_cost(prefix_nt);
+    prefix_all = prefix_cost * prefix_mt * a.H;
     const int per = (a.B + blockDim.x - 1) / blockDim.x;
-    const int b0 = min(a.B, tid * per), b1 = min(a.B, b0 + per);
-    int64_t sum = 0;
+    b0 = min(a.B, tid * per), b1 = min(a.B, b0 + per);
+    sum = 0;
     for (int i = b0; i < b1; ++i) sum += head_cost(attn_request(a, i), a.G) * a.H;
     int64_t inc = sum;
 #pragma unroll
@@ -154,51 +167,67 @@ struct AttnWalk {
       if (lane >= o) inc += v;
     }
     if (lane == 31) s_sum[warp] = inc;
-    if (tid == 0) s_b = a.B;
     __syncthreads();
-    int64_t before = prefix_all + inc - sum;
+    before = prefix_all + inc - sum;
     U = prefix_all;
     for (int w = 0; w < n_warps; ++w) {
       if (w < warp) before += s_sum[w];
       U += s_sum[w];
     }
-    const int64_t most = U / (C::C0 + C::WMAX);
-    n_cta = (int)max((int64_t)1, min((int64_t)grid, most));
-    u0 = cta < n_cta ? U * cta / n_cta : U;
-    u1 = cta < n_cta ? U * (cta + 1) / n_cta : U;
-    if (u0 >= prefix_all && before <= u0 && u0 < before + sum) {
-      int64_t p = before;
-      int i = b0;
-      for (; i < b1; ++i) {
-        const int64_t c = head_cost(attn_request(a, i), a.G) * a.H;
-        if (u0 < p + c) break;
-        p += c;
-      }
-      s_b = i;
-      s_at = p;
+    n = (int)max((int64_t)1, min((int64_t)most_shares, U / (C::C0 + C::W)));
+    __syncthreads();  // s_sum may be used again
+  }
+  __device__ __forceinline__ int64_t bound(int i) const { return i < n ? U * i / n : U; }
+  // Called by every thread: the one whose requests hold the beginning of share
+  // i leaves the request and the cost before it (to be read after a barrier).
+  __device__ void find(const AttnArgs& a, int i, int* s_b, int64_t* s_at) const {
+    const int64_t u = bound(i);
+    if (u < prefix_all || u < before || u >= before + sum) return;
+    int64_t p = before;
+    int b = b0;
+    for (; b < b1; ++b) {
+      const int64_t c = head_cost(attn_request(a, b), a.G) * a.H;
+      if (u < p + c) break;
+      p += c;
     }
-    __syncthreads();
-    own = u0 >= prefix_all;
+    *s_b = b;
+    *s_at = p;
+  }
+  // share that holds cost position p
+  __device__ __forceinline__ int share_of(int64_t p) const { return (int)(((p + 1) * n - 1) / U); }
+};
+
+// Walks share i of a line; the state is the calling thread's.
+template <class C>
+struct AttnWalk {
+  int64_t u0, u1, at;
+  int own, b, h, m;
+  AttnRequest req;
+
+  __device__ void begin(const AttnArgs& a, const AttnLine<C>& ln, int i, int s_b, int64_t s_at) {
+    u0 = ln.bound(i);
+    u1 = ln.bound(i + 1);
+    own = u0 >= ln.prefix_all;
     m = h = b = 0;
     at = 0;
-    if (u0 >= U) {  // nothing for this CTA
+    if (u0 >= u1) {  // nothing in this share
       own = 1;
       b = a.B;
-      at = U;
+      at = u1;
     } else if (!own) {
-      const int64_t i = u0 / prefix_cost;
-      h = (int)(i / prefix_mt);
-      m = (int)(i - (int64_t)h * prefix_mt);
-      at = i * prefix_cost;
+      const int64_t k = u0 / ln.prefix_cost;
+      h = (int)(k / ln.prefix_mt);
+      m = (int)(k - (int64_t)h * ln.prefix_mt);
+      at = k * ln.prefix_cost;
     } else {
       b = s_b;
       at = s_at;
       req = attn_request(a, b);
-      const int64_t hc = head_cost(req, a.G);
+      const int64_t hc = ln.head_cost(req, a.G);
       h = (int)((u0 - at) / hc);
       at += hc * h;
       for (;;) {
-        const int64_t c = own_item_cost(req, m, a.G);
+        const int64_t c = ln.item_cost(ln.own_tiles(req, m, a.G));
         if (u0 < at + c) break;
         at += c;
         ++m;
@@ -206,79 +235,65 @@ struct AttnWalk {
     }
   }
 
-  // CTA whose share holds cost position p
-  __device__ __forceinline__ int cta_of(int64_t p) const { return (int)(((p + 1) * n_cta - 1) / U); }
-
   // The next part with at least one tile; false at the end of the share.
-  __device__ bool next(const AttnArgs& a, AttnPart& it) {
+  __device__ bool next(const AttnArgs& a, const AttnLine<C>& ln, AttnPart& it) {
     for (;;) {
       if (at >= u1 || (own && b >= a.B)) return false;
-      int rows, nt;
-      int64_t cost;
+      const int R = own ? req.n * a.G : ln.prefix_rows;
+      int nt;
       it.own = own;
       it.h = h;
+      it.row0 = C::row0(R, m);
+      it.rows = C::rows(R, m);
       if (!own) {
-        rows = min(C::MR, prefix_rows - m * C::MR);
-        nt = prefix_nt;
-        cost = prefix_cost;
+        nt = ln.prefix_nt;
         it.b = -1;
         it.tok0 = 0;
-        it.len = prefix_len;
+        it.len = ln.prefix_len;
         it.see0 = 0;
       } else {
-        rows = min(C::MR, req.n * a.G - m * C::MR);
-        const int last = see(req, m * C::MR + rows - 1, a.G);
-        nt = tiles(last);
-        cost = C::C0 + (int64_t)C::weight(rows) * nt;
         it.b = b;
         it.tok0 = req.tok0;
-        it.len = last;
+        it.len = ln.see(req, it.row0 + it.rows - 1, a.G);
         it.see0 = req.len - req.n;
+        nt = ln.tiles(it.len);
       }
-      it.row0 = m * C::MR;
-      it.rows = rows;
-      // tile j begins at cost position at + C0 + j * w
-      const int w = C::weight(own ? rows : prefix_rows);
+      // tile j begins at cost position base + j * W
       const int64_t base = at + C::C0;
       auto tile_from = [&](int64_t u) -> int {
-        return u <= base ? 0 : (int)min((int64_t)nt, (u - base + w - 1) / w);
+        return u <= base ? 0 : (int)min((int64_t)nt, (u - base + C::W - 1) / C::W);
       };
       it.t0 = tile_from(u0);
       it.t1 = tile_from(u1);
       it.first = it.t0 == 0;
       it.n_cont = 0;
-      if (it.first && it.t1 < nt) it.n_cont = cta_of(base + (int64_t)(nt - 1) * w) - cta_of(base);
+      if (it.first && it.t1 < nt) it.n_cont = ln.share_of(base + (int64_t)(nt - 1) * C::W) - ln.share_of(base);
       // step to the next item
-      at += cost;
+      at += ln.item_cost(nt);
       ++m;
-      if (!own) {
-        if (m == prefix_mt) {
-          m = 0;
-          if (++h == a.H) {
-            h = 0;
-            own = 1;
-            b = -1;
-            advance_request(a);
-          }
-        }
-      } else if (m * C::MR >= req.n * a.G) {
+      if (m >= C::count(R)) {
         m = 0;
         if (++h == a.H) {
           h = 0;
-          advance_request(a);
+          if (!own) {
+            own = 1;
+            b = -1;
+          }
+          do {
+            if (++b >= a.B) break;
+            req = attn_request(a, b);
+          } while (C::count(req.n * a.G) == 0);
         }
       }
       if (it.t1 > it.t0) return true;
     }
   }
-
-  __device__ __forceinline__ void advance_request(const AttnArgs& a) {
-    do {
-      if (++b >= a.B) return;
-      req = attn_request(a, b);
-    } while (req.n == 0);
-  }
 };
+
+// part_next of a row: where its continuations begin and how far they lie apart
+__device__ __forceinline__ int2 attn_next(int cont_row, int n_cont, int stride) {
+  return make_int2(cont_row, n_cont * 512 + stride);
+}
 
 // Block holding position p (or -1 where the table names none of the pool's).
 __device__ __forceinline__ int attn_block(const AttnArgs& a, const AttnPart& it, int index) {
@@ -295,10 +310,16 @@ __device__ __forceinline__ void attn_row(const AttnArgs& a, const AttnPart& it, 
   hq = it.h * a.G + rg - t * a.G;
 }
 
-// device kernels' launchers (each returns a status)
-constexpr int kAttnMaxGrid = 320;      // continuation buffers
-constexpr int kAttnFmaRows = 32;       // MR of the FP32 kernel
-constexpr int kAttnTcRows = 256;       // MR of the tensor-core kernel
+// the kernels' launchers (each returns a status)
+constexpr int kAttnMaxGrid = 160;      // CTAs of a launch (two per SM of the FP32 kernel count as one here)
+constexpr int kAttnFmaRows = 32;       // rows of an item of the FP32 kernel
+constexpr int kAttnTcHalf = 128;       // rows of a tile of the tensor-core kernel
+// continuation rows: 32 for each of 320 CTAs of the FP32 kernel; 256 for a CTA's
+// pairs and 128 for each of its two streams of the tensor-core kernel
+constexpr int kAttnFmaContRows = 2 * kAttnMaxGrid * kAttnFmaRows;
+constexpr int kAttnTcContRows = kAttnMaxGrid * 4 * kAttnTcHalf;
 int launch_prefix_attention_fma(const AttnArgs& a, int dtype, int sms, cudaStream_t stream);
+bool prefix_attention_tc_takes(const AttnArgs& a, int dtype);
+int launch_prefix_attention_tc(const AttnArgs& a, int dtype, int sms, cudaStream_t stream);
 
 }  // namespace gfst

@@ -24,8 +24,7 @@ constexpr int kKeys = 64;
 constexpr int kThreads = 256;
 constexpr int kWarps = kThreads / 32;
 // An item's fixed cost is about two 64-key tiles (queries in, partials out).
-using FmaCost = AttnCost<kRows, kKeys, 2, 1, 1, kRows>;
-using Walk = AttnWalk<FmaCost>;
+using Cut = AttnCutAll<kRows, kKeys, 2, 1>;
 
 template <typename T>
 struct Vec;  // 16 bytes of T as floats
@@ -109,11 +108,17 @@ __global__ void __launch_bounds__(kThreads) prefix_attention_fma_kernel(const At
   const int grp = tid / n_col, col = (tid - grp * n_col) * 4;
   constexpr int kAcc = 8;                // rows per thread at dv = 256; fewer below
 
-  Walk walk;
-  walk.init(a, gridDim.x, blockIdx.x);
+  __shared__ int64_t s_sum[32], s_at;
+  __shared__ int s_b;
+  AttnLine<Cut> line;
+  line.init(a, gridDim.x, s_sum);
+  line.find(a, blockIdx.x, &s_b, &s_at);
+  __syncthreads();
+  AttnWalk<Cut> walk;
+  walk.begin(a, line, blockIdx.x, s_b, s_at);
   AttnPart it;
   bool bad = false;
-  while (walk.next(a, it)) {
+  while (walk.next(a, line, it)) {
     __syncthreads();
     for (int i = tid; i < it.rows * kvr; i += kThreads) {
       const int r = i / kvr;
@@ -242,7 +247,7 @@ __global__ void __launch_bounds__(kThreads) prefix_attention_fma_kernel(const At
             const float2 ml = make_float2(s_m[r], s_l[r]);
             if (it.first) {
               a.part_ml[it.own][row] = ml;
-              a.part_next[it.own][row] = make_int2((blockIdx.x + 1) * kRows + r, it.n_cont);
+              a.part_next[it.own][row] = attn_next((blockIdx.x + 1) * kRows + r, it.n_cont, kRows);
             } else {
               a.cont_ml[crow] = ml;
             }
@@ -261,7 +266,7 @@ int launch(const AttnArgs& a, int sms, cudaStream_t stream) {
   cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, FmaLayout(256, 256).bytes);
   GFST_REQUIRE(e == cudaSuccess, GFST_ERR_DEVICE, "cudaFuncSetAttribute: %s", cudaGetErrorString(e));
   const int per_sm = ly.bytes <= 110 * 1024 ? 2 : 1;
-  const int grid = sms * per_sm < kAttnMaxGrid ? sms * per_sm : kAttnMaxGrid;
+  const int grid = (sms < kAttnMaxGrid ? sms : kAttnMaxGrid) * per_sm;
   kern<<<grid, kThreads, ly.bytes, stream>>>(a);
   return check_launch("prefix_attention_fma_kernel");
 }

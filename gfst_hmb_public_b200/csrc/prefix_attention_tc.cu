@@ -1,0 +1,709 @@
+// Shared-prefix attention on the 5th-generation tensor cores: bf16 or fp16,
+// d = dv = 64 or 128, blocks that tile 128 keys (L a divisor of 128 from 8 up,
+// or a multiple of 128).
+//
+// A CTA (one per SM) runs two streams, each with a 128-row query tile:
+//   S = Q K^T     tcgen05.mma, both operands in shared memory, S in TMEM
+//   P = 2^(c S - m) by four warps, one row per thread, rounded to the pools'
+//                 type and stored back to TMEM over S
+//   O += P V      tcgen05.mma, P from TMEM, V from shared memory (keys along
+//                 the contraction: V is the MN-major operand), O in TMEM
+// While one stream's rows are exponentiated, the other's products run.  Per
+// 128 x 128 tile at d = 128 the products take 1024 tensor cycles and the 16,384
+// exponentials 1024 cycles of the SM's special-function units: with many rows
+// the two bound the kernel together; with few rows the bytes of K and V do.
+//
+// Two kinds of work (prefix_attention.cuh), each cut evenly over the CTAs:
+//   pairs   items of more than 128 rows: both streams take the same K and V
+//           tiles (one load for 256 rows), through a ring of all stages
+//   rest    items of up to 128 rows: every stream walks its own share with its
+//           own stages, so two items are in flight on an SM
+//
+// Warps: 0-3 and 4-7 softmax of stream 0 and 1 (warp w reads TMEM lanes 32 (w %
+// 4) ..); 8, 9 the streams' producers (work list, queries by cp.async, K and V by
+// TMA, one box per block and 64 columns); 10, 11 their MMA issuers.
+//
+// The maximum is followed lazily: m only moves when a row's new maximum exceeds
+// it by more than 8 (in log2), so O in TMEM is rescaled a few times per row and
+// not once a tile; sums then stay below 2^8 times their keys, exact softmax all
+// the same because every term uses the same m.  For fp16 the reference is
+// lowered by 7, so that p lies in [2^7, 2^15] at the top and the smallest
+// weights keep their bits.
+//
+// Masked keys get p = 0 by selection.  Since 0 * (inf or NaN) is NaN in the
+// product, value rows behind the last key are zeroed in shared memory, and a
+// value row that only some of the tile's rows see and that is not finite is
+// taken out of the product and added by the threads whose rows see it.
+//
+// Every wait is bounded; one that gives up sets the CTA's abort flag, every role
+// leaves its loop, copies in flight are waited for, TMEM is freed and the sticky
+// error word records GFST_ERR_TIMEOUT.
+#include <cuda_fp16.h>
+
+#include "prefix_attention.cuh"
+#include "umma.cuh"
+
+namespace gfst {
+
+GFST_DEFINE_ERROR_WORD(g_attn_tc_error, read_attn_tc_error, "attention")
+
+namespace {
+
+constexpr int kHalf = kAttnTcHalf;  // rows of a stream's tile
+constexpr int kKeys = 128;          // keys of a tile
+constexpr int kThreads = 384;
+constexpr int kProducer = 8, kMma = 10;
+constexpr int kItems = 4;           // parts announced ahead
+constexpr uint32_t kTmemCols = 512; // per stream: S (P over it) 128, O 128
+constexpr float kLazy = 8.f;
+
+// An item's fixed cost (queries, first scores, last values, partials out) is
+// that of about two tiles.
+using Pairs = AttnCutPairs<kHalf, kKeys, 2, 1>;
+using Rest = AttnCutRest<kHalf, kKeys, 2, 1>;
+
+template <int D>
+struct TcAttn {
+  static constexpr int NC = D / 64;                // 64-column chunks (128-byte swizzle rows)
+  static constexpr int TILE_BYTES = NC * 128 * 128;  // a 128-row tile of Q, K or V
+  static constexpr int NS = D == 64 ? 4 : 2;       // stages of a stream
+  static constexpr int RING = 2 * NS;              // stages of the pairs' ring
+  static constexpr int Q_OFF = 0;
+  static constexpr int KV_OFF = 2 * TILE_BYTES;
+  static constexpr int CTRL_OFF = KV_OFF + RING * TILE_BYTES;
+};
+
+struct StreamCtrl {
+  uint64_t item_full[kItems], item_empty[kItems];
+  uint64_t q_full, q_empty, s_full, p_ready, pv_done;
+  uint64_t care;               // the softmax warps among themselves
+  uint64_t full[4], empty[4];  // the stream's own stages
+  AttnPart item[kItems];
+  int paired[kItems];          // 1: pair, 0: rest, -1: no more work
+  uint32_t bad[4];             // value rows that are not finite (one bit each)
+  int accumulate;              // the tile's first product adds to O
+  int at_b[2];
+  int64_t at_u[2];
+};
+struct Ctrl {
+  StreamCtrl s[2];
+  uint64_t full[8], empty[8];  // the pairs' ring
+  uint64_t care;                 // both streams' softmax warps
+  uint64_t drained;              // the pairs are done with the ring
+  uint64_t done[2];              // a stream's products are done
+  int64_t sum[32];
+  uint32_t tmem;
+  int abort;
+};
+
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+template <bool F16>
+__device__ __forceinline__ uint32_t pack2(float lo, float hi) {
+  uint32_t r;
+  if constexpr (F16) asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+  else asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+  return r;
+}
+
+__device__ __forceinline__ void tmem_ld32(uint32_t taddr, float* v) {
+  uint32_t* r = reinterpret_cast<uint32_t*>(v);
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 "
+      "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
+      "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+        "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]),
+        "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]),
+        "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+      : "r"(taddr));
+}
+__device__ __forceinline__ void tmem_st32(uint32_t taddr, const uint32_t* r) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], "
+      "{%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, "
+      "%17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31, %32};" ::"r"(taddr),
+      "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
+      "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]), "r"(r[17]), "r"(r[18]),
+      "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]),
+      "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31])
+      : "memory");
+}
+__device__ __forceinline__ float tmem_ld1(uint32_t taddr) {
+  uint32_t r;
+  asm volatile("tcgen05.ld.sync.aligned.32x32b.x1.b32 {%0}, [%1];" : "=r"(r) : "r"(taddr));
+  return __uint_as_float(r);
+}
+__device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+__device__ __forceinline__ void fence_async_smem() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
+
+// D[tmem] += A[tmem] B[smem]
+__device__ __forceinline__ void umma_ts(uint32_t d, uint32_t a, uint64_t bdesc, uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d),
+      "r"(a), "l"(bdesc), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+// 128B-swizzled, MN-major operand: 64-element column chunks `chunk` bytes apart,
+// groups of 8 contraction rows 1024 bytes apart.
+__device__ __forceinline__ uint64_t sw128_mn_desc(uint32_t saddr, uint32_t chunk) {
+  return (uint64_t)((saddr & 0x3FFFFu) >> 4) | ((uint64_t)(chunk >> 4) << 16) | ((uint64_t)(1024 >> 4) << 32) |
+         ((uint64_t)1 << 46) | ((uint64_t)2 << 61);
+}
+// kind::f16 instruction descriptor, 128 x N, A and B of one 16-bit type; b_mn: B is MN-major
+__host__ __device__ constexpr uint32_t idesc16(bool f16, int N, bool b_mn) {
+  return (1u << 4) | (f16 ? 0u : (1u << 7) | (1u << 10)) | (b_mn ? 1u << 16 : 0u) | ((uint32_t)(N >> 3) << 17) |
+         ((uint32_t)(128 >> 4) << 24);
+}
+
+// One role's waits: after a wait that gave up (or another role's), false.
+struct Waiter {
+  volatile int* abort;
+  __device__ __forceinline__ bool operator()(uint64_t* bar, uint32_t parity) const {
+    if (!mbar_wait(bar, parity)) *abort = 1;
+    return *abort == 0;
+  }
+  // the whole warp waits; lanes leave together
+  __device__ __forceinline__ bool warp(uint64_t* bar, uint32_t parity) const {
+    int ok = (*this)(bar, parity) ? 1 : 0;
+    return __all_sync(0xffffffffu, ok);
+  }
+};
+
+template <int D, bool F16>
+__global__ void __launch_bounds__(kThreads, 1)
+    prefix_attention_tc_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV,
+                               const __grid_constant__ AttnArgs a, int64_t pool_rows) {
+  using TC = TcAttn<D>;
+  constexpr int NS = TC::NS, RING = TC::RING, NC = TC::NC, TILE = TC::TILE_BYTES;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  Ctrl* ctl = reinterpret_cast<Ctrl*>(smem + TC::CTRL_OFF);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+
+  if (threadIdx.x == 0) {
+    for (int j = 0; j < 2; ++j) {
+      StreamCtrl& c = ctl->s[j];
+      for (int i = 0; i < kItems; ++i) {
+        mbar_init(&c.item_full[i], 1);
+        mbar_init(&c.item_empty[i], 5);  // four softmax warps, the MMA warp
+      }
+      mbar_init(&c.q_full, 1);
+      mbar_init(&c.q_empty, 1);
+      mbar_init(&c.s_full, 1);
+      mbar_init(&c.p_ready, 4);
+      mbar_init(&c.pv_done, 1);
+      mbar_init(&c.care, 4);
+      for (int i = 0; i < 4; ++i) {
+        mbar_init(&c.full[i], 1);
+        mbar_init(&c.empty[i], 1);
+      }
+      c.accumulate = 0;
+      mbar_init(&ctl->done[j], 1);
+    }
+    for (int i = 0; i < 8; ++i) {
+      mbar_init(&ctl->full[i], 1);
+      mbar_init(&ctl->empty[i], 2);  // both streams' products
+    }
+    mbar_init(&ctl->care, 8);
+    mbar_init(&ctl->drained, 1);
+    ctl->abort = 0;
+    mbar_init_fence();
+  }
+  if (warp == kMma) tmem_alloc(&ctl->tmem, kTmemCols);
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = ctl->tmem;
+
+  // the work: this CTA's share of the pairs, and one share of the rest per
+  // stream (stream 1's behind all of stream 0's, so few items spread over the SMs)
+  AttnLine<Pairs> pl;
+  AttnLine<Rest> rl;
+  pl.init(a, gridDim.x, ctl->sum);
+  rl.init(a, 2 * gridDim.x, ctl->sum);
+  pl.find(a, blockIdx.x, &ctl->s[0].at_b[0], &ctl->s[0].at_u[0]);
+  for (int j = 0; j < 2; ++j) rl.find(a, blockIdx.x + j * gridDim.x, &ctl->s[j].at_b[1], &ctl->s[j].at_u[1]);
+  __syncthreads();
+
+  const Waiter wait{&ctl->abort};
+  uint32_t issued_own = 0, issued_ring = 0;  // stages filled by this producer (for the drain)
+
+  if (warp >= kProducer && warp < kProducer + 2) {
+    // ------------------------------------------------------------- producer
+    const int j = warp - kProducer;
+    StreamCtrl& c = ctl->s[j];
+    uint8_t* sq = smem + TC::Q_OFF + j * TILE;
+    uint32_t n_item = 0;
+    bool bad = false, ok = true;
+
+    // one part: announce it, its queries, its keys and values (for pairs the
+    // first stream's producer loads them for both)
+    auto part = [&](const AttnPart& it, int paired) -> bool {
+      const int slot = n_item % kItems;
+      if (!wait.warp(&c.item_empty[slot], ((n_item / kItems) & 1) ^ 1)) return false;
+      if (lane == 0) {
+        c.item[slot] = it;
+        c.paired[slot] = paired;
+        mbar_arrive(&c.item_full[slot]);
+      }
+      if (!wait.warp(&c.q_empty, (n_item & 1) ^ 1)) return false;
+      ++n_item;
+      // query rows of this stream, 16 bytes a copy, swizzled as TMA would
+      const int r_first = paired ? j * kHalf : 0;
+      const int rows = min(kHalf, it.rows - r_first);
+      const uint16_t* Q = static_cast<const uint16_t*>(a.Q);
+      for (int i = lane; i < rows * (D / 8); i += 32) {
+        const int r = i / (D / 8), v = i % (D / 8);
+        int tok, hq;
+        attn_row(a, it, r_first + r, tok, hq);
+        const uint32_t dst = smem_u32(sq + (v >> 3) * (128 * 128) + r * 128 + (((v & 7) ^ (r & 7)) << 4));
+        asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst),
+                     "l"(Q + tok * a.q_st + hq * a.q_sh + v * 8)
+                     : "memory");
+      }
+      asm volatile("cp.async.commit_group;" ::: "memory");
+      bool q_sent = false;
+      auto send_q = [&]() {
+        asm volatile("cp.async.wait_all;" ::: "memory");
+        fence_async_smem();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&c.q_full);
+        q_sent = true;
+      };
+      if (paired && j == 1) {
+        send_q();
+        return true;
+      }
+      const int box = min(a.L, kKeys);         // rows of a copy
+      const int boxes = kKeys / box;           // copies of a full tile, one per lane
+      auto block_row = [&](int t) -> int64_t {  // pool row of this lane's box in tile t
+        const int p = t * kKeys + lane * box;
+        if (lane >= boxes || p >= it.len) return -1;
+        const int idx = p / a.L;
+        const int blk = attn_block(a, it, idx);
+        // an entry outside the pool: a row behind its end, which TMA fills with zeros
+        if (blk < 0) return pool_rows;
+        return ((int64_t)blk * a.H + it.h) * a.L + (p - idx * a.L);
+      };
+      int64_t row = block_row(it.t0);
+      for (int t = it.t0; t < it.t1; ++t) {
+        const int64_t ahead = t + 1 < it.t1 ? block_row(t + 1) : -1;
+        if (row == pool_rows) bad = true;
+        const int n = __popc(__ballot_sync(0xffffffffu, row >= 0));
+#pragma unroll
+        for (int kv = 0; kv < 2; ++kv) {
+          uint64_t *full, *empty;
+          uint8_t* dst;
+          uint32_t parity;
+          if (paired) {
+            const uint32_t st = issued_ring % RING;
+            full = &ctl->full[st], empty = &ctl->empty[st];
+            parity = (issued_ring / RING) & 1;
+            dst = smem + TC::KV_OFF + st * TILE;
+            ++issued_ring;
+          } else {
+            const uint32_t st = issued_own % NS;
+            full = &c.full[st], empty = &c.empty[st];
+            parity = (issued_own / NS) & 1;
+            dst = smem + TC::KV_OFF + (j * NS + st) * TILE;
+            ++issued_own;
+          }
+          if (!wait.warp(empty, parity ^ 1)) {
+            if (paired) --issued_ring;
+            else --issued_own;
+            return false;
+          }
+          if (lane == 0) mbar_arrive_expect_tx(full, (uint32_t)(n * box * NC * 128));
+          __syncwarp();
+          if (row >= 0) {
+#pragma unroll
+            for (int ch = 0; ch < NC; ++ch)
+              tma_load_2d(dst + ch * (128 * 128) + lane * box * 128, kv ? &tmV : &tmK, full, ch * 64, (int)row);
+          }
+        }
+        if (!q_sent) send_q();
+        row = ahead;
+      }
+      return true;
+    };
+
+    AttnPart it;
+    {
+      AttnWalk<Pairs> w;
+      w.begin(a, pl, blockIdx.x, ctl->s[0].at_b[0], ctl->s[0].at_u[0]);
+      while (ok && w.next(a, pl, it)) ok = part(it, 1);
+      // the rest's stages lie in the ring: the pairs' products have to be done with it
+      if (j == 0) {
+        const uint32_t total = issued_ring;
+        for (uint32_t i = total > RING ? total - RING : 0; ok && i < total; ++i)
+          ok = wait.warp(&ctl->empty[i % RING], (i / RING) & 1);
+        if (lane == 0) mbar_arrive(&ctl->drained);
+      } else if (ok) {
+        ok = wait.warp(&ctl->drained, 0);
+      }
+    }
+    {
+      AttnWalk<Rest> w;
+      const int i = blockIdx.x + j * gridDim.x;
+      w.begin(a, rl, i, c.at_b[1], c.at_u[1]);
+      while (ok && w.next(a, rl, it)) ok = part(it, 0);
+    }
+    const int slot = n_item % kItems;
+    if (ok && wait.warp(&c.item_empty[slot], ((n_item / kItems) & 1) ^ 1) && lane == 0) {
+      c.paired[slot] = -1;
+      mbar_arrive(&c.item_full[slot]);
+    }
+    asm volatile("cp.async.wait_all;" ::: "memory");
+    if (bad) atomicExch(&g_attn_tc_error, (unsigned)GFST_ERR_ARG);
+  } else if (warp >= kMma) {
+    // ------------------------------------------------------------------ MMA
+    const int j = warp - kMma;
+    StreamCtrl& c = ctl->s[j];
+    if (lane == 0) {
+      constexpr uint32_t idesc_s = idesc16(F16, kKeys, false), idesc_o = idesc16(F16, D, true);
+      const uint32_t tS = tmem + j * 256, tO = tS + 128;
+      const uint32_t sq = smem_u32(smem + TC::Q_OFF + j * TILE);
+      uint32_t n_item = 0, n_tile = 0, n_own = 0, n_ring = 0;
+      bool ok = true;
+      while (ok) {
+        const int slot = n_item % kItems;
+        if (!wait(&c.item_full[slot], (n_item / kItems) & 1)) break;
+        const int paired = c.paired[slot], t0 = c.item[slot].t0, t1 = c.item[slot].t1;
+        if (paired < 0) break;
+        mbar_arrive(&c.item_empty[slot]);
+        if (!wait(&c.q_full, n_item & 1)) break;
+        ++n_item;
+        for (int t = t0; t < t1; ++t) {
+          uint64_t *kf, *ke, *vf, *ve;
+          uint32_t kp, vp;
+          uint8_t *ks, *vs;
+          auto stage = [&](uint64_t*& full, uint64_t*& empty, uint32_t& parity, uint8_t*& at) {
+            if (paired) {
+              const uint32_t st = n_ring % RING;
+              full = &ctl->full[st], empty = &ctl->empty[st], parity = (n_ring / RING) & 1;
+              at = smem + TC::KV_OFF + st * TILE;
+              ++n_ring;
+            } else {
+              const uint32_t st = n_own % NS;
+              full = &c.full[st], empty = &c.empty[st], parity = (n_own / NS) & 1;
+              at = smem + TC::KV_OFF + (j * NS + st) * TILE;
+              ++n_own;
+            }
+          };
+          stage(kf, ke, kp, ks);
+          stage(vf, ve, vp, vs);
+          // P of the last tile lies over S: its product has to be done
+          if (!(ok = wait(kf, kp) && (n_tile == 0 || wait(&c.pv_done, (n_tile - 1) & 1)))) break;
+          tc_fence_after();
+#pragma unroll
+          for (int kk = 0; kk < D / 16; ++kk) {
+            const uint32_t off = (kk >> 2) * (128 * 128) + (kk & 3) * 32;
+            umma_bf16(tS, sw128_desc(sq + off), sw128_desc(smem_u32(ks) + off), idesc_s, kk > 0 ? 1u : 0u);
+          }
+          umma_commit(&c.s_full);
+          umma_commit(ke);
+          if (t == t1 - 1) umma_commit(&c.q_empty);
+          if (!(ok = wait(&c.p_ready, n_tile & 1) && wait(vf, vp))) break;
+          tc_fence_after();
+          const uint32_t acc = t > t0 || c.accumulate != 0 ? 1u : 0u;
+          c.accumulate = 0;
+#pragma unroll
+          for (int kk = 0; kk < kKeys / 16; ++kk)
+            umma_ts(tO, tS + kk * 8, sw128_mn_desc(smem_u32(vs) + kk * 2048, 128 * 128), idesc_o,
+                    kk > 0 ? 1u : acc);
+          umma_commit(&c.pv_done);
+          umma_commit(ve);
+          ++n_tile;
+        }
+      }
+      umma_commit(&ctl->done[j]);
+    }
+    __syncwarp();
+  } else if (warp < kProducer) {
+    // -------------------------------------------------------------- softmax
+    const int j = warp >> 2, quad = warp & 3;
+    StreamCtrl& c = ctl->s[j];
+    const int tid = threadIdx.x & 127;         // row of the stream's tile
+    const uint32_t lanes = (uint32_t)(quad * 32) << 16;
+    const uint32_t tS = tmem + j * 256 + lanes, tO = tS + 128;
+    const float scale = a.scale_log2;
+    constexpr float kBias = F16 ? 7.f : 0.f;
+    uint32_t n_item = 0, n_tile = 0, n_own = 0, n_ring = 0, n_care = 0, n_care2 = 0;
+    bool ok = true;
+    while (ok) {
+      const int slot = n_item % kItems;
+      if (!wait.warp(&c.item_full[slot], (n_item / kItems) & 1)) break;
+      const int paired = c.paired[slot];
+      if (paired < 0) break;
+      const AttnPart it = c.item[slot];
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&c.item_empty[slot]);
+      ++n_item;
+      const int r = (paired ? j * kHalf : 0) + tid;        // row of the item
+      const bool live = r < it.rows;
+      const bool warp_live = __any_sync(0xffffffffu, live);
+      // keys this row sees, and the first row of the item (fewest)
+      const int sees = it.own ? min(it.len, it.see0 + (it.row0 + r) / a.G + 1) : it.len;
+      const int fewest = it.own ? min(it.len, it.see0 + it.row0 / a.G + 1) : it.len;
+      float m = -INFINITY, l = 0.f;                        // m: reference, bias included
+      for (int t = it.t0; t < it.t1; ++t) {
+        const int key0 = t * kKeys;
+        // the value stage (for tiles that need care)
+        uint64_t* vf;
+        uint32_t vp;
+        uint8_t* vs;
+        if (paired) {
+          const uint32_t st = (n_ring + 1) % RING;
+          vf = &ctl->full[st], vp = ((n_ring + 1) / RING) & 1, vs = smem + TC::KV_OFF + st * TILE;
+          n_ring += 2;
+        } else {
+          const uint32_t st = (n_own + 1) % NS;
+          vf = &c.full[st], vp = ((n_own + 1) / NS) & 1, vs = smem + TC::KV_OFF + (j * NS + st) * TILE;
+          n_own += 2;
+        }
+        if (!(ok = wait.warp(&c.s_full, n_tile & 1))) break;
+        ++n_tile;
+        tc_fence_after();
+        const bool care = key0 + kKeys > fewest;
+        float s[kKeys];
+        if (warp_live) {
+#pragma unroll
+          for (int i = 0; i < 4; ++i) tmem_ld32(tS + i * 32, s + i * 32);
+          tmem_wait_ld();
+          if (care) {
+            const int n = sees - key0;
+#pragma unroll
+            for (int i = 0; i < kKeys; ++i) s[i] = i < n ? s[i] : -INFINITY;
+          }
+          float m0 = s[0], m1 = s[1], m2 = s[2], m3 = s[3];
+#pragma unroll
+          for (int i = 4; i < kKeys; i += 4) {
+            m0 = fmaxf(m0, s[i]), m1 = fmaxf(m1, s[i + 1]);
+            m2 = fmaxf(m2, s[i + 2]), m3 = fmaxf(m3, s[i + 3]);
+          }
+          const float top = fmaxf(fmaxf(m0, m1), fmaxf(m2, m3)) * scale - kBias;
+          const bool move = top > m + kLazy || (m == -INFINITY && top > m);
+          if (__any_sync(0xffffffffu, move)) {
+            const float al = move ? ex2(m - top) : 1.f;  // m = -inf: 0
+            if (move) m = top;
+            l *= al;
+            if (t > it.t0) {
+#pragma unroll 1
+              for (int i = 0; i < D; i += 32) {
+                float o[32];
+                tmem_ld32(tO + i, o);
+                tmem_wait_ld();
+#pragma unroll
+                for (int k = 0; k < 32; ++k) o[k] *= al;
+                tmem_st32(tO + i, reinterpret_cast<const uint32_t*>(o));
+              }
+              tmem_wait_st();
+            }
+          }
+        }
+        const float base = m == -INFINITY ? 0.f : m;
+        if (care) {
+          // values: rows behind the last key become zero; rows that only some
+          // query rows see are looked at
+          if (!(ok = wait.warp(vf, vp))) break;
+          const int valid = min(kKeys, it.len - key0), from = fewest - key0;
+          auto zero_row = [&]() {
+#pragma unroll
+            for (int i = 0; i < NC * 8; ++i)
+              *reinterpret_cast<uint4*>(vs + (i >> 3) * (128 * 128) + tid * 128 + (i & 7) * 16) = make_uint4(0, 0, 0, 0);
+          };
+          if (tid >= valid) zero_row();
+          if (from < valid) {
+            // a bounded barrier of the softmax warps (of both streams for a
+            // pair: they look at the same rows of the same stage)
+            auto meet = [&]() -> bool {
+              __syncwarp();
+              uint64_t* bar = paired ? &ctl->care : &c.care;
+              uint32_t& n = paired ? n_care2 : n_care;
+              if (lane == 0) mbar_arrive(bar);
+              return wait.warp(bar, n++ & 1);
+            };
+            bool odd = false;
+            if (tid >= from && tid < valid) {
+              constexpr uint32_t E = F16 ? 0x7c00u : 0x7f80u;
+#pragma unroll
+              for (int i = 0; i < NC * 8; ++i) {
+                const uint4 v = *reinterpret_cast<const uint4*>(vs + (i >> 3) * (128 * 128) + tid * 128 + (i & 7) * 16);
+                const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+                for (int q = 0; q < 4; ++q) odd |= (w[q] & E) == E || ((w[q] >> 16) & E) == E;
+              }
+            }
+            const uint32_t mask = __ballot_sync(0xffffffffu, odd);
+            if (lane == 0) c.bad[quad] = mask;
+            if (!(ok = meet())) break;
+            if ((c.bad[0] | c.bad[1] | c.bad[2] | c.bad[3]) != 0) {
+              bool fresh = t == it.t0;  // O holds nothing yet
+              if (tid == 0 && fresh) c.accumulate = 1;
+#pragma unroll 1
+              for (int k = 0; k < kKeys; ++k) {
+                if (!((c.bad[k >> 5] >> (k & 31)) & 1)) continue;
+                if (warp_live) {
+                  const float sk = tmem_ld1(tS + k);
+                  tmem_wait_ld();
+                  const bool seen = key0 + k < sees;
+                  const float p = seen ? ex2(fmaf(sk, scale, -base)) : 0.f;
+#pragma unroll 1
+                  for (int i = 0; i < D; i += 32) {
+                    float o[32];
+                    tmem_ld32(tO + i, o);
+                    tmem_wait_ld();
+#pragma unroll
+                    for (int q = 0; q < 32; q += 8) {
+                      const int col = i + q;
+                      const uint4 v = *reinterpret_cast<const uint4*>(
+                          vs + (col >> 6) * (128 * 128) + k * 128 + ((((col & 63) >> 3) ^ (k & 7)) << 4));
+                      const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+                      for (int x = 0; x < 4; ++x) {
+                        float lo, hi;
+                        if constexpr (F16) {
+                          const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w[x]));
+                          lo = f.x, hi = f.y;
+                        } else {
+                          lo = bf16_lo(w[x]), hi = bf16_hi(w[x]);
+                        }
+                        const float a0 = fresh ? 0.f : o[q + 2 * x], a1 = fresh ? 0.f : o[q + 2 * x + 1];
+                        o[q + 2 * x] = seen ? fmaf(p, lo, a0) : a0;
+                        o[q + 2 * x + 1] = seen ? fmaf(p, hi, a1) : a1;
+                      }
+                    }
+                    tmem_st32(tO + i, reinterpret_cast<const uint32_t*>(o));
+                    tmem_wait_st();
+                  }
+                }
+                fresh = false;
+              }
+              if (!(ok = meet())) break;  // every row has read them
+              if (odd) zero_row();
+            }
+          }
+          fence_async_smem();
+        }
+        if (warp_live) {
+          float2 sum0 = make_float2(0.f, 0.f), sum1 = sum0;
+          const float2 sc = make_float2(scale, scale), nb = make_float2(-base, -base);
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            uint32_t p[32];
+#pragma unroll
+            for (int i = 0; i < 32; ++i) {
+              float2 x = ffma2(make_float2(s[h * 64 + 2 * i], s[h * 64 + 2 * i + 1]), sc, nb);
+              x.x = ex2(x.x);
+              x.y = ex2(x.y);
+              if (i & 1) sum1 = __fadd2_rn(sum1, x);
+              else sum0 = __fadd2_rn(sum0, x);
+              p[i] = pack2<F16>(x.x, x.y);
+            }
+            tmem_st32(tS + h * 32, p);
+          }
+          l += (sum0.x + sum0.y) + (sum1.x + sum1.y);
+          tmem_wait_st();
+        }
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&c.p_ready);
+      }
+      if (!ok) break;
+      // the part's last product, then its rows out
+      if (!(ok = wait.warp(&c.pv_done, (n_tile - 1) & 1))) break;
+      tc_fence_after();
+      if (warp_live) {
+        int tok, hq;
+        attn_row(a, it, r, tok, hq);
+        const int64_t row = (int64_t)tok * (a.H * a.G) + hq;
+        // continuation rows: the pairs' of all CTAs, then the streams'
+        const int64_t crow = paired ? (int64_t)blockIdx.x * (2 * kHalf) + r
+                                    : (int64_t)gridDim.x * (2 * kHalf) + (int64_t)(blockIdx.x + j * gridDim.x) * kHalf + r;
+        const int stride = paired ? 2 * kHalf : kHalf;
+        float* dst = it.first ? a.part_o[it.own] + row * D : a.cont_o + crow * D;
+#pragma unroll 1
+        for (int i = 0; i < D; i += 32) {
+          float o[32];
+          tmem_ld32(tO + i, o);
+          tmem_wait_ld();
+          if (live) {
+#pragma unroll
+            for (int k = 0; k < 32; k += 4)
+              *reinterpret_cast<float4*>(dst + i + k) = make_float4(o[k], o[k + 1], o[k + 2], o[k + 3]);
+          }
+        }
+        if (live) {
+          const float2 ml = make_float2(m, l);
+          if (it.first) {
+            a.part_ml[it.own][row] = ml;
+            a.part_next[it.own][row] = attn_next((int)(crow + stride), it.n_cont, stride);
+          } else {
+            a.cont_ml[crow] = ml;
+          }
+        }
+      }
+      tc_fence_before();
+    }
+  }
+  __syncthreads();
+  if (ctl->abort) {
+    // copies that were issued and may still land
+    if (warp >= kProducer && warp < kProducer + 2 && lane == 0) {
+      StreamCtrl& c = ctl->s[warp - kProducer];
+      for (uint32_t i = issued_own > NS ? issued_own - NS : 0; i < issued_own; ++i)
+        mbar_wait(&c.full[i % NS], (i / NS) & 1);
+      for (uint32_t i = issued_ring > RING ? issued_ring - RING : 0; i < issued_ring; ++i)
+        mbar_wait(&ctl->full[i % RING], (i / RING) & 1);
+    }
+    __syncthreads();
+  }
+  if (warp == kMma) {
+    for (int j = 0; j < 2; ++j) mbar_wait(&ctl->done[j], 0);
+    __syncwarp();
+    tc_fence_after();
+    tmem_dealloc(tmem, kTmemCols);
+  }
+  if (threadIdx.x == 0 && ctl->abort) atomicExch(&g_attn_tc_error, (unsigned)GFST_ERR_TIMEOUT);
+}
+
+template <int D, bool F16>
+int launch(const AttnArgs& a, int sms, cudaStream_t stream) {
+  constexpr int smem = 1024 + TcAttn<D>::CTRL_OFF + (int)sizeof(Ctrl);
+  static_assert(smem <= 227 * 1024, "shared memory");
+  auto kern = prefix_attention_tc_kernel<D, F16>;
+  cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+  GFST_REQUIRE(e == cudaSuccess, GFST_ERR_DEVICE, "cudaFuncSetAttribute: %s", cudaGetErrorString(e));
+  const int64_t rows = a.n_blocks * a.H * a.L;
+  CUtensorMap mk, mv;
+  const int box = a.L < kKeys ? a.L : kKeys;
+  int st = make_bf16_map(&mk, a.pool_K, (uint64_t)rows, D, box);  // 16-bit elements, copied as they are
+  if (st == GFST_OK) st = make_bf16_map(&mv, a.pool_V, (uint64_t)rows, D, box);
+  if (st != GFST_OK) return st;
+  const int grid = sms < kAttnMaxGrid ? sms : kAttnMaxGrid;
+  kern<<<grid, kThreads, smem, stream>>>(mk, mv, a, rows);
+  return check_launch("prefix_attention_tc_kernel");
+}
+
+}  // namespace
+
+bool prefix_attention_tc_takes(const AttnArgs& a, int dtype) {
+  return (dtype == GFST_BF16 || dtype == GFST_F16) && a.d == a.dv && (a.d == 64 || a.d == 128) &&
+         ((a.L >= 8 && kKeys % a.L == 0) || a.L % kKeys == 0) && a.n_blocks * a.H * a.L < (1LL << 31) - kKeys &&
+         a.scale_log2 > 0.f;  // the row maximum is taken before scaling
+}
+
+int launch_prefix_attention_tc(const AttnArgs& a, int dtype, int sms, cudaStream_t stream) {
+  const bool f16 = dtype == GFST_F16;
+  if (a.d == 64) return f16 ? launch<64, true>(a, sms, stream) : launch<64, false>(a, sms, stream);
+  return f16 ? launch<128, true>(a, sms, stream) : launch<128, false>(a, sms, stream);
+}
+
+}  // namespace gfst
