@@ -75,7 +75,7 @@ struct TcAttn {
 
 struct StreamCtrl {
   uint64_t item_full[kItems], item_empty[kItems];
-  uint64_t q_full, q_empty, s_full, p_ready, pv_done;
+  uint64_t q_full, q_empty, s_full, p_ready[2], pv_done;  // p_ready: keys 0-63, 64-127
   uint64_t care;               // the softmax warps among themselves
   uint64_t full[4], empty[4];  // the stream's own stages
   AttnPart item[kItems];
@@ -92,6 +92,8 @@ struct Ctrl {
   uint64_t drained;              // the pairs are done with the ring
   uint64_t done[2];              // a stream's products are done
   int64_t sum[32];
+  AttnLine<Pairs> pairs;         // the lines (their common part)
+  AttnLine<Rest> rest;
   uint32_t tmem;
   int abort;
 };
@@ -111,7 +113,7 @@ __device__ __forceinline__ uint32_t pack2(float lo, float hi) {
 }
 
 __device__ __forceinline__ void tmem_ld32(uint32_t taddr, float* v) {
-  uint32_t* r = reinterpret_cast<uint32_t*>(v);
+  uint32_t r[32];
   asm volatile(
       "tcgen05.ld.sync.aligned.32x32b.x32.b32 "
       "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
@@ -121,8 +123,10 @@ __device__ __forceinline__ void tmem_ld32(uint32_t taddr, float* v) {
         "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]),
         "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
       : "r"(taddr));
+#pragma unroll
+  for (int i = 0; i < 32; ++i) v[i] = __uint_as_float(r[i]);
 }
-__device__ __forceinline__ void tmem_st32(uint32_t taddr, const uint32_t* r) {
+__device__ __forceinline__ void tmem_st32(uint32_t taddr, const uint32_t (&r)[32]) {
   asm volatile(
       "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], "
       "{%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, "
@@ -133,6 +137,12 @@ __device__ __forceinline__ void tmem_st32(uint32_t taddr, const uint32_t* r) {
       "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31])
       : "memory");
 }
+__device__ __forceinline__ void tmem_st32(uint32_t taddr, const float (&v)[32]) {
+  uint32_t r[32];
+#pragma unroll
+  for (int i = 0; i < 32; ++i) r[i] = __float_as_uint(v[i]);
+  tmem_st32(taddr, r);
+}
 __device__ __forceinline__ float tmem_ld1(uint32_t taddr) {
   uint32_t r;
   asm volatile("tcgen05.ld.sync.aligned.32x32b.x1.b32 {%0}, [%1];" : "=r"(r) : "r"(taddr));
@@ -140,6 +150,13 @@ __device__ __forceinline__ float tmem_ld1(uint32_t taddr) {
 }
 __device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 __device__ __forceinline__ void fence_async_smem() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
+
+// 32 bytes (one sector) of a row
+__device__ __forceinline__ void store_sector(float* dst, const float* v) {
+  asm volatile("st.global.v8.f32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(dst), "f"(v[0]), "f"(v[1]), "f"(v[2]),
+               "f"(v[3]), "f"(v[4]), "f"(v[5]), "f"(v[6]), "f"(v[7])
+               : "memory");
+}
 
 // D[tmem] += A[tmem] B[smem]
 __device__ __forceinline__ void umma_ts(uint32_t d, uint32_t a, uint64_t bdesc, uint32_t idesc, uint32_t accumulate) {
@@ -160,6 +177,13 @@ __device__ __forceinline__ uint64_t sw128_mn_desc(uint32_t saddr, uint32_t chunk
 __host__ __device__ constexpr uint32_t idesc16(bool f16, int N, bool b_mn) {
   return (1u << 4) | (f16 ? 0u : (1u << 7) | (1u << 10)) | (b_mn ? 1u << 16 : 0u) | ((uint32_t)(N >> 3) << 17) |
          ((uint32_t)(128 >> 4) << 24);
+}
+
+// the lane that issues for its warp (always the same one)
+__device__ __forceinline__ bool elect_one() {
+  uint32_t r;
+  asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(r));
+  return r != 0;
 }
 
 // One role's waits: after a wait that gave up (or another role's), false.
@@ -197,7 +221,8 @@ __global__ void __launch_bounds__(kThreads, 1)
       mbar_init(&c.q_full, 1);
       mbar_init(&c.q_empty, 1);
       mbar_init(&c.s_full, 1);
-      mbar_init(&c.p_ready, 4);
+      mbar_init(&c.p_ready[0], 4);
+      mbar_init(&c.p_ready[1], 4);
       mbar_init(&c.pv_done, 1);
       mbar_init(&c.care, 4);
       for (int i = 0; i < 4; ++i) {
@@ -224,18 +249,26 @@ __global__ void __launch_bounds__(kThreads, 1)
 
   // the work: this CTA's share of the pairs, and one share of the rest per
   // stream (stream 1's behind all of stream 0's, so few items spread over the SMs)
-  AttnLine<Pairs> pl;
-  AttnLine<Rest> rl;
-  pl.init(a, gridDim.x, ctl->sum);
-  rl.init(a, 2 * gridDim.x, ctl->sum);
-  pl.find(a, blockIdx.x, &ctl->s[0].at_b[0], &ctl->s[0].at_u[0]);
-  for (int j = 0; j < 2; ++j) rl.find(a, blockIdx.x + j * gridDim.x, &ctl->s[j].at_b[1], &ctl->s[j].at_u[1]);
+  {
+    AttnLine<Pairs> pl;
+    pl.init(a, gridDim.x, ctl->sum);
+    pl.find(a, blockIdx.x, &ctl->s[0].at_b[0], &ctl->s[0].at_u[0]);
+    if (threadIdx.x == 0) ctl->pairs = pl;
+    AttnLine<Rest> rl;
+    rl.init(a, 2 * gridDim.x, ctl->sum);
+    for (int j = 0; j < 2; ++j) rl.find(a, blockIdx.x + j * gridDim.x, &ctl->s[j].at_b[1], &ctl->s[j].at_u[1]);
+    if (threadIdx.x == 0) ctl->rest = rl;
+  }
   __syncthreads();
 
   const Waiter wait{&ctl->abort};
   uint32_t issued_own = 0, issued_ring = 0;  // stages filled by this producer (for the drain)
 
-  if (warp >= kProducer && warp < kProducer + 2) {
+  // the softmax threads hold a row of scores: they take registers from the other
+  // four warps (2 x 128 x 200 + 128 x 104 of the 384 x 168 launched)
+  if (warp >= kProducer) {
+  asm volatile("setmaxnreg.dec.sync.aligned.u32 104;");
+  if (warp < kMma) {
     // ------------------------------------------------------------- producer
     const int j = warp - kProducer;
     StreamCtrl& c = ctl->s[j];
@@ -337,8 +370,8 @@ __global__ void __launch_bounds__(kThreads, 1)
     AttnPart it;
     {
       AttnWalk<Pairs> w;
-      w.begin(a, pl, blockIdx.x, ctl->s[0].at_b[0], ctl->s[0].at_u[0]);
-      while (ok && w.next(a, pl, it)) ok = part(it, 1);
+      w.begin(a, ctl->pairs, blockIdx.x, ctl->s[0].at_b[0], ctl->s[0].at_u[0]);
+      while (ok && w.next(a, ctl->pairs, it)) ok = part(it, 1);
       // the rest's stages lie in the ring: the pairs' products have to be done with it
       if (j == 0) {
         const uint32_t total = issued_ring;
@@ -352,8 +385,8 @@ __global__ void __launch_bounds__(kThreads, 1)
     {
       AttnWalk<Rest> w;
       const int i = blockIdx.x + j * gridDim.x;
-      w.begin(a, rl, i, c.at_b[1], c.at_u[1]);
-      while (ok && w.next(a, rl, it)) ok = part(it, 0);
+      w.begin(a, ctl->rest, i, c.at_b[1], c.at_u[1]);
+      while (ok && w.next(a, ctl->rest, it)) ok = part(it, 0);
     }
     const int slot = n_item % kItems;
     if (ok && wait.warp(&c.item_empty[slot], ((n_item / kItems) & 1) ^ 1) && lane == 0) {
@@ -362,72 +395,86 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
     asm volatile("cp.async.wait_all;" ::: "memory");
     if (bad) atomicExch(&g_attn_tc_error, (unsigned)GFST_ERR_ARG);
-  } else if (warp >= kMma) {
+  } else {
     // ------------------------------------------------------------------ MMA
+    // the whole warp walks the loop on warp-uniform values (descriptors then come
+    // from uniform registers); one elected lane issues
     const int j = warp - kMma;
     StreamCtrl& c = ctl->s[j];
-    if (lane == 0) {
-      constexpr uint32_t idesc_s = idesc16(F16, kKeys, false), idesc_o = idesc16(F16, D, true);
-      const uint32_t tS = tmem + j * 256, tO = tS + 128;
-      const uint32_t sq = smem_u32(smem + TC::Q_OFF + j * TILE);
-      uint32_t n_item = 0, n_tile = 0, n_own = 0, n_ring = 0;
-      bool ok = true;
-      while (ok) {
-        const int slot = n_item % kItems;
-        if (!wait(&c.item_full[slot], (n_item / kItems) & 1)) break;
-        const int paired = c.paired[slot], t0 = c.item[slot].t0, t1 = c.item[slot].t1;
-        if (paired < 0) break;
-        mbar_arrive(&c.item_empty[slot]);
-        if (!wait(&c.q_full, n_item & 1)) break;
-        ++n_item;
-        for (int t = t0; t < t1; ++t) {
-          uint64_t *kf, *ke, *vf, *ve;
-          uint32_t kp, vp;
-          uint8_t *ks, *vs;
-          auto stage = [&](uint64_t*& full, uint64_t*& empty, uint32_t& parity, uint8_t*& at) {
-            if (paired) {
-              const uint32_t st = n_ring % RING;
-              full = &ctl->full[st], empty = &ctl->empty[st], parity = (n_ring / RING) & 1;
-              at = smem + TC::KV_OFF + st * TILE;
-              ++n_ring;
-            } else {
-              const uint32_t st = n_own % NS;
-              full = &c.full[st], empty = &c.empty[st], parity = (n_own / NS) & 1;
-              at = smem + TC::KV_OFF + (j * NS + st) * TILE;
-              ++n_own;
-            }
-          };
-          stage(kf, ke, kp, ks);
-          stage(vf, ve, vp, vs);
-          // P of the last tile lies over S: its product has to be done
-          if (!(ok = wait(kf, kp) && (n_tile == 0 || wait(&c.pv_done, (n_tile - 1) & 1)))) break;
-          tc_fence_after();
+    constexpr uint32_t idesc_s = idesc16(F16, kKeys, false), idesc_o = idesc16(F16, D, true);
+    const uint32_t tbase = __shfl_sync(0xffffffffu, tmem, 0) + j * 256;
+    const uint32_t tS = tbase, tO = tbase + 128;
+    const uint32_t base = smem_u32(smem);
+    const uint64_t q_desc = sw128_desc(base + TC::Q_OFF + j * TILE);
+    const bool issuer = elect_one();
+    uint32_t n_item = 0, n_tile = 0, n_own = 0, n_ring = 0;
+    bool ok = true;
+    while (ok) {
+      const int slot = n_item % kItems;
+      if (!wait.warp(&c.item_full[slot], (n_item / kItems) & 1)) break;
+      const int paired = __shfl_sync(0xffffffffu, c.paired[slot], 0);
+      if (paired < 0) break;
+      const int t0 = __shfl_sync(0xffffffffu, c.item[slot].t0, 0), t1 = __shfl_sync(0xffffffffu, c.item[slot].t1, 0);
+      if (lane == 0) mbar_arrive(&c.item_empty[slot]);
+      if (!wait.warp(&c.q_full, n_item & 1)) break;
+      ++n_item;
+      for (int t = t0; t < t1; ++t) {
+        // stages of this tile's keys and values
+        const uint32_t n = paired ? n_ring : n_own, stages = paired ? RING : NS;
+        uint64_t* fulls = paired ? ctl->full : c.full;
+        uint64_t* empties = paired ? ctl->empty : c.empty;
+        const uint32_t ks = n % stages, vs = (n + 1) % stages;
+        const uint32_t kp = (n / stages) & 1, vp = ((n + 1) / stages) & 1;
+        const uint32_t stage0 = base + TC::KV_OFF + (paired ? 0 : j * NS * TILE);
+        n_ring += paired ? 2 : 0;
+        n_own += paired ? 0 : 2;
+        // P of the last tile lies over S: its product has to be done
+        if (!(ok = wait.warp(&fulls[ks], kp) && (n_tile == 0 || wait.warp(&c.pv_done, (n_tile - 1) & 1)))) break;
+        tc_fence_after();
+        if (issuer) {
+          const uint64_t k_desc = sw128_desc(stage0 + ks * TILE);
 #pragma unroll
           for (int kk = 0; kk < D / 16; ++kk) {
-            const uint32_t off = (kk >> 2) * (128 * 128) + (kk & 3) * 32;
-            umma_bf16(tS, sw128_desc(sq + off), sw128_desc(smem_u32(ks) + off), idesc_s, kk > 0 ? 1u : 0u);
+            const uint32_t off = ((kk >> 2) * (128 * 128) + (kk & 3) * 32) >> 4;
+            umma_bf16(tS, q_desc + off, k_desc + off, idesc_s, kk > 0 ? 1u : 0u);
           }
           umma_commit(&c.s_full);
-          umma_commit(ke);
+          umma_commit(&empties[ks]);
           if (t == t1 - 1) umma_commit(&c.q_empty);
-          if (!(ok = wait(&c.p_ready, n_tile & 1) && wait(vf, vp))) break;
-          tc_fence_after();
-          const uint32_t acc = t > t0 || c.accumulate != 0 ? 1u : 0u;
-          c.accumulate = 0;
-#pragma unroll
-          for (int kk = 0; kk < kKeys / 16; ++kk)
-            umma_ts(tO, tS + kk * 8, sw128_mn_desc(smem_u32(vs) + kk * 2048, 128 * 128), idesc_o,
-                    kk > 0 ? 1u : acc);
-          umma_commit(&c.pv_done);
-          umma_commit(ve);
-          ++n_tile;
         }
+        __syncwarp();
+        // the values' product follows the weights half a tile at a time
+        if (!(ok = wait.warp(&fulls[vs], vp))) break;
+        const uint64_t v_desc = sw128_mn_desc(stage0 + vs * TILE, 128 * 128);
+        uint32_t acc = t > t0 ? 1u : 0u;
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          if (!(ok = wait.warp(&c.p_ready[h], n_tile & 1))) break;
+          tc_fence_after();
+          if (h == 0) acc |= __shfl_sync(0xffffffffu, c.accumulate, 0);
+          if (issuer) {
+#pragma unroll
+            for (int kk = h * 4; kk < h * 4 + 4; ++kk)
+              umma_ts(tO, tS + kk * 8, v_desc + kk * (2048 >> 4), idesc_o, kk > 0 ? 1u : acc);
+            if (h == 0) {
+              c.accumulate = 0;
+            } else {
+              umma_commit(&c.pv_done);
+              umma_commit(&empties[vs]);
+            }
+          }
+          __syncwarp();
+        }
+        if (!ok) break;
+        ++n_tile;
       }
-      umma_commit(&ctl->done[j]);
     }
+    if (issuer) umma_commit(&ctl->done[j]);
     __syncwarp();
-  } else if (warp < kProducer) {
+  }
+  } else {
     // -------------------------------------------------------------- softmax
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 200;");
     const int j = warp >> 2, quad = warp & 3;
     StreamCtrl& c = ctl->s[j];
     const int tid = threadIdx.x & 127;         // row of the stream's tile
@@ -502,7 +549,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                 tmem_wait_ld();
 #pragma unroll
                 for (int k = 0; k < 32; ++k) o[k] *= al;
-                tmem_st32(tO + i, reinterpret_cast<const uint32_t*>(o));
+                tmem_st32(tO + i, o);
               }
               tmem_wait_st();
             }
@@ -580,7 +627,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                         o[q + 2 * x + 1] = seen ? fmaf(p, hi, a1) : a1;
                       }
                     }
-                    tmem_st32(tO + i, reinterpret_cast<const uint32_t*>(o));
+                    tmem_st32(tO + i, o);
                     tmem_wait_st();
                   }
                 }
@@ -592,11 +639,11 @@ __global__ void __launch_bounds__(kThreads, 1)
           }
           fence_async_smem();
         }
-        if (warp_live) {
-          float2 sum0 = make_float2(0.f, 0.f), sum1 = sum0;
-          const float2 sc = make_float2(scale, scale), nb = make_float2(-base, -base);
+        float2 sum0 = make_float2(0.f, 0.f), sum1 = sum0;
 #pragma unroll
-          for (int h = 0; h < 2; ++h) {
+        for (int h = 0; h < 2; ++h) {
+          if (warp_live) {
+            const float2 sc = make_float2(scale, scale), nb = make_float2(-base, -base);
             uint32_t p[32];
 #pragma unroll
             for (int i = 0; i < 32; ++i) {
@@ -608,13 +655,13 @@ __global__ void __launch_bounds__(kThreads, 1)
               p[i] = pack2<F16>(x.x, x.y);
             }
             tmem_st32(tS + h * 32, p);
+            tmem_wait_st();
           }
-          l += (sum0.x + sum0.y) + (sum1.x + sum1.y);
-          tmem_wait_st();
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&c.p_ready[h]);
         }
-        tc_fence_before();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&c.p_ready);
+        l += (sum0.x + sum0.y) + (sum1.x + sum1.y);
       }
       if (!ok) break;
       // the part's last product, then its rows out
@@ -636,8 +683,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           tmem_wait_ld();
           if (live) {
 #pragma unroll
-            for (int k = 0; k < 32; k += 4)
-              *reinterpret_cast<float4*>(dst + i + k) = make_float4(o[k], o[k + 1], o[k + 2], o[k + 3]);
+            for (int k = 0; k < 32; k += 8) store_sector(dst + i + k, o + k);
           }
         }
         if (live) {
