@@ -30,30 +30,6 @@ __device__ __forceinline__ void store4<__half>(__half* dst, float4 v) {
   *reinterpret_cast<uint2*>(dst) = make_uint2(*reinterpret_cast<const uint32_t*>(&a), *reinterpret_cast<const uint32_t*>(&b));
 }
 
-// joins one set (m, l, o) into the running one
-struct Join {
-  float m = -INFINITY, l = 0.f;
-  float4 o[2] = {make_float4(0, 0, 0, 0), make_float4(0, 0, 0, 0)};
-  __device__ __forceinline__ void add(float2 ml, const float* src, int lane, int dv) {
-    if (!(ml.y > 0.f) && ml.y == ml.y) return;  // an empty set (a NaN sum is kept)
-    const float now = fmaxf(m, ml.x);
-    const float wa = m == -INFINITY ? 0.f : exp2f(m - now), wb = ml.x == now ? 1.f : exp2f(ml.x - now);
-    m = now;
-    l = l * wa + ml.y * wb;
-#pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      const int c = (i * 32 + lane) * 4;
-      if (c < dv) {
-        const float4 v = *reinterpret_cast<const float4*>(src + c);
-        o[i].x = o[i].x * wa + v.x * wb;
-        o[i].y = o[i].y * wa + v.y * wb;
-        o[i].z = o[i].z * wa + v.z * wb;
-        o[i].w = o[i].w * wa + v.w * wb;
-      }
-    }
-  }
-};
-
 template <typename T>
 __global__ void __launch_bounds__(kMergeThreads) prefix_attention_merge_kernel(const AttnArgs a, int cont_rows) {
   const int lane = threadIdx.x & 31;
@@ -61,34 +37,95 @@ __global__ void __launch_bounds__(kMergeThreads) prefix_attention_merge_kernel(c
   const int heads = a.H * a.G;
   const int64_t tok = row / heads;
   if (tok >= a.n_tokens) return;
-  const bool live = a.B > 0 && tok < attn_tokens(a) && tok >= a.cu[0];
-  Join j;
+  const bool live = tok < attn_tokens(a) && tok >= a.cu[0];
+  if (!live && !a.fill_tail) return;
+  // the row's sets: [0, n0) prefix, [n0, n0 + n1) own, each its own place and
+  // then its continuations (offsets that cover no item leave next unset: sets
+  // outside the buffer are left out)
+  int n0 = 0, n1 = 0;
+  int2 x0 = make_int2(0, 0), x1 = x0;
   if (live) {
-#pragma unroll
-    for (int own = 0; own < 2; ++own) {
-      if (!own && attn_prefix_len(a) == 0) continue;
-      j.add(a.part_ml[own][row], a.part_o[own] + row * a.dv, lane, a.dv);
-      const int2 nx = a.part_next[own][row];
-      const int n = nx.y >> 9, stride = nx.y & 511;
-      for (int i = 0; i < n; ++i) {
-        const int64_t c = nx.x + (int64_t)i * stride;
-        if (c < 0 || c >= cont_rows) break;  // offsets that cover no item leave this unset
-        j.add(a.cont_ml[c], a.cont_o + c * a.dv, lane, a.dv);
+    x1 = a.part_next[1][row];
+    if (attn_prefix_len(a) > 0) {
+      x0 = a.part_next[0][row];
+      n0 = 1 + min(max(x0.y >> 9, 0), cont_rows);
+    }
+    n1 = 1 + min(max(x1.y >> 9, 0), cont_rows);
+  }
+  float m = -INFINITY, l = 0.f;
+  float4 o[2] = {make_float4(0, 0, 0, 0), make_float4(0, 0, 0, 0)};
+  // 32 sets at a time, one per lane: weights first, then the values with their
+  // loads in flight together
+  for (int s0 = 0; s0 < n0 + n1; s0 += 32) {
+    const int s = s0 + lane;
+    const float* src = nullptr;
+    float2 ml = make_float2(-INFINITY, 0.f);
+    if (s < n0 + n1) {
+      const int own = s >= n0, i = own ? s - n0 : s;
+      const int2 nx = own ? x1 : x0;
+      const int64_t c = nx.x + (int64_t)(i - 1) * (nx.y & 511);
+      if (i == 0) {
+        ml = a.part_ml[own][row];
+        src = a.part_o[own] + row * a.dv;
+      } else if (c >= 0 && c < cont_rows) {
+        ml = a.cont_ml[c];
+        src = a.cont_o + c * a.dv;
       }
     }
-  } else if (!a.fill_tail) {
-    return;
+    if (!(ml.y > 0.f) && ml.y == ml.y) src = nullptr;  // an empty set (a NaN sum is kept)
+    if (src == nullptr) ml = make_float2(-INFINITY, 0.f);
+    float now = fmaxf(m, ml.x);
+#pragma unroll
+    for (int i = 16; i >= 1; i >>= 1) now = fmaxf(now, __shfl_xor_sync(0xffffffffu, now, i));
+    // equal references need no exponential (and no inf - inf)
+    const float w = src == nullptr ? 0.f : ml.x == now ? 1.f : exp2f(ml.x - now);
+    float sum = ml.y * w;
+#pragma unroll
+    for (int i = 16; i >= 1; i >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, i);
+    const float keep = m == -INFINITY ? 0.f : m == now ? 1.f : exp2f(m - now);
+    m = now;
+    l = l * keep + sum;
+#pragma unroll
+    for (int i = 0; i < 2; ++i) o[i].x *= keep, o[i].y *= keep, o[i].z *= keep, o[i].w *= keep;
+    const int n = min(32, n0 + n1 - s0);
+    for (int g = 0; g < n; g += 4) {
+      float wt[4];
+      float4 v[4][2];
+#pragma unroll
+      for (int u = 0; u < 4; ++u) {
+        const int k = g + u;
+        const float* p = reinterpret_cast<const float*>(
+            __shfl_sync(0xffffffffu, reinterpret_cast<unsigned long long>(src), k & 31));
+        wt[u] = __shfl_sync(0xffffffffu, w, k & 31);
+        if (k >= n) p = nullptr;
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          const int c = (i * 32 + lane) * 4;
+          v[u][i] = p != nullptr && c < a.dv ? *reinterpret_cast<const float4*>(p + c) : make_float4(0, 0, 0, 0);
+        }
+      }
+#pragma unroll
+      for (int u = 0; u < 4; ++u) {
+        if (g + u >= n) break;
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          o[i].x = fmaf(v[u][i].x, wt[u], o[i].x);
+          o[i].y = fmaf(v[u][i].y, wt[u], o[i].y);
+          o[i].z = fmaf(v[u][i].z, wt[u], o[i].z);
+          o[i].w = fmaf(v[u][i].w, wt[u], o[i].w);
+        }
+      }
+    }
   }
   // a row that sees nothing: zeros and -inf
-  const float inv = j.l == 0.f ? 0.f : 1.f / j.l;
+  const float inv = l == 0.f ? 0.f : 1.f / l;
   T* out = static_cast<T*>(a.out) + row * a.dv;
 #pragma unroll
   for (int i = 0; i < 2; ++i) {
     const int c = (i * 32 + lane) * 4;
-    if (c < a.dv) store4<T>(out + c, make_float4(j.o[i].x * inv, j.o[i].y * inv, j.o[i].z * inv, j.o[i].w * inv));
+    if (c < a.dv) store4<T>(out + c, make_float4(o[i].x * inv, o[i].y * inv, o[i].z * inv, o[i].w * inv));
   }
-  if (a.lse != nullptr && lane == 0)
-    a.lse[row] = j.l == 0.f ? -INFINITY : (j.m + log2f(j.l)) * 0.69314718055994531f;
+  if (a.lse != nullptr && lane == 0) a.lse[row] = l == 0.f ? -INFINITY : (m + log2f(l)) * 0.69314718055994531f;
 }
 
 template <typename T>

@@ -50,12 +50,14 @@ GFST_DEFINE_ERROR_WORD(g_attn_tc_error, read_attn_tc_error, "attention")
 namespace {
 
 constexpr int kHalf = kAttnTcHalf;  // rows of a stream's tile
-constexpr int kKeys = 128;          // keys of a tile
+constexpr int kKeys = 128;          // keys of a tile (a stage)
+constexpr int kUnit = 64;           // keys of a score buffer
 constexpr int kThreads = 384;
 constexpr int kProducer = 8, kMma = 10;
 constexpr int kItems = 4;           // parts announced ahead
 constexpr uint32_t kTmemCols = 512; // per stream: S (P over it) 128, O 128
 constexpr float kLazy = 8.f;
+constexpr int kPolyEvery = 4;       // one pair of weights in four on the FP32 pipe
 
 // An item's fixed cost (queries, first scores, last values, partials out) is
 // that of about two tiles.
@@ -75,12 +77,13 @@ struct TcAttn {
 
 struct StreamCtrl {
   uint64_t item_full[kItems], item_empty[kItems];
-  uint64_t q_full, q_empty, s_full, p_ready[2], pv_done;  // p_ready: keys 0-63, 64-127
+  uint64_t q_full, q_empty;
+  uint64_t s_full[2], p_ready[2], pv_done[2];  // of the two score buffers
   uint64_t care;               // the softmax warps among themselves
   uint64_t full[4], empty[4];  // the stream's own stages
   AttnPart item[kItems];
   int paired[kItems];          // 1: pair, 0: rest, -1: no more work
-  uint32_t bad[4];             // value rows that are not finite (one bit each)
+  uint32_t bad[2][4];          // value rows that are not finite (one bit each), two tiles in turn
   int accumulate;              // the tile's first product adds to O
   int at_b[2];
   int64_t at_u[2];
@@ -102,6 +105,28 @@ __device__ __forceinline__ float ex2(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
+}
+
+// 2^x of two numbers on the FP32 pipe, x <= 127: 2^n times a polynomial of degree
+// 5 in f = x - n in [-1/2, 1/2] (coefficients from an exchange iteration on the
+// relative error: 7.5e-8, 2.1e-7 with the FP32 evaluation).  NaN stays NaN;
+// below 2^-125 the result is 2^-125.
+__device__ __forceinline__ float2 ex2_poly(float2 x) {
+  asm("max.NaN.f32 %0, %0, %1;" : "+f"(x.x) : "f"(-125.f));
+  asm("max.NaN.f32 %0, %0, %1;" : "+f"(x.y) : "f"(-125.f));
+  const float2 magic = make_float2(12582912.f, 12582912.f);  // 1.5 * 2^23: rounds to an integer
+  const float2 t = __fadd2_rn(x, magic);
+  const float2 r = __fadd2_rn(t, make_float2(-12582912.f, -12582912.f));
+  const float2 f = ffma2(r, make_float2(-1.f, -1.f), x);
+  float2 y = make_float2(1.327647245e-03f, 1.327647245e-03f);
+  y = ffma2(y, f, make_float2(9.675540961e-03f, 9.675540961e-03f));
+  y = ffma2(y, f, make_float2(5.550713092e-02f, 5.550713092e-02f));
+  y = ffma2(y, f, make_float2(2.402212024e-01f, 2.402212024e-01f));
+  y = ffma2(y, f, make_float2(6.931469440e-01f, 6.931469440e-01f));
+  y = ffma2(y, f, make_float2(1.000000119e+00f, 1.000000119e+00f));
+  const float2 p2 = make_float2(__uint_as_float((__float_as_uint(t.x) << 23) + 0x3f800000u),
+                                __uint_as_float((__float_as_uint(t.y) << 23) + 0x3f800000u));
+  return __fmul2_rn(y, p2);
 }
 
 template <bool F16>
@@ -186,17 +211,25 @@ __device__ __forceinline__ bool elect_one() {
   return r != 0;
 }
 
-// One role's waits: after a wait that gave up (or another role's), false.
+// One role's waits.  A wait that gives up, or finds that another role has, sets
+// the CTA's abort flag and is false.
 struct Waiter {
   volatile int* abort;
-  __device__ __forceinline__ bool operator()(uint64_t* bar, uint32_t parity) const {
-    if (!mbar_wait(bar, parity)) *abort = 1;
-    return *abort == 0;
+  __device__ __forceinline__ bool spin(uint64_t* bar, uint32_t parity) const {
+    const long long t0 = clock64();
+    for (int i = 1; !mbar_try_wait(bar, parity); ++i) {
+      if ((i & 15) == 0 && (*abort != 0 || clock64() - t0 > kMbarWaitCycles)) {
+        *abort = 1;
+        return false;
+      }
+    }
+    return true;
   }
   // the whole warp waits; lanes leave together
   __device__ __forceinline__ bool warp(uint64_t* bar, uint32_t parity) const {
-    int ok = (*this)(bar, parity) ? 1 : 0;
-    return __all_sync(0xffffffffu, ok);
+    const bool ok = mbar_try_wait(bar, parity);
+    if (__all_sync(0xffffffffu, ok)) return true;
+    return __all_sync(0xffffffffu, ok || spin(bar, parity));
   }
 };
 
@@ -220,10 +253,11 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
       mbar_init(&c.q_full, 1);
       mbar_init(&c.q_empty, 1);
-      mbar_init(&c.s_full, 1);
-      mbar_init(&c.p_ready[0], 4);
-      mbar_init(&c.p_ready[1], 4);
-      mbar_init(&c.pv_done, 1);
+      for (int i = 0; i < 2; ++i) {
+        mbar_init(&c.s_full[i], 1);
+        mbar_init(&c.p_ready[i], 4);
+        mbar_init(&c.pv_done[i], 1);
+      }
       mbar_init(&c.care, 4);
       for (int i = 0; i < 4; ++i) {
         mbar_init(&c.full[i], 1);
@@ -360,8 +394,8 @@ __global__ void __launch_bounds__(kThreads, 1)
             for (int ch = 0; ch < NC; ++ch)
               tma_load_2d(dst + ch * (128 * 128) + lane * box * 128, kv ? &tmV : &tmK, full, ch * 64, (int)row);
           }
+          if (!q_sent) send_q();
         }
-        if (!q_sent) send_q();
         row = ahead;
       }
       return true;
@@ -401,13 +435,13 @@ __global__ void __launch_bounds__(kThreads, 1)
     // from uniform registers); one elected lane issues
     const int j = warp - kMma;
     StreamCtrl& c = ctl->s[j];
-    constexpr uint32_t idesc_s = idesc16(F16, kKeys, false), idesc_o = idesc16(F16, D, true);
+    constexpr uint32_t idesc_s = idesc16(F16, kUnit, false), idesc_o = idesc16(F16, D, true);
     const uint32_t tbase = __shfl_sync(0xffffffffu, tmem, 0) + j * 256;
     const uint32_t tS = tbase, tO = tbase + 128;
     const uint32_t base = smem_u32(smem);
     const uint64_t q_desc = sw128_desc(base + TC::Q_OFF + j * TILE);
     const bool issuer = elect_one();
-    uint32_t n_item = 0, n_tile = 0, n_own = 0, n_ring = 0;
+    uint32_t n_item = 0, n_unit = 0, n_own = 0, n_ring = 0;
     bool ok = true;
     while (ok) {
       const int slot = n_item % kItems;
@@ -415,59 +449,63 @@ __global__ void __launch_bounds__(kThreads, 1)
       const int paired = __shfl_sync(0xffffffffu, c.paired[slot], 0);
       if (paired < 0) break;
       const int t0 = __shfl_sync(0xffffffffu, c.item[slot].t0, 0), t1 = __shfl_sync(0xffffffffu, c.item[slot].t1, 0);
+      const int len_of_slot = c.item[slot].len;
+      __syncwarp();
       if (lane == 0) mbar_arrive(&c.item_empty[slot]);
       if (!wait.warp(&c.q_full, n_item & 1)) break;
+      const int len = __shfl_sync(0xffffffffu, len_of_slot, 0);
       ++n_item;
-      for (int t = t0; t < t1; ++t) {
-        // stages of this tile's keys and values
-        const uint32_t n = paired ? n_ring : n_own, stages = paired ? RING : NS;
-        uint64_t* fulls = paired ? ctl->full : c.full;
-        uint64_t* empties = paired ? ctl->empty : c.empty;
-        const uint32_t ks = n % stages, vs = (n + 1) % stages;
-        const uint32_t kp = (n / stages) & 1, vp = ((n + 1) / stages) & 1;
-        const uint32_t stage0 = base + TC::KV_OFF + (paired ? 0 : j * NS * TILE);
-        n_ring += paired ? 2 : 0;
-        n_own += paired ? 0 : 2;
-        // P of the last tile lies over S: its product has to be done
-        if (!(ok = wait.warp(&fulls[ks], kp) && (n_tile == 0 || wait.warp(&c.pv_done, (n_tile - 1) & 1)))) break;
+      const uint32_t stages = paired ? RING : NS;
+      uint64_t* fulls = paired ? ctl->full : c.full;
+      uint64_t* empties = paired ? ctl->empty : c.empty;
+      const uint32_t stage0 = base + TC::KV_OFF + (paired ? 0 : j * NS * TILE);
+      const uint32_t n0 = paired ? n_ring : n_own;  // stage number of the part's first tile
+      n_ring += paired ? 2 * (t1 - t0) : 0;
+      n_own += paired ? 0 : 2 * (t1 - t0);
+      // units of 64 keys; the last tile has one if its second half holds no key
+      const int units = 2 * (t1 - t0) - (len - (t1 - 1) * kKeys > kUnit ? 0 : 1);
+      // scores of unit u, into buffer (n_unit + u) & 1: its weights two units ago
+      // lie there, so their product has to be done
+      auto scores = [&](int u) -> bool {
+        const uint32_t n = n0 + 2 * (u >> 1), ks = n % stages, g = n_unit + u, buf = g & 1;
+        if ((u & 1) == 0 && !wait.warp(&fulls[ks], (n / stages) & 1)) return false;
+        if (g >= 2 && !wait.warp(&c.pv_done[buf], ((g >> 1) & 1) ^ 1)) return false;
         tc_fence_after();
         if (issuer) {
-          const uint64_t k_desc = sw128_desc(stage0 + ks * TILE);
+          const uint64_t k_desc = sw128_desc(stage0 + ks * TILE + (u & 1) * (kUnit * 128));
 #pragma unroll
           for (int kk = 0; kk < D / 16; ++kk) {
             const uint32_t off = ((kk >> 2) * (128 * 128) + (kk & 3) * 32) >> 4;
-            umma_bf16(tS, q_desc + off, k_desc + off, idesc_s, kk > 0 ? 1u : 0u);
+            umma_bf16(tS + buf * kUnit, q_desc + off, k_desc + off, idesc_s, kk > 0 ? 1u : 0u);
           }
-          umma_commit(&c.s_full);
-          umma_commit(&empties[ks]);
-          if (t == t1 - 1) umma_commit(&c.q_empty);
+          umma_commit(&c.s_full[buf]);
+          if ((u & 1) || u == units - 1) umma_commit(&empties[ks]);
+          if (u == units - 1) umma_commit(&c.q_empty);
         }
         __syncwarp();
-        // the values' product follows the weights half a tile at a time
-        if (!(ok = wait.warp(&fulls[vs], vp))) break;
-        const uint64_t v_desc = sw128_mn_desc(stage0 + vs * TILE, 128 * 128);
-        uint32_t acc = t > t0 ? 1u : 0u;
+        return true;
+      };
+      if (!(ok = scores(0))) break;
+      for (int u = 0; u < units; ++u) {
+        if (u + 1 < units && !(ok = scores(u + 1))) break;
+        const uint32_t n = n0 + 2 * (u >> 1) + 1, vs = n % stages, g = n_unit + u, buf = g & 1;
+        if ((u & 1) == 0 && !(ok = wait.warp(&fulls[vs], (n / stages) & 1))) break;
+        if (!(ok = wait.warp(&c.p_ready[buf], (g >> 1) & 1))) break;
+        tc_fence_after();
+        uint32_t acc = 1;
+        if (u == 0) acc = __shfl_sync(0xffffffffu, c.accumulate, 0);
+        if (issuer) {
+          const uint64_t v_desc = sw128_mn_desc(stage0 + vs * TILE, 128 * 128) + (u & 1) * (kUnit * 128 >> 4);
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          if (!(ok = wait.warp(&c.p_ready[h], n_tile & 1))) break;
-          tc_fence_after();
-          if (h == 0) acc |= __shfl_sync(0xffffffffu, c.accumulate, 0);
-          if (issuer) {
-#pragma unroll
-            for (int kk = h * 4; kk < h * 4 + 4; ++kk)
-              umma_ts(tO, tS + kk * 8, v_desc + kk * (2048 >> 4), idesc_o, kk > 0 ? 1u : acc);
-            if (h == 0) {
-              c.accumulate = 0;
-            } else {
-              umma_commit(&c.pv_done);
-              umma_commit(&empties[vs]);
-            }
-          }
-          __syncwarp();
+          for (int kk = 0; kk < kUnit / 16; ++kk)
+            umma_ts(tO, tS + buf * kUnit + kk * 8, v_desc + kk * (2048 >> 4), idesc_o, kk > 0 ? 1u : acc);
+          umma_commit(&c.pv_done[buf]);
+          if ((u & 1) || u == units - 1) umma_commit(&empties[vs]);
+          if (u == 0) c.accumulate = 0;
         }
-        if (!ok) break;
-        ++n_tile;
+        __syncwarp();
       }
+      n_unit += units;
     }
     if (issuer) umma_commit(&ctl->done[j]);
     __syncwarp();
@@ -482,7 +520,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     const uint32_t tS = tmem + j * 256 + lanes, tO = tS + 128;
     const float scale = a.scale_log2;
     constexpr float kBias = F16 ? 7.f : 0.f;
-    uint32_t n_item = 0, n_tile = 0, n_own = 0, n_ring = 0, n_care = 0, n_care2 = 0;
+    uint32_t n_item = 0, n_tile = 0, n_unit = 0, n_own = 0, n_ring = 0, n_care = 0, n_care2 = 0;
     bool ok = true;
     while (ok) {
       const int slot = n_item % kItems;
@@ -500,107 +538,120 @@ __global__ void __launch_bounds__(kThreads, 1)
       const int sees = it.own ? min(it.len, it.see0 + (it.row0 + r) / a.G + 1) : it.len;
       const int fewest = it.own ? min(it.len, it.see0 + it.row0 / a.G + 1) : it.len;
       float m = -INFINITY, l = 0.f;                        // m: reference, bias included
-      for (int t = it.t0; t < it.t1; ++t) {
-        const int key0 = t * kKeys;
+      uint64_t* fulls = paired ? ctl->full : c.full;
+      for (int t = it.t0; ok && t < it.t1; ++t) {
         // the value stage (for tiles that need care)
-        uint64_t* vf;
-        uint32_t vp;
-        uint8_t* vs;
-        if (paired) {
-          const uint32_t st = (n_ring + 1) % RING;
-          vf = &ctl->full[st], vp = ((n_ring + 1) / RING) & 1, vs = smem + TC::KV_OFF + st * TILE;
-          n_ring += 2;
-        } else {
-          const uint32_t st = (n_own + 1) % NS;
-          vf = &c.full[st], vp = ((n_own + 1) / NS) & 1, vs = smem + TC::KV_OFF + (j * NS + st) * TILE;
-          n_own += 2;
-        }
-        if (!(ok = wait.warp(&c.s_full, n_tile & 1))) break;
-        ++n_tile;
-        tc_fence_after();
-        const bool care = key0 + kKeys > fewest;
-        float s[kKeys];
-        if (warp_live) {
+        const uint32_t n = (paired ? n_ring : n_own) + 1, stages = paired ? RING : NS;
+        const uint32_t v_stage = n % stages;
+        uint8_t* vs = smem + TC::KV_OFF + ((paired ? 0 : j * NS) + v_stage) * TILE;
+        n_ring += paired ? 2 : 0;
+        n_own += paired ? 0 : 2;
+        const bool care = t * kKeys + kKeys > fewest;
+        uint32_t any_bad = 0;
+        const int units = it.len - t * kKeys > kUnit ? 2 : 1;
+        for (int u = 0; u < units; ++u) {
+          const int key0 = t * kKeys + u * kUnit;
+          const uint32_t buf = n_unit & 1, phase = (n_unit >> 1) & 1;
+          const uint32_t tP = tS + buf * kUnit;
+          const bool first_unit = t == it.t0 && u == 0;
+          // the product before this unit's (still running unless waited for)
+          auto o_stable = [&]() -> bool {
+            if (first_unit) return true;
+            const bool done = wait.warp(&c.pv_done[buf ^ 1], ((n_unit - 1) >> 1) & 1);
+            tc_fence_after();
+            return done;
+          };
+          if (!(ok = wait.warp(&c.s_full[buf], phase))) break;
+          tc_fence_after();
+          float s[kUnit];
+          if (warp_live) {
+            tmem_ld32(tP, s);
+            tmem_ld32(tP + 32, s + 32);
+            tmem_wait_ld();
+            if (care) {
+              const int seen = sees - key0;
 #pragma unroll
-          for (int i = 0; i < 4; ++i) tmem_ld32(tS + i * 32, s + i * 32);
-          tmem_wait_ld();
-          if (care) {
-            const int n = sees - key0;
+              for (int i = 0; i < kUnit; ++i) s[i] = i < seen ? s[i] : -INFINITY;
+            }
+            float m0 = s[0], m1 = s[1], m2 = s[2], m3 = s[3];
 #pragma unroll
-            for (int i = 0; i < kKeys; ++i) s[i] = i < n ? s[i] : -INFINITY;
-          }
-          float m0 = s[0], m1 = s[1], m2 = s[2], m3 = s[3];
-#pragma unroll
-          for (int i = 4; i < kKeys; i += 4) {
-            m0 = fmaxf(m0, s[i]), m1 = fmaxf(m1, s[i + 1]);
-            m2 = fmaxf(m2, s[i + 2]), m3 = fmaxf(m3, s[i + 3]);
-          }
-          const float top = fmaxf(fmaxf(m0, m1), fmaxf(m2, m3)) * scale - kBias;
-          const bool move = top > m + kLazy || (m == -INFINITY && top > m);
-          if (__any_sync(0xffffffffu, move)) {
-            const float al = move ? ex2(m - top) : 1.f;  // m = -inf: 0
-            if (move) m = top;
-            l *= al;
-            if (t > it.t0) {
+            for (int i = 4; i < kUnit; i += 4) {
+              m0 = fmaxf(m0, s[i]), m1 = fmaxf(m1, s[i + 1]);
+              m2 = fmaxf(m2, s[i + 2]), m3 = fmaxf(m3, s[i + 3]);
+            }
+            const float top = fmaxf(fmaxf(m0, m1), fmaxf(m2, m3)) * scale - kBias;
+            const bool move = top > m + kLazy;
+            if (__any_sync(0xffffffffu, move)) {
+              const float al = move ? ex2(m - top) : 1.f;  // m = -inf: 0
+              if (move) m = top;
+              l *= al;
+              if (!first_unit) {
+                if (!(ok = o_stable())) break;
 #pragma unroll 1
-              for (int i = 0; i < D; i += 32) {
-                float o[32];
-                tmem_ld32(tO + i, o);
-                tmem_wait_ld();
+                for (int i = 0; i < D; i += 32) {
+                  float o[32];
+                  tmem_ld32(tO + i, o);
+                  tmem_wait_ld();
 #pragma unroll
-                for (int k = 0; k < 32; ++k) o[k] *= al;
-                tmem_st32(tO + i, o);
+                  for (int k = 0; k < 32; ++k) o[k] *= al;
+                  tmem_st32(tO + i, o);
+                }
+                tmem_wait_st();
               }
-              tmem_wait_st();
             }
           }
-        }
-        const float base = m == -INFINITY ? 0.f : m;
-        if (care) {
-          // values: rows behind the last key become zero; rows that only some
-          // query rows see are looked at
-          if (!(ok = wait.warp(vf, vp))) break;
-          const int valid = min(kKeys, it.len - key0), from = fewest - key0;
-          auto zero_row = [&]() {
-#pragma unroll
-            for (int i = 0; i < NC * 8; ++i)
-              *reinterpret_cast<uint4*>(vs + (i >> 3) * (128 * 128) + tid * 128 + (i & 7) * 16) = make_uint4(0, 0, 0, 0);
-          };
-          if (tid >= valid) zero_row();
-          if (from < valid) {
-            // a bounded barrier of the softmax warps (of both streams for a
-            // pair: they look at the same rows of the same stage)
+          const float base = m == -INFINITY ? 0.f : m;
+          if (care) {
+            // a bounded barrier of the softmax warps (of both streams for a pair:
+            // they look at the same rows of the same stage)
             auto meet = [&]() -> bool {
               __syncwarp();
               uint64_t* bar = paired ? &ctl->care : &c.care;
-              uint32_t& n = paired ? n_care2 : n_care;
+              uint32_t& n_meet = paired ? n_care2 : n_care;
               if (lane == 0) mbar_arrive(bar);
-              return wait.warp(bar, n++ & 1);
+              return wait.warp(bar, n_meet++ & 1);
             };
-            bool odd = false;
-            if (tid >= from && tid < valid) {
-              constexpr uint32_t E = F16 ? 0x7c00u : 0x7f80u;
+            auto zero_row = [&]() {
 #pragma unroll
-              for (int i = 0; i < NC * 8; ++i) {
-                const uint4 v = *reinterpret_cast<const uint4*>(vs + (i >> 3) * (128 * 128) + tid * 128 + (i & 7) * 16);
-                const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+              for (int i = 0; i < NC * 8; ++i)
+                *reinterpret_cast<uint4*>(vs + (i >> 3) * (128 * 128) + tid * 128 + (i & 7) * 16) = make_uint4(0, 0, 0, 0);
+            };
+            uint32_t* bad = c.bad[n_tile & 1];
+            if (u == 0) {
+              // values: rows behind the last key become zero; rows that only some
+              // query rows see are looked at
+              if (!(ok = wait.warp(&fulls[v_stage], (n / stages) & 1))) break;
+              const int valid = min(kKeys, it.len - key0), from = fewest - key0;
+              if (tid >= valid) zero_row();
+              if (from < valid) {
+                bool odd = false;
+                if (tid >= from && tid < valid) {
+                  constexpr uint32_t E = F16 ? 0x7c00u : 0x7f80u;
 #pragma unroll
-                for (int q = 0; q < 4; ++q) odd |= (w[q] & E) == E || ((w[q] >> 16) & E) == E;
+                  for (int i = 0; i < NC * 8; ++i) {
+                    const uint4 v = *reinterpret_cast<const uint4*>(vs + (i >> 3) * (128 * 128) + tid * 128 + (i & 7) * 16);
+                    const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+                    for (int q = 0; q < 4; ++q) odd |= (w[q] & E) == E || ((w[q] >> 16) & E) == E;
+                  }
+                }
+                const uint32_t mask = __ballot_sync(0xffffffffu, odd);
+                if (lane == 0) bad[quad] = mask;
+                if (!(ok = meet())) break;
+                any_bad = bad[0] | bad[1] | bad[2] | bad[3];
               }
             }
-            const uint32_t mask = __ballot_sync(0xffffffffu, odd);
-            if (lane == 0) c.bad[quad] = mask;
-            if (!(ok = meet())) break;
-            if ((c.bad[0] | c.bad[1] | c.bad[2] | c.bad[3]) != 0) {
-              bool fresh = t == it.t0;  // O holds nothing yet
-              if (tid == 0 && fresh) c.accumulate = 1;
+            if (any_bad != 0) {
+              if (!(ok = o_stable())) break;
+              bool fresh = first_unit;  // O holds nothing yet
 #pragma unroll 1
-              for (int k = 0; k < kKeys; ++k) {
-                if (!((c.bad[k >> 5] >> (k & 31)) & 1)) continue;
+              for (int k = u * kUnit; k < u * kUnit + kUnit; ++k) {
+                if (!((bad[k >> 5] >> (k & 31)) & 1)) continue;
+                if (tid == 0 && first_unit) c.accumulate = 1;
                 if (warp_live) {
-                  const float sk = tmem_ld1(tS + k);
+                  const float sk = tmem_ld1(tP + (k - u * kUnit));
                   tmem_wait_ld();
-                  const bool seen = key0 + k < sees;
+                  const bool seen = t * kKeys + k < sees;
                   const float p = seen ? ex2(fmaf(sk, scale, -base)) : 0.f;
 #pragma unroll 1
                   for (int i = 0; i < D; i += 32) {
@@ -634,38 +685,45 @@ __global__ void __launch_bounds__(kThreads, 1)
                 fresh = false;
               }
               if (!(ok = meet())) break;  // every row has read them
-              if (odd) zero_row();
+              if ((tid >> 6) == u && ((bad[quad] >> lane) & 1)) zero_row();
             }
+            fence_async_smem();
           }
-          fence_async_smem();
-        }
-        float2 sum0 = make_float2(0.f, 0.f), sum1 = sum0;
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
           if (warp_live) {
-            const float2 sc = make_float2(scale, scale), nb = make_float2(-base, -base);
             uint32_t p[32];
+            float2 sum0 = make_float2(0.f, 0.f), sum1 = sum0;
+            const float2 sc = make_float2(scale, scale), nb = make_float2(-base, -base);
+            auto weights = [&](auto poly) {
 #pragma unroll
-            for (int i = 0; i < 32; ++i) {
-              float2 x = ffma2(make_float2(s[h * 64 + 2 * i], s[h * 64 + 2 * i + 1]), sc, nb);
-              x.x = ex2(x.x);
-              x.y = ex2(x.y);
-              if (i & 1) sum1 = __fadd2_rn(sum1, x);
-              else sum0 = __fadd2_rn(sum0, x);
-              p[i] = pack2<F16>(x.x, x.y);
-            }
-            tmem_st32(tS + h * 32, p);
+              for (int i = 0; i < 32; ++i) {
+                float2 x = ffma2(make_float2(s[2 * i], s[2 * i + 1]), sc, nb);
+                if (decltype(poly)::value && i % kPolyEvery == kPolyEvery - 1) {
+                  x = ex2_poly(x);
+                } else {
+                  x.x = ex2(x.x);
+                  x.y = ex2(x.y);
+                }
+                if (i & 1) sum1 = __fadd2_rn(sum1, x);
+                else sum0 = __fadd2_rn(sum0, x);
+                p[i] = pack2<F16>(x.x, x.y);
+              }
+            };
+            if (care) weights(IC<0>{});
+            else weights(IC<1>{});
+            tmem_st32(tP, p);
+            l += (sum0.x + sum0.y) + (sum1.x + sum1.y);
             tmem_wait_st();
           }
           tc_fence_before();
           __syncwarp();
-          if (lane == 0) mbar_arrive(&c.p_ready[h]);
+          if (lane == 0) mbar_arrive(&c.p_ready[buf]);
+          ++n_unit;
         }
-        l += (sum0.x + sum0.y) + (sum1.x + sum1.y);
+        n_tile += care ? 1 : 0;
       }
       if (!ok) break;
       // the part's last product, then its rows out
-      if (!(ok = wait.warp(&c.pv_done, (n_tile - 1) & 1))) break;
+      if (!(ok = wait.warp(&c.pv_done[(n_unit - 1) & 1], ((n_unit - 1) >> 1) & 1))) break;
       tc_fence_after();
       if (warp_live) {
         int tok, hq;
