@@ -57,7 +57,7 @@ constexpr int kProducer = 8, kMma = 10;
 constexpr int kItems = 4;           // parts announced ahead
 constexpr uint32_t kTmemCols = 512; // per stream: S (P over it) 128, O 128
 constexpr float kLazy = 8.f;
-constexpr int kPolyEvery = 4;       // one pair of weights in four on the FP32 pipe
+constexpr int kPolyEvery = 8;       // one pair of weights in eight on the FP32 pipe
 
 // An item's fixed cost (queries, first scores, last values, partials out) is
 // that of about two tiles.
@@ -325,15 +325,25 @@ __global__ void __launch_bounds__(kThreads, 1)
       // query rows of this stream, 16 bytes a copy, swizzled as TMA would
       const int r_first = paired ? j * kHalf : 0;
       const int rows = min(kHalf, it.rows - r_first);
-      const uint16_t* Q = static_cast<const uint16_t*>(a.Q);
-      for (int i = lane; i < rows * (D / 8); i += 32) {
-        const int r = i / (D / 8), v = i % (D / 8);
-        int tok, hq;
+      {
+        // lane: piece `v` of rows r, r + step, ...; token and head are stepped, not divided
+        constexpr int PIECES = D / 8, STEP = 32 / PIECES;
+        const int v = lane % PIECES;
+        int r = lane / PIECES, g, tok, hq;
         attn_row(a, it, r_first + r, tok, hq);
-        const uint32_t dst = smem_u32(sq + (v >> 3) * (128 * 128) + r * 128 + (((v & 7) ^ (r & 7)) << 4));
-        asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst),
-                     "l"(Q + tok * a.q_st + hq * a.q_sh + v * 8)
-                     : "memory");
+        g = hq - it.h * a.G;
+        const uint16_t* src = static_cast<const uint16_t*>(a.Q) + tok * a.q_st + hq * a.q_sh + v * 8;
+        const uint32_t col = smem_u32(sq) + (v >> 3) * (128 * 128);
+        const int64_t over = a.q_st - a.G * a.q_sh;  // to the next token's first head
+#pragma unroll 4
+        for (; r < rows; r += STEP) {
+          asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(col + r * 128 + (((v & 7) ^ (r & 7)) << 4)),
+                       "l"(src)
+                       : "memory");
+          g += STEP;
+          src += STEP * a.q_sh;
+          while (g >= a.G) g -= a.G, src += over;
+        }
       }
       asm volatile("cp.async.commit_group;" ::: "memory");
       bool q_sent = false;
