@@ -32,6 +32,8 @@ __device__ __forceinline__ void store4<__half>(__half* dst, float4 v) {
 
 template <typename T>
 __global__ void __launch_bounds__(kMergeThreads) prefix_attention_merge_kernel(const AttnArgs a, int cont_rows) {
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   const int lane = threadIdx.x & 31;
   const int64_t row = (int64_t)blockIdx.x * (kMergeThreads / 32) + (threadIdx.x >> 5);
   const int heads = a.H * a.G;
@@ -132,9 +134,8 @@ template <typename T>
 int launch_merge(const AttnArgs& a, cudaStream_t stream) {
   const int64_t rows = (int64_t)a.n_tokens * a.H * a.G;
   const int64_t blocks = (rows + kMergeThreads / 32 - 1) / (kMergeThreads / 32);
-  prefix_attention_merge_kernel<T>
-      <<<(unsigned)blocks, kMergeThreads, 0, stream>>>(a, a.dv <= 128 ? kAttnTcContRows : kAttnFmaContRows);
-  return check_launch("prefix_attention_merge_kernel");
+  return attn_launch("prefix_attention_merge_kernel", prefix_attention_merge_kernel<T>, blocks, kMergeThreads, 0, stream,
+                     a, a.dv <= 128 ? kAttnTcContRows : kAttnFmaContRows);
 }
 
 struct Workspace {

@@ -95,7 +95,7 @@ struct AttnPart {
 // tile.  MR is the most rows of an item.
 template <int MR_, int KT_, int C0_, int W_>
 struct AttnCutAll {
-  static constexpr int MR = MR_, KT = KT_, C0 = C0_, W = W_;
+  static constexpr int MR = MR_, KT = KT_, C0 = C0_, W = W_, SHARES = 1;
   __device__ static __forceinline__ int count(int R) { return (R + MR - 1) / MR; }
   __device__ static __forceinline__ int row0(int, int m) { return m * MR; }
   __device__ static __forceinline__ int rows(int R, int m) { return min(MR, R - m * MR); }
@@ -103,7 +103,7 @@ struct AttnCutAll {
 // Items of more than HALF rows, up to two HALF-row tiles that share their keys ...
 template <int HALF, int KT_, int C0_, int W_>
 struct AttnCutPairs {
-  static constexpr int MR = 2 * HALF, KT = KT_, C0 = C0_, W = W_;
+  static constexpr int MR = 2 * HALF, KT = KT_, C0 = C0_, W = W_, SHARES = 1;
   __device__ static __forceinline__ int count(int R) { return R > HALF ? (R - HALF + MR - 1) / MR : 0; }
   __device__ static __forceinline__ int row0(int, int m) { return m * MR; }
   __device__ static __forceinline__ int rows(int R, int m) { return min(MR, R - m * MR); }
@@ -112,7 +112,7 @@ struct AttnCutPairs {
 template <int HALF, int KT_, int C0_, int W_>
 struct AttnCutRest {
   using Pairs = AttnCutPairs<HALF, KT_, C0_, W_>;
-  static constexpr int MR = HALF, KT = KT_, C0 = C0_, W = W_;
+  static constexpr int MR = HALF, KT = KT_, C0 = C0_, W = W_, SHARES = 2;  // shares of a CTA
   __device__ static __forceinline__ int row0(int R, int) { return Pairs::count(R) * 2 * HALF; }
   __device__ static __forceinline__ int rows(int R, int) { return R - row0(R, 0); }
   __device__ static __forceinline__ int count(int R) { return rows(R, 0) > 0 ? 1 : 0; }
@@ -145,39 +145,45 @@ struct AttnLine {
     return c;
   }
 
-  // Called by every thread of the CTA.  No share is smaller than an item's
-  // fixed cost and one tile, so every share between the first and the last of
-  // an item holds one of its tiles.
-  __device__ void init(const AttnArgs& a, int most_shares, int64_t* s_sum) {
-    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, n_warps = (blockDim.x + 31) >> 5;
-    prefix_len = attn_prefix_len(a);
-    prefix_rows = prefix_len > 0 ? attn_tokens(a) * a.G : 0;
+  // attn_lines() in pieces: the prefix's part; one request; the scan over threads
+  __device__ __forceinline__ void begin(const AttnArgs& a, int prefix, int tokens) {
+    prefix_len = prefix;
+    prefix_rows = prefix > 0 ? tokens * a.G : 0;
     prefix_mt = C::count(prefix_rows);
     prefix_nt = tiles(prefix_len);
     prefix_cost = item_cost(prefix_nt);
     prefix_all = prefix_cost * prefix_mt * a.H;
-    const int per = (a.B + blockDim.x - 1) / blockDim.x;
-    b0 = min(a.B, tid * per), b1 = min(a.B, b0 + per);
     sum = 0;
-    for (int i = b0; i < b1; ++i) sum += head_cost(attn_request(a, i), a.G) * a.H;
+  }
+  __device__ __forceinline__ void add(const AttnArgs& a, const AttnRequest& r) { sum += head_cost(r, a.G) * a.H; }
+  __device__ __forceinline__ void scan_warp(int64_t* s_sum) {
+    const int lane = threadIdx.x & 31;
     int64_t inc = sum;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
       const int64_t v = __shfl_up_sync(0xffffffffu, inc, o);
       if (lane >= o) inc += v;
     }
-    if (lane == 31) s_sum[warp] = inc;
-    __syncthreads();
+    if (lane == 31) s_sum[threadIdx.x >> 5] = inc;
     before = prefix_all + inc - sum;
+  }
+  __device__ __forceinline__ void scan_block(const int64_t* s_sum, int most_shares) {
+    const int warp = threadIdx.x >> 5, n_warps = (blockDim.x + 31) >> 5;
     U = prefix_all;
     for (int w = 0; w < n_warps; ++w) {
       if (w < warp) before += s_sum[w];
       U += s_sum[w];
     }
-    n = (int)max((int64_t)1, min((int64_t)most_shares, U / (C::C0 + C::W)));
-    __syncthreads();  // s_sum may be used again
+    // no share is smaller than an item's fixed cost and one tile, so every share
+    // between the first and the last of an item holds one of its tiles
+    constexpr int least = C::C0 + C::W;
+    n = U >= (int64_t)most_shares * least ? most_shares : max(1, (int)U / least);
   }
-  __device__ __forceinline__ int64_t bound(int i) const { return i < n ? U * i / n : U; }
+  // share i is [bound(i), bound(i + 1))
+  __device__ __forceinline__ int64_t bound(int i) const {
+    if (i >= n) return U;
+    return (U >> 22) == 0 ? (int64_t)((uint32_t)U * (uint32_t)i / (uint32_t)n) : U * i / n;  // n <= 640
+  }
   // Called by every thread: the one whose requests hold the beginning of share
   // i leaves the request and the cost before it (to be read after a barrier).
   __device__ void find(const AttnArgs& a, int i, int* s_b, int64_t* s_at) const {
@@ -194,8 +200,32 @@ struct AttnLine {
     *s_at = p;
   }
   // share that holds cost position p
-  __device__ __forceinline__ int share_of(int64_t p) const { return (int)(((p + 1) * n - 1) / U); }
+  __device__ __forceinline__ int share_of(int64_t p) const {
+    return (U >> 22) == 0 ? (int)(((uint32_t)(p + 1) * (uint32_t)n - 1) / (uint32_t)U) : (int)(((p + 1) * n - 1) / U);
+  }
 };
+
+// Sums up one or more lines; called by every thread of the CTA with its own
+// line objects.  One barrier; s_sum (one row a line) may be used again after
+// the caller's next one.
+template <class... C>
+__device__ __forceinline__ void attn_lines(const AttnArgs& a, int64_t (*s_sum)[32], int most_shares,
+                                           AttnLine<C>&... line) {
+  const int prefix = attn_prefix_len(a), tokens = attn_tokens(a);
+  (line.begin(a, prefix, tokens), ...);
+  const int per = (a.B + blockDim.x - 1) / blockDim.x;
+  const int b0 = min(a.B, (int)threadIdx.x * per), b1 = min(a.B, b0 + per);
+  ((line.b0 = b0, line.b1 = b1), ...);
+  for (int b = b0; b < b1; ++b) {
+    const AttnRequest r = attn_request(a, b);
+    (line.add(a, r), ...);
+  }
+  int k = 0;
+  (line.scan_warp(s_sum[k++]), ...);
+  __syncthreads();
+  k = 0;
+  (line.scan_block(s_sum[k++], most_shares * C::SHARES), ...);
+}
 
 // Walks share i of a line; the state is the calling thread's.
 template <class C>
@@ -308,6 +338,28 @@ __device__ __forceinline__ void attn_row(const AttnArgs& a, const AttnPart& it, 
   const int t = rg / a.G;
   tok = it.tok0 + t;
   hq = it.h * a.G + rg - t * a.G;
+}
+
+// A launch that may begin while the one before it on the stream ends: the
+// kernels wait (griddepcontrol.wait) before they touch memory.
+template <typename... P, typename... A>
+int attn_launch(const char* what, void (*kern)(P...), int64_t grid, int threads, int smem, cudaStream_t stream,
+                const A&... args) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)grid);
+  cfg.blockDim = dim3((unsigned)threads);
+  cfg.dynamicSmemBytes = (size_t)smem;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, kern, P(args)...);
+  if (e == cudaSuccess) return GFST_OK;
+  cudaGetLastError();  // reported here
+  set_last_error("%s: %s", what, cudaGetErrorString(e));
+  return GFST_ERR_LAUNCH;
 }
 
 // the kernels' launchers (each returns a status)

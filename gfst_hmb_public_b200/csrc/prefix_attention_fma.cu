@@ -108,10 +108,12 @@ __global__ void __launch_bounds__(kThreads) prefix_attention_fma_kernel(const At
   const int grp = tid / n_col, col = (tid - grp * n_col) * 4;
   constexpr int kAcc = 8;                // rows per thread at dv = 256; fewer below
 
-  __shared__ int64_t s_sum[32], s_at;
+  __shared__ int64_t s_sum[1][32], s_at;
   __shared__ int s_b;
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   AttnLine<Cut> line;
-  line.init(a, gridDim.x, s_sum);
+  attn_lines(a, s_sum, gridDim.x, line);
   line.find(a, blockIdx.x, &s_b, &s_at);
   __syncthreads();
   AttnWalk<Cut> walk;
@@ -267,8 +269,7 @@ int launch(const AttnArgs& a, int sms, cudaStream_t stream) {
   GFST_REQUIRE(e == cudaSuccess, GFST_ERR_DEVICE, "cudaFuncSetAttribute: %s", cudaGetErrorString(e));
   const int per_sm = ly.bytes <= 110 * 1024 ? 2 : 1;
   const int grid = (sms < kAttnMaxGrid ? sms : kAttnMaxGrid) * per_sm;
-  kern<<<grid, kThreads, ly.bytes, stream>>>(a);
-  return check_launch("prefix_attention_fma_kernel");
+  return attn_launch("prefix_attention_fma_kernel", kern, grid, kThreads, ly.bytes, stream, a);
 }
 
 }  // namespace

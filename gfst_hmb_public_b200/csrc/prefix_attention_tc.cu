@@ -59,6 +59,9 @@ constexpr uint32_t kTmemCols = 512; // per stream: S (P over it) 128, O 128
 constexpr float kLazy = 8.f;
 constexpr int kPolyEvery = 8;       // one pair of weights in eight on the FP32 pipe
 
+constexpr int kJoinRows = 16;                       // rows of an item of two copies; half of it of four
+constexpr int kStageBytes = 2 * kJoinRows * 128 * 4;  // a stream's rows of joining copies (copies_of)
+
 // An item's fixed cost (queries, first scores, last values, partials out) is
 // that of about two tiles.
 using Pairs = AttnCutPairs<kHalf, kKeys, 2, 1>;
@@ -72,7 +75,8 @@ struct TcAttn {
   static constexpr int RING = 2 * NS;              // stages of the pairs' ring
   static constexpr int Q_OFF = 0;
   static constexpr int KV_OFF = 2 * TILE_BYTES;
-  static constexpr int CTRL_OFF = KV_OFF + RING * TILE_BYTES;
+  static constexpr int STAGE_OFF = KV_OFF + RING * TILE_BYTES;  // rows of joining copies
+  static constexpr int CTRL_OFF = STAGE_OFF + 2 * kStageBytes;
 };
 
 struct StreamCtrl {
@@ -84,7 +88,8 @@ struct StreamCtrl {
   AttnPart item[kItems];
   int paired[kItems];          // 1: pair, 0: rest, -1: no more work
   uint32_t bad[2][4];          // value rows that are not finite (one bit each), two tiles in turn
-  int accumulate;              // the tile's first product adds to O
+  int accumulate;              // the part's first product adds to O
+  float2 ml[2 * kJoinRows];    // joining copies' references and sums
   int at_b[2];
   int64_t at_u[2];
 };
@@ -94,7 +99,7 @@ struct Ctrl {
   uint64_t care;                 // both streams' softmax warps
   uint64_t drained;              // the pairs are done with the ring
   uint64_t done[2];              // a stream's products are done
-  int64_t sum[32];
+  int64_t sum[2][32];
   AttnLine<Pairs> pairs;         // the lines (their common part)
   AttnLine<Rest> rest;
   uint32_t tmem;
@@ -161,6 +166,25 @@ __device__ __forceinline__ void tmem_st32(uint32_t taddr, const uint32_t (&r)[32
       "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]),
       "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31])
       : "memory");
+}
+__device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t (&r)[16]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], "
+      "{%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16};" ::"r"(taddr),
+      "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
+      "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
+      : "memory");
+}
+__device__ __forceinline__ void tmem_st8(uint32_t taddr, const uint32_t (&r)[8]) {
+  asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"r"(taddr), "r"(r[0]),
+               "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7])
+               : "memory");
+}
+template <int N>
+__device__ __forceinline__ void tmem_st(uint32_t taddr, const uint32_t (&r)[N]) {
+  if constexpr (N == 32) tmem_st32(taddr, r);
+  else if constexpr (N == 16) tmem_st16(taddr, r);
+  else tmem_st8(taddr, r);
 }
 __device__ __forceinline__ void tmem_st32(uint32_t taddr, const float (&v)[32]) {
   uint32_t r[32];
@@ -233,39 +257,385 @@ struct Waiter {
   }
 };
 
+// An item of few rows would leave three quarters of the softmax threads idle and
+// its one warp with all 64 scores of a unit to exponentiate.  Its rows are laid
+// out C times in the query tile (128 / C rows apart): the products give every
+// copy all scores, copy k takes only its 64 / C keys of each unit (its other
+// weights are 0), and the copies' rows, softmaxes over disjoint keys, are joined
+// when the part ends.  C = 4 up to 8 rows, 2 up to 16: the joining rows then fit
+// what shared memory is left.
+__device__ __forceinline__ int copies_of(int paired, int rows) {
+  return paired || rows > kJoinRows ? 1 : rows > kJoinRows / 2 ? 2 : 4;
+}
+
+// One softmax thread: a row of its stream's tile.
+template <int D, bool F16>
+struct Softmax {
+  using TC = TcAttn<D>;
+  static constexpr int NS = TC::NS, RING = TC::RING, NC = TC::NC, TILE = TC::TILE_BYTES;
+  static constexpr float kBias = F16 ? 7.f : 0.f;
+  const AttnArgs& a;
+  Ctrl* ctl;
+  uint8_t* smem;
+  const int j, quad, lane, tid;
+  StreamCtrl& c;
+  const uint32_t tS, tO;
+  const Waiter wait;
+  uint32_t n_tile = 0, n_unit = 0, n_own = 0, n_ring = 0, n_care = 0, n_care2 = 0;
+
+  __device__ __forceinline__ Softmax(const AttnArgs& a_, Ctrl* ctl_, uint8_t* smem_, uint32_t tmem, int j_)
+      : a(a_), ctl(ctl_), smem(smem_), j(j_), quad((threadIdx.x >> 5) & 3), lane(threadIdx.x & 31),
+        tid(threadIdx.x & 127), c(ctl_->s[j_]), tS(tmem + j_ * 256 + ((uint32_t)(quad * 32) << 16)), tO(tS + 128),
+        wait{&ctl_->abort} {}
+
+  // a bounded barrier of the stream's softmax warps, for a pair of both streams'
+  __device__ __forceinline__ bool meet(int paired) {
+    __syncwarp();
+    uint64_t* bar = paired ? &ctl->care : &c.care;
+    uint32_t& n = paired ? n_care2 : n_care;
+    if (lane == 0) mbar_arrive(bar);
+    return wait.warp(bar, n++ & 1);
+  }
+  __device__ __forceinline__ void zero_row(uint8_t* vs) const {
+#pragma unroll
+    for (int i = 0; i < NC * 8; ++i)
+      *reinterpret_cast<uint4*>(vs + (i >> 3) * (128 * 128) + tid * 128 + (i & 7) * 16) = make_uint4(0, 0, 0, 0);
+  }
+  // O += p v for the value row k, over this thread's row (fresh: O holds nothing yet)
+  __device__ __forceinline__ void add_row(const uint8_t* vs, int k, float p, bool add, bool fresh) const {
+#pragma unroll 1
+    for (int i = 0; i < D; i += 32) {
+      float o[32];
+      tmem_ld32(tO + i, o);
+      tmem_wait_ld();
+#pragma unroll
+      for (int q = 0; q < 32; q += 8) {
+        const int col = i + q;
+        const uint4 v = *reinterpret_cast<const uint4*>(vs + (col >> 6) * (128 * 128) + k * 128 +
+                                                        ((((col & 63) >> 3) ^ (k & 7)) << 4));
+        const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+        for (int x = 0; x < 4; ++x) {
+          float lo, hi;
+          if constexpr (F16) {
+            const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w[x]));
+            lo = f.x, hi = f.y;
+          } else {
+            lo = bf16_lo(w[x]), hi = bf16_hi(w[x]);
+          }
+          const float a0 = fresh ? 0.f : o[q + 2 * x], a1 = fresh ? 0.f : o[q + 2 * x + 1];
+          o[q + 2 * x] = add ? fmaf(p, lo, a0) : a0;
+          o[q + 2 * x + 1] = add ? fmaf(p, hi, a1) : a1;
+        }
+      }
+      tmem_st32(tO + i, o);
+      tmem_wait_st();
+    }
+  }
+
+  // N scores (or O columns) at TMEM address t
+  template <int N>
+  __device__ static __forceinline__ void load(uint32_t t, float (&s)[N]) {
+    if constexpr (N == 16) {
+      tmem_ld16(t, s);
+    } else {
+#pragma unroll
+      for (int i = 0; i < N; i += 32) tmem_ld32(t + i, s + i);
+    }
+    tmem_wait_ld();
+  }
+
+  template <int C>
+  __device__ __forceinline__ bool part(const AttnPart& it, int paired) {
+    constexpr int N = kUnit / C;                         // keys of a unit that this thread takes
+    const int copy = tid / (kHalf / C);
+    const int key_off = copy * N;
+    const int r = C > 1 ? tid % (kHalf / C) : (paired ? j * kHalf : 0) + tid;  // row of the item
+    const bool live = r < it.rows;
+    const bool warp_live = __any_sync(0xffffffffu, live);
+    const float scale = a.scale_log2;
+    // keys this row sees, and the first row of the item (fewest)
+    const int sees = it.own ? min(it.len, it.see0 + (it.row0 + r) / a.G + 1) : it.len;
+    const int fewest = it.own ? min(it.len, it.see0 + it.row0 / a.G + 1) : it.len;
+    const uint32_t stages = paired ? RING : NS;
+    uint64_t* fulls = paired ? ctl->full : c.full;
+    float m = -INFINITY, l = 0.f;                        // m: reference, bias included
+    for (int t = it.t0; t < it.t1; ++t) {
+      const uint32_t n = (paired ? n_ring : n_own) + 1;  // the value stage (for tiles that need care)
+      const uint32_t v_stage = n % stages;
+      uint8_t* vs = smem + TC::KV_OFF + ((paired ? 0 : j * NS) + v_stage) * TILE;
+      n_ring += paired ? 2 : 0;
+      n_own += paired ? 0 : 2;
+      const bool care = t * kKeys + kKeys > fewest;
+      uint32_t any_bad = 0;
+      const int units = it.len - t * kKeys > kUnit ? 2 : 1;
+      for (int u = 0; u < units; ++u, ++n_unit) {
+        const uint32_t buf = n_unit & 1;
+        const uint32_t tP = tS + buf * kUnit;
+        const bool first_unit = t == it.t0 && u == 0;
+        // keys of this thread's N that the row sees
+        const int seen = sees - (t * kKeys + u * kUnit + key_off);
+        // O as the products up to the last unit left it (they may still run)
+        auto o_stable = [&]() -> bool {
+          if (first_unit) return true;
+          const bool done = wait.warp(&c.pv_done[buf ^ 1], ((n_unit - 1) >> 1) & 1);
+          tc_fence_after();
+          return done;
+        };
+        if (!wait.warp(&c.s_full[buf], (n_unit >> 1) & 1)) return false;
+        tc_fence_after();
+        float s[N];
+        if (warp_live) {
+          load<N>(tP + key_off, s);
+          if (care) {
+#pragma unroll
+            for (int i = 0; i < N; ++i) s[i] = i < seen ? s[i] : -INFINITY;
+          }
+          float m0 = s[0], m1 = s[1], m2 = s[2], m3 = s[3];
+#pragma unroll
+          for (int i = 4; i < N; i += 4) {
+            m0 = fmaxf(m0, s[i]), m1 = fmaxf(m1, s[i + 1]);
+            m2 = fmaxf(m2, s[i + 2]), m3 = fmaxf(m3, s[i + 3]);
+          }
+          const float top = fmaxf(fmaxf(m0, m1), fmaxf(m2, m3)) * scale - kBias;
+          const bool move = live && top > m + kLazy;
+          if (__any_sync(0xffffffffu, move)) {
+            const float al = move ? ex2(m - top) : 1.f;  // m = -inf: 0
+            if (move) m = top;
+            l *= al;
+            if (!first_unit) {
+              if (!o_stable()) return false;
+#pragma unroll 1
+              for (int i = 0; i < D; i += 32) {
+                float o[32];
+                load<32>(tO + i, o);
+#pragma unroll
+                for (int k = 0; k < 32; ++k) o[k] *= al;
+                tmem_st32(tO + i, o);
+              }
+              tmem_wait_st();
+            }
+          }
+        }
+        const float base = m == -INFINITY ? 0.f : m;
+        if (care) {
+          uint32_t* bad = c.bad[n_tile & 1];
+          if (u == 0) {
+            // values: rows behind the last key become zero; rows that only some
+            // query rows see are looked at
+            if (!wait.warp(&fulls[v_stage], (n / stages) & 1)) return false;
+            const int valid = min(kKeys, it.len - t * kKeys), from = fewest - t * kKeys;
+            if (tid >= valid) zero_row(vs);
+            if (from < valid) {
+              bool odd = false;
+              if (tid >= from && tid < valid) {
+                constexpr uint32_t E = F16 ? 0x7c00u : 0x7f80u;
+#pragma unroll
+                for (int i = 0; i < NC * 8; ++i) {
+                  const uint4 v = *reinterpret_cast<const uint4*>(vs + (i >> 3) * (128 * 128) + tid * 128 + (i & 7) * 16);
+                  const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+                  for (int q = 0; q < 4; ++q) odd |= (w[q] & E) == E || ((w[q] >> 16) & E) == E;
+                }
+              }
+              const uint32_t mask = __ballot_sync(0xffffffffu, odd);
+              if (lane == 0) bad[quad] = mask;
+              // both streams of a pair look at the same rows of the same stage
+              if (!meet(paired)) return false;
+              any_bad = bad[0] | bad[1] | bad[2] | bad[3];
+            }
+          }
+          if (any_bad != 0) {
+            if (!o_stable()) return false;
+            bool fresh = first_unit;
+#pragma unroll 1
+            for (int k = u * kUnit; k < u * kUnit + kUnit; ++k) {
+              if (!((bad[k >> 5] >> (k & 31)) & 1)) continue;
+              if (tid == 0 && first_unit) c.accumulate = 1;
+              if (warp_live) {
+                const float sk = tmem_ld1(tP + (k - u * kUnit));
+                tmem_wait_ld();
+                const int mine = k - u * kUnit - key_off;
+                const bool add = mine >= 0 && mine < N && mine < seen;
+                add_row(vs, k, add ? ex2(fmaf(sk, scale, -base)) : 0.f, add, fresh);
+              }
+              fresh = false;
+            }
+            if (!meet(paired)) return false;  // every row has read them
+            if ((tid >> 6) == u && ((bad[quad] >> lane) & 1)) zero_row(vs);
+          }
+          fence_async_smem();
+        }
+        if (warp_live) {
+          uint32_t p[N / 2];
+          float2 sum0 = make_float2(0.f, 0.f), sum1 = sum0;
+          const float2 sc = make_float2(scale, scale), nb = make_float2(-base, -base);
+          auto weights = [&](auto poly) {
+#pragma unroll
+            for (int i = 0; i < N / 2; ++i) {
+              float2 x = ffma2(make_float2(s[2 * i], s[2 * i + 1]), sc, nb);
+              if (decltype(poly)::value && i % kPolyEvery == kPolyEvery - 1) {
+                x = ex2_poly(x);
+              } else {
+                x.x = ex2(x.x);
+                x.y = ex2(x.y);
+              }
+              if (i & 1) sum1 = __fadd2_rn(sum1, x);
+              else sum0 = __fadd2_rn(sum0, x);
+              p[i] = pack2<F16>(x.x, x.y);
+            }
+          };
+          if (care) weights(IC<0>{});
+          else weights(IC<1>{});
+          tmem_st(tP + copy * (N / 2), p);
+          if constexpr (C > 1) {
+            const uint32_t zero[N / 2] = {};
+#pragma unroll
+            for (int k = 1; k < C; ++k) tmem_st(tP + ((copy + k) % C) * (N / 2), zero);
+          }
+          l += (sum0.x + sum0.y) + (sum1.x + sum1.y);
+          tmem_wait_st();
+        }
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&c.p_ready[buf]);
+      }
+      n_tile += care ? 1 : 0;
+    }
+    // the part's last product, then its rows out
+    // continuation rows: the pairs' of all CTAs, then the streams'
+    const int64_t crow0 = paired ? (int64_t)blockIdx.x * (2 * kHalf)
+                                 : (int64_t)gridDim.x * (2 * kHalf) + (int64_t)(blockIdx.x + j * gridDim.x) * kHalf;
+    const int stride = paired ? 2 * kHalf : kHalf;
+    auto put_ml = [&](int64_t row, int r_, float2 ml) {
+      if (it.first) {
+        a.part_ml[it.own][row] = ml;
+        a.part_next[it.own][row] = attn_next((int)(crow0 + r_ + stride), it.n_cont, stride);
+      } else {
+        a.cont_ml[crow0 + r_] = ml;
+      }
+    };
+    if constexpr (C == 1) {
+      if (!wait.warp(&c.pv_done[(n_unit - 1) & 1], ((n_unit - 1) >> 1) & 1)) return false;
+      tc_fence_after();
+      if (warp_live) {
+        int tok, hq;
+        attn_row(a, it, r, tok, hq);
+        const int64_t row = (int64_t)tok * (a.H * a.G) + hq;
+        float* dst = it.first ? a.part_o[it.own] + row * D : a.cont_o + (crow0 + r) * D;
+#pragma unroll 1
+        for (int i = 0; i < D; i += 32) {
+          float o[32];
+          load<32>(tO + i, o);
+          if (live) {
+#pragma unroll
+            for (int k = 0; k < 32; k += 8) store_sector(dst + i + k, o + k);
+          }
+        }
+        if (live) put_ml(row, r, make_float2(m, l));
+      }
+    } else {
+      // the copies' references and sums, then their rows at the largest reference
+      // through shared memory; four warps add them, a row of D values a warp
+      constexpr int P = D / 4;                           // 16-byte pieces of a row
+      float4* st = reinterpret_cast<float4*>(smem + TC::STAGE_OFF + j * kStageBytes);
+      if (live) c.ml[copy * (kJoinRows * 2 / C) + r] = make_float2(m, l);
+      if (!meet(0)) return false;
+      const float2* mls = c.ml;
+      auto at = [&](int k, int r_) { return k * (kJoinRows * 2 / C) + r_; };
+      auto top_of = [&](int r_) {
+        float top = mls[at(0, r_)].x;
+#pragma unroll
+        for (int k = 1; k < C; ++k) top = fmaxf(top, mls[at(k, r_)].x);
+        return top;
+      };
+      if (!wait.warp(&c.pv_done[(n_unit - 1) & 1], ((n_unit - 1) >> 1) & 1)) return false;
+      tc_fence_after();
+      if (warp_live) {
+        const float top = live ? top_of(r) : 0.f;
+        const float f = m == top ? 1.f : ex2(m - top);   // all empty: 1
+#pragma unroll 1
+        for (int i = 0; i < D; i += 32) {
+          float o[32];
+          load<32>(tO + i, o);
+          if (live) {
+            float4* dst = st + (copy * it.rows + r) * P;
+#pragma unroll
+            for (int k = 0; k < 32; k += 4)  // pieces in an order that spreads the rows over the banks
+              dst[((i + k) / 4) ^ (r & 7)] = make_float4(o[k] * f, o[k + 1] * f, o[k + 2] * f, o[k + 3] * f);
+          }
+        }
+      }
+      if (!meet(0)) return false;
+      for (int r_ = quad; r_ < it.rows; r_ += 4) {
+        int tok, hq;
+        attn_row(a, it, r_, tok, hq);
+        const int64_t row = (int64_t)tok * (a.H * a.G) + hq;
+        float* dst = it.first ? a.part_o[it.own] + row * D : a.cont_o + (crow0 + r_) * D;
+        if (lane < P) {
+          float4 o = st[r_ * P + (lane ^ (r_ & 7))];
+#pragma unroll
+          for (int k = 1; k < C; ++k) {
+            const float4 v = st[(k * it.rows + r_) * P + (lane ^ (r_ & 7))];
+            o.x += v.x, o.y += v.y, o.z += v.z, o.w += v.w;
+          }
+          *reinterpret_cast<float4*>(dst + lane * 4) = o;
+        }
+        if (lane == 0) {
+          const float top = top_of(r_);
+          float sum = 0.f;
+#pragma unroll
+          for (int k = 0; k < C; ++k) {
+            const float2 v = mls[at(k, r_)];
+            sum += v.x == top ? v.y : v.y * ex2(v.x - top);
+          }
+          put_ml(row, r_, make_float2(top, sum));
+        }
+      }
+    }
+    tc_fence_before();
+    return true;
+  }
+};
+
 template <int D, bool F16>
 __global__ void __launch_bounds__(kThreads, 1)
     prefix_attention_tc_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV,
                                const __grid_constant__ AttnArgs a, int64_t pool_rows) {
   using TC = TcAttn<D>;
   constexpr int NS = TC::NS, RING = TC::RING, NC = TC::NC, TILE = TC::TILE_BYTES;
-  extern __shared__ uint8_t smem_raw[];
-  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  extern __shared__ __align__(1024) uint8_t smem[];  // tiles in 1024-byte swizzle atoms
   Ctrl* ctl = reinterpret_cast<Ctrl*>(smem + TC::CTRL_OFF);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  if ((smem_u32(smem) & 1023u) != 0) {  // cannot be: no other shared memory
+    if (threadIdx.x == 0) atomicExch(&g_attn_tc_error, (unsigned)GFST_ERR_ALIGN);
+    return;
+  }
 
-  if (threadIdx.x == 0) {
-    for (int j = 0; j < 2; ++j) {
-      StreamCtrl& c = ctl->s[j];
-      for (int i = 0; i < kItems; ++i) {
-        mbar_init(&c.item_full[i], 1);
-        mbar_init(&c.item_empty[i], 5);  // four softmax warps, the MMA warp
-      }
-      mbar_init(&c.q_full, 1);
-      mbar_init(&c.q_empty, 1);
-      for (int i = 0; i < 2; ++i) {
-        mbar_init(&c.s_full[i], 1);
-        mbar_init(&c.p_ready[i], 4);
-        mbar_init(&c.pv_done[i], 1);
-      }
-      mbar_init(&c.care, 4);
-      for (int i = 0; i < 4; ++i) {
-        mbar_init(&c.full[i], 1);
-        mbar_init(&c.empty[i], 1);
-      }
-      c.accumulate = 0;
-      mbar_init(&ctl->done[j], 1);
+  // Everything up to here and the barriers touch no memory of earlier work, so
+  // they run while the launch before this one ends.
+  if (lane == 0 && warp < 2) {
+    StreamCtrl& c = ctl->s[warp];
+    for (int i = 0; i < kItems; ++i) {
+      mbar_init(&c.item_full[i], 1);
+      mbar_init(&c.item_empty[i], 5);  // four softmax warps, the MMA warp
     }
+    mbar_init(&c.q_full, 1);
+    mbar_init(&c.q_empty, 1);
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&c.s_full[i], 1);
+      mbar_init(&c.p_ready[i], 4);
+      mbar_init(&c.pv_done[i], 1);
+    }
+    mbar_init(&c.care, 4);
+    for (int i = 0; i < 4; ++i) {
+      mbar_init(&c.full[i], 1);
+      mbar_init(&c.empty[i], 1);
+    }
+    c.accumulate = 0;
+    mbar_init(&ctl->done[warp], 1);
+    mbar_init_fence();
+  } else if (lane == 0 && warp == 2) {
     for (int i = 0; i < 8; ++i) {
       mbar_init(&ctl->full[i], 1);
       mbar_init(&ctl->empty[i], 2);  // both streams' products
@@ -277,31 +647,33 @@ __global__ void __launch_bounds__(kThreads, 1)
   }
   if (warp == kMma) tmem_alloc(&ctl->tmem, kTmemCols);
   tc_fence_before();
-  __syncthreads();
-  tc_fence_after();
-  const uint32_t tmem = ctl->tmem;
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
 
   // the work: this CTA's share of the pairs, and one share of the rest per
   // stream (stream 1's behind all of stream 0's, so few items spread over the SMs)
   {
     AttnLine<Pairs> pl;
-    pl.init(a, gridDim.x, ctl->sum);
-    pl.find(a, blockIdx.x, &ctl->s[0].at_b[0], &ctl->s[0].at_u[0]);
-    if (threadIdx.x == 0) ctl->pairs = pl;
     AttnLine<Rest> rl;
-    rl.init(a, 2 * gridDim.x, ctl->sum);
+    attn_lines(a, ctl->sum, gridDim.x, pl, rl);
+    pl.find(a, blockIdx.x, &ctl->s[0].at_b[0], &ctl->s[0].at_u[0]);
     for (int j = 0; j < 2; ++j) rl.find(a, blockIdx.x + j * gridDim.x, &ctl->s[j].at_b[1], &ctl->s[j].at_u[1]);
-    if (threadIdx.x == 0) ctl->rest = rl;
+    if (threadIdx.x == 0) {
+      ctl->pairs = pl;
+      ctl->rest = rl;
+    }
   }
   __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = ctl->tmem;
 
   const Waiter wait{&ctl->abort};
   uint32_t issued_own = 0, issued_ring = 0;  // stages filled by this producer (for the drain)
 
   // the softmax threads hold a row of scores: they take registers from the other
-  // four warps (2 x 128 x 200 + 128 x 104 of the 384 x 168 launched)
+  // four warps (2 x 128 x 208 + 128 x 88 of the 384 x 168 launched)
   if (warp >= kProducer) {
-  asm volatile("setmaxnreg.dec.sync.aligned.u32 104;");
+  asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
   if (warp < kMma) {
     // ------------------------------------------------------------- producer
     const int j = warp - kProducer;
@@ -335,11 +707,14 @@ __global__ void __launch_bounds__(kThreads, 1)
         const uint16_t* src = static_cast<const uint16_t*>(a.Q) + tok * a.q_st + hq * a.q_sh + v * 8;
         const uint32_t col = smem_u32(sq) + (v >> 3) * (128 * 128);
         const int64_t over = a.q_st - a.G * a.q_sh;  // to the next token's first head
+        const int copies = copies_of(paired, it.rows);
 #pragma unroll 4
         for (; r < rows; r += STEP) {
-          asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(col + r * 128 + (((v & 7) ^ (r & 7)) << 4)),
-                       "l"(src)
-                       : "memory");
+          for (int k = 0; k < copies; ++k)
+            asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(
+                             col + (r + k * (kHalf / copies)) * 128 + (((v & 7) ^ (r & 7)) << 4)),
+                         "l"(src)
+                         : "memory");
           g += STEP;
           src += STEP * a.q_sh;
           while (g >= a.G) g -= a.G, src += over;
@@ -522,17 +897,11 @@ __global__ void __launch_bounds__(kThreads, 1)
   }
   } else {
     // -------------------------------------------------------------- softmax
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 200;");
-    const int j = warp >> 2, quad = warp & 3;
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 208;");
+    const int j = warp >> 2;
     StreamCtrl& c = ctl->s[j];
-    const int tid = threadIdx.x & 127;         // row of the stream's tile
-    const uint32_t lanes = (uint32_t)(quad * 32) << 16;
-    const uint32_t tS = tmem + j * 256 + lanes, tO = tS + 128;
-    const float scale = a.scale_log2;
-    constexpr float kBias = F16 ? 7.f : 0.f;
-    uint32_t n_item = 0, n_tile = 0, n_unit = 0, n_own = 0, n_ring = 0, n_care = 0, n_care2 = 0;
-    bool ok = true;
-    while (ok) {
+    Softmax<D, F16> sm(a, ctl, smem, tmem, j);
+    for (uint32_t n_item = 0;; ++n_item) {
       const int slot = n_item % kItems;
       if (!wait.warp(&c.item_full[slot], (n_item / kItems) & 1)) break;
       const int paired = c.paired[slot];
@@ -540,231 +909,11 @@ __global__ void __launch_bounds__(kThreads, 1)
       const AttnPart it = c.item[slot];
       __syncwarp();
       if (lane == 0) mbar_arrive(&c.item_empty[slot]);
-      ++n_item;
-      const int r = (paired ? j * kHalf : 0) + tid;        // row of the item
-      const bool live = r < it.rows;
-      const bool warp_live = __any_sync(0xffffffffu, live);
-      // keys this row sees, and the first row of the item (fewest)
-      const int sees = it.own ? min(it.len, it.see0 + (it.row0 + r) / a.G + 1) : it.len;
-      const int fewest = it.own ? min(it.len, it.see0 + it.row0 / a.G + 1) : it.len;
-      float m = -INFINITY, l = 0.f;                        // m: reference, bias included
-      uint64_t* fulls = paired ? ctl->full : c.full;
-      for (int t = it.t0; ok && t < it.t1; ++t) {
-        // the value stage (for tiles that need care)
-        const uint32_t n = (paired ? n_ring : n_own) + 1, stages = paired ? RING : NS;
-        const uint32_t v_stage = n % stages;
-        uint8_t* vs = smem + TC::KV_OFF + ((paired ? 0 : j * NS) + v_stage) * TILE;
-        n_ring += paired ? 2 : 0;
-        n_own += paired ? 0 : 2;
-        const bool care = t * kKeys + kKeys > fewest;
-        uint32_t any_bad = 0;
-        const int units = it.len - t * kKeys > kUnit ? 2 : 1;
-        for (int u = 0; u < units; ++u) {
-          const int key0 = t * kKeys + u * kUnit;
-          const uint32_t buf = n_unit & 1, phase = (n_unit >> 1) & 1;
-          const uint32_t tP = tS + buf * kUnit;
-          const bool first_unit = t == it.t0 && u == 0;
-          // the product before this unit's (still running unless waited for)
-          auto o_stable = [&]() -> bool {
-            if (first_unit) return true;
-            const bool done = wait.warp(&c.pv_done[buf ^ 1], ((n_unit - 1) >> 1) & 1);
-            tc_fence_after();
-            return done;
-          };
-          if (!(ok = wait.warp(&c.s_full[buf], phase))) break;
-          tc_fence_after();
-          float s[kUnit];
-          if (warp_live) {
-            tmem_ld32(tP, s);
-            tmem_ld32(tP + 32, s + 32);
-            tmem_wait_ld();
-            if (care) {
-              const int seen = sees - key0;
-#pragma unroll
-              for (int i = 0; i < kUnit; ++i) s[i] = i < seen ? s[i] : -INFINITY;
-            }
-            float m0 = s[0], m1 = s[1], m2 = s[2], m3 = s[3];
-#pragma unroll
-            for (int i = 4; i < kUnit; i += 4) {
-              m0 = fmaxf(m0, s[i]), m1 = fmaxf(m1, s[i + 1]);
-              m2 = fmaxf(m2, s[i + 2]), m3 = fmaxf(m3, s[i + 3]);
-            }
-            const float top = fmaxf(fmaxf(m0, m1), fmaxf(m2, m3)) * scale - kBias;
-            const bool move = top > m + kLazy;
-            if (__any_sync(0xffffffffu, move)) {
-              const float al = move ? ex2(m - top) : 1.f;  // m = -inf: 0
-              if (move) m = top;
-              l *= al;
-              if (!first_unit) {
-                if (!(ok = o_stable())) break;
-#pragma unroll 1
-                for (int i = 0; i < D; i += 32) {
-                  float o[32];
-                  tmem_ld32(tO + i, o);
-                  tmem_wait_ld();
-#pragma unroll
-                  for (int k = 0; k < 32; ++k) o[k] *= al;
-                  tmem_st32(tO + i, o);
-                }
-                tmem_wait_st();
-              }
-            }
-          }
-          const float base = m == -INFINITY ? 0.f : m;
-          if (care) {
-            // a bounded barrier of the softmax warps (of both streams for a pair:
-            // they look at the same rows of the same stage)
-            auto meet = [&]() -> bool {
-              __syncwarp();
-              uint64_t* bar = paired ? &ctl->care : &c.care;
-              uint32_t& n_meet = paired ? n_care2 : n_care;
-              if (lane == 0) mbar_arrive(bar);
-              return wait.warp(bar, n_meet++ & 1);
-            };
-            auto zero_row = [&]() {
-#pragma unroll
-              for (int i = 0; i < NC * 8; ++i)
-                *reinterpret_cast<uint4*>(vs + (i >> 3) * (128 * 128) + tid * 128 + (i & 7) * 16) = make_uint4(0, 0, 0, 0);
-            };
-            uint32_t* bad = c.bad[n_tile & 1];
-            if (u == 0) {
-              // values: rows behind the last key become zero; rows that only some
-              // query rows see are looked at
-              if (!(ok = wait.warp(&fulls[v_stage], (n / stages) & 1))) break;
-              const int valid = min(kKeys, it.len - key0), from = fewest - key0;
-              if (tid >= valid) zero_row();
-              if (from < valid) {
-                bool odd = false;
-                if (tid >= from && tid < valid) {
-                  constexpr uint32_t E = F16 ? 0x7c00u : 0x7f80u;
-#pragma unroll
-                  for (int i = 0; i < NC * 8; ++i) {
-                    const uint4 v = *reinterpret_cast<const uint4*>(vs + (i >> 3) * (128 * 128) + tid * 128 + (i & 7) * 16);
-                    const uint32_t w[4] = {v.x, v.y, v.z, v.w};
-#pragma unroll
-                    for (int q = 0; q < 4; ++q) odd |= (w[q] & E) == E || ((w[q] >> 16) & E) == E;
-                  }
-                }
-                const uint32_t mask = __ballot_sync(0xffffffffu, odd);
-                if (lane == 0) bad[quad] = mask;
-                if (!(ok = meet())) break;
-                any_bad = bad[0] | bad[1] | bad[2] | bad[3];
-              }
-            }
-            if (any_bad != 0) {
-              if (!(ok = o_stable())) break;
-              bool fresh = first_unit;  // O holds nothing yet
-#pragma unroll 1
-              for (int k = u * kUnit; k < u * kUnit + kUnit; ++k) {
-                if (!((bad[k >> 5] >> (k & 31)) & 1)) continue;
-                if (tid == 0 && first_unit) c.accumulate = 1;
-                if (warp_live) {
-                  const float sk = tmem_ld1(tP + (k - u * kUnit));
-                  tmem_wait_ld();
-                  const bool seen = t * kKeys + k < sees;
-                  const float p = seen ? ex2(fmaf(sk, scale, -base)) : 0.f;
-#pragma unroll 1
-                  for (int i = 0; i < D; i += 32) {
-                    float o[32];
-                    tmem_ld32(tO + i, o);
-                    tmem_wait_ld();
-#pragma unroll
-                    for (int q = 0; q < 32; q += 8) {
-                      const int col = i + q;
-                      const uint4 v = *reinterpret_cast<const uint4*>(
-                          vs + (col >> 6) * (128 * 128) + k * 128 + ((((col & 63) >> 3) ^ (k & 7)) << 4));
-                      const uint32_t w[4] = {v.x, v.y, v.z, v.w};
-#pragma unroll
-                      for (int x = 0; x < 4; ++x) {
-                        float lo, hi;
-                        if constexpr (F16) {
-                          const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w[x]));
-                          lo = f.x, hi = f.y;
-                        } else {
-                          lo = bf16_lo(w[x]), hi = bf16_hi(w[x]);
-                        }
-                        const float a0 = fresh ? 0.f : o[q + 2 * x], a1 = fresh ? 0.f : o[q + 2 * x + 1];
-                        o[q + 2 * x] = seen ? fmaf(p, lo, a0) : a0;
-                        o[q + 2 * x + 1] = seen ? fmaf(p, hi, a1) : a1;
-                      }
-                    }
-                    tmem_st32(tO + i, o);
-                    tmem_wait_st();
-                  }
-                }
-                fresh = false;
-              }
-              if (!(ok = meet())) break;  // every row has read them
-              if ((tid >> 6) == u && ((bad[quad] >> lane) & 1)) zero_row();
-            }
-            fence_async_smem();
-          }
-          if (warp_live) {
-            uint32_t p[32];
-            float2 sum0 = make_float2(0.f, 0.f), sum1 = sum0;
-            const float2 sc = make_float2(scale, scale), nb = make_float2(-base, -base);
-            auto weights = [&](auto poly) {
-#pragma unroll
-              for (int i = 0; i < 32; ++i) {
-                float2 x = ffma2(make_float2(s[2 * i], s[2 * i + 1]), sc, nb);
-                if (decltype(poly)::value && i % kPolyEvery == kPolyEvery - 1) {
-                  x = ex2_poly(x);
-                } else {
-                  x.x = ex2(x.x);
-                  x.y = ex2(x.y);
-                }
-                if (i & 1) sum1 = __fadd2_rn(sum1, x);
-                else sum0 = __fadd2_rn(sum0, x);
-                p[i] = pack2<F16>(x.x, x.y);
-              }
-            };
-            if (care) weights(IC<0>{});
-            else weights(IC<1>{});
-            tmem_st32(tP, p);
-            l += (sum0.x + sum0.y) + (sum1.x + sum1.y);
-            tmem_wait_st();
-          }
-          tc_fence_before();
-          __syncwarp();
-          if (lane == 0) mbar_arrive(&c.p_ready[buf]);
-          ++n_unit;
-        }
-        n_tile += care ? 1 : 0;
-      }
-      if (!ok) break;
-      // the part's last product, then its rows out
-      if (!(ok = wait.warp(&c.pv_done[(n_unit - 1) & 1], ((n_unit - 1) >> 1) & 1))) break;
-      tc_fence_after();
-      if (warp_live) {
-        int tok, hq;
-        attn_row(a, it, r, tok, hq);
-        const int64_t row = (int64_t)tok * (a.H * a.G) + hq;
-        // continuation rows: the pairs' of all CTAs, then the streams'
-        const int64_t crow = paired ? (int64_t)blockIdx.x * (2 * kHalf) + r
-                                    : (int64_t)gridDim.x * (2 * kHalf) + (int64_t)(blockIdx.x + j * gridDim.x) * kHalf + r;
-        const int stride = paired ? 2 * kHalf : kHalf;
-        float* dst = it.first ? a.part_o[it.own] + row * D : a.cont_o + crow * D;
-#pragma unroll 1
-        for (int i = 0; i < D; i += 32) {
-          float o[32];
-          tmem_ld32(tO + i, o);
-          tmem_wait_ld();
-          if (live) {
-#pragma unroll
-            for (int k = 0; k < 32; k += 8) store_sector(dst + i + k, o + k);
-          }
-        }
-        if (live) {
-          const float2 ml = make_float2(m, l);
-          if (it.first) {
-            a.part_ml[it.own][row] = ml;
-            a.part_next[it.own][row] = attn_next((int)(crow + stride), it.n_cont, stride);
-          } else {
-            a.cont_ml[crow] = ml;
-          }
-        }
-      }
-      tc_fence_before();
+      const int copies = copies_of(paired, it.rows);
+      if (!(copies == 4   ? sm.template part<4>(it, 0)
+            : copies == 2 ? sm.template part<2>(it, 0)
+                          : sm.template part<1>(it, paired)))
+        break;
     }
   }
   __syncthreads();
@@ -790,7 +939,7 @@ __global__ void __launch_bounds__(kThreads, 1)
 
 template <int D, bool F16>
 int launch(const AttnArgs& a, int sms, cudaStream_t stream) {
-  constexpr int smem = 1024 + TcAttn<D>::CTRL_OFF + (int)sizeof(Ctrl);
+  constexpr int smem = TcAttn<D>::CTRL_OFF + (int)sizeof(Ctrl);
   static_assert(smem <= 227 * 1024, "shared memory");
   auto kern = prefix_attention_tc_kernel<D, F16>;
   cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
@@ -802,8 +951,7 @@ int launch(const AttnArgs& a, int sms, cudaStream_t stream) {
   if (st == GFST_OK) st = make_bf16_map(&mv, a.pool_V, (uint64_t)rows, D, box);
   if (st != GFST_OK) return st;
   const int grid = sms < kAttnMaxGrid ? sms : kAttnMaxGrid;
-  kern<<<grid, kThreads, smem, stream>>>(mk, mv, a, rows);
-  return check_launch("prefix_attention_tc_kernel");
+  return attn_launch("prefix_attention_tc_kernel", kern, grid, kThreads, smem, stream, mk, mv, a, rows);
 }
 
 }  // namespace
