@@ -17,14 +17,14 @@
 // request's positions, up to the last one its rows see.  An item's cost is
 // c0 + w * (number of KT-key tiles).
 //
-// Shares.  All items of a cut, in a fixed order, make one line of cost U;
-// worker c of n takes [U c / n, U (c + 1) / n) and computes the tiles that begin
-// there: any mixture of lengths loads all SMs alike, and a long request is
-// split over many workers without a plan made on the host.  The part of an item
-// that holds its first tile writes to the row's own place (prefix or own); a
-// later part is the first work of its worker, so one continuation buffer per
-// worker is enough.  The row records where its continuations lie: workers
-// first + 1 .. first + n.
+// Shares.  All items of a cut, in a fixed order, make one line of cost; a
+// worker (a CTA, or one of its two streams) takes an interval of it and computes
+// the tiles that begin there: any mixture of lengths loads all SMs alike, and a
+// long request is split over many workers without a plan made on the host.  The
+// part of an item that holds its first tile writes to the row's own place
+// (prefix or own); a later part is the first work of its worker, so one
+// continuation buffer per worker is enough.  The row records where its
+// continuations lie: those of the next workers in order.
 #pragma once
 
 #include "gfst_common.cuh"
@@ -95,7 +95,7 @@ struct AttnPart {
 // tile.  MR is the most rows of an item.
 template <int MR_, int KT_, int C0_, int W_>
 struct AttnCutAll {
-  static constexpr int MR = MR_, KT = KT_, C0 = C0_, W = W_, SHARES = 1;
+  static constexpr int MR = MR_, KT = KT_, C0 = C0_, W = W_;
   __device__ static __forceinline__ int count(int R) { return (R + MR - 1) / MR; }
   __device__ static __forceinline__ int row0(int, int m) { return m * MR; }
   __device__ static __forceinline__ int rows(int R, int m) { return min(MR, R - m * MR); }
@@ -103,7 +103,7 @@ struct AttnCutAll {
 // Items of more than HALF rows, up to two HALF-row tiles that share their keys ...
 template <int HALF, int KT_, int C0_, int W_>
 struct AttnCutPairs {
-  static constexpr int MR = 2 * HALF, KT = KT_, C0 = C0_, W = W_, SHARES = 1;
+  static constexpr int MR = 2 * HALF, KT = KT_, C0 = C0_, W = W_;
   __device__ static __forceinline__ int count(int R) { return R > HALF ? (R - HALF + MR - 1) / MR : 0; }
   __device__ static __forceinline__ int row0(int, int m) { return m * MR; }
   __device__ static __forceinline__ int rows(int R, int m) { return min(MR, R - m * MR); }
@@ -112,17 +112,16 @@ struct AttnCutPairs {
 template <int HALF, int KT_, int C0_, int W_>
 struct AttnCutRest {
   using Pairs = AttnCutPairs<HALF, KT_, C0_, W_>;
-  static constexpr int MR = HALF, KT = KT_, C0 = C0_, W = W_, SHARES = 2;  // shares of a CTA
+  static constexpr int MR = HALF, KT = KT_, C0 = C0_, W = W_;
   __device__ static __forceinline__ int row0(int R, int) { return Pairs::count(R) * 2 * HALF; }
   __device__ static __forceinline__ int rows(int R, int) { return R - row0(R, 0); }
   __device__ static __forceinline__ int count(int R) { return rows(R, 0) > 0 ? 1 : 0; }
 };
 
-// The line of all items of one cut, over n shares.
+// The line of all items of one cut.
 template <class C>
 struct AttnLine {
   int64_t U, prefix_all, prefix_cost;
-  int n;
   int prefix_len, prefix_rows, prefix_mt, prefix_nt;
   // this thread's requests [b0, b1): their cost and the cost before them
   int b0, b1;
@@ -141,10 +140,10 @@ struct AttnLine {
   __device__ static __forceinline__ int64_t head_cost(const AttnRequest& r, int G) {
     int64_t c = 0;
     const int mt = C::count(r.n * G);
+#pragma unroll 1
     for (int m = 0; m < mt; ++m) c += item_cost(own_tiles(r, m, G));
     return c;
   }
-
   // attn_lines() in pieces: the prefix's part; one request; the scan over threads
   __device__ __forceinline__ void begin(const AttnArgs& a, int prefix, int tokens) {
     prefix_len = prefix;
@@ -167,30 +166,22 @@ struct AttnLine {
     if (lane == 31) s_sum[threadIdx.x >> 5] = inc;
     before = prefix_all + inc - sum;
   }
-  __device__ __forceinline__ void scan_block(const int64_t* s_sum, int most_shares) {
+  __device__ __forceinline__ void scan_block(const int64_t* s_sum) {
     const int warp = threadIdx.x >> 5, n_warps = (blockDim.x + 31) >> 5;
     U = prefix_all;
+#pragma unroll 1
     for (int w = 0; w < n_warps; ++w) {
       if (w < warp) before += s_sum[w];
       U += s_sum[w];
     }
-    // no share is smaller than an item's fixed cost and one tile, so every share
-    // between the first and the last of an item holds one of its tiles
-    constexpr int least = C::C0 + C::W;
-    n = U >= (int64_t)most_shares * least ? most_shares : max(1, (int)U / least);
   }
-  // share i is [bound(i), bound(i + 1))
-  __device__ __forceinline__ int64_t bound(int i) const {
-    if (i >= n) return U;
-    return (U >> 22) == 0 ? (int64_t)((uint32_t)U * (uint32_t)i / (uint32_t)n) : U * i / n;  // n <= 640
-  }
-  // Called by every thread: the one whose requests hold the beginning of share
-  // i leaves the request and the cost before it (to be read after a barrier).
-  __device__ void find(const AttnArgs& a, int i, int* s_b, int64_t* s_at) const {
-    const int64_t u = bound(i);
+  // Called by every thread: the one whose requests hold position u leaves the
+  // request and the cost before it (to be read after a barrier).
+  __device__ void find(const AttnArgs& a, int64_t u, int* s_b, int64_t* s_at) const {
     if (u < prefix_all || u < before || u >= before + sum) return;
     int64_t p = before;
     int b = b0;
+#pragma unroll 1
     for (; b < b1; ++b) {
       const int64_t c = head_cost(attn_request(a, b), a.G) * a.H;
       if (u < p + c) break;
@@ -199,23 +190,19 @@ struct AttnLine {
     *s_b = b;
     *s_at = p;
   }
-  // share that holds cost position p
-  __device__ __forceinline__ int share_of(int64_t p) const {
-    return (U >> 22) == 0 ? (int)(((uint32_t)(p + 1) * (uint32_t)n - 1) / (uint32_t)U) : (int)(((p + 1) * n - 1) / U);
-  }
 };
 
 // Sums up one or more lines; called by every thread of the CTA with its own
 // line objects.  One barrier; s_sum (one row a line) may be used again after
 // the caller's next one.
 template <class... C>
-__device__ __forceinline__ void attn_lines(const AttnArgs& a, int64_t (*s_sum)[32], int most_shares,
-                                           AttnLine<C>&... line) {
+__device__ __forceinline__ void attn_lines(const AttnArgs& a, int64_t (*s_sum)[32], AttnLine<C>&... line) {
   const int prefix = attn_prefix_len(a), tokens = attn_tokens(a);
   (line.begin(a, prefix, tokens), ...);
   const int per = (a.B + blockDim.x - 1) / blockDim.x;
   const int b0 = min(a.B, (int)threadIdx.x * per), b1 = min(a.B, b0 + per);
   ((line.b0 = b0, line.b1 = b1), ...);
+#pragma unroll 1
   for (int b = b0; b < b1; ++b) {
     const AttnRequest r = attn_request(a, b);
     (line.add(a, r), ...);
@@ -224,19 +211,70 @@ __device__ __forceinline__ void attn_lines(const AttnArgs& a, int64_t (*s_sum)[3
   (line.scan_warp(s_sum[k++]), ...);
   __syncthreads();
   k = 0;
-  (line.scan_block(s_sum[k++], most_shares * C::SHARES), ...);
+  (line.scan_block(s_sum[k++]), ...);
 }
 
-// Walks share i of a line; the state is the calling thread's.
+// How the lines are shared.  P (pairs, or the only line) and then S (rest) make
+// one line of cost T = P + S over n CTAs: CTA c has [T c / n, T (c + 1) / n), so
+// most CTAs work on one kind only, a pair's rows are split over no more CTAs
+// than its cost needs, and compute-bound and memory-bound work run side by
+// side.  A CTA's part of S is halved over its two streams if a half is at least
+// `least`; CTA cb, the first with a part of S, may have a short one.
+struct AttnShares {
+  int64_t P, T;
+  int n, two, cb, nb;  // nb: workers of CTA cb
+  int least;
+
+  __device__ void init(int64_t p, int64_t s, int grid, int least_p, int least_s, bool streams) {
+    P = p, T = p + s;
+    least = least_s;
+    const int small = p > 0 ? max(least_p, least_s) : least_s;
+    n = T >= (int64_t)grid * small ? grid : max(1, (int)T / small);
+    two = streams && T / n >= 2 * least_s;
+    cb = P < T ? cta_of(P) : n;
+    nb = 1;
+    if (cb < n) nb = two && bound(cb + 1) - P >= 2 * least_s ? 2 : 1;
+  }
+  __device__ __forceinline__ int64_t bound(int i) const {  // n <= 320
+    if (i >= n) return T;
+    return (T >> 22) == 0 ? (int64_t)((uint32_t)T * (uint32_t)i / (uint32_t)n) : T * i / n;
+  }
+  __device__ __forceinline__ int cta_of(int64_t t) const {
+    return (T >> 22) == 0 ? (int)(((uint32_t)(t + 1) * (uint32_t)n - 1) / (uint32_t)T) : (int)(((t + 1) * n - 1) / T);
+  }
+  __device__ __forceinline__ int workers(int c) const { return c == cb ? nb : two ? 2 : 1; }
+  // CTA c's share [u0, u1) of P, in P's positions
+  __device__ __forceinline__ void share_p(int c, int64_t& u0, int64_t& u1) const {
+    u0 = min(bound(c), P), u1 = min(bound(c + 1), P);
+  }
+  // stream j of CTA c: its share of S, in S's positions
+  __device__ __forceinline__ void share_s(int c, int j, int64_t& u0, int64_t& u1) const {
+    const int64_t lo = max(bound(c) - P, (int64_t)0), hi = max(bound(c + 1) - P, (int64_t)0);
+    const int64_t mid = c >= cb && workers(c) == 2 ? lo + (hi - lo) / 2 : hi;
+    u0 = j == 0 ? lo : mid, u1 = j == 0 ? mid : hi;
+  }
+  // number of the worker that holds S's position u, and of a CTA's stream
+  __device__ __forceinline__ int worker(int c, int j) const {
+    return c == cb ? j : nb + (c - cb - 1) * (two ? 2 : 1) + j;
+  }
+  __device__ __forceinline__ int worker_of(int64_t u) const {
+    const int c = cta_of(P + u);
+    int64_t u0, u1;
+    share_s(c, 0, u0, u1);
+    return worker(c, u < u1 ? 0 : 1);
+  }
+};
+
+// Walks a share [u0, u1) of a line; the state is the calling thread's.
 template <class C>
 struct AttnWalk {
   int64_t u0, u1, at;
   int own, b, h, m;
   AttnRequest req;
 
-  __device__ void begin(const AttnArgs& a, const AttnLine<C>& ln, int i, int s_b, int64_t s_at) {
-    u0 = ln.bound(i);
-    u1 = ln.bound(i + 1);
+  __device__ void begin(const AttnArgs& a, const AttnLine<C>& ln, int64_t from, int64_t to, int s_b, int64_t s_at) {
+    u0 = from;
+    u1 = to;
     own = u0 >= ln.prefix_all;
     m = h = b = 0;
     at = 0;
@@ -256,6 +294,7 @@ struct AttnWalk {
       const int64_t hc = ln.head_cost(req, a.G);
       h = (int)((u0 - at) / hc);
       at += hc * h;
+#pragma unroll 1
       for (;;) {
         const int64_t c = ln.item_cost(ln.own_tiles(req, m, a.G));
         if (u0 < at + c) break;
@@ -266,7 +305,10 @@ struct AttnWalk {
   }
 
   // The next part with at least one tile; false at the end of the share.
-  __device__ bool next(const AttnArgs& a, const AttnLine<C>& ln, AttnPart& it) {
+  // share_of(p): number of the worker whose share holds position p.
+  template <class F>
+  __device__ __forceinline__ bool next(const AttnArgs& a, const AttnLine<C>& ln, F&& share_of, AttnPart& it) {
+#pragma unroll 1
     for (;;) {
       if (at >= u1 || (own && b >= a.B)) return false;
       const int R = own ? req.n * a.G : ln.prefix_rows;
@@ -297,7 +339,7 @@ struct AttnWalk {
       it.t1 = tile_from(u1);
       it.first = it.t0 == 0;
       it.n_cont = 0;
-      if (it.first && it.t1 < nt) it.n_cont = ln.share_of(base + (int64_t)(nt - 1) * C::W) - ln.share_of(base);
+      if (it.first && it.t1 < nt) it.n_cont = share_of(base + (int64_t)(nt - 1) * C::W) - share_of(base);
       // step to the next item
       at += ln.item_cost(nt);
       ++m;

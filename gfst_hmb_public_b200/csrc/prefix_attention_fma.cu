@@ -113,14 +113,19 @@ __global__ void __launch_bounds__(kThreads) prefix_attention_fma_kernel(const At
   asm volatile("griddepcontrol.wait;" ::: "memory");
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   AttnLine<Cut> line;
-  attn_lines(a, s_sum, gridDim.x, line);
-  line.find(a, blockIdx.x, &s_b, &s_at);
+  attn_lines(a, s_sum, line);
+  AttnShares shares;
+  shares.init(line.U, 0, gridDim.x, Cut::C0 + Cut::W, Cut::C0 + Cut::W, false);
+  int64_t u0, u1;
+  shares.share_p(blockIdx.x, u0, u1);
+  line.find(a, u0, &s_b, &s_at);
   __syncthreads();
   AttnWalk<Cut> walk;
-  walk.begin(a, line, blockIdx.x, s_b, s_at);
+  walk.begin(a, line, u0, u1, s_b, s_at);
+  auto share_of = [&](int64_t p) { return shares.cta_of(p); };
   AttnPart it;
   bool bad = false;
-  while (walk.next(a, line, it)) {
+  while (walk.next(a, line, share_of, it)) {
     __syncthreads();
     for (int i = tid; i < it.rows * kvr; i += kThreads) {
       const int r = i / kvr;

@@ -57,15 +57,15 @@ constexpr int kProducer = 8, kMma = 10;
 constexpr int kItems = 4;           // parts announced ahead
 constexpr uint32_t kTmemCols = 512; // per stream: S (P over it) 128, O 128
 constexpr float kLazy = 8.f;
-constexpr int kPolyEvery = 8;       // one pair of weights in eight on the FP32 pipe
 
-constexpr int kJoinRows = 16;                       // rows of an item of two copies; half of it of four
+constexpr int kJoinRows = 16;                         // rows of joining copies staged at a time
 constexpr int kStageBytes = 2 * kJoinRows * 128 * 4;  // a stream's rows of joining copies (copies_of)
 
-// An item's fixed cost (queries, first scores, last values, partials out) is
-// that of about two tiles.
-using Pairs = AttnCutPairs<kHalf, kKeys, 2, 1>;
-using Rest = AttnCutRest<kHalf, kKeys, 2, 1>;
+// Costs in units of about 500 cycles of a CTA: a 256-row tile takes about 4000
+// cycles and its item 5000 more (queries in, partials out); of the rest two
+// streams run at once, so a tile counts 1500 and an item 2500.
+using Pairs = AttnCutPairs<kHalf, kKeys, 10, 8>;
+using Rest = AttnCutRest<kHalf, kKeys, 5, 3>;
 
 template <int D>
 struct TcAttn {
@@ -89,7 +89,7 @@ struct StreamCtrl {
   int paired[kItems];          // 1: pair, 0: rest, -1: no more work
   uint32_t bad[2][4];          // value rows that are not finite (one bit each), two tiles in turn
   int accumulate;              // the part's first product adds to O
-  float2 ml[2 * kJoinRows];    // joining copies' references and sums
+  float2 ml[2][32];            // joining copies' references and sums
   int at_b[2];
   int64_t at_u[2];
 };
@@ -102,6 +102,7 @@ struct Ctrl {
   int64_t sum[2][32];
   AttnLine<Pairs> pairs;         // the lines (their common part)
   AttnLine<Rest> rest;
+  AttnShares shares;
   uint32_t tmem;
   int abort;
 };
@@ -110,28 +111,6 @@ __device__ __forceinline__ float ex2(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
-}
-
-// 2^x of two numbers on the FP32 pipe, x <= 127: 2^n times a polynomial of degree
-// 5 in f = x - n in [-1/2, 1/2] (coefficients from an exchange iteration on the
-// relative error: 7.5e-8, 2.1e-7 with the FP32 evaluation).  NaN stays NaN;
-// below 2^-125 the result is 2^-125.
-__device__ __forceinline__ float2 ex2_poly(float2 x) {
-  asm("max.NaN.f32 %0, %0, %1;" : "+f"(x.x) : "f"(-125.f));
-  asm("max.NaN.f32 %0, %0, %1;" : "+f"(x.y) : "f"(-125.f));
-  const float2 magic = make_float2(12582912.f, 12582912.f);  // 1.5 * 2^23: rounds to an integer
-  const float2 t = __fadd2_rn(x, magic);
-  const float2 r = __fadd2_rn(t, make_float2(-12582912.f, -12582912.f));
-  const float2 f = ffma2(r, make_float2(-1.f, -1.f), x);
-  float2 y = make_float2(1.327647245e-03f, 1.327647245e-03f);
-  y = ffma2(y, f, make_float2(9.675540961e-03f, 9.675540961e-03f));
-  y = ffma2(y, f, make_float2(5.550713092e-02f, 5.550713092e-02f));
-  y = ffma2(y, f, make_float2(2.402212024e-01f, 2.402212024e-01f));
-  y = ffma2(y, f, make_float2(6.931469440e-01f, 6.931469440e-01f));
-  y = ffma2(y, f, make_float2(1.000000119e+00f, 1.000000119e+00f));
-  const float2 p2 = make_float2(__uint_as_float((__float_as_uint(t.x) << 23) + 0x3f800000u),
-                                __uint_as_float((__float_as_uint(t.y) << 23) + 0x3f800000u));
-  return __fmul2_rn(y, p2);
 }
 
 template <bool F16>
@@ -257,16 +236,12 @@ struct Waiter {
   }
 };
 
-// An item of few rows would leave three quarters of the softmax threads idle and
-// its one warp with all 64 scores of a unit to exponentiate.  Its rows are laid
-// out C times in the query tile (128 / C rows apart): the products give every
-// copy all scores, copy k takes only its 64 / C keys of each unit (its other
-// weights are 0), and the copies' rows, softmaxes over disjoint keys, are joined
-// when the part ends.  C = 4 up to 8 rows, 2 up to 16: the joining rows then fit
-// what shared memory is left.
-__device__ __forceinline__ int copies_of(int paired, int rows) {
-  return paired || rows > kJoinRows ? 1 : rows > kJoinRows / 2 ? 2 : 4;
-}
+// An item of few rows would leave most softmax threads idle and one warp with all
+// 64 scores of a unit to exponentiate.  Up to 32 rows are laid out twice in the
+// query tile (64 rows apart): the products give both copies all scores, copy k
+// takes only its 32 keys of each unit (its other weights are 0), and the copies'
+// rows, softmaxes over disjoint keys, are joined when the part ends.
+__device__ __forceinline__ int copies_of(int paired, int rows) { return paired || rows > 32 ? 1 : 2; }
 
 // One softmax thread: a row of its stream's tile.
 template <int D, bool F16>
@@ -333,33 +308,22 @@ struct Softmax {
     }
   }
 
-  // N scores (or O columns) at TMEM address t
-  template <int N>
-  __device__ static __forceinline__ void load(uint32_t t, float (&s)[N]) {
-    if constexpr (N == 16) {
-      tmem_ld16(t, s);
-    } else {
-#pragma unroll
-      for (int i = 0; i < N; i += 32) tmem_ld32(t + i, s + i);
-    }
-    tmem_wait_ld();
-  }
-
-  template <int C>
   __device__ __forceinline__ bool part(const AttnPart& it, int paired) {
-    constexpr int N = kUnit / C;                         // keys of a unit that this thread takes
-    const int copy = tid / (kHalf / C);
-    const int key_off = copy * N;
-    const int r = C > 1 ? tid % (kHalf / C) : (paired ? j * kHalf : 0) + tid;  // row of the item
+    const int copies = copies_of(paired, it.rows);
+    const int copy = copies > 1 ? tid >> 6 : 0;
+    const int r = copies > 1 ? tid & 63 : (paired ? j * kHalf : 0) + tid;  // row of the item
     const bool live = r < it.rows;
     const bool warp_live = __any_sync(0xffffffffu, live);
     const float scale = a.scale_log2;
+    // this thread's 32-key halves of a unit
+    const int q0 = copy, q1 = copies > 1 ? copy + 1 : 2;
     // keys this row sees, and the first row of the item (fewest)
     const int sees = it.own ? min(it.len, it.see0 + (it.row0 + r) / a.G + 1) : it.len;
     const int fewest = it.own ? min(it.len, it.see0 + it.row0 / a.G + 1) : it.len;
     const uint32_t stages = paired ? RING : NS;
     uint64_t* fulls = paired ? ctl->full : c.full;
     float m = -INFINITY, l = 0.f;                        // m: reference, bias included
+#pragma unroll 1
     for (int t = it.t0; t < it.t1; ++t) {
       const uint32_t n = (paired ? n_ring : n_own) + 1;  // the value stage (for tiles that need care)
       const uint32_t v_stage = n % stages;
@@ -369,12 +333,12 @@ struct Softmax {
       const bool care = t * kKeys + kKeys > fewest;
       uint32_t any_bad = 0;
       const int units = it.len - t * kKeys > kUnit ? 2 : 1;
+#pragma unroll 1
       for (int u = 0; u < units; ++u, ++n_unit) {
         const uint32_t buf = n_unit & 1;
         const uint32_t tP = tS + buf * kUnit;
         const bool first_unit = t == it.t0 && u == 0;
-        // keys of this thread's N that the row sees
-        const int seen = sees - (t * kKeys + u * kUnit + key_off);
+        const int seen = sees - (t * kKeys + u * kUnit);  // keys of the unit that the row sees
         // O as the products up to the last unit left it (they may still run)
         auto o_stable = [&]() -> bool {
           if (first_unit) return true;
@@ -384,20 +348,26 @@ struct Softmax {
         };
         if (!wait.warp(&c.s_full[buf], (n_unit >> 1) & 1)) return false;
         tc_fence_after();
-        float s[N];
         if (warp_live) {
-          load<N>(tP + key_off, s);
-          if (care) {
+          float top = -INFINITY;
+#pragma unroll 1
+          for (int q = q0; q < q1; ++q) {
+            float s[32];
+            tmem_ld32(tP + q * 32, s);
+            tmem_wait_ld();
+            if (care) {
 #pragma unroll
-            for (int i = 0; i < N; ++i) s[i] = i < seen ? s[i] : -INFINITY;
-          }
-          float m0 = s[0], m1 = s[1], m2 = s[2], m3 = s[3];
+              for (int i = 0; i < 32; ++i) s[i] = q * 32 + i < seen ? s[i] : -INFINITY;
+            }
+            float m0 = s[0], m1 = s[1], m2 = s[2], m3 = s[3];
 #pragma unroll
-          for (int i = 4; i < N; i += 4) {
-            m0 = fmaxf(m0, s[i]), m1 = fmaxf(m1, s[i + 1]);
-            m2 = fmaxf(m2, s[i + 2]), m3 = fmaxf(m3, s[i + 3]);
+            for (int i = 4; i < 32; i += 4) {
+              m0 = fmaxf(m0, s[i]), m1 = fmaxf(m1, s[i + 1]);
+              m2 = fmaxf(m2, s[i + 2]), m3 = fmaxf(m3, s[i + 3]);
+            }
+            top = fmaxf(top, fmaxf(fmaxf(m0, m1), fmaxf(m2, m3)));
           }
-          const float top = fmaxf(fmaxf(m0, m1), fmaxf(m2, m3)) * scale - kBias;
+          top = top * scale - kBias;
           const bool move = live && top > m + kLazy;
           if (__any_sync(0xffffffffu, move)) {
             const float al = move ? ex2(m - top) : 1.f;  // m = -inf: 0
@@ -408,7 +378,8 @@ struct Softmax {
 #pragma unroll 1
               for (int i = 0; i < D; i += 32) {
                 float o[32];
-                load<32>(tO + i, o);
+                tmem_ld32(tO + i, o);
+                tmem_wait_ld();
 #pragma unroll
                 for (int k = 0; k < 32; ++k) o[k] *= al;
                 tmem_st32(tO + i, o);
@@ -430,7 +401,7 @@ struct Softmax {
               bool odd = false;
               if (tid >= from && tid < valid) {
                 constexpr uint32_t E = F16 ? 0x7c00u : 0x7f80u;
-#pragma unroll
+#pragma unroll 1
                 for (int i = 0; i < NC * 8; ++i) {
                   const uint4 v = *reinterpret_cast<const uint4*>(vs + (i >> 3) * (128 * 128) + tid * 128 + (i & 7) * 16);
                   const uint32_t w[4] = {v.x, v.y, v.z, v.w};
@@ -455,8 +426,8 @@ struct Softmax {
               if (warp_live) {
                 const float sk = tmem_ld1(tP + (k - u * kUnit));
                 tmem_wait_ld();
-                const int mine = k - u * kUnit - key_off;
-                const bool add = mine >= 0 && mine < N && mine < seen;
+                const int mine = k - u * kUnit;
+                const bool add = mine >= q0 * 32 && mine < q1 * 32 && mine < seen;
                 add_row(vs, k, add ? ex2(fmaf(sk, scale, -base)) : 0.f, add, fresh);
               }
               fresh = false;
@@ -467,31 +438,33 @@ struct Softmax {
           fence_async_smem();
         }
         if (warp_live) {
-          uint32_t p[N / 2];
           float2 sum0 = make_float2(0.f, 0.f), sum1 = sum0;
           const float2 sc = make_float2(scale, scale), nb = make_float2(-base, -base);
-          auto weights = [&](auto poly) {
+          // weights go over scores already taken
+#pragma unroll 1
+          for (int q = q0; q < q1; ++q) {
+            float s[32];
+            uint32_t p[16];
+            tmem_ld32(tP + q * 32, s);
+            tmem_wait_ld();
+            if (care) {
 #pragma unroll
-            for (int i = 0; i < N / 2; ++i) {
+              for (int i = 0; i < 32; ++i) s[i] = q * 32 + i < seen ? s[i] : -INFINITY;
+            }
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
               float2 x = ffma2(make_float2(s[2 * i], s[2 * i + 1]), sc, nb);
-              if (decltype(poly)::value && i % kPolyEvery == kPolyEvery - 1) {
-                x = ex2_poly(x);
-              } else {
-                x.x = ex2(x.x);
-                x.y = ex2(x.y);
-              }
+              x.x = ex2(x.x);
+              x.y = ex2(x.y);
               if (i & 1) sum1 = __fadd2_rn(sum1, x);
               else sum0 = __fadd2_rn(sum0, x);
               p[i] = pack2<F16>(x.x, x.y);
             }
-          };
-          if (care) weights(IC<0>{});
-          else weights(IC<1>{});
-          tmem_st(tP + copy * (N / 2), p);
-          if constexpr (C > 1) {
-            const uint32_t zero[N / 2] = {};
-#pragma unroll
-            for (int k = 1; k < C; ++k) tmem_st(tP + ((copy + k) % C) * (N / 2), zero);
+            tmem_st16(tP + q * 16, p);
+          }
+          if (copies > 1) {
+            const uint32_t zero[16] = {};
+            tmem_st16(tP + (copy ^ 1) * 16, zero);
           }
           l += (sum0.x + sum0.y) + (sum1.x + sum1.y);
           tmem_wait_st();
@@ -502,95 +475,85 @@ struct Softmax {
       }
       n_tile += care ? 1 : 0;
     }
-    // the part's last product, then its rows out
-    // continuation rows: the pairs' of all CTAs, then the streams'
+    // the part's last product, then its rows out.  Continuation rows: the pairs'
+    // of all CTAs, then the workers' of the rest
     const int64_t crow0 = paired ? (int64_t)blockIdx.x * (2 * kHalf)
-                                 : (int64_t)gridDim.x * (2 * kHalf) + (int64_t)(blockIdx.x + j * gridDim.x) * kHalf;
+                                 : (int64_t)gridDim.x * (2 * kHalf) +
+                                       (int64_t)ctl->shares.worker(blockIdx.x, j) * kHalf;
     const int stride = paired ? 2 * kHalf : kHalf;
-    auto put_ml = [&](int64_t row, int r_, float2 ml) {
+    auto put = [&](int r_, float2 ml, bool write) -> float* {  // a row's (m, l) out; where its values go
+      int tok, hq;
+      attn_row(a, it, r_, tok, hq);
+      const int64_t row = (int64_t)tok * (a.H * a.G) + hq;
       if (it.first) {
-        a.part_ml[it.own][row] = ml;
-        a.part_next[it.own][row] = attn_next((int)(crow0 + r_ + stride), it.n_cont, stride);
-      } else {
-        a.cont_ml[crow0 + r_] = ml;
+        if (write) {
+          a.part_ml[it.own][row] = ml;
+          a.part_next[it.own][row] = attn_next((int)(crow0 + r_ + stride), it.n_cont, stride);
+        }
+        return a.part_o[it.own] + row * D;
       }
+      if (write) a.cont_ml[crow0 + r_] = ml;
+      return a.cont_o + (crow0 + r_) * D;
     };
-    if constexpr (C == 1) {
-      if (!wait.warp(&c.pv_done[(n_unit - 1) & 1], ((n_unit - 1) >> 1) & 1)) return false;
-      tc_fence_after();
+    if (copies > 1) {
+      if (live) c.ml[copy][r] = make_float2(m, l);
+      if (!meet(0)) return false;
+    }
+    if (!wait.warp(&c.pv_done[(n_unit - 1) & 1], ((n_unit - 1) >> 1) & 1)) return false;
+    tc_fence_after();
+    if (copies == 1) {
       if (warp_live) {
-        int tok, hq;
-        attn_row(a, it, r, tok, hq);
-        const int64_t row = (int64_t)tok * (a.H * a.G) + hq;
-        float* dst = it.first ? a.part_o[it.own] + row * D : a.cont_o + (crow0 + r) * D;
+        float* dst = live ? put(r, make_float2(m, l), true) : nullptr;
 #pragma unroll 1
         for (int i = 0; i < D; i += 32) {
           float o[32];
-          load<32>(tO + i, o);
+          tmem_ld32(tO + i, o);
+          tmem_wait_ld();
           if (live) {
 #pragma unroll
             for (int k = 0; k < 32; k += 8) store_sector(dst + i + k, o + k);
           }
         }
-        if (live) put_ml(row, r, make_float2(m, l));
       }
     } else {
-      // the copies' references and sums, then their rows at the largest reference
-      // through shared memory; four warps add them, a row of D values a warp
+      // both copies at the larger reference through shared memory, 16 rows at a
+      // time; the four warps add them, a row of D values a warp
       constexpr int P = D / 4;                           // 16-byte pieces of a row
       float4* st = reinterpret_cast<float4*>(smem + TC::STAGE_OFF + j * kStageBytes);
-      if (live) c.ml[copy * (kJoinRows * 2 / C) + r] = make_float2(m, l);
-      if (!meet(0)) return false;
-      const float2* mls = c.ml;
-      auto at = [&](int k, int r_) { return k * (kJoinRows * 2 / C) + r_; };
-      auto top_of = [&](int r_) {
-        float top = mls[at(0, r_)].x;
-#pragma unroll
-        for (int k = 1; k < C; ++k) top = fmaxf(top, mls[at(k, r_)].x);
-        return top;
-      };
-      if (!wait.warp(&c.pv_done[(n_unit - 1) & 1], ((n_unit - 1) >> 1) & 1)) return false;
-      tc_fence_after();
-      if (warp_live) {
-        const float top = live ? top_of(r) : 0.f;
-        const float f = m == top ? 1.f : ex2(m - top);   // all empty: 1
+      const float top = live ? fmaxf(m, c.ml[copy ^ 1][r].x) : m;
+      const float f = m == top ? 1.f : ex2(m - top);     // both empty: 1
 #pragma unroll 1
-        for (int i = 0; i < D; i += 32) {
-          float o[32];
-          load<32>(tO + i, o);
-          if (live) {
-            float4* dst = st + (copy * it.rows + r) * P;
+      for (int r0 = 0; r0 < it.rows; r0 += kJoinRows) {
+        const bool mine = live && r >= r0 && r < r0 + kJoinRows;
+        if (__any_sync(0xffffffffu, mine)) {
+#pragma unroll 1
+          for (int i = 0; i < D; i += 32) {
+            float o[32];
+            tmem_ld32(tO + i, o);
+            tmem_wait_ld();
+            if (mine) {
+              float4* dst = st + (copy * kJoinRows + r - r0) * P;
 #pragma unroll
-            for (int k = 0; k < 32; k += 4)  // pieces in an order that spreads the rows over the banks
-              dst[((i + k) / 4) ^ (r & 7)] = make_float4(o[k] * f, o[k + 1] * f, o[k + 2] * f, o[k + 3] * f);
+              for (int k = 0; k < 32; k += 4)  // pieces in an order that spreads the rows over the banks
+                dst[((i + k) / 4) ^ (r & 7)] = make_float4(o[k] * f, o[k + 1] * f, o[k + 2] * f, o[k + 3] * f);
+            }
           }
         }
-      }
-      if (!meet(0)) return false;
-      for (int r_ = quad; r_ < it.rows; r_ += 4) {
-        int tok, hq;
-        attn_row(a, it, r_, tok, hq);
-        const int64_t row = (int64_t)tok * (a.H * a.G) + hq;
-        float* dst = it.first ? a.part_o[it.own] + row * D : a.cont_o + (crow0 + r_) * D;
-        if (lane < P) {
-          float4 o = st[r_ * P + (lane ^ (r_ & 7))];
-#pragma unroll
-          for (int k = 1; k < C; ++k) {
-            const float4 v = st[(k * it.rows + r_) * P + (lane ^ (r_ & 7))];
-            o.x += v.x, o.y += v.y, o.z += v.z, o.w += v.w;
+        if (!meet(0)) return false;
+        const int rows = min(kJoinRows, it.rows - r0);
+#pragma unroll 1
+        for (int x = quad; x < rows; x += 4) {
+          const float2 v0 = c.ml[0][r0 + x], v1 = c.ml[1][r0 + x];
+          const float mx = fmaxf(v0.x, v1.x);
+          const float sum = (v0.x == mx ? v0.y : v0.y * ex2(v0.x - mx)) + (v1.x == mx ? v1.y : v1.y * ex2(v1.x - mx));
+          float* dst = put(r0 + x, make_float2(mx, sum), lane == 0);
+          if (lane < P) {
+            const float4 u = st[x * P + (lane ^ (x & 7))], w = st[(kJoinRows + x) * P + (lane ^ (x & 7))];
+            *reinterpret_cast<float4*>(dst + lane * 4) = make_float4(u.x + w.x, u.y + w.y, u.z + w.z, u.w + w.w);
           }
-          *reinterpret_cast<float4*>(dst + lane * 4) = o;
         }
-        if (lane == 0) {
-          const float top = top_of(r_);
-          float sum = 0.f;
-#pragma unroll
-          for (int k = 0; k < C; ++k) {
-            const float2 v = mls[at(k, r_)];
-            sum += v.x == top ? v.y : v.y * ex2(v.x - top);
-          }
-          put_ml(row, r_, make_float2(top, sum));
-        }
+        // the stage, and the sums of the next part, may be written again
+        if (!meet(0)) return false;
       }
     }
     tc_fence_before();
@@ -650,17 +613,24 @@ __global__ void __launch_bounds__(kThreads, 1)
   asm volatile("griddepcontrol.wait;" ::: "memory");
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
 
-  // the work: this CTA's share of the pairs, and one share of the rest per
-  // stream (stream 1's behind all of stream 0's, so few items spread over the SMs)
+  // the work: this CTA's share of the pairs, and its streams' shares of the rest
   {
     AttnLine<Pairs> pl;
     AttnLine<Rest> rl;
-    attn_lines(a, ctl->sum, gridDim.x, pl, rl);
-    pl.find(a, blockIdx.x, &ctl->s[0].at_b[0], &ctl->s[0].at_u[0]);
-    for (int j = 0; j < 2; ++j) rl.find(a, blockIdx.x + j * gridDim.x, &ctl->s[j].at_b[1], &ctl->s[j].at_u[1]);
+    attn_lines(a, ctl->sum, pl, rl);
+    AttnShares sh;
+    sh.init(pl.U, rl.U, gridDim.x, Pairs::C0 + Pairs::W, Rest::C0 + Rest::W, true);
+    int64_t u0, u1;
+    sh.share_p(blockIdx.x, u0, u1);
+    if (u0 < u1) pl.find(a, u0, &ctl->s[0].at_b[0], &ctl->s[0].at_u[0]);
+    for (int j = 0; j < 2; ++j) {
+      sh.share_s(blockIdx.x, j, u0, u1);
+      if (u0 < u1) rl.find(a, u0, &ctl->s[j].at_b[1], &ctl->s[j].at_u[1]);
+    }
     if (threadIdx.x == 0) {
       ctl->pairs = pl;
       ctl->rest = rl;
+      ctl->shares = sh;
     }
   }
   __syncthreads();
@@ -670,10 +640,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   const Waiter wait{&ctl->abort};
   uint32_t issued_own = 0, issued_ring = 0;  // stages filled by this producer (for the drain)
 
-  // the softmax threads hold a row of scores: they take registers from the other
-  // four warps (2 x 128 x 208 + 128 x 88 of the 384 x 168 launched)
   if (warp >= kProducer) {
-  asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
   if (warp < kMma) {
     // ------------------------------------------------------------- producer
     const int j = warp - kProducer;
@@ -692,46 +659,37 @@ __global__ void __launch_bounds__(kThreads, 1)
         c.paired[slot] = paired;
         mbar_arrive(&c.item_full[slot]);
       }
-      if (!wait.warp(&c.q_empty, (n_item & 1) ^ 1)) return false;
-      ++n_item;
-      // query rows of this stream, 16 bytes a copy, swizzled as TMA would
-      const int r_first = paired ? j * kHalf : 0;
-      const int rows = min(kHalf, it.rows - r_first);
-      {
-        // lane: piece `v` of rows r, r + step, ...; token and head are stepped, not divided
-        constexpr int PIECES = D / 8, STEP = 32 / PIECES;
-        const int v = lane % PIECES;
-        int r = lane / PIECES, g, tok, hq;
-        attn_row(a, it, r_first + r, tok, hq);
-        g = hq - it.h * a.G;
-        const uint16_t* src = static_cast<const uint16_t*>(a.Q) + tok * a.q_st + hq * a.q_sh + v * 8;
-        const uint32_t col = smem_u32(sq) + (v >> 3) * (128 * 128);
-        const int64_t over = a.q_st - a.G * a.q_sh;  // to the next token's first head
+      // query rows of this stream: a row a lane, 16 bytes a copy, swizzled as TMA would
+      auto queries = [&]() -> bool {
+        if (!wait.warp(&c.q_empty, (n_item & 1) ^ 1)) return false;
+        const int r_first = paired ? j * kHalf : 0, rows = min(kHalf, it.rows - r_first);
         const int copies = copies_of(paired, it.rows);
-#pragma unroll 4
-        for (; r < rows; r += STEP) {
-          for (int k = 0; k < copies; ++k)
-            asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(
-                             col + (r + k * (kHalf / copies)) * 128 + (((v & 7) ^ (r & 7)) << 4)),
-                         "l"(src)
-                         : "memory");
-          g += STEP;
-          src += STEP * a.q_sh;
-          while (g >= a.G) g -= a.G, src += over;
+#pragma unroll 1
+        for (int r = lane; r < rows; r += 32) {
+          int tok, hq;
+          attn_row(a, it, r_first + r, tok, hq);
+          const uint16_t* src = static_cast<const uint16_t*>(a.Q) + tok * a.q_st + hq * a.q_sh;
+#pragma unroll 1
+          for (int k = 0; k < copies; ++k) {
+            const uint32_t dst = smem_u32(sq) + (r + k * (kHalf / 2)) * 128;
+#pragma unroll
+            for (int v = 0; v < D / 8; ++v)
+              asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(
+                               dst + (v >> 3) * (128 * 128) + (((v & 7) ^ (r & 7)) << 4)),
+                           "l"(src + v * 8)
+                           : "memory");
+          }
         }
-      }
-      asm volatile("cp.async.commit_group;" ::: "memory");
-      bool q_sent = false;
-      auto send_q = [&]() {
         asm volatile("cp.async.wait_all;" ::: "memory");
         fence_async_smem();
         __syncwarp();
         if (lane == 0) mbar_arrive(&c.q_full);
-        q_sent = true;
+        return true;
       };
       if (paired && j == 1) {
-        send_q();
-        return true;
+        const bool sent = queries();
+        ++n_item;
+        return sent;
       }
       const int box = min(a.L, kKeys);         // rows of a copy
       const int boxes = kKeys / box;           // copies of a full tile, one per lane
@@ -779,18 +737,23 @@ __global__ void __launch_bounds__(kThreads, 1)
             for (int ch = 0; ch < NC; ++ch)
               tma_load_2d(dst + ch * (128 * 128) + lane * box * 128, kv ? &tmV : &tmK, full, ch * 64, (int)row);
           }
-          if (!q_sent) send_q();
+          if (kv == 0 && t == it.t0 && !queries()) return false;  // while the first keys are on their way
         }
         row = ahead;
       }
+      ++n_item;
       return true;
     };
 
     AttnPart it;
-    {
+    const AttnShares& sh = ctl->shares;
+    int64_t u0, u1;
+    sh.share_p(blockIdx.x, u0, u1);
+    if (u0 < u1) {
       AttnWalk<Pairs> w;
-      w.begin(a, ctl->pairs, blockIdx.x, ctl->s[0].at_b[0], ctl->s[0].at_u[0]);
-      while (ok && w.next(a, ctl->pairs, it)) ok = part(it, 1);
+      w.begin(a, ctl->pairs, u0, u1, ctl->s[0].at_b[0], ctl->s[0].at_u[0]);
+#pragma unroll 1
+      while (ok && w.next(a, ctl->pairs, [&](int64_t p) { return sh.cta_of(p); }, it)) ok = part(it, 1);
       // the rest's stages lie in the ring: the pairs' products have to be done with it
       if (j == 0) {
         const uint32_t total = issued_ring;
@@ -801,11 +764,12 @@ __global__ void __launch_bounds__(kThreads, 1)
         ok = wait.warp(&ctl->drained, 0);
       }
     }
-    {
+    sh.share_s(blockIdx.x, j, u0, u1);
+    if (u0 < u1) {
       AttnWalk<Rest> w;
-      const int i = blockIdx.x + j * gridDim.x;
-      w.begin(a, ctl->rest, i, c.at_b[1], c.at_u[1]);
-      while (ok && w.next(a, ctl->rest, it)) ok = part(it, 0);
+      w.begin(a, ctl->rest, u0, u1, c.at_b[1], c.at_u[1]);
+#pragma unroll 1
+      while (ok && w.next(a, ctl->rest, [&](int64_t p) { return sh.worker_of(p); }, it)) ok = part(it, 0);
     }
     const int slot = n_item % kItems;
     if (ok && wait.warp(&c.item_empty[slot], ((n_item / kItems) & 1) ^ 1) && lane == 0) {
@@ -897,7 +861,6 @@ __global__ void __launch_bounds__(kThreads, 1)
   }
   } else {
     // -------------------------------------------------------------- softmax
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 208;");
     const int j = warp >> 2;
     StreamCtrl& c = ctl->s[j];
     Softmax<D, F16> sm(a, ctl, smem, tmem, j);
@@ -909,11 +872,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       const AttnPart it = c.item[slot];
       __syncwarp();
       if (lane == 0) mbar_arrive(&c.item_empty[slot]);
-      const int copies = copies_of(paired, it.rows);
-      if (!(copies == 4   ? sm.template part<4>(it, 0)
-            : copies == 2 ? sm.template part<2>(it, 0)
-                          : sm.template part<1>(it, paired)))
-        break;
+      if (!sm.part(it, paired)) break;
     }
   }
   __syncthreads();
