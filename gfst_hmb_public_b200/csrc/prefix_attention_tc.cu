@@ -61,11 +61,12 @@ constexpr float kLazy = 8.f;
 constexpr int kJoinRows = 16;                         // rows of joining copies staged at a time
 constexpr int kStageBytes = 2 * kJoinRows * 128 * 4;  // a stream's rows of joining copies (copies_of)
 
-// Costs in units of about 500 cycles of a CTA: a 256-row tile takes about 4000
-// cycles and its item 5000 more (queries in, partials out); of the rest two
-// streams run at once, so a tile counts 1500 and an item 2500.
-using Pairs = AttnCutPairs<kHalf, kKeys, 10, 8>;
-using Rest = AttnCutRest<kHalf, kKeys, 5, 3>;
+// Costs in units of about 500 cycles of a CTA, from measured parts: a 256-row
+// tile takes about 4200 cycles and its item 16,000 more (queries in, first
+// scores, partials out); of the rest two streams run at once, so a tile of 3400
+// counts 1700 and an item's 8000 count 4000.
+using Pairs = AttnCutPairs<kHalf, kKeys, 30, 8>;
+using Rest = AttnCutRest<kHalf, kKeys, 8, 3>;
 
 template <int D>
 struct TcAttn {
@@ -308,15 +309,16 @@ struct Softmax {
     }
   }
 
+  // C: copies of the rows
+  template <int C>
   __device__ __forceinline__ bool part(const AttnPart& it, int paired) {
-    const int copies = copies_of(paired, it.rows);
+    constexpr int copies = C, N = kUnit / C;              // N: keys of a unit that this thread takes
     const int copy = copies > 1 ? tid >> 6 : 0;
     const int r = copies > 1 ? tid & 63 : (paired ? j * kHalf : 0) + tid;  // row of the item
     const bool live = r < it.rows;
     const bool warp_live = __any_sync(0xffffffffu, live);
     const float scale = a.scale_log2;
-    // this thread's 32-key halves of a unit
-    const int q0 = copy, q1 = copies > 1 ? copy + 1 : 2;
+    const int key_off = copy * N;
     // keys this row sees, and the first row of the item (fewest)
     const int sees = it.own ? min(it.len, it.see0 + (it.row0 + r) / a.G + 1) : it.len;
     const int fewest = it.own ? min(it.len, it.see0 + it.row0 / a.G + 1) : it.len;
@@ -338,7 +340,7 @@ struct Softmax {
         const uint32_t buf = n_unit & 1;
         const uint32_t tP = tS + buf * kUnit;
         const bool first_unit = t == it.t0 && u == 0;
-        const int seen = sees - (t * kKeys + u * kUnit);  // keys of the unit that the row sees
+        const int seen = sees - (t * kKeys + u * kUnit + key_off);  // of this thread's keys, those the row sees
         // O as the products up to the last unit left it (they may still run)
         auto o_stable = [&]() -> bool {
           if (first_unit) return true;
@@ -348,26 +350,25 @@ struct Softmax {
         };
         if (!wait.warp(&c.s_full[buf], (n_unit >> 1) & 1)) return false;
         tc_fence_after();
+        float2 x[N / 2];
         if (warp_live) {
-          float top = -INFINITY;
-#pragma unroll 1
-          for (int q = q0; q < q1; ++q) {
-            float s[32];
-            tmem_ld32(tP + q * 32, s);
-            tmem_wait_ld();
-            if (care) {
+          float s[N];
 #pragma unroll
-              for (int i = 0; i < 32; ++i) s[i] = q * 32 + i < seen ? s[i] : -INFINITY;
-            }
-            float m0 = s[0], m1 = s[1], m2 = s[2], m3 = s[3];
+          for (int q = 0; q < N; q += 32) tmem_ld32(tP + key_off + q, s + q);
+          tmem_wait_ld();
+          if (care) {
 #pragma unroll
-            for (int i = 4; i < 32; i += 4) {
-              m0 = fmaxf(m0, s[i]), m1 = fmaxf(m1, s[i + 1]);
-              m2 = fmaxf(m2, s[i + 2]), m3 = fmaxf(m3, s[i + 3]);
-            }
-            top = fmaxf(top, fmaxf(fmaxf(m0, m1), fmaxf(m2, m3)));
+            for (int i = 0; i < N; ++i) s[i] = i < seen ? s[i] : -INFINITY;
           }
-          top = top * scale - kBias;
+          float m0 = s[0], m1 = s[1], m2 = s[2], m3 = s[3];
+#pragma unroll
+          for (int i = 4; i < N; i += 4) {
+            m0 = fmaxf(m0, s[i]), m1 = fmaxf(m1, s[i + 1]);
+            m2 = fmaxf(m2, s[i + 2]), m3 = fmaxf(m3, s[i + 3]);
+          }
+#pragma unroll
+          for (int i = 0; i < N / 2; ++i) x[i] = make_float2(s[2 * i], s[2 * i + 1]);
+          const float top = fmaxf(fmaxf(m0, m1), fmaxf(m2, m3)) * scale - kBias;
           const bool move = live && top > m + kLazy;
           if (__any_sync(0xffffffffu, move)) {
             const float al = move ? ex2(m - top) : 1.f;  // m = -inf: 0
@@ -426,8 +427,8 @@ struct Softmax {
               if (warp_live) {
                 const float sk = tmem_ld1(tP + (k - u * kUnit));
                 tmem_wait_ld();
-                const int mine = k - u * kUnit;
-                const bool add = mine >= q0 * 32 && mine < q1 * 32 && mine < seen;
+                const int mine = k - u * kUnit - key_off;
+                const bool add = mine >= 0 && mine < N && mine < seen;
                 add_row(vs, k, add ? ex2(fmaf(sk, scale, -base)) : 0.f, add, fresh);
               }
               fresh = false;
@@ -438,31 +439,29 @@ struct Softmax {
           fence_async_smem();
         }
         if (warp_live) {
-          float2 sum0 = make_float2(0.f, 0.f), sum1 = sum0;
           const float2 sc = make_float2(scale, scale), nb = make_float2(-base, -base);
-          // weights go over scores already taken
-#pragma unroll 1
-          for (int q = q0; q < q1; ++q) {
-            float s[32];
-            uint32_t p[16];
-            tmem_ld32(tP + q * 32, s);
-            tmem_wait_ld();
-            if (care) {
 #pragma unroll
-              for (int i = 0; i < 32; ++i) s[i] = q * 32 + i < seen ? s[i] : -INFINITY;
-            }
+          for (int i = 0; i < N / 2; ++i) x[i] = ffma2(x[i], sc, nb);
 #pragma unroll
-            for (int i = 0; i < 16; ++i) {
-              float2 x = ffma2(make_float2(s[2 * i], s[2 * i + 1]), sc, nb);
-              x.x = ex2(x.x);
-              x.y = ex2(x.y);
-              if (i & 1) sum1 = __fadd2_rn(sum1, x);
-              else sum0 = __fadd2_rn(sum0, x);
-              p[i] = pack2<F16>(x.x, x.y);
-            }
-            tmem_st16(tP + q * 16, p);
+          for (int i = 0; i < N / 2; ++i) {
+            x[i].x = ex2(x[i].x);
+            x[i].y = ex2(x[i].y);
           }
-          if (copies > 1) {
+          float2 sum0 = x[0], sum1 = x[1];
+#pragma unroll
+          for (int i = 2; i < N / 2; i += 2) {
+            sum0 = __fadd2_rn(sum0, x[i]);
+            sum1 = __fadd2_rn(sum1, x[i + 1]);
+          }
+          // weights go over scores already taken
+#pragma unroll
+          for (int q = 0; q < N / 2; q += 16) {
+            uint32_t p[16];
+#pragma unroll
+            for (int i = 0; i < 16; ++i) p[i] = pack2<F16>(x[q + i].x, x[q + i].y);
+            tmem_st16(tP + key_off / 2 + q, p);
+          }
+          if constexpr (C > 1) {
             const uint32_t zero[16] = {};
             tmem_st16(tP + (copy ^ 1) * 16, zero);
           }
@@ -495,13 +494,10 @@ struct Softmax {
       if (write) a.cont_ml[crow0 + r_] = ml;
       return a.cont_o + (crow0 + r_) * D;
     };
-    if (copies > 1) {
-      if (live) c.ml[copy][r] = make_float2(m, l);
-      if (!meet(0)) return false;
-    }
+    if (C > 1 && live) c.ml[copy][r] = make_float2(m, l);  // read behind the next meeting
     if (!wait.warp(&c.pv_done[(n_unit - 1) & 1], ((n_unit - 1) >> 1) & 1)) return false;
     tc_fence_after();
-    if (copies == 1) {
+    if constexpr (C == 1) {
       if (warp_live) {
         float* dst = live ? put(r, make_float2(m, l), true) : nullptr;
 #pragma unroll 1
@@ -516,14 +512,14 @@ struct Softmax {
         }
       }
     } else {
-      // both copies at the larger reference through shared memory, 16 rows at a
-      // time; the four warps add them, a row of D values a warp
+      // both copies through shared memory, 16 rows at a time; the four warps join
+      // them at the larger reference, a row of D values a warp.  (The next part
+      // writes the stage and c.ml behind products that wait for all four warps.)
       constexpr int P = D / 4;                           // 16-byte pieces of a row
       float4* st = reinterpret_cast<float4*>(smem + TC::STAGE_OFF + j * kStageBytes);
-      const float top = live ? fmaxf(m, c.ml[copy ^ 1][r].x) : m;
-      const float f = m == top ? 1.f : ex2(m - top);     // both empty: 1
 #pragma unroll 1
       for (int r0 = 0; r0 < it.rows; r0 += kJoinRows) {
+        if (r0 > 0 && !meet(0)) return false;            // the rows before are out
         const bool mine = live && r >= r0 && r < r0 + kJoinRows;
         if (__any_sync(0xffffffffu, mine)) {
 #pragma unroll 1
@@ -535,7 +531,7 @@ struct Softmax {
               float4* dst = st + (copy * kJoinRows + r - r0) * P;
 #pragma unroll
               for (int k = 0; k < 32; k += 4)  // pieces in an order that spreads the rows over the banks
-                dst[((i + k) / 4) ^ (r & 7)] = make_float4(o[k] * f, o[k + 1] * f, o[k + 2] * f, o[k + 3] * f);
+                dst[((i + k) / 4) ^ (r & 7)] = make_float4(o[k], o[k + 1], o[k + 2], o[k + 3]);
             }
           }
         }
@@ -545,15 +541,15 @@ struct Softmax {
         for (int x = quad; x < rows; x += 4) {
           const float2 v0 = c.ml[0][r0 + x], v1 = c.ml[1][r0 + x];
           const float mx = fmaxf(v0.x, v1.x);
-          const float sum = (v0.x == mx ? v0.y : v0.y * ex2(v0.x - mx)) + (v1.x == mx ? v1.y : v1.y * ex2(v1.x - mx));
-          float* dst = put(r0 + x, make_float2(mx, sum), lane == 0);
+          // equal references (both empty: -inf) need no exponential
+          const float f0 = v0.x == mx ? 1.f : ex2(v0.x - mx), f1 = v1.x == mx ? 1.f : ex2(v1.x - mx);
+          float* dst = put(r0 + x, make_float2(mx, fmaf(v0.y, f0, v1.y * f1)), lane == 0);
           if (lane < P) {
             const float4 u = st[x * P + (lane ^ (x & 7))], w = st[(kJoinRows + x) * P + (lane ^ (x & 7))];
-            *reinterpret_cast<float4*>(dst + lane * 4) = make_float4(u.x + w.x, u.y + w.y, u.z + w.z, u.w + w.w);
+            *reinterpret_cast<float4*>(dst + lane * 4) =
+                make_float4(fmaf(u.x, f0, w.x * f1), fmaf(u.y, f0, w.y * f1), fmaf(u.z, f0, w.z * f1), fmaf(u.w, f0, w.w * f1));
           }
         }
-        // the stage, and the sums of the next part, may be written again
-        if (!meet(0)) return false;
       }
     }
     tc_fence_before();
@@ -640,7 +636,10 @@ __global__ void __launch_bounds__(kThreads, 1)
   const Waiter wait{&ctl->abort};
   uint32_t issued_own = 0, issued_ring = 0;  // stages filled by this producer (for the drain)
 
+  // the softmax threads hold 64 scores: they take registers from the other four
+  // warps (2 x 128 x 208 + 128 x 88 of the 384 x 168 launched)
   if (warp >= kProducer) {
+  asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
   if (warp < kMma) {
     // ------------------------------------------------------------- producer
     const int j = warp - kProducer;
@@ -861,6 +860,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   }
   } else {
     // -------------------------------------------------------------- softmax
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 208;");
     const int j = warp >> 2;
     StreamCtrl& c = ctl->s[j];
     Softmax<D, F16> sm(a, ctl, smem, tmem, j);
@@ -872,7 +872,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       const AttnPart it = c.item[slot];
       __syncwarp();
       if (lane == 0) mbar_arrive(&c.item_empty[slot]);
-      if (!sm.part(it, paired)) break;
+      if (!(copies_of(paired, it.rows) > 1 ? sm.template part<2>(it, 0) : sm.template part<1>(it, paired))) break;
     }
   }
   __syncthreads();
