@@ -41,6 +41,7 @@ struct TablesArgs {
   int32_t* n_short;
   int B, W, L, F;
   int64_t n_tokens;
+  int lane_bits;  // lanes of a table row, as a power of two
 };
 
 struct Need {
@@ -54,9 +55,10 @@ __device__ __forceinline__ Need need_of(const TablesArgs& a, int b) {
   const int64_t len = max(a.lens[b], 0);
   const int nw = a.new_lens[b];
   r.add = nw > 0 ? nw : 0;
-  const int64_t held = (len + a.L - 1) / a.L;
-  r.held = (int)min(held, (int64_t)a.W);
-  r.want = nw < 0 ? r.held : (len + r.add + a.L - 1) / a.L;
+  const int held = (int)(((uint32_t)len + (uint32_t)a.L - 1u) / (uint32_t)a.L);  // both below 2^31
+  r.held = min(held, a.W);
+  const int64_t end = len + r.add + a.L - 1;
+  r.want = nw < 0 ? r.held : (end >> 32) == 0 ? (int64_t)((uint32_t)end / (uint32_t)a.L) : end / a.L;
   r.need = nw < 0 ? r.held : (int)min(r.want, (int64_t)a.W);
   r.back = nw < 0 ? r.held : 0;
   return r;
@@ -150,31 +152,54 @@ __global__ void __launch_bounds__(kTablesMaxThreads) block_tables_kernel(const T
     }
   }
 
+  // ring position of `head + offset`, offset < 2 F
+  auto ring_at = [&](int64_t offset) -> int64_t {
+    const int64_t at = head + offset;
+    return at >= a.F ? (at - a.F >= a.F ? at % a.F : at - a.F) : at;
+  };
   // the entry of block j >= held of request b
   auto fresh = [&](int b, int j, int held) -> int32_t {
     const int64_t rank = (int64_t)s_first[b] + j - held;
-    return rank < count ? a.free_ring[(head + rank) % a.F] : -1;
+    return rank < count ? a.free_ring[ring_at(rank)] : -1;
   };
 
-  const int64_t entries = (int64_t)a.B * a.W;
-  for (int64_t i = first; i < entries; i += stride) {
-    const int b = (int)(i / a.W), j = (int)(i - (int64_t)b * a.W);
-    const Need n = need_of(a, b);
-    int32_t v = -1;
-    if (j < n.held) {
-      v = a.tables[i];
-      if (n.back > 0) {
-        const int64_t rank = (int64_t)count + s_back[b] + j;
-        // returned entries past the ring's room (a block listed twice) are dropped
-        if (rank < a.F) a.free_ring[(head + rank) % a.F] = v;
-        v = -1;
+  // Table rows: a group of lanes a row (a power of two near the width, so that
+  // short rows leave few lanes idle), four entries a lane in flight.
+  const int lanes = 1 << a.lane_bits;
+  const int64_t groups = ((int64_t)gridDim.x * blockDim.x) >> a.lane_bits;
+  const int gl = tid & (lanes - 1);
+  for (int64_t b = ((int64_t)blockIdx.x * blockDim.x + tid) >> a.lane_bits; b < a.B; b += groups) {
+    const Need n = need_of(a, (int)b);
+    const int32_t* row = a.tables + b * a.W;
+    int32_t* out = a.tables_out + b * a.W;
+    for (int j0 = gl; j0 < a.W; j0 += 4 * lanes) {
+      int32_t v[4];
+#pragma unroll
+      for (int u = 0; u < 4; ++u) {
+        const int j = j0 + u * lanes;
+        v[u] = -1;
+        if (j >= a.W) continue;
+        if (j < n.held) v[u] = row[j];
+        else if (j < n.need) v[u] = fresh((int)b, j, n.held);
       }
-    } else if (j < n.need) {
-      v = fresh(b, j, n.held);
+#pragma unroll
+      for (int u = 0; u < 4; ++u) {
+        const int j = j0 + u * lanes;
+        if (j >= a.W) continue;
+        if (n.back > 0) {
+          if (j < n.held) {
+            const int64_t rank = (int64_t)count + s_back[b] + j;
+            // returned entries past the ring's room (a block listed twice) are dropped
+            if (rank < a.F) a.free_ring[ring_at(rank)] = v[u];
+          }
+          v[u] = -1;
+        }
+        out[j] = v[u];
+      }
     }
-    a.tables_out[i] = v;
   }
 
+  // Slots: a token a thread, its request found by bisection in shared memory.
   const int total = s_cu[a.B];
   for (int64_t i = first; i < a.n_tokens; i += stride) {
     int32_t slot = -1;
@@ -188,7 +213,7 @@ __global__ void __launch_bounds__(kTablesMaxThreads) block_tables_kernel(const T
       }
       const Need n = need_of(a, lo);
       const int64_t p = (int64_t)max(a.lens[lo], 0) + (i - s_cu[lo]);
-      const int64_t j = p / a.L;
+      const int64_t j = (p >> 32) == 0 ? (int64_t)((uint32_t)p / (uint32_t)a.L) : p / a.L;
       if (j < a.W) {
         const int32_t blk = j < n.held ? a.tables[(int64_t)lo * a.W + j] : fresh(lo, (int)j, n.held);
         if (blk >= 0 && blk < a.F) slot = (int32_t)((int64_t)blk * a.L + (p - j * a.L));
@@ -198,41 +223,57 @@ __global__ void __launch_bounds__(kTablesMaxThreads) block_tables_kernel(const T
   }
 }
 
-// 16-byte vectors of one row group: token t, head h, vector v of the row.  A
-// thread moves kAppendIlp vectors with their loads in flight together.
+// A token's keys and values are H (kv + vv) 16-byte vectors.  A thread keeps its
+// vector (head and piece) and walks tokens, so the only division left is the
+// slot's block (a shift where L is a power of two); kAppendIlp tokens are in
+// flight at once.  A copy: the bytes of K and V read and written bound it.
 constexpr int kAppendIlp = 4;
 constexpr int kAppendThreads = 256;
 
-__global__ void __launch_bounds__(kAppendThreads) paged_append_kernel(
-    const uint4* __restrict__ K, int64_t k_st, int64_t k_sh, const uint4* __restrict__ V, int64_t v_st, int64_t v_sh,
-    uint4* __restrict__ pool_K, uint4* __restrict__ pool_V, const int32_t* __restrict__ slot_map, int64_t n_tokens,
-    int64_t n_slots, int L, int H, int kv, int vv, int64_t k_items, int64_t items) {
-  const int64_t base = (int64_t)blockIdx.x * (kAppendThreads * kAppendIlp) + threadIdx.x;
-  uint4 x[kAppendIlp];
-  uint4* dst[kAppendIlp];
+struct AppendArgs {
+  const uint4* K;
+  const uint4* V;
+  int64_t k_st, k_sh, v_st, v_sh;  // strides in vectors
+  uint4* pool_K;
+  uint4* pool_V;
+  const int32_t* slot_map;
+  int64_t n_tokens, n_slots;
+  int L, shift;       // L == 1 << shift, or shift < 0
+  int H, kv, vv;      // vectors of a key and of a value row
+  int per, abreast;   // vectors of a token; tokens side by side in a CTA
+};
+
+__global__ void __launch_bounds__(kAppendThreads) paged_append_kernel(const AppendArgs a) {
+  const int side = a.abreast > 1 ? (int)threadIdx.x / a.per : 0;
+  const int64_t t0 = (int64_t)blockIdx.x * (a.abreast * kAppendIlp) + side;
+  for (int x = a.abreast > 1 ? (int)threadIdx.x - side * a.per : (int)threadIdx.x; x < a.per && side < a.abreast;
+       x += a.abreast > 1 ? a.per : kAppendThreads) {
+    const bool is_v = x >= a.H * a.kv;
+    const int y = is_v ? x - a.H * a.kv : x, row = is_v ? a.vv : a.kv;
+    const int h = y / row, v = y - h * row;
+    const uint4* src = is_v ? a.V + h * a.v_sh + v : a.K + h * a.k_sh + v;
+    const int64_t st = is_v ? a.v_st : a.k_st;
+    uint4* pool = (is_v ? a.pool_V : a.pool_K) + (int64_t)h * a.L * row + v;
+    const int64_t block = (int64_t)a.H * a.L * row;
+    int slot[kAppendIlp];
+    uint4 d[kAppendIlp];
 #pragma unroll
-  for (int u = 0; u < kAppendIlp; ++u) {
-    const int64_t i = base + u * kAppendThreads;
-    dst[u] = nullptr;
-    if (i >= items) continue;
-    const bool is_v = i >= k_items;
-    const int64_t r = is_v ? i - k_items : i;
-    const int vpr = is_v ? vv : kv;
-    const int64_t row = r / vpr;
-    const int v = (int)(r - row * vpr);
-    const int64_t t = row / H;
-    const int h = (int)(row - t * H);
-    const int64_t slot = slot_map[t];
-    if (slot < 0 || slot >= n_slots) continue;
-    const int64_t blk = slot / L;
-    const int off = (int)(slot - blk * L);
-    const uint4* src = is_v ? V + t * v_st + h * v_sh + v : K + t * k_st + h * k_sh + v;
-    x[u] = __ldg(src);
-    dst[u] = (is_v ? pool_V : pool_K) + ((blk * H + h) * L + off) * vpr + v;
+    for (int u = 0; u < kAppendIlp; ++u) {
+      const int64_t t = t0 + u * a.abreast;
+      slot[u] = t < a.n_tokens ? a.slot_map[t] : -1;
+    }
+#pragma unroll
+    for (int u = 0; u < kAppendIlp; ++u) {
+      if (slot[u] >= a.n_slots) slot[u] = -1;
+      if (slot[u] >= 0) d[u] = __ldg(src + (t0 + u * a.abreast) * st);
+    }
+#pragma unroll
+    for (int u = 0; u < kAppendIlp; ++u) {
+      if (slot[u] < 0) continue;
+      const int blk = a.shift >= 0 ? slot[u] >> a.shift : (int)((uint32_t)slot[u] / (uint32_t)a.L);
+      pool[blk * block + (int64_t)(slot[u] - blk * a.L) * row] = d[u];
+    }
   }
-#pragma unroll
-  for (int u = 0; u < kAppendIlp; ++u)
-    if (dst[u] != nullptr) *dst[u] = x[u];
 }
 
 int sm_count() {
@@ -268,8 +309,10 @@ extern "C" int gfst_block_tables(const int32_t* lens, const int32_t* new_lens, c
                "lens_out and free_state_out must not alias the inputs");
   const int sms = sm_count();
   GFST_REQUIRE(sms > 0, GFST_ERR_DEVICE, "no CUDA device");
+  int lane_bits = 0;
+  while (lane_bits < 5 && (4 << lane_bits) < width) ++lane_bits;
   const TablesArgs a{lens,     new_lens, tables,         free_ring, free_state, tables_out, lens_out, cu_new,
-                     slot_map, free_state_out, n_short, n_requests, width, L, (int)n_blocks, n_tokens};
+                     slot_map, free_state_out, n_short, n_requests, width, L, (int)n_blocks, n_tokens, lane_bits};
   const int threads = n_requests <= 1024 ? 256 : kTablesMaxThreads;
   const int64_t work = (int64_t)n_requests * width + n_tokens;
   // four elements per thread before a CTA more; every CTA repeats the scan
@@ -303,13 +346,17 @@ extern "C" int gfst_paged_append(const void* K, int64_t k_stride_t, int64_t k_st
   GFST_REQUIRE(aligned16(K) && aligned16(V) && aligned16(pool_K) && aligned16(pool_V) && k_stride_t % pv == 0 &&
                    k_stride_h % pv == 0 && v_stride_t % pv == 0 && v_stride_h % pv == 0,
                GFST_ERR_ALIGN, "K, V and the pools need 16-byte aligned rows");
-  const int kv = d / pv, vv = dv / pv;
-  const int64_t k_items = n_tokens * n_heads * kv, items = k_items + n_tokens * n_heads * vv;
-  const int64_t grid = (items + kAppendThreads * kAppendIlp - 1) / (kAppendThreads * kAppendIlp);
-  GFST_REQUIRE(grid < (1LL << 31), GFST_ERR_SHAPE, "too many rows for one launch");
-  paged_append_kernel<<<(unsigned)grid, kAppendThreads, 0, stream>>>(
-      static_cast<const uint4*>(K), k_stride_t / pv, k_stride_h / pv, static_cast<const uint4*>(V), v_stride_t / pv,
-      v_stride_h / pv, static_cast<uint4*>(pool_K), static_cast<uint4*>(pool_V), slot_map, n_tokens, n_blocks * L, L,
-      n_heads, kv, vv, k_items, items);
+  GFST_REQUIRE((int64_t)n_heads * (d + dv) < (1LL << 30), GFST_ERR_SHAPE, "rows of %d heads are too long", n_heads);
+  AppendArgs a;
+  a.K = static_cast<const uint4*>(K), a.V = static_cast<const uint4*>(V);
+  a.k_st = k_stride_t / pv, a.k_sh = k_stride_h / pv, a.v_st = v_stride_t / pv, a.v_sh = v_stride_h / pv;
+  a.pool_K = static_cast<uint4*>(pool_K), a.pool_V = static_cast<uint4*>(pool_V);
+  a.slot_map = slot_map, a.n_tokens = n_tokens, a.n_slots = n_blocks * L;
+  a.L = L, a.shift = (L & (L - 1)) == 0 ? ilog2(L) : -1;
+  a.H = n_heads, a.kv = d / pv, a.vv = dv / pv;
+  a.per = n_heads * (a.kv + a.vv);
+  a.abreast = a.per < kAppendThreads ? kAppendThreads / a.per : 1;
+  const int64_t grid = (n_tokens + a.abreast * kAppendIlp - 1) / (a.abreast * kAppendIlp);
+  paged_append_kernel<<<(unsigned)grid, kAppendThreads, 0, stream>>>(a);
   return check_launch("paged_append_kernel");
 }
