@@ -42,7 +42,13 @@ struct TablesArgs {
   int B, W, L, F;
   int64_t n_tokens;
   int lane_bits;  // lanes of a table row, as a power of two
+  int shift;      // L == 1 << shift, or shift < 0
 };
+
+// v / L for v below 2^32
+__device__ __forceinline__ uint32_t over_L(const TablesArgs& a, uint32_t v) {
+  return a.shift >= 0 ? v >> a.shift : v / (uint32_t)a.L;
+}
 
 struct Need {
   int64_t add;   // new tokens
@@ -55,10 +61,10 @@ __device__ __forceinline__ Need need_of(const TablesArgs& a, int b) {
   const int64_t len = max(a.lens[b], 0);
   const int nw = a.new_lens[b];
   r.add = nw > 0 ? nw : 0;
-  const int held = (int)(((uint32_t)len + (uint32_t)a.L - 1u) / (uint32_t)a.L);  // both below 2^31
+  const int held = (int)over_L(a, (uint32_t)len + (uint32_t)a.L - 1u);  // both below 2^31
   r.held = min(held, a.W);
   const int64_t end = len + r.add + a.L - 1;
-  r.want = nw < 0 ? r.held : (end >> 32) == 0 ? (int64_t)((uint32_t)end / (uint32_t)a.L) : end / a.L;
+  r.want = nw < 0 ? r.held : (end >> 32) == 0 ? (int64_t)over_L(a, (uint32_t)end) : end / a.L;
   r.need = nw < 0 ? r.held : (int)min(r.want, (int64_t)a.W);
   r.back = nw < 0 ? r.held : 0;
   return r;
@@ -80,21 +86,33 @@ __global__ void __launch_bounds__(kTablesMaxThreads) block_tables_kernel(const T
   int32_t* s_cu = sm;               // [B + 1] first packed position of each request
   int32_t* s_first = sm + a.B + 1;  // [B] rank of its first new block
   int32_t* s_back = s_first + a.B;  // [B] rank of its first returned block
-  __shared__ int64_t w_add[32], w_want[32];
-  __shared__ int w_grow[32], w_back[32];
+  __shared__ int64_t w_add[33], w_want[33];  // by warp, then exclusive sums and the total
+  __shared__ int w_grow[33], w_back[33];
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, n_warps = blockDim.x >> 5;
 
-  // thread t owns requests [t * per, (t + 1) * per)
-  const int per = (a.B + blockDim.x - 1) / blockDim.x;
+  const int head = min(max(a.free_state[0], 0), a.F - 1);
+  const int count = min(max(a.free_state[1], 0), a.F);
+  // each request's numbers, a request a thread at a time (coalesced) ...
+  int64_t want = 0;
+#pragma unroll 4
+  for (int b = tid; b < a.B; b += blockDim.x) {
+    const Need n = need_of(a, b);
+    s_cu[b] = (int)n.add;
+    s_first[b] = n.need - n.held;
+    s_back[b] = n.back;
+    want += n.want - n.need;
+  }
+  __syncthreads();
+  // ... and their prefix sums, thread t over requests [t * per, (t + 1) * per)
+  // (an odd run: the threads' reads then fall on different banks)
+  const int per = ((a.B + blockDim.x - 1) / blockDim.x) | 1;
   const int b0 = min(a.B, tid * per), b1 = min(a.B, b0 + per);
-  int64_t add = 0, want = 0;
+  int64_t add = 0;
   int grow = 0, back = 0;
   for (int b = b0; b < b1; ++b) {
-    const Need n = need_of(a, b);
-    add += n.add;
-    grow += n.need - n.held;
-    back += n.back;
-    want += n.want - n.need;
+    add += s_cu[b];
+    grow += s_first[b];
+    back += s_back[b];
   }
   const int64_t i_add = warp_inclusive(add), i_want = warp_inclusive(want);
   const int i_grow = warp_inclusive(grow), i_back = warp_inclusive(back);
@@ -105,35 +123,34 @@ __global__ void __launch_bounds__(kTablesMaxThreads) block_tables_kernel(const T
     w_back[warp] = i_back;
   }
   __syncthreads();
-  int64_t x_add = i_add - add, t_add = 0, t_want = 0;
-  int x_grow = i_grow - grow, x_back = i_back - back, t_grow = 0, t_back = 0;
-  for (int w = 0; w < n_warps; ++w) {
-    if (w < warp) {
-      x_add += w_add[w];
-      x_grow += w_grow[w];
-      x_back += w_back[w];
-    }
-    t_add += w_add[w];
-    t_want += w_want[w];
-    t_grow += w_grow[w];
-    t_back += w_back[w];
+  if (warp == 0) {
+    const bool in = lane < n_warps;
+    const int64_t a0 = in ? w_add[lane] : 0, a1 = in ? w_want[lane] : 0;
+    const int a2 = in ? w_grow[lane] : 0, a3 = in ? w_back[lane] : 0;
+    const int64_t s0 = warp_inclusive(a0), s1 = warp_inclusive(a1);
+    const int s2 = warp_inclusive(a2), s3 = warp_inclusive(a3);
+    w_add[lane] = s0 - a0, w_grow[lane] = s2 - a2, w_back[lane] = s3 - a3;
+    if (lane == 31) w_add[32] = s0, w_want[32] = s1, w_grow[32] = s2, w_back[32] = s3;
   }
+  __syncthreads();
+  int64_t x_add = w_add[warp] + i_add - add;
+  int x_grow = w_grow[warp] + i_grow - grow, x_back = w_back[warp] + i_back - back;
+  const int64_t t_add = w_add[32], t_want = w_want[32];
+  const int t_grow = w_grow[32], t_back = w_back[32];
   // packed positions past the int32 range are past every slot map as well
   auto clamp32 = [](int64_t v) { return (int32_t)min(v, (int64_t)0x7fffffff); };
   for (int b = b0; b < b1; ++b) {
-    const Need n = need_of(a, b);
+    const int na = s_cu[b], ng = s_first[b], nb = s_back[b];
     s_cu[b] = clamp32(x_add);
     s_first[b] = x_grow;
     s_back[b] = x_back;
-    x_add += n.add;
-    x_grow += n.need - n.held;
-    x_back += n.back;
+    x_add += na;
+    x_grow += ng;
+    x_back += nb;
   }
   if (tid == 0) s_cu[a.B] = clamp32(t_add);
   __syncthreads();
 
-  const int head = min(max(a.free_state[0], 0), a.F - 1);
-  const int count = min(max(a.free_state[1], 0), a.F);
   const int taken = min(t_grow, count);
   const int64_t stride = (int64_t)gridDim.x * blockDim.x;
   const int64_t first = (int64_t)blockIdx.x * blockDim.x + tid;
@@ -152,15 +169,22 @@ __global__ void __launch_bounds__(kTablesMaxThreads) block_tables_kernel(const T
     }
   }
 
-  // ring position of `head + offset`, offset < 2 F
-  auto ring_at = [&](int64_t offset) -> int64_t {
-    const int64_t at = head + offset;
-    return at >= a.F ? (at - a.F >= a.F ? at % a.F : at - a.F) : at;
+  // ring position of `head + offset`, offset below F (and F below 2^31)
+  auto ring_at = [&](int offset) -> uint32_t {
+    const uint32_t at = (uint32_t)head + (uint32_t)offset;
+    return at >= (uint32_t)a.F ? at - (uint32_t)a.F : at;
   };
-  // the entry of block j >= held of request b
+  // the entry of block j >= held of request b, j < W
   auto fresh = [&](int b, int j, int held) -> int32_t {
-    const int64_t rank = (int64_t)s_first[b] + j - held;
+    const int rank = s_first[b] + j - held;
     return rank < count ? a.free_ring[ring_at(rank)] : -1;
+  };
+  // slot of position p of request b (held blocks); positions lie below 2^32
+  auto slot_of = [&](int b, int held, uint32_t p) -> int32_t {
+    const uint32_t j = over_L(a, p);
+    if (j >= (uint32_t)a.W) return -1;
+    const int32_t blk = (int)j < held ? a.tables[(int64_t)b * a.W + j] : fresh(b, (int)j, held);
+    return blk >= 0 && blk < a.F ? (int32_t)((uint32_t)blk * (uint32_t)a.L + (p - j * (uint32_t)a.L)) : -1;
   };
 
   // Table rows: a group of lanes a row (a power of two near the width, so that
@@ -190,7 +214,7 @@ __global__ void __launch_bounds__(kTablesMaxThreads) block_tables_kernel(const T
           if (j < n.held) {
             const int64_t rank = (int64_t)count + s_back[b] + j;
             // returned entries past the ring's room (a block listed twice) are dropped
-            if (rank < a.F) a.free_ring[ring_at(rank)] = v[u];
+            if (rank < a.F) a.free_ring[ring_at((int)rank)] = v[u];
           }
           v[u] = -1;
         }
@@ -199,27 +223,53 @@ __global__ void __launch_bounds__(kTablesMaxThreads) block_tables_kernel(const T
     }
   }
 
-  // Slots: a token a thread, its request found by bisection in shared memory.
-  const int total = s_cu[a.B];
-  for (int64_t i = first; i < a.n_tokens; i += stride) {
-    int32_t slot = -1;
-    if (i < total) {
-      // the last request whose first packed position is <= i (idle requests share it with the next one)
-      int lo = 0, hi = a.B;
-      while (hi - lo > 1) {
-        const int mid = (lo + hi) >> 1;
-        if (s_cu[mid] <= i) lo = mid;
-        else hi = mid;
+  // Slots: four tokens in a row a thread (one while there are threads enough), the
+  // last CTAs first, which have the fewest rows.  The first token's request, the
+  // last whose first packed position is not behind it (idle requests share theirs
+  // with the next), is found by bisection in shared memory; the others follow it.
+  const int total = (int)min((int64_t)s_cu[a.B], a.n_tokens);
+  int step0 = 1;
+  while (step0 * 2 < a.B) step0 *= 2;
+  const int run = a.n_tokens > stride ? 4 : 1;
+  const bool vec = run == 4 && (reinterpret_cast<uintptr_t>(a.slot_map) & 15) == 0;
+#pragma unroll 1
+  for (int64_t i0 = (stride - 1 - first) * run; i0 < a.n_tokens; i0 += stride * run) {
+    int32_t slot[4] = {-1, -1, -1, -1};
+    int b = 0, held = 0, end = -1;  // request, its blocks, where its tokens end
+    uint32_t p = 0;
+    if (i0 < total) {
+#pragma unroll 1
+      for (int step = step0; step > 0; step >>= 1) {
+        const int x = b + step;
+        if (x < a.B && s_cu[x] <= (int)i0) b = x;
       }
-      const Need n = need_of(a, lo);
-      const int64_t p = (int64_t)max(a.lens[lo], 0) + (i - s_cu[lo]);
-      const int64_t j = (p >> 32) == 0 ? (int64_t)((uint32_t)p / (uint32_t)a.L) : p / a.L;
-      if (j < a.W) {
-        const int32_t blk = j < n.held ? a.tables[(int64_t)lo * a.W + j] : fresh(lo, (int)j, n.held);
-        if (blk >= 0 && blk < a.F) slot = (int32_t)((int64_t)blk * a.L + (p - j * a.L));
+#pragma unroll
+      for (int u = 0; u < 4; ++u) {
+        const int i = (int)i0 + u;
+        if (i >= total || u >= run) break;
+        if (u == 0 || i >= end) {
+          if (u > 0) {
+            do ++b;
+            while (s_cu[b + 1] <= i);
+          }
+          end = s_cu[b + 1];
+          held = need_of(a, b).held;
+          p = (uint32_t)max(a.lens[b], 0) + (uint32_t)(i - s_cu[b]);
+          slot[u] = slot_of(b, held, p);
+        } else {
+          ++p;
+          const bool same = a.shift >= 0 ? (p & (uint32_t)(a.L - 1)) != 0 : p % (uint32_t)a.L != 0;
+          slot[u] = same ? (slot[u - 1] < 0 ? -1 : slot[u - 1] + 1) : slot_of(b, held, p);
+        }
       }
     }
-    a.slot_map[i] = slot;
+    if (vec && i0 + 4 <= a.n_tokens) {
+      *reinterpret_cast<int4*>(a.slot_map + i0) = make_int4(slot[0], slot[1], slot[2], slot[3]);
+    } else {
+#pragma unroll
+      for (int u = 0; u < 4; ++u)
+        if (u < run && i0 + u < a.n_tokens) a.slot_map[i0 + u] = slot[u];
+    }
   }
 }
 
@@ -312,12 +362,14 @@ extern "C" int gfst_block_tables(const int32_t* lens, const int32_t* new_lens, c
   int lane_bits = 0;
   while (lane_bits < 5 && (4 << lane_bits) < width) ++lane_bits;
   const TablesArgs a{lens,     new_lens, tables,         free_ring, free_state, tables_out, lens_out, cu_new,
-                     slot_map, free_state_out, n_short, n_requests, width, L, (int)n_blocks, n_tokens, lane_bits};
+                     slot_map, free_state_out, n_short, n_requests, width, L, (int)n_blocks, n_tokens, lane_bits,
+                     (L & (L - 1)) == 0 ? ilog2(L) : -1};
   const int threads = n_requests <= 1024 ? 256 : kTablesMaxThreads;
   const int64_t work = (int64_t)n_requests * width + n_tokens;
-  // four elements per thread before a CTA more; every CTA repeats the scan
+  // four elements per thread before a CTA more; every CTA repeats the scan, so one wave
   const int64_t want = (work + 4 * threads - 1) / (4 * threads);
-  const int grid = (int)(want < 2 * sms ? want : 2 * sms);
+  const int64_t wave = (int64_t)sms * (threads < kTablesMaxThreads ? 2 : 1);
+  const int grid = (int)(want < wave ? want : wave);
   const size_t smem = ((size_t)3 * n_requests + 1) * 4;
   if (smem > 48 * 1024) {
     const cudaError_t e = cudaFuncSetAttribute(block_tables_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
