@@ -27,6 +27,8 @@
 // continuations lie: those of the next workers in order.
 #pragma once
 
+#include <atomic>
+
 #include "gfst_common.cuh"
 
 namespace gfst {
@@ -380,6 +382,18 @@ __device__ __forceinline__ void attn_row(const AttnArgs& a, const AttnPart& it, 
   const int t = rg / a.G;
   tok = it.tok0 + t;
   hq = it.h * a.G + rg - t * a.G;
+}
+
+// Largest dynamic shared memory of a kernel, set once per device.
+template <typename K>
+int attn_allow_smem(K kern, int bytes, std::atomic<uint64_t>& done) {
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e == cudaSuccess && dev < 64 && (done.load(std::memory_order_relaxed) >> dev & 1)) return GFST_OK;
+  if (e == cudaSuccess) e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+  GFST_REQUIRE(e == cudaSuccess, GFST_ERR_DEVICE, "cudaFuncSetAttribute: %s", cudaGetErrorString(e));
+  if (dev < 64) done.fetch_or(1ull << dev, std::memory_order_relaxed);
+  return GFST_OK;
 }
 
 // A launch that may begin while the one before it on the stream ends: the

@@ -270,8 +270,9 @@ template <typename T>
 int launch(const AttnArgs& a, int sms, cudaStream_t stream) {
   const FmaLayout ly(a.d, a.dv);
   auto kern = prefix_attention_fma_kernel<T>;
-  cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, FmaLayout(256, 256).bytes);
-  GFST_REQUIRE(e == cudaSuccess, GFST_ERR_DEVICE, "cudaFuncSetAttribute: %s", cudaGetErrorString(e));
+  static std::atomic<uint64_t> allowed{0};
+  const int st = attn_allow_smem(kern, FmaLayout(256, 256).bytes, allowed);
+  if (st != GFST_OK) return st;
   const int per_sm = ly.bytes <= 110 * 1024 ? 2 : 1;
   const int grid = (sms < kAttnMaxGrid ? sms : kAttnMaxGrid) * per_sm;
   return attn_launch("prefix_attention_fma_kernel", kern, grid, kThreads, ly.bytes, stream, a);

@@ -901,12 +901,13 @@ int launch(const AttnArgs& a, int sms, cudaStream_t stream) {
   constexpr int smem = TcAttn<D>::CTRL_OFF + (int)sizeof(Ctrl);
   static_assert(smem <= 227 * 1024, "shared memory");
   auto kern = prefix_attention_tc_kernel<D, F16>;
-  cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
-  GFST_REQUIRE(e == cudaSuccess, GFST_ERR_DEVICE, "cudaFuncSetAttribute: %s", cudaGetErrorString(e));
+  static std::atomic<uint64_t> allowed{0};
+  int st = attn_allow_smem(kern, smem, allowed);
+  if (st != GFST_OK) return st;
   const int64_t rows = a.n_blocks * a.H * a.L;
   CUtensorMap mk, mv;
   const int box = a.L < kKeys ? a.L : kKeys;
-  int st = make_bf16_map(&mk, a.pool_K, (uint64_t)rows, D, box);  // 16-bit elements, copied as they are
+  st = make_bf16_map(&mk, a.pool_K, (uint64_t)rows, D, box);  // 16-bit elements, copied as they are
   if (st == GFST_OK) st = make_bf16_map(&mv, a.pool_V, (uint64_t)rows, D, box);
   if (st != GFST_OK) return st;
   const int grid = sms < kAttnMaxGrid ? sms : kAttnMaxGrid;

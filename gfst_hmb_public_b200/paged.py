@@ -25,6 +25,7 @@ Serving operators: nothing here records gradients.  The reference
 from __future__ import annotations
 
 import ctypes
+import functools
 import math
 from typing import NamedTuple
 
@@ -36,34 +37,68 @@ _DTYPES = {torch.float32: nat.DTYPE_F32, torch.bfloat16: nat.DTYPE_BF16, torch.f
 
 
 def _dtype_code(what: str, *tensors: torch.Tensor) -> int:
-    dtypes = {t.dtype for t in tensors}
-    if len(dtypes) != 1:
-        raise RuntimeError(f"{what}: mixed dtypes {dtypes}")
-    dtype = dtypes.pop()
+    dtype = tensors[0].dtype
+    for t in tensors:
+        if t.dtype != dtype:
+            raise RuntimeError(f"{what}: mixed dtypes {({t.dtype for t in tensors})}")
     if dtype not in _DTYPES:
         raise RuntimeError(f"{what}: unsupported dtype {dtype} (float32, bfloat16 or float16)")
     return _DTYPES[dtype]
 
 
 def _no_grad(what: str, *tensors: torch.Tensor) -> None:
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
-        raise RuntimeError(f"{what} has no backward pass; call it under torch.no_grad()")
+    if torch.is_grad_enabled():
+        for t in tensors:
+            if t.requires_grad:
+                raise RuntimeError(f"{what} has no backward pass; call it under torch.no_grad()")
+
+
+def _cuda(what: str, *tensors: torch.Tensor | None) -> int:
+    """Index of the CUDA device that holds every given tensor; raises as nat.require_cuda does."""
+    first = tensors[0]
+    if isinstance(first, torch.Tensor) and first.is_cuda:
+        index = first.get_device()
+        for t in tensors:
+            if t is not None and not (isinstance(t, torch.Tensor) and t.is_cuda and t.get_device() == index):
+                break
+        else:
+            return index
+    return nat.require_cuda(*tensors, what=what).index
+
+
+def _call(index: int, name: str, *args) -> None:
+    """Entry point ``name`` on device ``index`` and its current stream."""
+    stream = torch.cuda.current_stream(index).cuda_stream
+    if torch.cuda.current_device() == index:
+        nat.call(name, *args, stream)
+    else:
+        with torch.cuda.device(index):
+            nat.call(name, *args, stream)
 
 
 def _int32(what: str, name: str, t: torch.Tensor, shape: tuple) -> torch.Tensor:
     if t.dtype != torch.int32:
         raise RuntimeError(f"{what}: {name} must be int32 (got {t.dtype})")
-    if tuple(t.shape) != shape:
+    if t.shape != shape:
         raise ValueError(f"{what}: {name} has shape {tuple(t.shape)}, expected {shape}")
-    return t.contiguous()
+    return t if t.is_contiguous() else t.contiguous()
 
 
 def _rows(t: torch.Tensor) -> torch.Tensor:
     """t [n, heads, width] with contiguous 16-byte aligned rows (a copy where it has none)."""
     per = 16 // t.element_size()
-    if t.stride(2) == 1 and t.stride(0) % per == 0 and t.stride(1) % per == 0 and t.data_ptr() % 16 == 0:
+    a, b, c = t.stride()
+    if c == 1 and a % per == 0 and b % per == 0 and t.data_ptr() % 16 == 0:
         return t
     return t.contiguous().clone() if t.is_contiguous() else t.contiguous()
+
+
+@functools.lru_cache(maxsize=256)
+def _workspace_bytes(n: int, heads: int, group: int, dv: int) -> int:
+    nbytes = ctypes.c_size_t(0)
+    nat.check(nat.load().gfst_prefix_attention_workspace_bytes(n, heads, group, dv, ctypes.byref(nbytes)),
+              "gfst_prefix_attention_workspace_bytes")
+    return int(nbytes.value)
 
 
 class BlockTables(NamedTuple):
@@ -92,17 +127,19 @@ def block_tables(lens: torch.Tensor, new_lens: torch.Tensor, tables: torch.Tenso
     the sum of the positive new_lens.  ``tables_out`` (may be ``tables``)
     receives the new tables in place of a new tensor.  All int32."""
     what = "block_tables"
-    nat.require_cuda(lens, new_lens, tables, free_ring, free_state, tables_out, what=what)
+    index = _cuda(what, lens, new_lens, tables, free_ring, free_state, tables_out)
     if tables.ndim != 2 or free_ring.ndim != 1:
         raise ValueError("block_tables expects tables [B, W] and free_ring [n_blocks]")
     B, W = tables.shape
+    n = int(n_tokens)
     lens, new_lens = _int32(what, "lens", lens, (B,)), _int32(what, "new_lens", new_lens, (B,))
     free_state = _int32(what, "free_state", free_state, (2,))
     if free_ring.dtype != torch.int32 or not free_ring.is_contiguous():
         raise RuntimeError("block_tables: free_ring must be contiguous int32")
+    if n < 0:
+        raise ValueError(f"block_tables: n_tokens {n} is negative")
     if tables_out is None:
         tables = _int32(what, "tables", tables, (B, W))
-        tables_out = torch.empty_like(tables)
     else:
         if not (tables.is_contiguous() and tables_out.is_contiguous()):
             raise ValueError("block_tables: tables and tables_out must be contiguous")
@@ -111,14 +148,23 @@ def block_tables(lens: torch.Tensor, new_lens: torch.Tensor, tables: torch.Tenso
         a, b, size = tables.data_ptr(), tables_out.data_ptr(), B * W * 4
         if a != b and a < b + size and b < a + size:
             raise ValueError("block_tables: tables_out overlaps tables without being it")
-    new = lambda *shape: torch.empty(shape, dtype=torch.int32, device=lens.device)  # noqa: E731
-    out = BlockTables(tables_out, new(B), new(B + 1), new(int(n_tokens)), new(2), new(1))
-    with torch.cuda.device(lens.device):
-        nat.call("gfst_block_tables", nat.ptr(lens), nat.ptr(new_lens), nat.ptr(tables), nat.ptr(free_ring),
-                 nat.ptr(free_state), B, W, int(block_len), int(free_ring.shape[0]), int(n_tokens),
-                 nat.ptr(out.tables), nat.ptr(out.lens), nat.ptr(out.cu_new), nat.ptr(out.slot_map),
-                 nat.ptr(out.free_state), nat.ptr(out.n_short), nat.stream_of(lens))
-    return out
+    # one buffer for all that is new; the slots first, at an allocation's alignment
+    sizes = [n, B, B + 1, 2, 1]
+    if tables_out is None:
+        sizes.append(B * W)
+    buffer = torch.empty((n + 2 * B + 4 + (B * W if tables_out is None else 0),), dtype=torch.int32,
+                         device=lens.device)
+    cut = torch.split_with_sizes(buffer, sizes)
+    if tables_out is None:
+        tables_out = cut[5].view(B, W)
+    at_slots = buffer.data_ptr()
+    at_lens = at_slots + 4 * n
+    at_cu = at_lens + 4 * B
+    at_state = at_cu + 4 * (B + 1)
+    _call(index, "gfst_block_tables", lens.data_ptr(), new_lens.data_ptr(), tables.data_ptr(), free_ring.data_ptr(),
+          free_state.data_ptr(), B, W, int(block_len), free_ring.shape[0], n, tables_out.data_ptr(), at_lens, at_cu,
+          at_slots, at_state, at_state + 8)
+    return BlockTables(tables_out, cut[1], cut[2], cut[0], cut[3], cut[4])
 
 
 def _check_pools(what: str, pool_K: torch.Tensor, pool_V: torch.Tensor) -> tuple:
@@ -137,19 +183,20 @@ def paged_append(K: torch.Tensor, V: torch.Tensor, pool_K: torch.Tensor, pool_V:
     so is a slot outside the pool; nothing else of the pools changes.  K and V
     may be strided views (a fused projection's output) with 16-byte rows."""
     what = "paged_append"
-    nat.require_cuda(K, V, pool_K, pool_V, slot_map, what=what)
+    index = _cuda(what, K, V, pool_K, pool_V, slot_map)
     n_blocks, H, L, d, dv = _check_pools(what, pool_K, pool_V)
-    if K.ndim != 3 or V.ndim != 3 or tuple(K.shape[1:]) != (H, d) or tuple(V.shape) != (K.shape[0], H, dv):
+    if K.ndim != 3 or V.ndim != 3 or K.shape[1:] != (H, d) or V.shape != (K.shape[0], H, dv):
         raise ValueError(f"paged_append: K{tuple(K.shape)} V{tuple(V.shape)} do not match pools of {H} heads, "
                          f"d={d}, dv={dv}")
     code = _dtype_code(what, K, V, pool_K, pool_V)
     _no_grad(what, K, V, pool_K, pool_V)
-    slot_map = _int32(what, "slot_map", slot_map, (K.shape[0],))
+    n = K.shape[0]
+    slot_map = _int32(what, "slot_map", slot_map, (n,))
     K, V = _rows(K), _rows(V)
-    with torch.cuda.device(K.device):
-        nat.call("gfst_paged_append", nat.ptr(K), K.stride(0), K.stride(1), nat.ptr(V), V.stride(0), V.stride(1),
-                 nat.ptr(pool_K), nat.ptr(pool_V), nat.ptr(slot_map), K.shape[0], n_blocks, L, H, d, dv, code,
-                 nat.stream_of(K))
+    kt, kh, _ = K.stride()
+    vt, vh, _ = V.stride()
+    _call(index, "gfst_paged_append", K.data_ptr(), kt, kh, V.data_ptr(), vt, vh, pool_K.data_ptr(), pool_V.data_ptr(),
+          slot_map.data_ptr(), n, n_blocks, L, H, d, dv, code)
 
 
 def prefix_attention(Q: torch.Tensor, pool_K: torch.Tensor, pool_V: torch.Tensor, tables: torch.Tensor,
@@ -175,13 +222,13 @@ def prefix_attention(Q: torch.Tensor, pool_K: torch.Tensor, pool_V: torch.Tensor
     pool within a request's length reads as zero keys and values and is
     reported by ``_native.check_device_errors``."""
     what = "prefix_attention"
-    nat.require_cuda(Q, pool_K, pool_V, tables, lens, cu_new, prefix_table, prefix_len, out, what=what)
+    index = _cuda(what, Q, pool_K, pool_V, tables, lens, cu_new, prefix_table, prefix_len, out)
     n_blocks, H, L, d, dv = _check_pools(what, pool_K, pool_V)
     if Q.ndim != 3 or Q.shape[2] != d or Q.shape[1] % H != 0 or Q.shape[1] == 0:
         raise ValueError(f"prefix_attention: Q{tuple(Q.shape)} does not match pools of {H} heads, d={d}")
     if tables.ndim != 2:
         raise ValueError("prefix_attention expects tables [B, W]")
-    n, heads = int(Q.shape[0]), int(Q.shape[1])
+    n, heads, _ = Q.shape
     B, W = tables.shape
     if tables.dtype != torch.int32:
         raise RuntimeError("prefix_attention: tables must be int32")
@@ -190,11 +237,12 @@ def prefix_attention(Q: torch.Tensor, pool_K: torch.Tensor, pool_V: torch.Tensor
     lens, cu_new = _int32(what, "lens", lens, (B,)), _int32(what, "cu_new", cu_new, (B + 1,))
     if (prefix_table is None) != (prefix_len is None):
         raise ValueError("prefix_attention: prefix_table and prefix_len go together")
-    P = 0
+    P, p_table, p_len = 0, None, None
     if prefix_table is not None:
-        P = int(prefix_table.numel())
+        P = prefix_table.numel()
         prefix_table = _int32(what, "prefix_table", prefix_table, (P,))
         prefix_len = _int32(what, "prefix_len", prefix_len, (1,))
+        p_table, p_len = prefix_table.data_ptr(), prefix_len.data_ptr()
     code = _dtype_code(what, Q, pool_K, pool_V)
     _no_grad(what, Q, pool_K, pool_V)
     scale = 1.0 / math.sqrt(d) if scale is None else float(scale)
@@ -202,22 +250,18 @@ def prefix_attention(Q: torch.Tensor, pool_K: torch.Tensor, pool_V: torch.Tensor
         raise ValueError(f"prefix_attention: scale {scale} is not finite")
     given = out is not None
     if given:
-        if tuple(out.shape) != (n, heads, dv) or out.dtype != Q.dtype or not out.is_contiguous():
+        if out.shape != (n, heads, dv) or out.dtype != Q.dtype or not out.is_contiguous():
             raise ValueError(f"prefix_attention: out must be contiguous {Q.dtype} [{n}, {heads}, {dv}]")
     else:
         out = torch.empty((n, heads, dv), dtype=Q.dtype, device=Q.device)
     lse = torch.empty((n, heads), dtype=torch.float32, device=Q.device) if return_lse else None
     Q = _rows(Q)
-    nbytes = ctypes.c_size_t(0)
-    lib = nat.load()
-    with torch.cuda.device(Q.device):
-        nat.check(lib.gfst_prefix_attention_workspace_bytes(n, H, heads // H, dv, ctypes.byref(nbytes)),
-                  "gfst_prefix_attention_workspace_bytes")
-        ws = torch.empty((int(nbytes.value),), dtype=torch.uint8, device=Q.device)
-        nat.call("gfst_prefix_attention", nat.ptr(Q), Q.stride(0), Q.stride(1), nat.ptr(pool_K), nat.ptr(pool_V),
-                 n_blocks, L, H, heads // H, d, dv, code, nat.ptr(tables), tables.stride(0), W, nat.ptr(lens),
-                 nat.ptr(cu_new), B, n, nat.ptr(prefix_table), P, nat.ptr(prefix_len), scale, nat.ptr(out),
-                 nat.ptr(lse), 0 if given else 1, nat.ptr(ws), int(ws.numel()), nat.stream_of(Q))
+    qt, qh, _ = Q.stride()
+    nbytes = _workspace_bytes(n, H, heads // H, dv)
+    ws = torch.empty((nbytes,), dtype=torch.uint8, device=Q.device)
+    _call(index, "gfst_prefix_attention", Q.data_ptr(), qt, qh, pool_K.data_ptr(), pool_V.data_ptr(), n_blocks, L, H,
+          heads // H, d, dv, code, tables.data_ptr(), tables.stride(0), W, lens.data_ptr(), cu_new.data_ptr(), B, n,
+          p_table, P, p_len, scale, out.data_ptr(), nat.ptr(lse), 0 if given else 1, ws.data_ptr(), nbytes)
     return out, lse
 
 
