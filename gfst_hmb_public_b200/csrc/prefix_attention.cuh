@@ -93,6 +93,16 @@ struct AttnPart {
   int n_cont;     // continuations of the item (first part only), by workers worker + 1 ..
 };
 
+// floor(x / n) for 0 <= x < 2^62 and an integer n, inv = 1 / n in double: the
+// product is within one of the quotient while that is below 2^50, and costs a
+// tenth of a 64-bit division.
+__device__ __forceinline__ int64_t attn_div(int64_t x, int64_t n, double inv) {
+  int64_t q = (int64_t)((double)x * inv);
+  const int64_t r = x - q * n;
+  q += r < 0 ? -1 : r >= n ? 1 : 0;
+  return q;
+}
+
 // How a group of R rows is cut into items, and what an item costs: C0 + W per
 // tile.  MR is the most rows of an item.
 template <int MR_, int KT_, int C0_, int W_>
@@ -224,26 +234,22 @@ __device__ __forceinline__ void attn_lines(const AttnArgs& a, int64_t (*s_sum)[3
 // `least`; CTA cb, the first with a part of S, may have a short one.
 struct AttnShares {
   int64_t P, T;
+  double inv_n, inv_T;
   int n, two, cb, nb;  // nb: workers of CTA cb
-  int least;
 
-  __device__ void init(int64_t p, int64_t s, int grid, int least_p, int least_s, bool streams) {
+  __device__ __forceinline__ void init(int64_t p, int64_t s, int grid, int least_p, int least_s, bool streams) {
     P = p, T = p + s;
-    least = least_s;
     const int small = p > 0 ? max(least_p, least_s) : least_s;
     n = T >= (int64_t)grid * small ? grid : max(1, (int)T / small);
-    two = streams && T / n >= 2 * least_s;
+    inv_n = 1.0 / n;
+    inv_T = T > 0 ? 1.0 / (double)T : 0.0;
+    two = streams && T >= (int64_t)n * (2 * least_s);
     cb = P < T ? cta_of(P) : n;
     nb = 1;
     if (cb < n) nb = two && bound(cb + 1) - P >= 2 * least_s ? 2 : 1;
   }
-  __device__ __forceinline__ int64_t bound(int i) const {  // n <= 320
-    if (i >= n) return T;
-    return (T >> 22) == 0 ? (int64_t)((uint32_t)T * (uint32_t)i / (uint32_t)n) : T * i / n;
-  }
-  __device__ __forceinline__ int cta_of(int64_t t) const {
-    return (T >> 22) == 0 ? (int)(((uint32_t)(t + 1) * (uint32_t)n - 1) / (uint32_t)T) : (int)(((t + 1) * n - 1) / T);
-  }
+  __device__ __forceinline__ int64_t bound(int i) const { return i >= n ? T : attn_div(T * i, n, inv_n); }
+  __device__ __forceinline__ int cta_of(int64_t t) const { return (int)attn_div((t + 1) * n - 1, T, inv_T); }
   __device__ __forceinline__ int workers(int c) const { return c == cb ? nb : two ? 2 : 1; }
   // CTA c's share [u0, u1) of P, in P's positions
   __device__ __forceinline__ void share_p(int c, int64_t& u0, int64_t& u1) const {
@@ -285,8 +291,8 @@ struct AttnWalk {
       b = a.B;
       at = u1;
     } else if (!own) {
-      const int64_t k = u0 / ln.prefix_cost;
-      h = (int)(k / ln.prefix_mt);
+      const int64_t k = attn_div(u0, ln.prefix_cost, 1.0 / (double)ln.prefix_cost);
+      h = (int)attn_div(k, ln.prefix_mt, 1.0 / ln.prefix_mt);
       m = (int)(k - (int64_t)h * ln.prefix_mt);
       at = k * ln.prefix_cost;
     } else {
@@ -294,7 +300,7 @@ struct AttnWalk {
       at = s_at;
       req = attn_request(a, b);
       const int64_t hc = ln.head_cost(req, a.G);
-      h = (int)((u0 - at) / hc);
+      h = (int)attn_div(u0 - at, hc, 1.0 / (double)hc);
       at += hc * h;
 #pragma unroll 1
       for (;;) {

@@ -155,17 +155,6 @@ __device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t (&r)[16
       "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
       : "memory");
 }
-__device__ __forceinline__ void tmem_st8(uint32_t taddr, const uint32_t (&r)[8]) {
-  asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"r"(taddr), "r"(r[0]),
-               "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7])
-               : "memory");
-}
-template <int N>
-__device__ __forceinline__ void tmem_st(uint32_t taddr, const uint32_t (&r)[N]) {
-  if constexpr (N == 32) tmem_st32(taddr, r);
-  else if constexpr (N == 16) tmem_st16(taddr, r);
-  else tmem_st8(taddr, r);
-}
 __device__ __forceinline__ void tmem_st32(uint32_t taddr, const float (&v)[32]) {
   uint32_t r[32];
 #pragma unroll
@@ -179,13 +168,6 @@ __device__ __forceinline__ float tmem_ld1(uint32_t taddr) {
 }
 __device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 __device__ __forceinline__ void fence_async_smem() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
-
-// 32 bytes (one sector) of a row
-__device__ __forceinline__ void store_sector(float* dst, const float* v) {
-  asm volatile("st.global.v8.f32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(dst), "f"(v[0]), "f"(v[1]), "f"(v[2]),
-               "f"(v[3]), "f"(v[4]), "f"(v[5]), "f"(v[6]), "f"(v[7])
-               : "memory");
-}
 
 // D[tmem] += A[tmem] B[smem]
 __device__ __forceinline__ void umma_ts(uint32_t d, uint32_t a, uint64_t bdesc, uint32_t idesc, uint32_t accumulate) {
@@ -499,15 +481,27 @@ struct Softmax {
     tc_fence_after();
     if constexpr (C == 1) {
       if (warp_live) {
+        // 32 columns of the warp's 32 rows at a time through shared memory, so that
+        // a store writes whole 128-byte lines (four rows) and not 32 sectors
+        float4* st = reinterpret_cast<float4*>(smem + TC::STAGE_OFF + j * kStageBytes) + quad * (32 * 8);
         float* dst = live ? put(r, make_float2(m, l), true) : nullptr;
 #pragma unroll 1
         for (int i = 0; i < D; i += 32) {
           float o[32];
           tmem_ld32(tO + i, o);
           tmem_wait_ld();
-          if (live) {
+          __syncwarp();
 #pragma unroll
-            for (int k = 0; k < 32; k += 8) store_sector(dst + i + k, o + k);
+          for (int k = 0; k < 8; ++k)
+            st[lane * 8 + (k ^ (lane & 7))] = make_float4(o[4 * k], o[4 * k + 1], o[4 * k + 2], o[4 * k + 3]);
+          __syncwarp();
+#pragma unroll
+          for (int k = 0; k < 8; ++k) {
+            const int row = k * 4 + (lane >> 3);
+            float* to = reinterpret_cast<float*>(
+                __shfl_sync(0xffffffffu, reinterpret_cast<unsigned long long>(dst), row));
+            const float4 v = st[row * 8 + ((lane & 7) ^ (row & 7))];
+            if (to != nullptr) *reinterpret_cast<float4*>(to + i + (lane & 7) * 4) = v;
           }
         }
       }
@@ -658,25 +652,31 @@ __global__ void __launch_bounds__(kThreads, 1)
         c.paired[slot] = paired;
         mbar_arrive(&c.item_full[slot]);
       }
-      // query rows of this stream: a row a lane, 16 bytes a copy, swizzled as TMA would
+      // query rows of this stream, swizzled as TMA would: a lane finds a row's place,
+      // then whole rows are copied, D / 8 lanes a row
       auto queries = [&]() -> bool {
         if (!wait.warp(&c.q_empty, (n_item & 1) ^ 1)) return false;
         const int r_first = paired ? j * kHalf : 0, rows = min(kHalf, it.rows - r_first);
         const int copies = copies_of(paired, it.rows);
+        constexpr int PIECES = D / 8, ROWS = 32 / PIECES;  // rows of a step
+        const int v = lane % PIECES, sub = lane / PIECES;
+        const uint32_t col = smem_u32(sq) + (v >> 3) * (128 * 128);
 #pragma unroll 1
-        for (int r = lane; r < rows; r += 32) {
+        for (int r0 = 0; r0 < rows; r0 += 32) {
           int tok, hq;
-          attn_row(a, it, r_first + r, tok, hq);
-          const uint16_t* src = static_cast<const uint16_t*>(a.Q) + tok * a.q_st + hq * a.q_sh;
-#pragma unroll 1
-          for (int k = 0; k < copies; ++k) {
-            const uint32_t dst = smem_u32(sq) + (r + k * (kHalf / 2)) * 128;
-#pragma unroll
-            for (int v = 0; v < D / 8; ++v)
-              asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(
-                               dst + (v >> 3) * (128 * 128) + (((v & 7) ^ (r & 7)) << 4)),
-                           "l"(src + v * 8)
-                           : "memory");
+          attn_row(a, it, r_first + min(r0 + lane, rows - 1), tok, hq);
+          const int64_t at = tok * a.q_st + hq * a.q_sh;
+#pragma unroll 4
+          for (int x = 0; x < 32; x += ROWS) {
+            const int r = r0 + x + sub;
+            const uint16_t* src = static_cast<const uint16_t*>(a.Q) + __shfl_sync(0xffffffffu, at, x + sub) + v * 8;
+            const uint32_t dst = col + r * 128 + (((v & 7) ^ (r & 7)) << 4);
+            if (r < rows) {
+              asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+              if (copies > 1)
+                asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst + (kHalf / 2) * 128), "l"(src)
+                             : "memory");
+            }
           }
         }
         asm volatile("cp.async.wait_all;" ::: "memory");
