@@ -226,50 +226,47 @@ __device__ __forceinline__ void attn_lines(const AttnArgs& a, int64_t (*s_sum)[3
   (line.scan_block(s_sum[k++]), ...);
 }
 
-// How the lines are shared.  P (pairs, or the only line) and then S (rest) make
-// one line of cost T = P + S over n CTAs: CTA c has [T c / n, T (c + 1) / n), so
-// most CTAs work on one kind only, a pair's rows are split over no more CTAs
-// than its cost needs, and compute-bound and memory-bound work run side by
-// side.  A CTA's part of S is halved over its two streams if a half is at least
-// `least`; CTA cb, the first with a part of S, may have a short one.
-struct AttnShares {
-  int64_t P, T;
-  double inv_n, inv_T;
-  int n, two, cb, nb;  // nb: workers of CTA cb
+// Equal shares of a line over n workers: worker i has [U i / n, U (i + 1) / n).
+struct AttnEven {
+  int64_t U;
+  double inv_n, inv_U;
+  int n;
+  __device__ __forceinline__ void init(int64_t u, int workers) {
+    U = u, n = workers;
+    inv_n = 1.0 / max(n, 1);
+    inv_U = U > 0 ? 1.0 / (double)U : 0.0;
+  }
+  __device__ __forceinline__ int64_t bound(int i) const { return i >= n ? U : attn_div(U * i, n, inv_n); }
+  __device__ __forceinline__ int worker_of(int64_t u) const { return (int)attn_div((u + 1) * n - 1, U, inv_U); }
+};
 
-  __device__ __forceinline__ void init(int64_t p, int64_t s, int grid, int least_p, int least_s, bool streams) {
-    P = p, T = p + s;
-    const int small = p > 0 ? max(least_p, least_s) : least_s;
-    n = T >= (int64_t)grid * small ? grid : max(1, (int)T / small);
-    inv_n = 1.0 / n;
-    inv_T = T > 0 ? 1.0 / (double)T : 0.0;
-    two = streams && T >= (int64_t)n * (2 * least_s);
-    cb = P < T ? cta_of(P) : n;
-    nb = 1;
-    if (cb < n) nb = two && bound(cb + 1) - P >= 2 * least_s ? 2 : 1;
+// How the two lines are shared: CTAs [0, pairs.n) take pairs and the others of n
+// the rest, in the ratio of their costs, so that a pair's rows are split over no
+// more CTAs than its cost needs and compute-bound and memory-bound work run side
+// by side.  A CTA of the rest is one worker, or two (its streams) if there is
+// enough.  No share but a line's only one is smaller than `least`, an item's
+// fixed cost and one tile, so every worker between the first and the last of an
+// item holds one of its tiles.
+struct AttnShares {
+  AttnEven pairs, rest;
+  int two;
+
+  __device__ __forceinline__ void init(int64_t P, int64_t S, int grid, int least_p, int least_s) {
+    const int64_t T = P + S;
+    const int least = P > 0 ? max(least_p, least_s) : least_s;
+    const int n = T >= (int64_t)grid * least ? grid : max(1, (int)T / least);
+    // a CTA more than the ratio's whole part once that would leave the pairs' 15 % behind
+    int np = (int)ceil((double)P * n / (double)max(T, (int64_t)1) - 0.15);
+    np = P == 0 ? 0 : S == 0 ? n : min(max(np, 1), max(n - 1, 1));
+    const int ns = S == 0 ? 0 : max(n - np, 1);
+    two = S >= (int64_t)ns * (2 * least_s);
+    pairs.init(P, np);
+    rest.init(S, two ? 2 * ns : ns);
   }
-  __device__ __forceinline__ int64_t bound(int i) const { return i >= n ? T : attn_div(T * i, n, inv_n); }
-  __device__ __forceinline__ int cta_of(int64_t t) const { return (int)attn_div((t + 1) * n - 1, T, inv_T); }
-  __device__ __forceinline__ int workers(int c) const { return c == cb ? nb : two ? 2 : 1; }
-  // CTA c's share [u0, u1) of P, in P's positions
-  __device__ __forceinline__ void share_p(int c, int64_t& u0, int64_t& u1) const {
-    u0 = min(bound(c), P), u1 = min(bound(c + 1), P);
-  }
-  // stream j of CTA c: its share of S, in S's positions
-  __device__ __forceinline__ void share_s(int c, int j, int64_t& u0, int64_t& u1) const {
-    const int64_t lo = max(bound(c) - P, (int64_t)0), hi = max(bound(c + 1) - P, (int64_t)0);
-    const int64_t mid = c >= cb && workers(c) == 2 ? lo + (hi - lo) / 2 : hi;
-    u0 = j == 0 ? lo : mid, u1 = j == 0 ? mid : hi;
-  }
-  // number of the worker that holds S's position u, and of a CTA's stream
-  __device__ __forceinline__ int worker(int c, int j) const {
-    return c == cb ? j : nb + (c - cb - 1) * (two ? 2 : 1) + j;
-  }
-  __device__ __forceinline__ int worker_of(int64_t u) const {
-    const int c = cta_of(P + u);
-    int64_t u0, u1;
-    share_s(c, 0, u0, u1);
-    return worker(c, u < u1 ? 0 : 1);
+  // worker number of stream j of CTA c among the rest, or -1
+  __device__ __forceinline__ int rest_worker(int c, int j) const {
+    const int w = two ? 2 * (c - pairs.n) + j : j == 0 ? c - pairs.n : -1;
+    return c < pairs.n || w >= rest.n ? -1 : w;
   }
 };
 

@@ -114,15 +114,15 @@ __global__ void __launch_bounds__(kThreads) prefix_attention_fma_kernel(const At
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   AttnLine<Cut> line;
   attn_lines(a, s_sum, line);
-  AttnShares shares;
-  shares.init(line.U, 0, gridDim.x, Cut::C0 + Cut::W, Cut::C0 + Cut::W, false);
-  int64_t u0, u1;
-  shares.share_p(blockIdx.x, u0, u1);
+  AttnEven shares;
+  constexpr int least = Cut::C0 + Cut::W;
+  shares.init(line.U, line.U >= (int64_t)gridDim.x * least ? (int)gridDim.x : max(1, (int)line.U / least));
+  const int64_t u0 = shares.bound(blockIdx.x), u1 = shares.bound(blockIdx.x + 1);
   line.find(a, u0, &s_b, &s_at);
   __syncthreads();
   AttnWalk<Cut> walk;
   walk.begin(a, line, u0, u1, s_b, s_at);
-  auto share_of = [&](int64_t p) { return shares.cta_of(p); };
+  auto share_of = [&](int64_t p) { return shares.worker_of(p); };
   AttnPart it;
   bool bad = false;
   while (walk.next(a, line, share_of, it)) {

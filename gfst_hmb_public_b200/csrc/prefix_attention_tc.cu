@@ -91,14 +91,13 @@ struct StreamCtrl {
   uint32_t bad[2][4];          // value rows that are not finite (one bit each), two tiles in turn
   int accumulate;              // the part's first product adds to O
   float2 ml[2][32];            // joining copies' references and sums
-  int at_b[2];
-  int64_t at_u[2];
+  int at_b;                    // where the stream's (the pairs': stream 0's) share begins
+  int64_t at_u;
 };
 struct Ctrl {
   StreamCtrl s[2];
   uint64_t full[8], empty[8];  // the pairs' ring
   uint64_t care;                 // both streams' softmax warps
-  uint64_t drained;              // the pairs are done with the ring
   uint64_t done[2];              // a stream's products are done
   int64_t sum[2][32];
   AttnLine<Pairs> pairs;         // the lines (their common part)
@@ -253,6 +252,21 @@ struct Softmax {
     uint32_t& n = paired ? n_care2 : n_care;
     if (lane == 0) mbar_arrive(bar);
     return wait.warp(bar, n++ & 1);
+  }
+  // A pair's streams tend to reach their exponentials together, share the
+  // special-function units and then leave them idle through the rest (the slow
+  // CTAs of a launch took 650,000 cycles where the others took 450,000).  Warps w
+  // and w + 4, on the same quarter of the SM, take turns instead, stream 0 first:
+  // named barriers of the two warps, 1 + quad for stream 0's turn and 5 + quad
+  // for stream 1's.  A warp that gives up sets the abort flag and gives the turn
+  // on, so the other one never stays in the barrier.
+  __device__ __forceinline__ void turn_give() const {
+    asm volatile("barrier.cta.arrive %0, 64;" ::"r"(1 + (j ^ 1) * 4 + quad) : "memory");
+  }
+  __device__ __forceinline__ bool turn_take() const {
+    if (__any_sync(0xffffffffu, *wait.abort != 0)) return false;
+    asm volatile("barrier.cta.sync %0, 64;" ::"r"(1 + j * 4 + quad) : "memory");
+    return true;
   }
   __device__ __forceinline__ void zero_row(uint8_t* vs) const {
 #pragma unroll
@@ -422,6 +436,7 @@ struct Softmax {
         }
         if (warp_live) {
           const float2 sc = make_float2(scale, scale), nb = make_float2(-base, -base);
+          if (paired && !turn_take()) return false;
 #pragma unroll
           for (int i = 0; i < N / 2; ++i) x[i] = ffma2(x[i], sc, nb);
 #pragma unroll
@@ -435,6 +450,7 @@ struct Softmax {
             sum0 = __fadd2_rn(sum0, x[i]);
             sum1 = __fadd2_rn(sum1, x[i + 1]);
           }
+          if (paired) turn_give();
           // weights go over scores already taken
 #pragma unroll
           for (int q = 0; q < N / 2; q += 16) {
@@ -449,6 +465,9 @@ struct Softmax {
           }
           l += (sum0.x + sum0.y) + (sum1.x + sum1.y);
           tmem_wait_st();
+        } else if (paired) {
+          if (!turn_take()) return false;
+          turn_give();
         }
         tc_fence_before();
         __syncwarp();
@@ -460,7 +479,7 @@ struct Softmax {
     // of all CTAs, then the workers' of the rest
     const int64_t crow0 = paired ? (int64_t)blockIdx.x * (2 * kHalf)
                                  : (int64_t)gridDim.x * (2 * kHalf) +
-                                       (int64_t)ctl->shares.worker(blockIdx.x, j) * kHalf;
+                                       (int64_t)ctl->shares.rest_worker(blockIdx.x, j) * kHalf;
     const int stride = paired ? 2 * kHalf : kHalf;
     auto put = [&](int r_, float2 ml, bool write) -> float* {  // a row's (m, l) out; where its values go
       int tok, hq;
@@ -594,7 +613,6 @@ __global__ void __launch_bounds__(kThreads, 1)
       mbar_init(&ctl->empty[i], 2);  // both streams' products
     }
     mbar_init(&ctl->care, 8);
-    mbar_init(&ctl->drained, 1);
     ctl->abort = 0;
     mbar_init_fence();
   }
@@ -609,13 +627,14 @@ __global__ void __launch_bounds__(kThreads, 1)
     AttnLine<Rest> rl;
     attn_lines(a, ctl->sum, pl, rl);
     AttnShares sh;
-    sh.init(pl.U, rl.U, gridDim.x, Pairs::C0 + Pairs::W, Rest::C0 + Rest::W, true);
-    int64_t u0, u1;
-    sh.share_p(blockIdx.x, u0, u1);
-    if (u0 < u1) pl.find(a, u0, &ctl->s[0].at_b[0], &ctl->s[0].at_u[0]);
-    for (int j = 0; j < 2; ++j) {
-      sh.share_s(blockIdx.x, j, u0, u1);
-      if (u0 < u1) rl.find(a, u0, &ctl->s[j].at_b[1], &ctl->s[j].at_u[1]);
+    sh.init(pl.U, rl.U, gridDim.x, Pairs::C0 + Pairs::W, Rest::C0 + Rest::W);
+    if (blockIdx.x < sh.pairs.n) {
+      pl.find(a, sh.pairs.bound(blockIdx.x), &ctl->s[0].at_b, &ctl->s[0].at_u);
+    } else {
+      for (int j = 0; j < 2; ++j) {
+        const int w = sh.rest_worker(blockIdx.x, j);
+        if (w >= 0) rl.find(a, sh.rest.bound(w), &ctl->s[j].at_b, &ctl->s[j].at_u);
+      }
     }
     if (threadIdx.x == 0) {
       ctl->pairs = pl;
@@ -746,29 +765,16 @@ __global__ void __launch_bounds__(kThreads, 1)
 
     AttnPart it;
     const AttnShares& sh = ctl->shares;
-    int64_t u0, u1;
-    sh.share_p(blockIdx.x, u0, u1);
-    if (u0 < u1) {
+    if (blockIdx.x < sh.pairs.n) {
       AttnWalk<Pairs> w;
-      w.begin(a, ctl->pairs, u0, u1, ctl->s[0].at_b[0], ctl->s[0].at_u[0]);
+      w.begin(a, ctl->pairs, sh.pairs.bound(blockIdx.x), sh.pairs.bound(blockIdx.x + 1), ctl->s[0].at_b, ctl->s[0].at_u);
 #pragma unroll 1
-      while (ok && w.next(a, ctl->pairs, [&](int64_t p) { return sh.cta_of(p); }, it)) ok = part(it, 1);
-      // the rest's stages lie in the ring: the pairs' products have to be done with it
-      if (j == 0) {
-        const uint32_t total = issued_ring;
-        for (uint32_t i = total > RING ? total - RING : 0; ok && i < total; ++i)
-          ok = wait.warp(&ctl->empty[i % RING], (i / RING) & 1);
-        if (lane == 0) mbar_arrive(&ctl->drained);
-      } else if (ok) {
-        ok = wait.warp(&ctl->drained, 0);
-      }
-    }
-    sh.share_s(blockIdx.x, j, u0, u1);
-    if (u0 < u1) {
+      while (ok && w.next(a, ctl->pairs, [&](int64_t p) { return sh.pairs.worker_of(p); }, it)) ok = part(it, 1);
+    } else if (const int i = sh.rest_worker(blockIdx.x, j); i >= 0) {
       AttnWalk<Rest> w;
-      w.begin(a, ctl->rest, u0, u1, c.at_b[1], c.at_u[1]);
+      w.begin(a, ctl->rest, sh.rest.bound(i), sh.rest.bound(i + 1), c.at_b, c.at_u);
 #pragma unroll 1
-      while (ok && w.next(a, ctl->rest, [&](int64_t p) { return sh.worker_of(p); }, it)) ok = part(it, 0);
+      while (ok && w.next(a, ctl->rest, [&](int64_t p) { return sh.rest.worker_of(p); }, it)) ok = part(it, 0);
     }
     const int slot = n_item % kItems;
     if (ok && wait.warp(&c.item_empty[slot], ((n_item / kItems) & 1) ^ 1) && lane == 0) {
@@ -864,16 +870,22 @@ __global__ void __launch_bounds__(kThreads, 1)
     const int j = warp >> 2;
     StreamCtrl& c = ctl->s[j];
     Softmax<D, F16> sm(a, ctl, smem, tmem, j);
+    // pairs: the first turn is stream 0's, and stream 0 takes the one left at the end
+    const bool turns = blockIdx.x < ctl->shares.pairs.n;
+    if (turns && j == 1) sm.turn_give();
+    bool ok = false;
     for (uint32_t n_item = 0;; ++n_item) {
       const int slot = n_item % kItems;
       if (!wait.warp(&c.item_full[slot], (n_item / kItems) & 1)) break;
       const int paired = c.paired[slot];
-      if (paired < 0) break;
+      if ((ok = paired < 0)) break;
       const AttnPart it = c.item[slot];
       __syncwarp();
       if (lane == 0) mbar_arrive(&c.item_empty[slot]);
       if (!(copies_of(paired, it.rows) > 1 ? sm.template part<2>(it, 0) : sm.template part<1>(it, paired))) break;
     }
+    if (turns && !ok) sm.turn_give();
+    if (turns && ok && j == 0) sm.turn_take();
   }
   __syncthreads();
   if (ctl->abort) {
