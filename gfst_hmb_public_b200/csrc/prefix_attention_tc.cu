@@ -103,6 +103,7 @@ struct Ctrl {
   AttnLine<Pairs> pairs;         // the lines (their common part)
   AttnLine<Rest> rest;
   AttnShares shares;
+  int gone[2][4];                // softmax warps of pairs that have left
   uint32_t tmem;
   int abort;
 };
@@ -258,8 +259,9 @@ struct Softmax {
   // CTAs of a launch took 650,000 cycles where the others took 450,000).  Warps w
   // and w + 4, on the same quarter of the SM, take turns instead, stream 0 first:
   // named barriers of the two warps, 1 + quad for stream 0's turn and 5 + quad
-  // for stream 1's.  A warp that gives up sets the abort flag and gives the turn
-  // on, so the other one never stays in the barrier.
+  // for stream 1's (through an mbarrier a handover took 200 cycles more).  A warp
+  // that gives up sets the abort flag and goes on giving turns until the other
+  // one, which looks at the flag before it takes one, has left too (turn_leave).
   __device__ __forceinline__ void turn_give() const {
     asm volatile("barrier.cta.arrive %0, 64;" ::"r"(1 + (j ^ 1) * 4 + quad) : "memory");
   }
@@ -267,6 +269,18 @@ struct Softmax {
     if (__any_sync(0xffffffffu, *wait.abort != 0)) return false;
     asm volatile("barrier.cta.sync %0, 64;" ::"r"(1 + j * 4 + quad) : "memory");
     return true;
+  }
+  // After the pairs; ok: this warp did all its work.  Bounded by a few seconds:
+  // the other warp's waits are.
+  __device__ __forceinline__ void turn_leave(bool ok) const {
+    if (ok && j == 0) ok = turn_take();  // the turn that stream 1 gave last
+    volatile int* gone = &ctl->gone[0][0];
+    if (lane == 0) gone[j * 4 + quad] = 1;
+    for (int i = 0; !ok && i < 4000000; ++i) {
+      if (__any_sync(0xffffffffu, gone[(j ^ 1) * 4 + quad] != 0)) break;
+      turn_give();
+      __nanosleep(1000);
+    }
   }
   __device__ __forceinline__ void zero_row(uint8_t* vs) const {
 #pragma unroll
@@ -613,6 +627,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       mbar_init(&ctl->empty[i], 2);  // both streams' products
     }
     mbar_init(&ctl->care, 8);
+    for (int i = 0; i < 8; ++i) (&ctl->gone[0][0])[i] = 0;
     ctl->abort = 0;
     mbar_init_fence();
   }
@@ -870,7 +885,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     const int j = warp >> 2;
     StreamCtrl& c = ctl->s[j];
     Softmax<D, F16> sm(a, ctl, smem, tmem, j);
-    // pairs: the first turn is stream 0's, and stream 0 takes the one left at the end
+    // pairs: the first turn is stream 0's
     const bool turns = blockIdx.x < ctl->shares.pairs.n;
     if (turns && j == 1) sm.turn_give();
     bool ok = false;
@@ -884,8 +899,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       if (lane == 0) mbar_arrive(&c.item_empty[slot]);
       if (!(copies_of(paired, it.rows) > 1 ? sm.template part<2>(it, 0) : sm.template part<1>(it, paired))) break;
     }
-    if (turns && !ok) sm.turn_give();
-    if (turns && ok && j == 0) sm.turn_take();
+    if (turns) sm.turn_leave(ok);
   }
   __syncthreads();
   if (ctl->abort) {
