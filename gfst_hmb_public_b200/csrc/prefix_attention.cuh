@@ -15,7 +15,7 @@
 // read once for MR queries and not once per request.  An own item is MR rows
 // of one request and KV head (row = (token - first) * G + g) against that
 // request's positions, up to the last one its rows see.  An item's cost is
-// c0 + w * (number of KT-key tiles).
+// c0 + w * (number of KT-key tiles), w by its rows.
 //
 // Shares.  All items of a cut, in a fixed order, make one line of cost; a
 // worker (a CTA, or one of its two streams) takes an interval of it and computes
@@ -103,11 +103,16 @@ __device__ __forceinline__ int64_t attn_div(int64_t x, int64_t n, double inv) {
   return q;
 }
 
-// How a group of R rows is cut into items, and what an item costs: C0 + W per
-// tile.  MR is the most rows of an item.
+// How a group of R rows is cut into items, and what an item costs: C0 + weight()
+// per tile, which is at most W.  MR is the most rows of an item.  (Here items of
+// up to four rows weigh 1 where `few` rows have a way of their own, and others
+// the more the more rows they have.)
 template <int MR_, int KT_, int C0_, int W_>
 struct AttnCutAll {
   static constexpr int MR = MR_, KT = KT_, C0 = C0_, W = W_;
+  __device__ static __forceinline__ int weight(int rows, int few) {
+    return few && rows <= 4 ? 1 : min(W, 2 + rows * W / MR * 3 / 4);
+  }
   __device__ static __forceinline__ int count(int R) { return (R + MR - 1) / MR; }
   __device__ static __forceinline__ int row0(int, int m) { return m * MR; }
   __device__ static __forceinline__ int rows(int R, int m) { return min(MR, R - m * MR); }
@@ -116,6 +121,7 @@ struct AttnCutAll {
 template <int HALF, int KT_, int C0_, int W_>
 struct AttnCutPairs {
   static constexpr int MR = 2 * HALF, KT = KT_, C0 = C0_, W = W_;
+  __device__ static __forceinline__ int weight(int, int) { return W; }
   __device__ static __forceinline__ int count(int R) { return R > HALF ? (R - HALF + MR - 1) / MR : 0; }
   __device__ static __forceinline__ int row0(int, int m) { return m * MR; }
   __device__ static __forceinline__ int rows(int R, int m) { return min(MR, R - m * MR); }
@@ -125,6 +131,7 @@ template <int HALF, int KT_, int C0_, int W_>
 struct AttnCutRest {
   using Pairs = AttnCutPairs<HALF, KT_, C0_, W_>;
   static constexpr int MR = HALF, KT = KT_, C0 = C0_, W = W_;
+  __device__ static __forceinline__ int weight(int, int) { return W; }
   __device__ static __forceinline__ int row0(int R, int) { return Pairs::count(R) * 2 * HALF; }
   __device__ static __forceinline__ int rows(int R, int) { return R - row0(R, 0); }
   __device__ static __forceinline__ int count(int R) { return rows(R, 0) > 0 ? 1 : 0; }
@@ -134,11 +141,12 @@ struct AttnCutRest {
 template <class C>
 struct AttnLine {
   int64_t U, prefix_all, prefix_cost;
-  int prefix_len, prefix_rows, prefix_mt, prefix_nt;
+  int prefix_len, prefix_rows, prefix_mt, prefix_nt, few;
   // this thread's requests [b0, b1): their cost and the cost before them
   int b0, b1;
   int64_t before, sum;
 
+  __device__ __forceinline__ int prefix_w_rows() const { return min(C::MR, prefix_rows); }
   __device__ static __forceinline__ int tiles(int len) { return max(1, (len + C::KT - 1) / C::KT); }
   // positions that the rows up to `last_row` of a request see between them
   __device__ static __forceinline__ int see(const AttnRequest& r, int last_row, int G) {
@@ -148,21 +156,28 @@ struct AttnLine {
     const int R = r.n * G;
     return tiles(see(r, C::row0(R, m) + C::rows(R, m) - 1, G));
   }
-  __device__ static __forceinline__ int64_t item_cost(int nt) { return C::C0 + (int64_t)C::W * nt; }
-  __device__ static __forceinline__ int64_t head_cost(const AttnRequest& r, int G) {
+  // cost of an item of nt tiles and of `rows` rows (the prefix's items all count as their first)
+  __device__ __forceinline__ int64_t item_cost(int nt, int rows) const {
+    return C::C0 + (int64_t)C::weight(rows, few) * nt;
+  }
+  __device__ __forceinline__ int64_t own_cost(const AttnRequest& r, int m, int G) const {
+    return item_cost(own_tiles(r, m, G), C::rows(r.n * G, m));
+  }
+  __device__ __forceinline__ int64_t head_cost(const AttnRequest& r, int G) const {
     int64_t c = 0;
     const int mt = C::count(r.n * G);
 #pragma unroll 1
-    for (int m = 0; m < mt; ++m) c += item_cost(own_tiles(r, m, G));
+    for (int m = 0; m < mt; ++m) c += own_cost(r, m, G);
     return c;
   }
   // attn_lines() in pieces: the prefix's part; one request; the scan over threads
   __device__ __forceinline__ void begin(const AttnArgs& a, int prefix, int tokens) {
+    few = a.d <= 128 && a.dv <= 128;
     prefix_len = prefix;
     prefix_rows = prefix > 0 ? tokens * a.G : 0;
     prefix_mt = C::count(prefix_rows);
     prefix_nt = tiles(prefix_len);
-    prefix_cost = item_cost(prefix_nt);
+    prefix_cost = item_cost(prefix_nt, prefix_w_rows());
     prefix_all = prefix_cost * prefix_mt * a.H;
     sum = 0;
   }
@@ -301,7 +316,7 @@ struct AttnWalk {
       at += hc * h;
 #pragma unroll 1
       for (;;) {
-        const int64_t c = ln.item_cost(ln.own_tiles(req, m, a.G));
+        const int64_t c = ln.own_cost(req, m, a.G);
         if (u0 < at + c) break;
         at += c;
         ++m;
@@ -335,18 +350,20 @@ struct AttnWalk {
         it.see0 = req.len - req.n;
         nt = ln.tiles(it.len);
       }
-      // tile j begins at cost position base + j * W
+      // tile j begins at cost position base + j * w
+      const int w_rows = own ? it.rows : ln.prefix_w_rows();
+      const int w = C::weight(w_rows, ln.few);
       const int64_t base = at + C::C0;
       auto tile_from = [&](int64_t u) -> int {
-        return u <= base ? 0 : (int)min((int64_t)nt, (u - base + C::W - 1) / C::W);
+        return u <= base ? 0 : (int)min((int64_t)nt, (u - base + w - 1) / w);
       };
       it.t0 = tile_from(u0);
       it.t1 = tile_from(u1);
       it.first = it.t0 == 0;
       it.n_cont = 0;
-      if (it.first && it.t1 < nt) it.n_cont = share_of(base + (int64_t)(nt - 1) * C::W) - share_of(base);
+      if (it.first && it.t1 < nt) it.n_cont = share_of(base + (int64_t)(nt - 1) * w) - share_of(base);
       // step to the next item
-      at += ln.item_cost(nt);
+      at += ln.item_cost(nt, w_rows);
       ++m;
       if (m >= C::count(R)) {
         m = 0;

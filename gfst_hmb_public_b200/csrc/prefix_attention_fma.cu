@@ -3,12 +3,21 @@
 // the 32-bit memory, whose products the tensor cores would round, and the
 // shapes the tensor-core kernel does not tile.
 //
-// One CTA walks its share of the items (prefix_attention.cuh): 32 query rows
-// and a 64-key tile in shared memory as fp32, scores one key per thread and
-// four rows a pass, running maximum and sum per row in shared memory, values
-// accumulated in registers (four columns per thread).  Row groups without
-// valid rows are skipped, so a decode step of a few rows reads each key from
-// shared memory once.
+// One CTA walks its share of the items (prefix_attention.cuh), 32 query rows
+// against 32-key tiles.  Keys and values arrive by cp.async in the pools' own
+// type, the next tile under this one's arithmetic.  Warp w has rows w, w + 8,
+// w + 16, w + 24 to itself: a lane scores one key against its rows, the warp
+// reduces maximum and sum by shuffles, leaves the weights in its own corner of
+// shared memory and then adds value rows, four columns a lane -- no barrier but
+// the tile's two.  What bounds it: shared-memory reads, 8 wavefronts for 16 warp
+// FMAs of the scores.
+//
+// Items of up to four rows (a decode step's) would leave warps idle and wait for
+// each tile: they go key by key instead, straight from memory.  Eight lanes have
+// a key, 16 bytes of every 128 each; a warp four keys of the 32-key tile.  Every
+// group of eight lanes keeps its own maximum, sum and values over its keys and
+// all are joined when the part ends, so the loop has no barrier at all and the
+// bytes of K and V bound it.
 #include <cuda_fp16.h>
 
 #include "prefix_attention.cuh"
@@ -20,11 +29,14 @@ GFST_DEFINE_ERROR_WORD(g_attn_fma_error, read_attn_fma_error, "attention")
 namespace {
 
 constexpr int kRows = kAttnFmaRows;   // 32
-constexpr int kKeys = 64;
+constexpr int kKeys = 32;
 constexpr int kThreads = 256;
 constexpr int kWarps = kThreads / 32;
-// An item's fixed cost is about two 64-key tiles (queries in, partials out).
-using Cut = AttnCutAll<kRows, kKeys, 2, 1>;
+constexpr int kPer = kRows / kWarps;  // rows of a warp
+// A 32-key tile of up to four rows is memory bound, one of 32 rows took seven
+// times as long; an item's fixed cost is about four of the first (queries in,
+// partials out).
+using Cut = AttnCutAll<kRows, kKeys, 4, 8>;
 
 template <typename T>
 struct Vec;  // 16 bytes of T as floats
@@ -55,212 +67,407 @@ struct Vec<__half> {
     }
   }
 };
+// A row's partial result out: to its own place, or to this CTA's continuation
+// buffer.  A lane has columns k * 128 + 4 lane of n such runs.
+__device__ __forceinline__ void fma_put(const AttnArgs& a, const AttnPart& it, int r, int lane, float2 ml,
+                                        const float4* v, int n) {
+  int tok, hq;
+  attn_row(a, it, r, tok, hq);
+  const int64_t row = (int64_t)tok * (a.H * a.G) + hq;
+  const int64_t crow = (int64_t)blockIdx.x * kRows + r;
+  float* o = it.first ? a.part_o[it.own] + row * a.dv : a.cont_o + crow * a.dv;
+#pragma unroll
+  for (int k = 0; k < 2; ++k)
+    if (k < n && k * 128 + lane * 4 < a.dv) *reinterpret_cast<float4*>(o + k * 128 + lane * 4) = v[k];
+  if (lane == 0) {
+    if (it.first) {
+      a.part_ml[it.own][row] = ml;
+      a.part_next[it.own][row] = attn_next((blockIdx.x + 1) * kRows + r, it.n_cont, kRows);
+    } else {
+      a.cont_ml[crow] = ml;
+    }
+  }
+}
 
-// shared memory: rows padded by 4 floats, so that the float4 reads of eight
-// consecutive rows cover all banks once
+// four elements of a row in shared memory
+template <typename T>
+__device__ __forceinline__ float4 four(const uint8_t* row, int c) {
+  if constexpr (sizeof(T) == 4) {
+    return *reinterpret_cast<const float4*>(row + c * 4);
+  } else {
+    const uint2 v = *reinterpret_cast<const uint2*>(row + c * 2);
+    float f[8];
+    Vec<T>::get(make_uint4(v.x, v.y, 0, 0), f);
+    return make_float4(f[0], f[1], f[2], f[3]);
+  }
+}
+
+// Shared memory, in bytes.  Key and value rows are padded by 16 bytes, so that a
+// quarter-warp's 16-byte reads of eight rows cover all banks.
 struct FmaLayout {
-  int qp, vp, q, k, v, s, stat, rows, bytes;
-  __host__ __device__ FmaLayout(int d, int dv) {
+  int kp, vp, qp;              // row pitches: keys, values (bytes), queries (floats)
+  int kv, stage, q, w, rows, bytes;
+  __host__ __device__ FmaLayout(int d, int dv, int es) {
+    kp = d * es + 16;
+    vp = dv * es + 16;
     qp = d + 4;
-    vp = dv + 4;
-    q = 0;
-    k = q + kRows * qp;
-    v = k + kKeys * qp;
-    s = v + kKeys * vp;
-    stat = s + kRows * (kKeys + 1);
-    rows = stat + 3 * kRows;      // int64 row offsets, 8-byte aligned below
-    rows = (rows + 1) & ~1;
-    bytes = (rows + 2 * kKeys) * 4;
+    stage = kKeys * (kp + vp);  // keys, then values
+    kv = 0;
+    q = 2 * stage;
+    w = q + kRows * qp * 4;
+    rows = w + kRows * kKeys * 4;
+    bytes = rows + 2 * kKeys * 8;
   }
 };
 
-template <typename T>
-__device__ __forceinline__ void stage_row(float* dst, const T* src, int v) {
-  float f[Vec<T>::N];
-  const uint4 x = src != nullptr ? __ldg(reinterpret_cast<const uint4*>(src) + v) : make_uint4(0, 0, 0, 0);
-  Vec<T>::get(x, f);
+// Up to NR rows, key by key (see above); d and dv up to 128.  sj: shared memory
+// for the warps' sets, NR rows of dv + 4 floats each.  Returns whether a table
+// entry outside the pool was met.
+template <typename T, int NR>
+__device__ __forceinline__ bool few_rows(const AttnArgs& a, const AttnPart& it, const float* sq, int qp, float* sj) {
+  constexpr int N = Vec<T>::N, S = 16 / N;            // elements and 16-byte pieces of a lane
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, grp = lane >> 3, piece = lane & 7;
+  const int kvr = a.d / N, vvr = a.dv / N;
+  bool bad = false;
+  // pool row of this group's key in tile t (-1: zeros, -2: none)
+  auto row_of = [&](int t) -> int64_t {
+    const int p = t * kKeys + warp * 4 + grp;
+    if (t >= it.t1 || p >= it.len) return -2;
+    const int j = p / a.L;
+    const int blk = attn_block(a, it, j);
+    bad |= blk < 0;
+    return blk >= 0 ? ((int64_t)blk * a.H + it.h) * a.L + (p - j * a.L) : -1;
+  };
+  float m[NR], l[NR], acc[NR][16];
+  int see[NR];
 #pragma unroll
-  for (int i = 0; i < Vec<T>::N; i += 4)
-    *reinterpret_cast<float4*>(dst + v * Vec<T>::N + i) = make_float4(f[i], f[i + 1], f[i + 2], f[i + 3]);
+  for (int i = 0; i < NR; ++i) {
+    m[i] = -INFINITY, l[i] = 0.f;
+    see[i] = i >= it.rows ? 0 : it.own ? min(it.len, it.see0 + (it.row0 + i) / a.G + 1) : it.len;
+#pragma unroll
+    for (int c = 0; c < 16; ++c) acc[i][c] = 0.f;
+  }
+  int64_t row = row_of(it.t0);
+#pragma unroll 1
+  for (int t = it.t0; t < it.t1; ++t) {
+    uint4 k[S], v[S];
+    const uint4* kp = reinterpret_cast<const uint4*>(static_cast<const T*>(a.pool_K) + row * a.d);
+    const uint4* vp = reinterpret_cast<const uint4*>(static_cast<const T*>(a.pool_V) + row * a.dv);
+#pragma unroll
+    for (int s = 0; s < S; ++s) {
+      const int x = s * 8 + piece;
+      k[s] = row >= 0 && x < kvr ? __ldg(kp + x) : make_uint4(0, 0, 0, 0);
+    }
+#pragma unroll
+    for (int s = 0; s < S; ++s) {
+      const int x = s * 8 + piece;
+      v[s] = row >= 0 && x < vvr ? __ldg(vp + x) : make_uint4(0, 0, 0, 0);
+    }
+    const int p0 = t * kKeys + warp * 4 + grp;
+    const bool key = row != -2;
+    row = row_of(t + 1);
+    float x[NR];
+#pragma unroll
+    for (int i = 0; i < NR; ++i) x[i] = 0.f;
+#pragma unroll
+    for (int s = 0; s < S; ++s) {
+      float f[N];
+      Vec<T>::get(k[s], f);
+      if (s * 8 + piece < kvr) {
+#pragma unroll
+        for (int i = 0; i < NR; ++i)
+#pragma unroll
+          for (int c = 0; c < N; c += 4) {
+            const float4 u = *reinterpret_cast<const float4*>(sq + i * qp + (s * 8 + piece) * N + c);
+            x[i] = fmaf(f[c], u.x, x[i]), x[i] = fmaf(f[c + 1], u.y, x[i]);
+            x[i] = fmaf(f[c + 2], u.z, x[i]), x[i] = fmaf(f[c + 3], u.w, x[i]);
+          }
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < NR; ++i) {
+#pragma unroll
+      for (int o = 4; o >= 1; o >>= 1) x[i] += __shfl_xor_sync(0xffffffffu, x[i], o);
+      // a key that the row does not see is left out (its values may be inf or NaN)
+      const bool seen = key && p0 < see[i];
+      const float s = x[i] * a.scale_log2;
+      if (seen) {
+        if (s > m[i]) {
+          const float al = exp2f(m[i] - s);
+          m[i] = s;
+          l[i] *= al;
+#pragma unroll
+          for (int c = 0; c < 16; ++c) acc[i][c] *= al;
+        }
+        // only scores of -inf seen: weight 0
+        const float w = exp2f(s - (m[i] == -INFINITY ? 0.f : m[i]));
+        l[i] += w;
+#pragma unroll
+        for (int q = 0; q < S; ++q) {
+          float f[N];
+          Vec<T>::get(v[q], f);
+#pragma unroll
+          for (int c = 0; c < N; ++c) acc[i][q * N + c] = fmaf(w, f[c], acc[i][q * N + c]);
+        }
+      }
+    }
+  }
+  // the warp's four groups, then the warps through shared memory
+#pragma unroll
+  for (int i = 0; i < NR; ++i) {
+#pragma unroll
+    for (int o = 8; o <= 16; o <<= 1) {
+      const float om = __shfl_xor_sync(0xffffffffu, m[i], o), ol = __shfl_xor_sync(0xffffffffu, l[i], o);
+      const float now = fmaxf(m[i], om);
+      const float fa = m[i] == now ? 1.f : exp2f(m[i] - now), fb = om == now ? 1.f : exp2f(om - now);
+      m[i] = now;
+      l[i] = l[i] * fa + ol * fb;
+#pragma unroll
+      for (int c = 0; c < 16; ++c) acc[i][c] = acc[i][c] * fa + __shfl_xor_sync(0xffffffffu, acc[i][c], o) * fb;
+    }
+    float* set = sj + (warp * NR + i) * (a.dv + 4);
+    if (grp == 0) {
+#pragma unroll
+      for (int s = 0; s < S; ++s)
+        if (s * 8 + piece < vvr) {
+#pragma unroll
+          for (int c = 0; c < N; c += 4)
+            *reinterpret_cast<float4*>(set + 4 + (s * 8 + piece) * N + c) =
+                make_float4(acc[i][s * N + c], acc[i][s * N + c + 1], acc[i][s * N + c + 2], acc[i][s * N + c + 3]);
+        }
+      if (piece == 0) set[0] = m[i], set[1] = l[i];
+    }
+  }
+  __syncthreads();
+  // row `warp` of the item: its eight sets, four columns a lane
+  if (warp < it.rows) {
+    float top = -INFINITY;
+#pragma unroll
+    for (int w = 0; w < kWarps; ++w) top = fmaxf(top, sj[(w * NR + warp) * (a.dv + 4)]);
+    float sum = 0.f;
+    float4 o = make_float4(0, 0, 0, 0);
+#pragma unroll
+    for (int w = 0; w < kWarps; ++w) {
+      const float* set = sj + (w * NR + warp) * (a.dv + 4);
+      const float f = set[0] == top ? 1.f : exp2f(set[0] - top);
+      sum += set[1] * f;
+      if (lane * 4 < a.dv) {
+        const float4 u = *reinterpret_cast<const float4*>(set + 4 + lane * 4);
+        o.x += u.x * f, o.y += u.y * f, o.z += u.z * f, o.w += u.w * f;
+      }
+    }
+    fma_put(a, it, warp, lane, make_float2(top, sum), &o, 1);
+  }
+  return bad;
 }
 
 template <typename T>
-__global__ void __launch_bounds__(kThreads) prefix_attention_fma_kernel(const AttnArgs a) {
-  extern __shared__ float4 smem4[];
-  float* sm = reinterpret_cast<float*>(smem4);
-  const FmaLayout ly(a.d, a.dv);
-  float* sq = sm + ly.q;
-  float* sk = sm + ly.k;
-  float* sv = sm + ly.v;
-  float* ss = sm + ly.s;                 // [kRows][kKeys + 1]
-  float* s_m = sm + ly.stat;             // running maximum (log2 units)
-  float* s_l = s_m + kRows;              // running sum
-  float* s_a = s_l + kRows;              // this tile's rescale
-  int64_t* s_row = reinterpret_cast<int64_t*>(sm + ly.rows);  // pool row of each key, -1 = none
+__global__ void __launch_bounds__(kThreads, 2) prefix_attention_fma_kernel(const __grid_constant__ AttnArgs a) {
+  extern __shared__ __align__(16) uint8_t smem[];
+  const FmaLayout ly(a.d, a.dv, (int)sizeof(T));
+  float* sq = reinterpret_cast<float*>(smem + ly.q);
+  int64_t* s_row = reinterpret_cast<int64_t*>(smem + ly.rows);  // [2][kKeys] pool row of a key, -1: zeros, -2: none
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  float* sw = reinterpret_cast<float*>(smem + ly.w) + warp * (kPer * kKeys);  // the warp's weights
   const T* Q = static_cast<const T*>(a.Q);
-  const T* pK = static_cast<const T*>(a.pool_K);
-  const T* pV = static_cast<const T*>(a.pool_V);
-  const int kvr = a.d / Vec<T>::N, vvr = a.dv / Vec<T>::N;
+  const int kvr = a.d / Vec<T>::N, vvr = a.dv / Vec<T>::N, vpr = kvr + vvr;
 
-  // value columns: thread owns columns [4 col, 4 col + 4) of rows grp, grp + n_grp, ...
-  const int n_col = a.dv / 4, n_grp = kThreads / n_col;
-  const int grp = tid / n_col, col = (tid - grp * n_col) * 4;
-  constexpr int kAcc = 8;                // rows per thread at dv = 256; fewer below
-
+  // the walk is one thread's, its state in shared memory: 40 registers less a thread
   __shared__ int64_t s_sum[1][32], s_at;
-  __shared__ int s_b;
+  __shared__ int s_b, s_more;
+  __shared__ AttnLine<Cut> s_line;
+  __shared__ AttnEven s_shares;
+  __shared__ AttnWalk<Cut> s_walk;
+  __shared__ AttnPart s_it;
   asm volatile("griddepcontrol.wait;" ::: "memory");
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-  AttnLine<Cut> line;
-  attn_lines(a, s_sum, line);
-  AttnEven shares;
-  constexpr int least = Cut::C0 + Cut::W;
-  shares.init(line.U, line.U >= (int64_t)gridDim.x * least ? (int)gridDim.x : max(1, (int)line.U / least));
-  const int64_t u0 = shares.bound(blockIdx.x), u1 = shares.bound(blockIdx.x + 1);
-  line.find(a, u0, &s_b, &s_at);
+  {
+    AttnLine<Cut> line;
+    attn_lines(a, s_sum, line);
+    AttnEven shares;
+    constexpr int least = Cut::C0 + Cut::W;
+    shares.init(line.U, line.U >= (int64_t)gridDim.x * least ? (int)gridDim.x : max(1, (int)line.U / least));
+    line.find(a, shares.bound(blockIdx.x), &s_b, &s_at);
+    if (tid == 0) s_line = line, s_shares = shares;
+  }
   __syncthreads();
-  AttnWalk<Cut> walk;
-  walk.begin(a, line, u0, u1, s_b, s_at);
-  auto share_of = [&](int64_t p) { return shares.worker_of(p); };
-  AttnPart it;
+  if (tid == 0)
+    s_walk.begin(a, s_line, s_shares.bound(blockIdx.x), s_shares.bound(blockIdx.x + 1), s_b, s_at);
   bool bad = false;
-  while (walk.next(a, line, share_of, it)) {
+#pragma unroll 1
+  for (;;) {
+    __syncthreads();  // the last part's reads of the stages, the queries and s_it are done
+    if (tid == 0) s_more = s_walk.next(a, s_line, [&](int64_t p) { return s_shares.worker_of(p); }, s_it);
     __syncthreads();
+    if (!s_more) break;
+    const AttnPart it = s_it;
+    // where a tile's keys lie (32 threads)
+    auto find_rows = [&](int t) {
+      if (tid >= kKeys || t >= it.t1) return;
+      const int p = t * kKeys + tid;
+      int64_t row = -2;
+      if (p < it.len) {
+        const int j = p / a.L;
+        const int blk = attn_block(a, it, j);
+        row = blk >= 0 ? ((int64_t)blk * a.H + it.h) * a.L + (p - j * a.L) : -1;
+        bad |= blk < 0;
+      }
+      s_row[(t & 1) * kKeys + tid] = row;
+    };
+    // a tile's keys and values on their way into stage t & 1
+    auto fetch = [&](int t) {
+      uint8_t* st = smem + (t & 1) * ly.stage;
+      for (int i = tid; i < kKeys * vpr; i += kThreads) {
+        const int key = i / vpr, v = i - key * vpr;
+        const int64_t row = s_row[(t & 1) * kKeys + key];
+        if (row == -2) continue;
+        const bool is_v = v >= kvr;
+        const int64_t at = max(row, (int64_t)0);
+        const T* src = is_v ? static_cast<const T*>(a.pool_V) + at * a.dv + (v - kvr) * Vec<T>::N
+                            : static_cast<const T*>(a.pool_K) + at * a.d + v * Vec<T>::N;
+        uint8_t* dst = is_v ? st + kKeys * ly.kp + key * ly.vp + (v - kvr) * 16 : st + key * ly.kp + v * 16;
+        // a table entry outside the pool: zeros
+        asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"((uint32_t)__cvta_generic_to_shared(dst)),
+                     "l"(src), "r"(row >= 0 ? 16 : 0)
+                     : "memory");
+      }
+      asm volatile("cp.async.commit_group;" ::: "memory");
+    };
+
     for (int i = tid; i < it.rows * kvr; i += kThreads) {
-      const int r = i / kvr;
+      const int r = i / kvr, v = i - r * kvr;
       int tok, hq;
       attn_row(a, it, r, tok, hq);
-      stage_row<T>(sq + r * ly.qp, Q + tok * a.q_st + hq * a.q_sh, i - r * kvr);
+      float f[Vec<T>::N];
+      Vec<T>::get(__ldg(reinterpret_cast<const uint4*>(Q + tok * a.q_st + hq * a.q_sh) + v), f);
+#pragma unroll
+      for (int x = 0; x < Vec<T>::N; x += 4)
+        *reinterpret_cast<float4*>(sq + r * ly.qp + v * Vec<T>::N + x) = make_float4(f[x], f[x + 1], f[x + 2], f[x + 3]);
     }
-    if (tid < kRows) {
-      s_m[tid] = -INFINITY;
-      s_l[tid] = 0.f;
+    if (it.rows <= 4 && s_line.few) {
+      __syncthreads();
+      float* sj = reinterpret_cast<float*>(smem);  // the stages' place
+      bad |= it.rows == 1   ? few_rows<T, 1>(a, it, sq, ly.qp, sj)
+             : it.rows == 2 ? few_rows<T, 2>(a, it, sq, ly.qp, sj)
+                            : few_rows<T, 4>(a, it, sq, ly.qp, sj);
+      continue;
     }
-    float acc[kAcc][4];
-#pragma unroll
-    for (int i = 0; i < kAcc; ++i) acc[i][0] = acc[i][1] = acc[i][2] = acc[i][3] = 0.f;
-
-    for (int t = it.t0; t < it.t1; ++t) {
-      const int key0 = t * kKeys;
-      __syncthreads();
-      if (tid < kKeys) {
-        const int p = key0 + tid;
-        int64_t row = -1;
-        if (p < it.len) {
-          const int j = p / a.L;
-          const int blk = attn_block(a, it, j);
-          if (blk >= 0) row = ((int64_t)blk * a.H + it.h) * a.L + (p - j * a.L);
-          else bad = true;
-        }
-        s_row[tid] = row;
-      }
-      __syncthreads();
-      for (int i = tid; i < kKeys * kvr; i += kThreads) {
-        const int r = i / kvr;
-        const int64_t row = s_row[r];
-        stage_row<T>(sk + r * ly.qp, row >= 0 ? pK + row * a.d : nullptr, i - r * kvr);
-      }
-      for (int i = tid; i < kKeys * vvr; i += kThreads) {
-        const int r = i / vvr;
-        const int64_t row = s_row[r];
-        stage_row<T>(sv + r * ly.vp, row >= 0 ? pV + row * a.dv : nullptr, i - r * vvr);
-      }
-      __syncthreads();
-      {  // scores: key tid % 64, rows tid / 64 + 4 i
-        const int key = tid & (kKeys - 1);
-        const float4* kr = reinterpret_cast<const float4*>(sk + key * ly.qp);
-        for (int r0 = 0; r0 < it.rows; r0 += 8) {
-          const int ra = min(r0 + (tid >> 6), it.rows - 1), rb = min(r0 + 4 + (tid >> 6), it.rows - 1);
-          const float4* qa = reinterpret_cast<const float4*>(sq + ra * ly.qp);
-          const float4* qb = reinterpret_cast<const float4*>(sq + rb * ly.qp);
-          float x = 0.f, y = 0.f;
-          for (int c = 0; c < a.d / 4; ++c) {
-            const float4 k = kr[c], u = qa[c], w = qb[c];
-            x = fmaf(k.x, u.x, x), x = fmaf(k.y, u.y, x), x = fmaf(k.z, u.z, x), x = fmaf(k.w, u.w, x);
-            y = fmaf(k.x, w.x, y), y = fmaf(k.y, w.y, y), y = fmaf(k.z, w.z, y), y = fmaf(k.w, w.w, y);
-          }
-          const int p = key0 + key;
-          auto put = [&](int r, float s) {
-            const int lim = it.own ? min(it.len, it.see0 + (it.row0 + r) / a.G + 1) : it.len;
-            ss[r * (kKeys + 1) + key] = p < lim ? s * a.scale_log2 : -INFINITY;
-          };
-          put(ra, x);
-          if (rb != ra) put(rb, y);
-        }
-      }
-      __syncthreads();
-      // running maximum and sum: warp w takes rows w, w + 8, ...
-      for (int r = warp; r < it.rows; r += kWarps) {
-        float* sr = ss + r * (kKeys + 1);
-        const float x = sr[lane], y = sr[lane + 32];
-        float m = fmaxf(x, y);
-#pragma unroll
-        for (int o = 16; o >= 1; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
-        const float old = s_m[r];
-        const float now = fmaxf(old, m);
-        // a row that has seen nothing keeps weight 0 (and no inf - inf)
-        const float base = now == -INFINITY ? 0.f : now;
-        const float px = exp2f(x - base), py = exp2f(y - base);
-        sr[lane] = px;
-        sr[lane + 32] = py;
-        float l = px + py;
-#pragma unroll
-        for (int o = 16; o >= 1; o >>= 1) l += __shfl_xor_sync(0xffffffffu, l, o);
-        if (lane == 0) {
-          const float al = exp2f(old - base);
-          s_a[r] = al;
-          s_m[r] = now;
-          s_l[r] = s_l[r] * al + l;
-        }
-      }
-      __syncthreads();
-      if (grp < n_grp) {
-        // keys beyond a row's own limit carry weight 0, but 0 * (inf or NaN) is NaN: they are left out
-        const bool ragged = it.own && key0 + kKeys > it.see0 + it.row0 / a.G + 1;
-#pragma unroll
-        for (int i = 0; i < kAcc; ++i) {
-          const int r = grp + i * n_grp;
-          if (r < it.rows) {
-            const float al = s_a[r];
-            float o0 = acc[i][0] * al, o1 = acc[i][1] * al, o2 = acc[i][2] * al, o3 = acc[i][3] * al;
-            const float* pr = ss + r * (kKeys + 1);
-            int n = min(kKeys, it.len - key0);
-            if (ragged) n = min(n, it.see0 + (it.row0 + r) / a.G + 1 - key0);
-            for (int j = 0; j < n; ++j) {
-              const float p = pr[j];
-              const float4 v = *reinterpret_cast<const float4*>(sv + j * ly.vp + col);
-              o0 = fmaf(p, v.x, o0), o1 = fmaf(p, v.y, o1), o2 = fmaf(p, v.z, o2), o3 = fmaf(p, v.w, o3);
-            }
-            acc[i][0] = o0, acc[i][1] = o1, acc[i][2] = o2, acc[i][3] = o3;
-          }
-        }
-      }
-    }
+    find_rows(it.t0);
+    find_rows(it.t0 + 1);
     __syncthreads();
-    // partial results: the row's own place, or this CTA's continuation buffer
-    if (grp < n_grp) {
+    fetch(it.t0);
+    float m[kPer], l[kPer];
+    float4 acc[kPer][2];
 #pragma unroll
-      for (int i = 0; i < kAcc; ++i) {
-        const int r = grp + i * n_grp;
-        if (r < it.rows) {
-          int tok, hq;
-          attn_row(a, it, r, tok, hq);
-          const int64_t row = (int64_t)tok * (a.H * a.G) + hq;
-          const int64_t crow = (int64_t)blockIdx.x * kRows + r;
-          float* o = it.first ? a.part_o[it.own] + row * a.dv : a.cont_o + crow * a.dv;
-          *reinterpret_cast<float4*>(o + col) = make_float4(acc[i][0], acc[i][1], acc[i][2], acc[i][3]);
-          if (col == 0) {
-            const float2 ml = make_float2(s_m[r], s_l[r]);
-            if (it.first) {
-              a.part_ml[it.own][row] = ml;
-              a.part_next[it.own][row] = attn_next((blockIdx.x + 1) * kRows + r, it.n_cont, kRows);
-            } else {
-              a.cont_ml[crow] = ml;
-            }
-          }
+    for (int i = 0; i < kPer; ++i) {
+      m[i] = -INFINITY, l[i] = 0.f;
+      acc[i][0] = acc[i][1] = make_float4(0, 0, 0, 0);
+    }
+
+    // NR: rows of the warp (its last ones repeat where the item has fewer)
+    auto run = [&](auto nr) {
+      constexpr int NR = decltype(nr)::value;
+#pragma unroll 1
+      for (int t = it.t0; t < it.t1; ++t) {
+        if (t + 1 < it.t1) {
+          fetch(t + 1);
+          asm volatile("cp.async.wait_group 1;" ::: "memory");
+        } else {
+          asm volatile("cp.async.wait_group 0;" ::: "memory");
         }
+        __syncthreads();
+        find_rows(t + 2);
+        const uint8_t* sk = smem + (t & 1) * ly.stage;
+        const uint8_t* sv = sk + kKeys * ly.kp;
+        const int key0 = t * kKeys, n = min(kKeys, it.len - key0);
+        if (warp < it.rows) {
+          // scores: key `lane`, the warp's rows
+          float x[NR];
+          const float* q[NR];
+#pragma unroll
+          for (int i = 0; i < NR; ++i) x[i] = 0.f, q[i] = sq + min(warp + i * kWarps, it.rows - 1) * ly.qp;
+          const uint8_t* kr = sk + lane * ly.kp;
+#pragma unroll 2
+          for (int v = 0; v < kvr; ++v) {
+            float f[Vec<T>::N];
+            Vec<T>::get(*reinterpret_cast<const uint4*>(kr + v * 16), f);
+#pragma unroll
+            for (int i = 0; i < NR; ++i)
+#pragma unroll
+              for (int c = 0; c < Vec<T>::N; c += 4) {
+                const float4 u = *reinterpret_cast<const float4*>(q[i] + v * Vec<T>::N + c);
+                x[i] = fmaf(f[c], u.x, x[i]), x[i] = fmaf(f[c + 1], u.y, x[i]);
+                x[i] = fmaf(f[c + 2], u.z, x[i]), x[i] = fmaf(f[c + 3], u.w, x[i]);
+              }
+          }
+          // keys that a row sees, running maximum and sum
+          int see[NR];
+#pragma unroll
+          for (int i = 0; i < NR; ++i) {
+            const int r = min(warp + i * kWarps, it.rows - 1);
+            see[i] = it.own ? min(n, it.see0 + (it.row0 + r) / a.G + 1 - key0) : n;
+            const float s = lane < see[i] ? x[i] * a.scale_log2 : -INFINITY;
+            float top = s;
+#pragma unroll
+            for (int o = 16; o >= 1; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+            const float now = fmaxf(m[i], top);
+            const float base = now == -INFINITY ? 0.f : now;  // nothing seen yet: weights 0, and no inf - inf
+            const float p = exp2f(s - base), al = exp2f(m[i] - base);
+            float sum = p;
+#pragma unroll
+            for (int o = 16; o >= 1; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+            m[i] = now;
+            l[i] = l[i] * al + sum;
+#pragma unroll
+            for (int k = 0; k < 2; ++k)
+              acc[i][k].x *= al, acc[i][k].y *= al, acc[i][k].z *= al, acc[i][k].w *= al;
+            sw[i * kKeys + lane] = p;
+          }
+          __syncwarp();
+          // values, four columns a lane (and four more beyond 128); a key beyond a
+          // row's own has weight 0, but 0 * (inf or NaN) is NaN, so it is left out
+          const bool ragged = it.own && key0 + n > it.see0 + it.row0 / a.G + 1;
+          auto add = [&](auto guard) {
+#pragma unroll 1
+            for (int j0 = 0; j0 < n; j0 += 4) {
+              float4 p[NR];
+#pragma unroll
+              for (int i = 0; i < NR; ++i) p[i] = *reinterpret_cast<const float4*>(sw + i * kKeys + j0);
+#pragma unroll
+              for (int u = 0; u < 4; ++u) {
+                if (j0 + u >= n) break;
+#pragma unroll
+                for (int k = 0; k < 2; ++k) {
+                  const int c = k * 128 + lane * 4;
+                  if (c >= a.dv) continue;
+                  const float4 v = four<T>(sv + (j0 + u) * ly.vp, c);
+#pragma unroll
+                  for (int i = 0; i < NR; ++i) {
+                    if (decltype(guard)::value && j0 + u >= see[i]) continue;
+                    const float w = u == 0 ? p[i].x : u == 1 ? p[i].y : u == 2 ? p[i].z : p[i].w;
+                    acc[i][k].x = fmaf(w, v.x, acc[i][k].x), acc[i][k].y = fmaf(w, v.y, acc[i][k].y);
+                    acc[i][k].z = fmaf(w, v.z, acc[i][k].z), acc[i][k].w = fmaf(w, v.w, acc[i][k].w);
+                  }
+                }
+              }
+            }
+          };
+          if (ragged) add(IC<1>{});
+          else add(IC<0>{});
+        }
+        __syncthreads();  // the stage may be filled again, and the next rows are known
       }
+    };
+    if (it.rows <= kWarps) run(IC<1>{});
+    else if (it.rows <= 2 * kWarps) run(IC<2>{});
+    else run(IC<4>{});
+
+    // partial results: the row's own place, or this CTA's continuation buffer
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) {
+      const int r = warp + i * kWarps;
+      if (r >= it.rows) break;
+      fma_put(a, it, r, lane, make_float2(m[i], l[i]), acc[i], 2);
     }
   }
   if (bad) atomicExch(&g_attn_fma_error, (unsigned)GFST_ERR_ARG);
@@ -268,10 +475,10 @@ __global__ void __launch_bounds__(kThreads) prefix_attention_fma_kernel(const At
 
 template <typename T>
 int launch(const AttnArgs& a, int sms, cudaStream_t stream) {
-  const FmaLayout ly(a.d, a.dv);
+  const FmaLayout ly(a.d, a.dv, (int)sizeof(T));
   auto kern = prefix_attention_fma_kernel<T>;
   static std::atomic<uint64_t> allowed{0};
-  const int st = attn_allow_smem(kern, FmaLayout(256, 256).bytes, allowed);
+  const int st = attn_allow_smem(kern, FmaLayout(256, 256, (int)sizeof(T)).bytes, allowed);
   if (st != GFST_OK) return st;
   const int per_sm = ly.bytes <= 110 * 1024 ? 2 : 1;
   const int grid = (sms < kAttnMaxGrid ? sms : kAttnMaxGrid) * per_sm;
