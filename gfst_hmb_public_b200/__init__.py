@@ -9,6 +9,8 @@ reference project's surface (pkhairkh/gfst-hmb-public):
 * ``memory``     block commit into the block memory pool (mean summary keys)
 * ``retrieval``  coarse block retrieval (BlockRetriever.search / exact_topk)
 * ``readout``    exact-token gather, score and argmax inside selected blocks
+* ``paged``      paged block memory for requests of ragged lengths: block tables,
+                 append, softmax attention behind a shared prefix
 * ``step``       the fused streaming step (frames + commit + readout)
 * ``sharding``   multi-GPU: stream sharding and block-range sharded retrieval
 * ``workloads``  seeded synthetic inputs

@@ -27,6 +27,12 @@ the last launch.  CASE is one of:
   exact_topk  one query against a bf16 bank (--streams = keys, default 8192; top-16)
   mpuc_scan   MPUC recurrent scan of a d_model 2048 cell (fast 1024, mid 512, slow 512,
               bridge rank 128) over 256 tokens (--streams = sequences, default 8)
+  block_tables  one step of the paged memory's block tables, one new token a request
+              (--streams = requests, default 256; 64-token blocks, up to 512 a request)
+  paged_append  keys and values of new tokens to their slots (--streams = tokens, default 65,000; 8 heads, bf16)
+  paged_decode  one token a request behind a shared prefix of 8192 tokens, 500 tokens of
+              its own (--streams = requests, default 64; 8 heads x 4, d=128, bf16)
+  paged_document  the same behind 32,768 shared tokens with 4 heads x 8 (--streams = requests, default 512)
 """
 from __future__ import annotations
 
@@ -35,7 +41,7 @@ import math
 
 import torch
 
-from . import block_commit, centroid, gfst, memory, mpuc, readout, retrieval, tracker, workloads as wl
+from . import block_commit, centroid, gfst, memory, mpuc, paged, readout, retrieval, tracker, workloads as wl
 
 
 def _timed(fn, repeat: int, batch: int = 1) -> float:
@@ -61,7 +67,8 @@ def main() -> None:
                                          "commit", "tracker",
                                          "readout_long", "commit_eig", "block_tracker", "centroid_commit",
                                          "centroid_readout", "segmented", "block_score", "heev", "open_block",
-                                         "exact_topk", "mpuc_scan"])
+                                         "exact_topk", "mpuc_scan", "block_tables", "paged_append", "paged_decode",
+                                         "paged_document"])
     parser.add_argument("--streams", type=int, default=None)
     parser.add_argument("--repeat", type=int, default=2)
     parser.add_argument("--batch", type=int, default=1, help="calls per timed round (segmented, block_score)")
@@ -210,6 +217,47 @@ def main() -> None:
         ins = [torch.randn((B, T, n), generator=g, device=dev) for n in (cell.F, cell.M, cell.S)]
         ms = _timed(lambda: mpuc.recurrent_scan(cell, *ins), args.repeat)
         units = f"{ms * 1e3 / T:.2f} us per token, {B * T / ms / 1e3:.3f} M sequence-tokens/s"
+    elif args.case == "block_tables":
+        B = args.streams or 256
+        lens = (torch.arange(B, device=dev) * 7919 % 32000).to(torch.int32)
+        need = (lens.long() + 63) // 64
+        n_blocks = int(need.sum()) + B
+        table = torch.full((B, 512), -1, dtype=torch.int32, device=dev)
+        held = torch.arange(512, device=dev) < need[:, None]
+        table[held] = torch.arange(int(need.sum()), dtype=torch.int32, device=dev)
+        ring = torch.arange(int(need.sum()), n_blocks + int(need.sum()), dtype=torch.int32, device=dev) % n_blocks
+        state = torch.tensor([0, B], dtype=torch.int32, device=dev)
+        new = torch.ones((B,), dtype=torch.int32, device=dev)
+        ms = _timed(lambda: paged.block_tables(lens, new, table, ring, state, block_len=64, n_tokens=B), args.repeat,
+                    args.batch)
+        units = f"{B * 512 / ms / 1e6:.2f} G entries/s"
+    elif args.case == "paged_append":
+        n = args.streams or 65000
+        mem = paged.PagedMemory(2 * n // 64 + 1, 64, 8, 128, max_requests=1, max_blocks=n // 64 + 1, device=dev)
+        t = mem.extend(torch.tensor([n], dtype=torch.int32, device=dev), n)
+        Kb = torch.randn((n, 8, 128), generator=g, device=dev).to(bf)
+        Vb = torch.randn((n, 8, 128), generator=g, device=dev).to(bf)
+        ms = _timed(lambda: mem.append(Kb, Vb, t), args.repeat, args.batch)
+        units = f"{n * 8 * 128 * 2 * 4 / ms / 1e6:.0f} GB/s"
+    elif args.case in ("paged_decode", "paged_document"):
+        B, P, H, G = (args.streams or 64, 8192, 8, 4) if args.case == "paged_decode" else \
+            (args.streams or 512, 32768, 4, 8)
+        mem = paged.PagedMemory(P // 64 + B * 8 + 1, 64, H, 128, max_requests=B + 1, max_blocks=P // 64, device=dev)
+        mem.pool_K.normal_(generator=g)
+        mem.pool_V.normal_(generator=g)
+        new = torch.zeros((B + 1,), dtype=torch.int32, device=dev)
+        new[B] = P
+        mem.extend(new, P)
+        mem.share(B)
+        new.fill_(499)
+        new[B] = 0
+        mem.extend(new, B * 499)
+        new[:B] = 1
+        t = mem.extend(new, B)
+        Q = torch.randn((B, H * G, 128), generator=g, device=dev).to(bf)
+        ms = _timed(lambda: mem.attend(Q, t), args.repeat, args.batch)
+        units = (f"{(P + B * 500) * H * 128 * 4 / ms / 1e6:.0f} GB/s, "
+                 f"{B * H * G * (P + 500) * 128 * 4 / ms / 1e9:.1f} TFLOP/s")
     else:  # commit
         S = args.streams or 2048
         mem = memory.BlockMemory(S, 4, 64, 128, dtype=bf, device=dev)

@@ -127,3 +127,25 @@ def test_oracle_tables_conserve_blocks(seed):
         free = [int(ring[(state[0] + i) % F]) for i in range(state[1])]
         assert short == 0 and sorted(held + free) == list(range(F))
         assert len(set(slots[slots >= 0].tolist())) == cu[-1]
+
+
+@pytest.mark.parametrize("seed", range(4))
+def test_oracle_attention_against_a_dense_softmax(seed):
+    rng = np.random.default_rng(seed)
+    H, G, d, L, P = 2, 3, 8, 4, int(rng.integers(0, 11))
+    pool_K, pool_V = rng.standard_normal((2, 12, H, L, d))
+    tables, lens, cu = np.array([[5, 1, 7], [9, -1, -1]]), np.array([10, 3]), np.array([0, 4, 5])
+    Q = rng.standard_normal((6, H * G, d))
+    out, lse, mean_abs, top = po.prefix_attention(Q, pool_K, pool_V, tables, lens, cu, np.array([0, 2, 3]), P, 0.3)
+    for t, (b, see) in enumerate([(0, 7), (0, 8), (0, 9), (0, 10), (1, 3)]):
+        for h in range(H * G):
+            rows = [pool_K[[0, 2, 3][p // L], h // G, p % L] for p in range(P)]
+            rows += [pool_K[tables[b, p // L], h // G, p % L] for p in range(see)]
+            vals = [pool_V[[0, 2, 3][p // L], h // G, p % L] for p in range(P)]
+            vals += [pool_V[tables[b, p // L], h // G, p % L] for p in range(see)]
+            s = np.stack(rows) @ Q[t, h] * 0.3
+            w = np.exp(s - s.max())
+            assert np.allclose(out[t, h], w @ np.stack(vals) / w.sum(), rtol=1e-12, atol=1e-12)
+            assert np.isclose(lse[t, h], s.max() + np.log(w.sum()))
+            assert np.allclose(mean_abs[t, h], w @ np.abs(np.stack(vals)) / w.sum())
+    assert (out[5] == 0).all() and np.isneginf(lse[5]).all()
