@@ -33,13 +33,15 @@ import torch
 
 from . import _native as nat
 
+_ENTRY: dict = {}  # entry points by name, as the loaded library gives them
+_I32 = torch.int32
 _DTYPES = {torch.float32: nat.DTYPE_F32, torch.bfloat16: nat.DTYPE_BF16, torch.float16: nat.DTYPE_F16}
 
 
 def _dtype_code(what: str, *tensors: torch.Tensor) -> int:
     dtype = tensors[0].dtype
     for t in tensors:
-        if t.dtype != dtype:
+        if t.dtype is not dtype:
             raise RuntimeError(f"{what}: mixed dtypes {({t.dtype for t in tensors})}")
     if dtype not in _DTYPES:
         raise RuntimeError(f"{what}: unsupported dtype {dtype} (float32, bfloat16 or float16)")
@@ -68,12 +70,17 @@ def _cuda(what: str, *tensors: torch.Tensor | None) -> int:
 
 def _call(index: int, name: str, *args) -> None:
     """Entry point ``name`` on device ``index`` and its current stream."""
+    fn = _ENTRY.get(name)
+    if fn is None:
+        fn = _ENTRY[name] = getattr(nat.load(), name)
     stream = torch.cuda.current_stream(index).cuda_stream
     if torch.cuda.current_device() == index:
-        nat.call(name, *args, stream)
+        status = fn(*args, stream)
     else:
         with torch.cuda.device(index):
-            nat.call(name, *args, stream)
+            status = fn(*args, stream)
+    if status != nat.GFST_OK:
+        nat.check(status, name)
 
 
 def _int32(what: str, name: str, t: torch.Tensor, shape: tuple) -> torch.Tensor:
@@ -132,8 +139,11 @@ def block_tables(lens: torch.Tensor, new_lens: torch.Tensor, tables: torch.Tenso
         raise ValueError("block_tables expects tables [B, W] and free_ring [n_blocks]")
     B, W = tables.shape
     n = int(n_tokens)
-    lens, new_lens = _int32(what, "lens", lens, (B,)), _int32(what, "new_lens", new_lens, (B,))
-    free_state = _int32(what, "free_state", free_state, (2,))
+    if not (lens.dtype is new_lens.dtype is free_state.dtype is _I32 and lens.shape == new_lens.shape == (B,) and
+            free_state.shape == (2,) and lens.is_contiguous() and new_lens.is_contiguous() and
+            free_state.is_contiguous()):
+        lens, new_lens = _int32(what, "lens", lens, (B,)), _int32(what, "new_lens", new_lens, (B,))
+        free_state = _int32(what, "free_state", free_state, (2,))
     if free_ring.dtype != torch.int32 or not free_ring.is_contiguous():
         raise RuntimeError("block_tables: free_ring must be contiguous int32")
     if n < 0:
@@ -152,8 +162,7 @@ def block_tables(lens: torch.Tensor, new_lens: torch.Tensor, tables: torch.Tenso
     sizes = [n, B, B + 1, 2, 1]
     if tables_out is None:
         sizes.append(B * W)
-    buffer = torch.empty((n + 2 * B + 4 + (B * W if tables_out is None else 0),), dtype=torch.int32,
-                         device=lens.device)
+    buffer = lens.new_empty((n + 2 * B + 4 + (B * W if tables_out is None else 0),))
     cut = torch.split_with_sizes(buffer, sizes)
     if tables_out is None:
         tables_out = cut[5].view(B, W)
@@ -234,14 +243,18 @@ def prefix_attention(Q: torch.Tensor, pool_K: torch.Tensor, pool_V: torch.Tensor
         raise RuntimeError("prefix_attention: tables must be int32")
     if W > 0 and tables.stride(1) != 1:
         tables = tables.contiguous()
-    lens, cu_new = _int32(what, "lens", lens, (B,)), _int32(what, "cu_new", cu_new, (B + 1,))
+    if not (lens.dtype is cu_new.dtype is _I32 and lens.shape == (B,) and cu_new.shape == (B + 1,) and
+            lens.is_contiguous() and cu_new.is_contiguous()):
+        lens, cu_new = _int32(what, "lens", lens, (B,)), _int32(what, "cu_new", cu_new, (B + 1,))
     if (prefix_table is None) != (prefix_len is None):
         raise ValueError("prefix_attention: prefix_table and prefix_len go together")
     P, p_table, p_len = 0, None, None
     if prefix_table is not None:
         P = prefix_table.numel()
-        prefix_table = _int32(what, "prefix_table", prefix_table, (P,))
-        prefix_len = _int32(what, "prefix_len", prefix_len, (1,))
+        if not (prefix_table.dtype is prefix_len.dtype is _I32 and prefix_len.shape == (1,) and
+                prefix_table.ndim == 1 and prefix_table.is_contiguous()):
+            prefix_table = _int32(what, "prefix_table", prefix_table, (P,))
+            prefix_len = _int32(what, "prefix_len", prefix_len, (1,))
         p_table, p_len = prefix_table.data_ptr(), prefix_len.data_ptr()
     code = _dtype_code(what, Q, pool_K, pool_V)
     _no_grad(what, Q, pool_K, pool_V)
@@ -253,12 +266,12 @@ def prefix_attention(Q: torch.Tensor, pool_K: torch.Tensor, pool_V: torch.Tensor
         if out.shape != (n, heads, dv) or out.dtype != Q.dtype or not out.is_contiguous():
             raise ValueError(f"prefix_attention: out must be contiguous {Q.dtype} [{n}, {heads}, {dv}]")
     else:
-        out = torch.empty((n, heads, dv), dtype=Q.dtype, device=Q.device)
-    lse = torch.empty((n, heads), dtype=torch.float32, device=Q.device) if return_lse else None
+        out = Q.new_empty((n, heads, dv))
+    lse = Q.new_empty((n, heads), dtype=torch.float32) if return_lse else None
     Q = _rows(Q)
     qt, qh, _ = Q.stride()
     nbytes = _workspace_bytes(n, H, heads // H, dv)
-    ws = torch.empty((nbytes,), dtype=torch.uint8, device=Q.device)
+    ws = tables.new_empty(((nbytes + 3) // 4,))
     _call(index, "gfst_prefix_attention", Q.data_ptr(), qt, qh, pool_K.data_ptr(), pool_V.data_ptr(), n_blocks, L, H,
           heads // H, d, dv, code, tables.data_ptr(), tables.stride(0), W, lens.data_ptr(), cu_new.data_ptr(), B, n,
           p_table, P, p_len, scale, out.data_ptr(), nat.ptr(lse), 0 if given else 1, ws.data_ptr(), nbytes)
