@@ -16,7 +16,9 @@
 // (new tokens, blocks taken, blocks returned).  One launch: every CTA computes
 // the sums itself (the lengths stay in L2 and a scan of 4096 requests is four
 // loads and one block scan), then fills its share of the table entries and of
-// the slots, each found by its own arithmetic -- no CTA waits for another.
+// the slots, each found by its own arithmetic -- no CTA waits for another.  A
+// step in place that wants more blocks than there are leaves everything as it
+// was (every CTA knows it from the sums), so that it can be taken again.
 // What bounds it: launch and scan latency for a decode batch; for thousands
 // of requests the table rows written, 4 B per entry.
 #include "gfst_common.cuh"
@@ -152,8 +154,24 @@ __global__ void __launch_bounds__(kTablesMaxThreads) block_tables_kernel(const T
   __syncthreads();
 
   const int taken = min(t_grow, count);
+  const int32_t lacking = clamp32((int64_t)(t_grow - taken) + t_want);
   const int64_t stride = (int64_t)gridDim.x * blockDim.x;
   const int64_t first = (int64_t)blockIdx.x * blockDim.x + tid;
+
+  if (lacking > 0 && a.tables == a.tables_out) {
+    // a step in place that cannot be had: lengths, tables and ring stay, no token has a slot
+    if (blockIdx.x == 0) {
+      for (int b = tid; b <= a.B; b += blockDim.x) a.cu_new[b] = 0;
+      for (int b = tid; b < a.B; b += blockDim.x) a.lens_out[b] = a.lens[b];
+      if (tid == 0) {
+        a.free_state_out[0] = a.free_state[0];
+        a.free_state_out[1] = a.free_state[1];
+        a.n_short[0] = lacking;
+      }
+    }
+    for (int64_t i = first; i < a.n_tokens; i += stride) a.slot_map[i] = -1;
+    return;
+  }
 
   if (blockIdx.x == 0) {
     for (int b = tid; b <= a.B; b += blockDim.x) a.cu_new[b] = s_cu[b];
@@ -165,7 +183,7 @@ __global__ void __launch_bounds__(kTablesMaxThreads) block_tables_kernel(const T
       a.free_state_out[0] = (int)(((int64_t)head + taken) % a.F);
       // a table that lists more blocks than the ring has room for overflows no count
       a.free_state_out[1] = (int)min((int64_t)a.F, (int64_t)count - taken + t_back);
-      a.n_short[0] = clamp32((int64_t)(t_grow - taken) + t_want);
+      a.n_short[0] = lacking;
     }
   }
 

@@ -132,7 +132,11 @@ def block_tables(lens: torch.Tensor, new_lens: torch.Tensor, tables: torch.Tenso
     not used can be taken again from the same lens, tables and free_state).
     ``n_tokens`` is the number of packed new tokens the caller holds, at least
     the sum of the positive new_lens.  ``tables_out`` (may be ``tables``)
-    receives the new tables in place of a new tensor.  All int32."""
+    receives the new tables in place of a new tensor.  All int32.
+
+    A step that wants more blocks than there are has n_short > 0 and is not to
+    be used; in place (``tables_out`` is ``tables``) it changes nothing, and no
+    token of it has a slot."""
     what = "block_tables"
     index = _cuda(what, lens, new_lens, tables, free_ring, free_state, tables_out)
     if tables.ndim != 2 or free_ring.ndim != 1:
@@ -189,7 +193,8 @@ def paged_append(K: torch.Tensor, V: torch.Tensor, pool_K: torch.Tensor, pool_V:
     """Write K [n, heads, d] and V [n, heads, dv] to their slots of the pools:
     pool[s // L, h, s % L] = row (t, h) with s = slot_map[t] (int32 [n]).  Tokens
     with a negative slot (padding, or a block that was not had) are left out, and
-    so is a slot outside the pool; nothing else of the pools changes.  K and V
+    so is a slot outside the pool; nothing else of the pools changes.  The slots
+    that are written must be distinct, as ``block_tables`` gives them.  K and V
     may be strided views (a fused projection's output) with 16-byte rows."""
     what = "paged_append"
     index = _cuda(what, K, V, pool_K, pool_V, slot_map)
@@ -317,8 +322,10 @@ class PagedMemory:
     def extend(self, new_lens: torch.Tensor, n_tokens: int) -> BlockTables:
         """Take and return blocks for one step; updates the memory's tables,
         lengths and free ring in place and returns the step (whose ``tables`` and
-        ``lens`` are the memory's own).  ``n_short`` of the step says whether the
-        pool was too small; read it when the host waits anyway."""
+        ``lens`` are the memory's own).  ``n_short`` of the step says how many
+        blocks the pool was short of; read it when the host waits anyway.  A step
+        with n_short > 0 did nothing: no request grew or ended, its tokens have no
+        slots and attend to nothing.  End a request and take it again."""
         t = block_tables(self.lens, new_lens, self.tables, self.free_ring, self.free_state,
                          block_len=self.block_len, n_tokens=n_tokens, tables_out=self.tables)
         self.lens.copy_(t.lens)

@@ -98,6 +98,42 @@ def test_block_tables_short_of_blocks(cuda_device, lack):
     _check_tables(cuda_device, (lens, new, tables, ring, state), 16, int(np.maximum(new, 0).sum()), False)
 
 
+@pytest.mark.parametrize("ring_short", [True, False])
+def test_block_tables_short_step_in_place_changes_nothing(cuda_device, ring_short):
+    # the ring is empty, or request 0 wants more than its table is wide
+    lens, new, want = [3, 5, 8, 0], *(([2, 5, -1, 3], 1) if ring_short else ([14, 1, -1, 3], 2))
+    tables = [[7, -1, -1], [2, 9, -1], [4, 1, -1], [-1, -1, -1]]
+    ring, state = [0, 3, 5, 6, 8, 10, 11, -1, -1, -1], [0, 2 if ring_short else 7]
+    d = [_dev(x, cuda_device) for x in (lens, new, tables, ring, state)]
+    t = paged.block_tables(*d, block_len=4, n_tokens=30, tables_out=d[2])
+    assert int(t.n_short) == want
+    assert t.tables.tolist() == tables and d[3].tolist() == ring
+    assert t.lens.tolist() == lens and t.free_state.tolist() == state
+    assert (t.cu_new == 0).all() and (t.slot_map == -1).all()
+
+
+def test_memory_takes_a_short_step_again(cuda_device):
+    mem = paged.PagedMemory(6, 16, 1, 64, max_requests=3, max_blocks=5, device=cuda_device)
+    g = torch.Generator(device=cuda_device).manual_seed(0)
+    make = lambda n, h: torch.randn((n, h, 64), generator=g, device=cuda_device).to(BF16)  # noqa: E731
+    K = make(60, 1)
+    mem.append(K, K, mem.extend(_dev([30, 30, 0], cuda_device), 60))
+    before = [x.clone() for x in (mem.tables, mem.lens, mem.free_ring, mem.free_state, mem.pool_K)]
+    new, more = _dev([3, 3, 17], cuda_device), make(23, 1)      # four blocks, two are free
+    t = mem.extend(new, 23)
+    mem.append(more, more, t)
+    out, lse = mem.attend(make(23, 2), t, return_lse=True)
+    assert int(t.n_short) == 2
+    assert all(torch.equal(a, b) for a, b in
+               zip(before, (mem.tables, mem.lens, mem.free_ring, mem.free_state, mem.pool_K)))
+    assert (out == 0).all() and torch.isneginf(lse).all()
+    t = mem.extend(_dev([0, -1, 0], cuda_device), 0)            # request 1 returns two
+    assert int(t.n_short) == 0 and int(mem.free_state[1]) == 4
+    t = mem.extend(_dev([3, 0, 17], cuda_device), 20)
+    assert int(t.n_short) == 0 and mem.lens.tolist() == [33, 0, 17]
+    assert int((mem.tables >= 0).sum()) == 5 and int(mem.free_state[1]) == 1
+
+
 def test_block_tables_beyond_the_width(cuda_device):
     # request 1 wants 4 blocks of a table 2 wide; its tokens there have no slot
     inputs = (np.array([3, 5, 0]), np.array([2, 11, 4]), np.array([[7, -1], [2, 9], [-1, -1]]),
@@ -296,6 +332,31 @@ def test_attention(cuda_device, dtype, shape):
 def test_attention_other_shapes(cuda_device, dtype, d, dv, L):
     s = Setup(cuda_device, dtype, [70, 1, 200], [3, 1, 60], 150, 2, 3, d, L, dv=dv, seed=d + L)
     s.check(*s.run())
+
+
+@pytest.mark.parametrize("dtype, d", [(BF16, 128), (FP16, 64), (F32, 128)])
+@pytest.mark.parametrize("rows", [3, 16, 17, 32, 33, 64, 100, 128, 129, 256, 257, 300, 385])
+def test_rows_of_the_prefix(cuda_device, dtype, d, rows):
+    # as many one-token requests as rows: every size of the prefix's last item
+    s = Setup(cuda_device, dtype, [1 + i % 70 for i in range(rows)], [1] * rows, 300, 1, 1, d, 32, seed=rows)
+    s.check(*s.run())
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("G", [1, 2, 3, 4, 5])
+def test_few_rows_over_long_requests(cuda_device, dtype, G):
+    # a block length that the tensor-core kernel does not take, 65 to 128 columns
+    s = Setup(cuda_device, dtype, [2000, 33, 1, 400], [1, 1, 1, 1], 0, 2, G, 104, 24, dv=128, seed=G)
+    s.check(*s.run())
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+def test_output_over_the_queries(cuda_device, dtype):
+    s = Setup(cuda_device, dtype, [200, 5], [130, 2], 64, 1, 2, 64, 16, seed=12)
+    want, lse = s.run()
+    q = s.Q.clone()
+    got, lse2 = s.run(Q=q, out=q)
+    assert got is q and torch.equal(q, want) and torch.equal(lse, lse2)
 
 
 @pytest.mark.parametrize("dtype", [BF16, F32])
