@@ -7,6 +7,8 @@
 // partial once; what bounds it is their 4 B per value.
 #include <cuda_fp16.h>
 
+#include <cmath>
+
 #include "prefix_attention.cuh"
 
 namespace gfst {
@@ -192,10 +194,13 @@ extern "C" int gfst_prefix_attention(const void* Q, int64_t q_stride_t, int64_t 
   GFST_REQUIRE(d >= 1 && d <= 256, GFST_ERR_SHAPE, "d=%d outside [1, 256]", d);
   GFST_REQUIRE(d % pv == 0 && dv % pv == 0, GFST_ERR_ALIGN, "rows of %d and %d elements are no multiple of 16 bytes", d,
                dv);
+  const float scale_log2 = (float)((double)scale * 1.4426950408889634);
+  GFST_REQUIRE(std::isfinite(scale_log2), GFST_ERR_ARG, "scale %g is not finite", (double)scale);
   GFST_REQUIRE(n_requests >= 1 && n_requests <= 65536 && width >= 1 && L >= 1 && n_blocks >= 1 && prefix_width >= 0,
                GFST_ERR_SHAPE, "requests %d width %d L %d blocks %lld prefix width %d", n_requests, width, L,
                (long long)n_blocks, prefix_width);
-  GFST_REQUIRE((int64_t)width * L < (1LL << 31) && (int64_t)prefix_width * L < (1LL << 31), GFST_ERR_SHAPE,
+  constexpr int64_t kMostKeys = (1LL << 31) - 1024;  // a tile's last position stays in range
+  GFST_REQUIRE((int64_t)width * L <= kMostKeys && (int64_t)prefix_width * L <= kMostKeys, GFST_ERR_SHAPE,
                "positions exceed the int32 range");
   if (n_tokens == 0) return GFST_OK;
   GFST_REQUIRE(Q && pool_K && pool_V && tables && lens && cu_new && out && workspace, GFST_ERR_ARG, "null pointer");
@@ -221,7 +226,7 @@ extern "C" int gfst_prefix_attention(const void* Q, int64_t q_stride_t, int64_t 
   a.tables = tables, a.table_st = table_stride, a.width = width, a.lens = lens, a.cu = cu_new, a.B = n_requests;
   a.n_tokens = (int)n_tokens;
   a.prefix_table = prefix_table, a.prefix_width = prefix_width, a.prefix_len = prefix_width > 0 ? prefix_len : nullptr;
-  a.scale_log2 = (float)((double)scale * 1.4426950408889634);
+  a.scale_log2 = scale_log2;
   a.out = out, a.lse = lse, a.fill_tail = fill_tail;
   a.part_o[0] = reinterpret_cast<float*>(w + ws.o);
   a.part_o[1] = reinterpret_cast<float*>(half(ws.o, ws.ml));

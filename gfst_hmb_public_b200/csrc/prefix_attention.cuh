@@ -259,9 +259,10 @@ struct AttnEven {
 // the rest, in the ratio of their costs, so that a pair's rows are split over no
 // more CTAs than its cost needs and compute-bound and memory-bound work run side
 // by side.  A CTA of the rest is one worker, or two (its streams) if there is
-// enough.  No share but a line's only one is smaller than `least`, an item's
-// fixed cost and one tile, so every worker between the first and the last of an
-// item holds one of its tiles.
+// enough.  There are workers for shares of `least`, an item's fixed cost and one
+// tile; the split by cost rounds them down by half at most, which still is more
+// than a tile, so every worker between the first and the last of an item holds
+// one of its tiles.
 struct AttnShares {
   AttnEven pairs, rest;
   int two;

@@ -80,6 +80,15 @@ def test_prefix_attention_refuses(kw, status):
     assert _attend(**kw) == status
 
 
+@pytest.mark.parametrize("kw, status", [
+    # the last position of a tile of 128 keys passes 2^31
+    (dict(W=(1 << 31) - 512, L=1), 2), (dict(P=(1 << 31) - 512, L=1), 2), (dict(W=(1 << 27) - 1), 2),
+    (dict(scale=float("nan")), 1), (dict(scale=float("inf")), 1), (dict(scale=3e38), 1), (dict(scale=-3e38), 1),
+])
+def test_prefix_attention_refuses_far_positions_and_scales(kw, status):
+    assert _attend(**kw) == status
+
+
 def test_prefix_attention_of_nothing():
     assert _attend(n=0, Q=None, out=None, ws=None) == 0
 
