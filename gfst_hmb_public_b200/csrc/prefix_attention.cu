@@ -3,8 +3,13 @@
 //
 // The merge is one warp per (token, query head): the prefix part, the own part
 // and their continuations, at most a few, weighted by 2^(m_i - max m), divided
-// by the joined sum and rounded once to the output type.  It reads each
-// partial once; what bounds it is their 4 B per value.
+// by the joined sum and rounded once to the output type.  It reads each partial
+// once; what bounds it is their 4 B per value: for 300,768 rows of two parts of
+// 128 columns, 385 MB, it takes 95 us (4.1 TB/s).  A row's two parts and their (m, l)
+// are loaded at once, before it is known which of them are needed: one memory
+// latency a warp instead of four in a chain (which took 217 us).  One row a warp:
+// two or four, with their loads together, were slower from 16 rows (11.7 and 13.0
+// us a call for 11.2) to those (934 and 979 for 931).
 #include <cuda_fp16.h>
 
 #include <cmath>
@@ -32,112 +37,143 @@ __device__ __forceinline__ void store4<__half>(__half* dst, float4 v) {
   *reinterpret_cast<uint2*>(dst) = make_uint2(*reinterpret_cast<const uint32_t*>(&a), *reinterpret_cast<const uint32_t*>(&b));
 }
 
-template <typename T>
+// What a row's sets have given so far: o is relative to 2^m.
+template <int V>
+struct MergeRow {
+  float m = -INFINITY, l = 0.f;
+  float4 o[V] = {};
+  // weight of a set of reference x under the reference `now` (equal ones need no
+  // exponential, and no inf - inf)
+  __device__ static __forceinline__ float weight(float x, float now) { return x == now ? 1.f : exp2f(x - now); }
+  __device__ __forceinline__ void add(int i, const float4& v, float w) {
+    o[i].x = fmaf(v.x, w, o[i].x), o[i].y = fmaf(v.y, w, o[i].y);
+    o[i].z = fmaf(v.z, w, o[i].z), o[i].w = fmaf(v.w, w, o[i].w);
+  }
+};
+// an empty set (a NaN sum is kept)
+__device__ __forceinline__ bool merge_empty(float2 ml) { return !(ml.y > 0.f) && ml.y == ml.y; }
+
+// V: runs of 128 columns.
+template <typename T, int V>
 __global__ void __launch_bounds__(kMergeThreads) prefix_attention_merge_kernel(const AttnArgs a, int cont_rows) {
+  const int lane = threadIdx.x & 31;
+  const int heads = a.H * a.G;
+  const int64_t row = (int64_t)blockIdx.x * (kMergeThreads / 32) + (threadIdx.x >> 5);
   asm volatile("griddepcontrol.wait;" ::: "memory");
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-  const int lane = threadIdx.x & 31;
-  const int64_t row = (int64_t)blockIdx.x * (kMergeThreads / 32) + (threadIdx.x >> 5);
-  const int heads = a.H * a.G;
-  const int64_t tok = row / heads;
-  if (tok >= a.n_tokens) return;
-  const bool live = tok < attn_tokens(a) && tok >= a.cu[0];
-  if (!live && !a.fill_tail) return;
-  // the row's sets: [0, n0) prefix, [n0, n0 + n1) own, each its own place and
-  // then its continuations (offsets that cover no item leave next unset: sets
-  // outside the buffer are left out)
-  int n0 = 0, n1 = 0;
-  int2 x0 = make_int2(0, 0), x1 = x0;
-  if (live) {
-    x1 = a.part_next[1][row];
-    if (attn_prefix_len(a) > 0) {
-      x0 = a.part_next[0][row];
-      n0 = 1 + min(max(x0.y >> 9, 0), cont_rows);
+  if (row >= (int64_t)a.n_tokens * heads) return;
+  // everything that lies at the row's own place in one go, whether it is needed or
+  // not (a set that was not written is not looked at)
+  int2 next[2] = {};
+  float2 ml[2];
+  float4 o[2][V];
+#pragma unroll
+  for (int k = 0; k < 2; ++k) {
+    if (k == 0 && a.prefix_len == nullptr) continue;
+    next[k] = a.part_next[k][row];
+    ml[k] = a.part_ml[k][row];
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+      const int c = (i * 32 + lane) * 4;
+      if (c < a.dv) o[k][i] = *reinterpret_cast<const float4*>(a.part_o[k] + row * a.dv + c);
     }
-    n1 = 1 + min(max(x1.y >> 9, 0), cont_rows);
   }
-  float m = -INFINITY, l = 0.f;
-  float4 o[2] = {make_float4(0, 0, 0, 0), make_float4(0, 0, 0, 0)};
-  // 32 sets at a time, one per lane: weights first, then the values with their
-  // loads in flight together
+  const int tok = (int)row / heads;
+  const bool live = tok < attn_tokens(a) && tok >= a.cu[0], prefix = live && attn_prefix_len(a) > 0;
+  if (!live && !a.fill_tail) return;
+  const bool has[2] = {prefix && !merge_empty(ml[0]), live && !merge_empty(ml[1])};
+  MergeRow<V> x;
+#pragma unroll
+  for (int k = 0; k < 2; ++k)
+    if (has[k]) x.m = fmaxf(x.m, ml[k].x);
+#pragma unroll
+  for (int k = 0; k < 2; ++k) {
+    if (!has[k]) continue;
+    const float w = MergeRow<V>::weight(ml[k].x, x.m);
+    x.l = fmaf(ml[k].y, w, x.l);
+#pragma unroll
+    for (int i = 0; i < V; ++i) x.add(i, o[k][i], w);
+  }
+  // Continuations, 32 sets at a time, one per lane: weights first, then the
+  // values with their loads in flight together.  (Offsets that cover no item leave
+  // `next` unset: sets outside the buffer are left out.)
+  const int n0 = prefix ? min(max(next[0].y >> 9, 0), cont_rows) : 0;
+  const int n1 = live ? min(max(next[1].y >> 9, 0), cont_rows) : 0;
   for (int s0 = 0; s0 < n0 + n1; s0 += 32) {
     const int s = s0 + lane;
     const float* src = nullptr;
-    float2 ml = make_float2(-INFINITY, 0.f);
+    float2 y = make_float2(-INFINITY, 0.f);
     if (s < n0 + n1) {
-      const int own = s >= n0, i = own ? s - n0 : s;
-      const int2 nx = own ? x1 : x0;
-      const int64_t c = nx.x + (int64_t)(i - 1) * (nx.y & 511);
-      if (i == 0) {
-        ml = a.part_ml[own][row];
-        src = a.part_o[own] + row * a.dv;
-      } else if (c >= 0 && c < cont_rows) {
-        ml = a.cont_ml[c];
+      const int own = s >= n0;
+      const int2 nx = own ? next[1] : next[0];
+      const int64_t c = nx.x + (int64_t)(own ? s - n0 : s) * (nx.y & 511);
+      if (c >= 0 && c < cont_rows) {
+        y = a.cont_ml[c];
         src = a.cont_o + c * a.dv;
       }
     }
-    if (!(ml.y > 0.f) && ml.y == ml.y) src = nullptr;  // an empty set (a NaN sum is kept)
-    if (src == nullptr) ml = make_float2(-INFINITY, 0.f);
-    float now = fmaxf(m, ml.x);
+    if (merge_empty(y)) src = nullptr;
+    if (src == nullptr) y = make_float2(-INFINITY, 0.f);
+    float now = fmaxf(x.m, y.x);
 #pragma unroll
     for (int i = 16; i >= 1; i >>= 1) now = fmaxf(now, __shfl_xor_sync(0xffffffffu, now, i));
-    // equal references need no exponential (and no inf - inf)
-    const float w = src == nullptr ? 0.f : ml.x == now ? 1.f : exp2f(ml.x - now);
-    float sum = ml.y * w;
+    const float w = src == nullptr ? 0.f : MergeRow<V>::weight(y.x, now);
+    float sum = y.y * w;
 #pragma unroll
     for (int i = 16; i >= 1; i >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, i);
-    const float keep = m == -INFINITY ? 0.f : m == now ? 1.f : exp2f(m - now);
-    m = now;
-    l = l * keep + sum;
+    const float keep = MergeRow<V>::weight(x.m, now);
+    x.m = now;
+    x.l = x.l * keep + sum;
 #pragma unroll
-    for (int i = 0; i < 2; ++i) o[i].x *= keep, o[i].y *= keep, o[i].z *= keep, o[i].w *= keep;
+    for (int i = 0; i < V; ++i) x.o[i].x *= keep, x.o[i].y *= keep, x.o[i].z *= keep, x.o[i].w *= keep;
     const int n = min(32, n0 + n1 - s0);
     for (int g = 0; g < n; g += 4) {
       float wt[4];
-      float4 v[4][2];
+      float4 v[4][V];
 #pragma unroll
-      for (int u = 0; u < 4; ++u) {
-        const int k = g + u;
+      for (int q = 0; q < 4; ++q) {
+        const int k = g + q;
         const float* p = reinterpret_cast<const float*>(
             __shfl_sync(0xffffffffu, reinterpret_cast<unsigned long long>(src), k & 31));
-        wt[u] = __shfl_sync(0xffffffffu, w, k & 31);
+        wt[q] = __shfl_sync(0xffffffffu, w, k & 31);
         if (k >= n) p = nullptr;
 #pragma unroll
-        for (int i = 0; i < 2; ++i) {
+        for (int i = 0; i < V; ++i) {
           const int c = (i * 32 + lane) * 4;
-          v[u][i] = p != nullptr && c < a.dv ? *reinterpret_cast<const float4*>(p + c) : make_float4(0, 0, 0, 0);
+          v[q][i] = p != nullptr && c < a.dv ? *reinterpret_cast<const float4*>(p + c) : make_float4(0, 0, 0, 0);
         }
       }
 #pragma unroll
-      for (int u = 0; u < 4; ++u) {
-        if (g + u >= n) break;
+      for (int q = 0; q < 4; ++q) {
+        if (g + q >= n) break;
 #pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          o[i].x = fmaf(v[u][i].x, wt[u], o[i].x);
-          o[i].y = fmaf(v[u][i].y, wt[u], o[i].y);
-          o[i].z = fmaf(v[u][i].z, wt[u], o[i].z);
-          o[i].w = fmaf(v[u][i].w, wt[u], o[i].w);
-        }
+        for (int i = 0; i < V; ++i) x.add(i, v[q][i], wt[q]);
       }
     }
   }
   // a row that sees nothing: zeros and -inf
-  const float inv = l == 0.f ? 0.f : 1.f / l;
+  const float inv = x.l == 0.f ? 0.f : 1.f / x.l;
   T* out = static_cast<T*>(a.out) + row * a.dv;
 #pragma unroll
-  for (int i = 0; i < 2; ++i) {
+  for (int i = 0; i < V; ++i) {
     const int c = (i * 32 + lane) * 4;
-    if (c < a.dv) store4<T>(out + c, make_float4(o[i].x * inv, o[i].y * inv, o[i].z * inv, o[i].w * inv));
+    if (c < a.dv) store4<T>(out + c, make_float4(x.o[i].x * inv, x.o[i].y * inv, x.o[i].z * inv, x.o[i].w * inv));
   }
-  if (a.lse != nullptr && lane == 0) a.lse[row] = l == 0.f ? -INFINITY : (m + log2f(l)) * 0.69314718055994531f;
+  if (a.lse != nullptr && lane == 0) a.lse[row] = x.l == 0.f ? -INFINITY : (x.m + log2f(x.l)) * 0.69314718055994531f;
+}
+
+template <typename T, int V>
+int launch_merge_of(const AttnArgs& a, int cont_rows, cudaStream_t stream) {
+  constexpr int per = kMergeThreads / 32;
+  const int64_t rows = (int64_t)a.n_tokens * a.H * a.G;
+  return attn_launch("prefix_attention_merge_kernel", prefix_attention_merge_kernel<T, V>, (rows + per - 1) / per,
+                     kMergeThreads, 0, stream, a, cont_rows);
 }
 
 template <typename T>
 int launch_merge(const AttnArgs& a, cudaStream_t stream) {
-  const int64_t rows = (int64_t)a.n_tokens * a.H * a.G;
-  const int64_t blocks = (rows + kMergeThreads / 32 - 1) / (kMergeThreads / 32);
-  return attn_launch("prefix_attention_merge_kernel", prefix_attention_merge_kernel<T>, blocks, kMergeThreads, 0, stream,
-                     a, a.dv <= 128 ? kAttnTcContRows : kAttnFmaContRows);
+  return a.dv > 128 ? launch_merge_of<T, 2>(a, kAttnFmaContRows, stream)
+                    : launch_merge_of<T, 1>(a, kAttnTcContRows, stream);
 }
 
 struct Workspace {
