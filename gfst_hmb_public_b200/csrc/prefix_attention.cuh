@@ -93,14 +93,10 @@ struct AttnPart {
   int n_cont;     // continuations of the item (first part only), by workers worker + 1 ..
 };
 
-// floor(x / n) for 0 <= x < 2^62 and an integer n, inv = 1 / n in double: the
-// product is within one of the quotient while that is below 2^50, and costs a
-// tenth of a 64-bit division.
-__device__ __forceinline__ int64_t attn_div(int64_t x, int64_t n, double inv) {
-  int64_t q = (int64_t)((double)x * inv);
-  const int64_t r = x - q * n;
-  q += r < 0 ? -1 : r >= n ? 1 : 0;
-  return q;
+// x / n for x >= 0, n > 0: costs hardly ever leave 32 bits, where a division is a
+// fifth as long.
+__device__ __forceinline__ int64_t attn_div(int64_t x, int64_t n) {
+  return ((x | n) >> 32) == 0 ? (int64_t)((uint32_t)x / (uint32_t)n) : x / n;
 }
 
 // How a group of R rows is cut into items, and what an item costs: C0 + weight()
@@ -145,6 +141,9 @@ struct AttnLine {
   // this thread's requests [b0, b1): their cost and the cost before them
   int b0, b1;
   int64_t before, sum;
+  // the last of them, and the cost of one of its heads
+  AttnRequest last;
+  int64_t last_cost;
 
   __device__ __forceinline__ int prefix_w_rows() const { return min(C::MR, prefix_rows); }
   __device__ static __forceinline__ int tiles(int len) { return max(1, (len + C::KT - 1) / C::KT); }
@@ -181,7 +180,11 @@ struct AttnLine {
     prefix_all = prefix_cost * prefix_mt * a.H;
     sum = 0;
   }
-  __device__ __forceinline__ void add(const AttnArgs& a, const AttnRequest& r) { sum += head_cost(r, a.G) * a.H; }
+  __device__ __forceinline__ void add(const AttnArgs& a, const AttnRequest& r) {
+    last = r;
+    last_cost = head_cost(r, a.G);
+    sum += last_cost * a.H;
+  }
   __device__ __forceinline__ void scan_warp(int64_t* s_sum) {
     const int lane = threadIdx.x & 31;
     int64_t inc = sum;
@@ -193,40 +196,27 @@ struct AttnLine {
     if (lane == 31) s_sum[threadIdx.x >> 5] = inc;
     before = prefix_all + inc - sum;
   }
+  template <int WARPS>
   __device__ __forceinline__ void scan_block(const int64_t* s_sum) {
-    const int warp = threadIdx.x >> 5, n_warps = (blockDim.x + 31) >> 5;
+    const int warp = threadIdx.x >> 5;
     U = prefix_all;
-#pragma unroll 1
-    for (int w = 0; w < n_warps; ++w) {
-      if (w < warp) before += s_sum[w];
-      U += s_sum[w];
+#pragma unroll
+    for (int w = 0; w < WARPS; ++w) {
+      const int64_t v = s_sum[w];
+      before += w < warp ? v : 0;
+      U += v;
     }
-  }
-  // Called by every thread: the one whose requests hold position u leaves the
-  // request and the cost before it (to be read after a barrier).
-  __device__ void find(const AttnArgs& a, int64_t u, int* s_b, int64_t* s_at) const {
-    if (u < prefix_all || u < before || u >= before + sum) return;
-    int64_t p = before;
-    int b = b0;
-#pragma unroll 1
-    for (; b < b1; ++b) {
-      const int64_t c = head_cost(attn_request(a, b), a.G) * a.H;
-      if (u < p + c) break;
-      p += c;
-    }
-    *s_b = b;
-    *s_at = p;
   }
 };
 
-// Sums up one or more lines; called by every thread of the CTA with its own
-// line objects.  One barrier; s_sum (one row a line) may be used again after
-// the caller's next one.
-template <class... C>
+// Sums up one or more lines; called by every thread of the CTA (WARPS warps) with
+// its own line objects.  One barrier; s_sum (one row a line) may be used again
+// after the caller's next one.
+template <int WARPS, class... C>
 __device__ __forceinline__ void attn_lines(const AttnArgs& a, int64_t (*s_sum)[32], AttnLine<C>&... line) {
   const int prefix = attn_prefix_len(a), tokens = attn_tokens(a);
   (line.begin(a, prefix, tokens), ...);
-  const int per = (a.B + blockDim.x - 1) / blockDim.x;
+  const int per = (a.B + WARPS * 32 - 1) / (WARPS * 32);
   const int b0 = min(a.B, (int)threadIdx.x * per), b1 = min(a.B, b0 + per);
   ((line.b0 = b0, line.b1 = b1), ...);
 #pragma unroll 1
@@ -238,21 +228,20 @@ __device__ __forceinline__ void attn_lines(const AttnArgs& a, int64_t (*s_sum)[3
   (line.scan_warp(s_sum[k++]), ...);
   __syncthreads();
   k = 0;
-  (line.scan_block(s_sum[k++]), ...);
+  (line.template scan_block<WARPS>(s_sum[k++]), ...);
 }
 
-// Equal shares of a line over n workers: worker i has [U i / n, U (i + 1) / n).
+// Equal shares of a line over n workers, rounded up: the last ones may be short
+// or empty.
 struct AttnEven {
-  int64_t U;
-  double inv_n, inv_U;
+  int64_t U, step;
   int n;
   __device__ __forceinline__ void init(int64_t u, int workers) {
     U = u, n = workers;
-    inv_n = 1.0 / max(n, 1);
-    inv_U = U > 0 ? 1.0 / (double)U : 0.0;
+    step = max(attn_div(u + n - 1, max(n, 1)), (int64_t)1);
   }
-  __device__ __forceinline__ int64_t bound(int i) const { return i >= n ? U : attn_div(U * i, n, inv_n); }
-  __device__ __forceinline__ int worker_of(int64_t u) const { return (int)attn_div((u + 1) * n - 1, U, inv_U); }
+  __device__ __forceinline__ int64_t bound(int i) const { return min(U, step * i); }
+  __device__ __forceinline__ int worker_of(int64_t u) const { return (int)attn_div(u, step); }
 };
 
 // How the two lines are shared: CTAs [0, pairs.n) take pairs and the others of n
@@ -272,7 +261,7 @@ struct AttnShares {
     const int least = P > 0 ? max(least_p, least_s) : least_s;
     const int n = T >= (int64_t)grid * least ? grid : max(1, (int)T / least);
     // a CTA more than the ratio's whole part once that would leave the pairs' 15 % behind
-    int np = (int)ceil((double)P * n / (double)max(T, (int64_t)1) - 0.15);
+    int np = (int)ceilf((float)P * n / (float)max(T, (int64_t)1) - 0.15f);
     np = P == 0 ? 0 : S == 0 ? n : min(max(np, 1), max(n - 1, 1));
     const int ns = S == 0 ? 0 : max(n - np, 1);
     two = S >= (int64_t)ns * (2 * least_s);
@@ -290,39 +279,75 @@ struct AttnShares {
 template <class C>
 struct AttnWalk {
   int64_t u0, u1, at;
+  int64_t cost;  // of the item at `at`, once it has been handed out
   int own, b, h, m;
   AttnRequest req;
 
-  __device__ void begin(const AttnArgs& a, const AttnLine<C>& ln, int64_t from, int64_t to, int s_b, int64_t s_at) {
-    u0 = from;
-    u1 = to;
-    own = u0 >= ln.prefix_all;
-    m = h = b = 0;
-    at = 0;
-    if (u0 >= u1) {  // nothing in this share
-      own = 1;
-      b = a.B;
-      at = u1;
-    } else if (!own) {
-      const int64_t k = attn_div(u0, ln.prefix_cost, 1.0 / (double)ln.prefix_cost);
-      h = (int)attn_div(k, ln.prefix_mt, 1.0 / ln.prefix_mt);
-      m = (int)(k - (int64_t)h * ln.prefix_mt);
-      at = k * ln.prefix_cost;
+  // The walk of the share [from, to) into *s (to be read behind a barrier); called
+  // by every thread with its line: the one whose requests hold `from`, or thread 0
+  // for the prefix and an empty share, knows where it begins.
+  __device__ static __forceinline__ void find(const AttnArgs& a, const AttnLine<C>& ln, int64_t from, int64_t to,
+                                              AttnWalk* s) {
+    const bool none = from >= to, prefix = from < ln.prefix_all;
+    if (none || prefix ? threadIdx.x != 0 : from < ln.before || from >= ln.before + ln.sum) return;
+    AttnWalk w;
+    w.u0 = from;
+    w.u1 = to;
+    w.own = !prefix;
+    w.m = w.h = w.b = 0;
+    w.at = 0;
+    if (none) {
+      w.own = 1;
+      w.b = a.B;
+      w.at = to;
+    } else if (prefix) {
+      const int64_t k = attn_div(from, ln.prefix_cost);
+      w.h = (int)attn_div(k, ln.prefix_mt);
+      w.m = (int)(k - (int64_t)w.h * ln.prefix_mt);
+      w.at = k * ln.prefix_cost;
     } else {
-      b = s_b;
-      at = s_at;
-      req = attn_request(a, b);
-      const int64_t hc = ln.head_cost(req, a.G);
-      h = (int)attn_div(u0 - at, hc, 1.0 / (double)hc);
-      at += hc * h;
+      w.at = ln.before;
+      w.b = ln.b1 - 1;
+      w.req = ln.last;
+      int64_t hc = ln.last_cost;
+      if (ln.b0 < w.b) {
 #pragma unroll 1
-      for (;;) {
-        const int64_t c = ln.own_cost(req, m, a.G);
-        if (u0 < at + c) break;
-        at += c;
-        ++m;
+        for (w.b = ln.b0;; ++w.b) {
+          w.req = attn_request(a, w.b);
+          hc = ln.head_cost(w.req, a.G);
+          if (from < w.at + hc * a.H) break;
+          w.at += hc * a.H;
+        }
+      }
+      w.h = (int)attn_div(from - w.at, hc);
+      w.at += hc * w.h;
+      const int items = C::count(w.req.n * a.G);
+#pragma unroll 1
+      for (; w.m + 1 < items; ++w.m) {
+        const int64_t c = ln.own_cost(w.req, w.m, a.G);
+        if (from < w.at + c) break;
+        w.at += c;
       }
     }
+    w.cost = -1;
+    *s = w;
+  }
+
+  // to the next item of the line
+  __device__ __forceinline__ void step(const AttnArgs& a, const AttnLine<C>& ln) {
+    at += cost;
+    if (++m < C::count(own ? req.n * a.G : ln.prefix_rows)) return;
+    m = 0;
+    if (++h < a.H) return;
+    h = 0;
+    if (!own) {
+      own = 1;
+      b = -1;
+    }
+    do {
+      if (++b >= a.B) break;
+      req = attn_request(a, b);
+    } while (C::count(req.n * a.G) == 0);
   }
 
   // The next part with at least one tile; false at the end of the share.
@@ -331,6 +356,7 @@ struct AttnWalk {
   __device__ __forceinline__ bool next(const AttnArgs& a, const AttnLine<C>& ln, F&& share_of, AttnPart& it) {
 #pragma unroll 1
     for (;;) {
+      if (cost >= 0) step(a, ln);  // only now: the next request's lengths are not waited for before
       if (at >= u1 || (own && b >= a.B)) return false;
       const int R = own ? req.n * a.G : ln.prefix_rows;
       int nt;
@@ -363,23 +389,7 @@ struct AttnWalk {
       it.first = it.t0 == 0;
       it.n_cont = 0;
       if (it.first && it.t1 < nt) it.n_cont = share_of(base + (int64_t)(nt - 1) * w) - share_of(base);
-      // step to the next item
-      at += ln.item_cost(nt, w_rows);
-      ++m;
-      if (m >= C::count(R)) {
-        m = 0;
-        if (++h == a.H) {
-          h = 0;
-          if (!own) {
-            own = 1;
-            b = -1;
-          }
-          do {
-            if (++b >= a.B) break;
-            req = attn_request(a, b);
-          } while (C::count(req.n * a.G) == 0);
-        }
-      }
+      cost = ln.item_cost(nt, w_rows);
       if (it.t1 > it.t0) return true;
     }
   }

@@ -273,8 +273,8 @@ __global__ void __launch_bounds__(kThreads, 2) prefix_attention_fma_kernel(const
   const int kvr = a.d / Vec<T>::N, vvr = a.dv / Vec<T>::N, vpr = kvr + vvr;
 
   // the walk is one thread's, its state in shared memory: 40 registers less a thread
-  __shared__ int64_t s_sum[1][32], s_at;
-  __shared__ int s_b, s_more;
+  __shared__ int64_t s_sum[1][32];
+  __shared__ int s_more;
   __shared__ AttnLine<Cut> s_line;
   __shared__ AttnEven s_shares;
   __shared__ AttnWalk<Cut> s_walk;
@@ -283,16 +283,14 @@ __global__ void __launch_bounds__(kThreads, 2) prefix_attention_fma_kernel(const
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   {
     AttnLine<Cut> line;
-    attn_lines(a, s_sum, line);
+    attn_lines<kWarps>(a, s_sum, line);
     AttnEven shares;
     constexpr int least = Cut::C0 + Cut::W;
     shares.init(line.U, line.U >= (int64_t)gridDim.x * least ? (int)gridDim.x : max(1, (int)line.U / least));
-    line.find(a, shares.bound(blockIdx.x), &s_b, &s_at);
-    if (tid == 0) s_line = line, s_shares = shares;
+    AttnWalk<Cut>::find(a, line, shares.bound(blockIdx.x), shares.bound(blockIdx.x + 1), &s_walk);
+    if (tid == 32) s_line = line;
+    if (tid == 64) s_shares = shares;
   }
-  __syncthreads();
-  if (tid == 0)
-    s_walk.begin(a, s_line, s_shares.bound(blockIdx.x), s_shares.bound(blockIdx.x + 1), s_b, s_at);
   bool bad = false;
 #pragma unroll 1
   for (;;) {

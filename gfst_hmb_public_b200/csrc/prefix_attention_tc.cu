@@ -91,8 +91,6 @@ struct StreamCtrl {
   uint32_t bad[2][4];          // value rows that are not finite (one bit each), two tiles in turn
   int accumulate;              // the part's first product adds to O
   float2 ml[2][32];            // joining copies' references and sums
-  int at_b;                    // where the stream's (the pairs': stream 0's) share begins
-  int64_t at_u;
 };
 struct Ctrl {
   StreamCtrl s[2];
@@ -103,6 +101,8 @@ struct Ctrl {
   AttnLine<Pairs> pairs;         // the lines (their common part)
   AttnLine<Rest> rest;
   AttnShares shares;
+  AttnWalk<Pairs> walk_pairs;    // where the shares begin
+  AttnWalk<Rest> walk_rest[2];
   int gone[2][4];                // softmax warps of pairs that have left
   uint32_t tmem;
   int abort;
@@ -640,22 +640,21 @@ __global__ void __launch_bounds__(kThreads, 1)
   {
     AttnLine<Pairs> pl;
     AttnLine<Rest> rl;
-    attn_lines(a, ctl->sum, pl, rl);
+    attn_lines<kThreads / 32>(a, ctl->sum, pl, rl);
     AttnShares sh;
     sh.init(pl.U, rl.U, gridDim.x, Pairs::C0 + Pairs::W, Rest::C0 + Rest::W);
     if (blockIdx.x < sh.pairs.n) {
-      pl.find(a, sh.pairs.bound(blockIdx.x), &ctl->s[0].at_b, &ctl->s[0].at_u);
+      AttnWalk<Pairs>::find(a, pl, sh.pairs.bound(blockIdx.x), sh.pairs.bound(blockIdx.x + 1), &ctl->walk_pairs);
     } else {
       for (int j = 0; j < 2; ++j) {
         const int w = sh.rest_worker(blockIdx.x, j);
-        if (w >= 0) rl.find(a, sh.rest.bound(w), &ctl->s[j].at_b, &ctl->s[j].at_u);
+        if (w >= 0) AttnWalk<Rest>::find(a, rl, sh.rest.bound(w), sh.rest.bound(w + 1), &ctl->walk_rest[j]);
       }
     }
-    if (threadIdx.x == 0) {
-      ctl->pairs = pl;
-      ctl->rest = rl;
-      ctl->shares = sh;
-    }
+    // (different warps: they run side by side)
+    if (threadIdx.x == 32) ctl->pairs = pl;
+    if (threadIdx.x == 64) ctl->rest = rl;
+    if (threadIdx.x == 96) ctl->shares = sh;
   }
   __syncthreads();
   tc_fence_after();
@@ -781,13 +780,11 @@ __global__ void __launch_bounds__(kThreads, 1)
     AttnPart it;
     const AttnShares& sh = ctl->shares;
     if (blockIdx.x < sh.pairs.n) {
-      AttnWalk<Pairs> w;
-      w.begin(a, ctl->pairs, sh.pairs.bound(blockIdx.x), sh.pairs.bound(blockIdx.x + 1), ctl->s[0].at_b, ctl->s[0].at_u);
+      AttnWalk<Pairs> w = ctl->walk_pairs;
 #pragma unroll 1
       while (ok && w.next(a, ctl->pairs, [&](int64_t p) { return sh.pairs.worker_of(p); }, it)) ok = part(it, 1);
-    } else if (const int i = sh.rest_worker(blockIdx.x, j); i >= 0) {
-      AttnWalk<Rest> w;
-      w.begin(a, ctl->rest, sh.rest.bound(i), sh.rest.bound(i + 1), c.at_b, c.at_u);
+    } else if (sh.rest_worker(blockIdx.x, j) >= 0) {
+      AttnWalk<Rest> w = ctl->walk_rest[j];
 #pragma unroll 1
       while (ok && w.next(a, ctl->rest, [&](int64_t p) { return sh.rest.worker_of(p); }, it)) ok = part(it, 0);
     }
