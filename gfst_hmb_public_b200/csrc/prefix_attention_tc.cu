@@ -226,6 +226,40 @@ struct Waiter {
 // rows, softmaxes over disjoint keys, are joined when the part ends.
 __device__ __forceinline__ int copies_of(int paired, int rows) { return paired || rows > 32 ? 1 : 2; }
 
+// Query rows [r0, r1) of a stream's tile by one warp, swizzled as TMA would: a lane
+// finds a row's place, then whole rows are copied, D / 8 lanes a row.
+template <int D>
+__device__ __forceinline__ void copy_queries(const AttnArgs& a, const AttnPart& it, int paired, int j, uint8_t* sq,
+                                             int r0, int r1) {
+  const int lane = threadIdx.x & 31;
+  const int r_first = paired ? j * kHalf : 0, rows = min(kHalf, it.rows - r_first);
+  const int copies = copies_of(paired, it.rows);
+  constexpr int PIECES = D / 8, ROWS = 32 / PIECES;  // rows of a step
+  const int v = lane % PIECES, sub = lane / PIECES;
+  const uint32_t col = smem_u32(sq) + (v >> 3) * (128 * 128);
+  r1 = min(r1, rows);
+#pragma unroll 1
+  for (; r0 < r1; r0 += 32) {
+    int tok, hq;
+    attn_row(a, it, r_first + min(r0 + lane, rows - 1), tok, hq);
+    const int64_t at = tok * a.q_st + hq * a.q_sh;
+#pragma unroll 4
+    for (int x = 0; x < 32; x += ROWS) {
+      const int r = r0 + x + sub;
+      const uint16_t* src = static_cast<const uint16_t*>(a.Q) + __shfl_sync(0xffffffffu, at, x + sub) + v * 8;
+      const uint32_t dst = col + r * 128 + (((v & 7) ^ (r & 7)) << 4);
+      if (r < rows) {
+        asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+        if (copies > 1)
+          asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst + (kHalf / 2) * 128), "l"(src) : "memory");
+      }
+    }
+  }
+  asm volatile("cp.async.wait_all;" ::: "memory");
+  fence_async_smem();
+  __syncwarp();
+}
+
 // One softmax thread: a row of its stream's tile.
 template <int D, bool F16>
 struct Softmax {
@@ -606,7 +640,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       mbar_init(&c.item_full[i], 1);
       mbar_init(&c.item_empty[i], 5);  // four softmax warps, the MMA warp
     }
-    mbar_init(&c.q_full, 1);
+    mbar_init(&c.q_full, 4);
     mbar_init(&c.q_empty, 1);
     for (int i = 0; i < 2; ++i) {
       mbar_init(&c.s_full[i], 1);
@@ -632,6 +666,10 @@ __global__ void __launch_bounds__(kThreads, 1)
     mbar_init_fence();
   }
   if (warp == kMma) tmem_alloc(&ctl->tmem, kTmemCols);
+  if (warp == kProducer && lane == 0) {
+    asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(&tmK)) : "memory");
+    asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(&tmV)) : "memory");
+  }
   tc_fence_before();
   asm volatile("griddepcontrol.wait;" ::: "memory");
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
@@ -685,37 +723,12 @@ __global__ void __launch_bounds__(kThreads, 1)
         c.paired[slot] = paired;
         mbar_arrive(&c.item_full[slot]);
       }
-      // query rows of this stream, swizzled as TMA would: a lane finds a row's place,
-      // then whole rows are copied, D / 8 lanes a row
+      // queries of this stream; those of its first part come by the softmax warps
       auto queries = [&]() -> bool {
+        if (n_item == 0) return true;
         if (!wait.warp(&c.q_empty, (n_item & 1) ^ 1)) return false;
-        const int r_first = paired ? j * kHalf : 0, rows = min(kHalf, it.rows - r_first);
-        const int copies = copies_of(paired, it.rows);
-        constexpr int PIECES = D / 8, ROWS = 32 / PIECES;  // rows of a step
-        const int v = lane % PIECES, sub = lane / PIECES;
-        const uint32_t col = smem_u32(sq) + (v >> 3) * (128 * 128);
-#pragma unroll 1
-        for (int r0 = 0; r0 < rows; r0 += 32) {
-          int tok, hq;
-          attn_row(a, it, r_first + min(r0 + lane, rows - 1), tok, hq);
-          const int64_t at = tok * a.q_st + hq * a.q_sh;
-#pragma unroll 4
-          for (int x = 0; x < 32; x += ROWS) {
-            const int r = r0 + x + sub;
-            const uint16_t* src = static_cast<const uint16_t*>(a.Q) + __shfl_sync(0xffffffffu, at, x + sub) + v * 8;
-            const uint32_t dst = col + r * 128 + (((v & 7) ^ (r & 7)) << 4);
-            if (r < rows) {
-              asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
-              if (copies > 1)
-                asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst + (kHalf / 2) * 128), "l"(src)
-                             : "memory");
-            }
-          }
-        }
-        asm volatile("cp.async.wait_all;" ::: "memory");
-        fence_async_smem();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&c.q_full);
+        copy_queries<D>(a, it, paired, j, sq, 0, kHalf);
+        if (lane < 4) mbar_arrive(&c.q_full);
         return true;
       };
       if (paired && j == 1) {
@@ -894,6 +907,12 @@ __global__ void __launch_bounds__(kThreads, 1)
       const AttnPart it = c.item[slot];
       __syncwarp();
       if (lane == 0) mbar_arrive(&c.item_empty[slot]);
+      if (n_item == 0) {
+        // nothing to do yet: these warps fetch the first queries, each its rows (the
+        // producer, which is ahead later on, needs 2000 cycles for them)
+        copy_queries<D>(a, it, paired, j, smem + TC::Q_OFF + j * TILE, (warp & 3) * 32, (warp & 3) * 32 + 32);
+        if (lane == 0) mbar_arrive(&c.q_full);
+      }
       if (!(copies_of(paired, it.rows) > 1 ? sm.template part<2>(it, 0) : sm.template part<1>(it, paired))) break;
     }
     if (turns) sm.turn_leave(ok);
