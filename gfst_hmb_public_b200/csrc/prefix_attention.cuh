@@ -451,9 +451,9 @@ int attn_launch(const char* what, void (*kern)(P...), int64_t grid, int threads,
 
 // the kernels' launchers (each returns a status)
 constexpr int kAttnMaxGrid = 160;      // CTAs of a launch (two per SM of the FP32 kernel count as one here)
-constexpr int kAttnFmaRows = 32;       // rows of an item of the FP32 kernel
+constexpr int kAttnFmaRows = 64;       // rows of an item of the FP32 kernel
 constexpr int kAttnTcHalf = 128;       // rows of a tile of the tensor-core kernel
-// continuation rows: 32 for each of 320 CTAs of the FP32 kernel; 256 for a CTA's
+// continuation rows: 64 for each of 320 CTAs of the FP32 kernel; 256 for a CTA's
 // pairs and 128 for each of its two streams of the tensor-core kernel
 constexpr int kAttnFmaContRows = 2 * kAttnMaxGrid * kAttnFmaRows;
 constexpr int kAttnTcContRows = kAttnMaxGrid * 4 * kAttnTcHalf;

@@ -28,11 +28,12 @@ GFST_DEFINE_ERROR_WORD(g_attn_fma_error, read_attn_fma_error, "attention")
 
 namespace {
 
-constexpr int kRows = kAttnFmaRows;   // 32
+constexpr int kRows = kAttnFmaRows;   // 64
 constexpr int kKeys = 32;
 constexpr int kThreads = 256;
 constexpr int kWarps = kThreads / 32;
 constexpr int kPer = kRows / kWarps;  // rows of a warp
+constexpr int kWeightPitch = kKeys + 4;  // floats of a row of weights
 // A 32-key tile of up to four rows is memory bound, one of 32 rows took seven
 // times as long; an item's fixed cost is about four of the first (queries in,
 // partials out).
@@ -67,19 +68,14 @@ struct Vec<__half> {
     }
   }
 };
-// A row's partial result out: to its own place, or to this CTA's continuation
-// buffer.  A lane has columns k * 128 + 4 lane of n such runs.
-__device__ __forceinline__ void fma_put(const AttnArgs& a, const AttnPart& it, int r, int lane, float2 ml,
-                                        const float4* v, int n) {
+// Where a row's partial result goes: its own place, or this CTA's continuation
+// buffer; writes its (m, l) if told to.
+__device__ __forceinline__ float* fma_put(const AttnArgs& a, const AttnPart& it, int r, float2 ml, bool write) {
   int tok, hq;
   attn_row(a, it, r, tok, hq);
   const int64_t row = (int64_t)tok * (a.H * a.G) + hq;
   const int64_t crow = (int64_t)blockIdx.x * kRows + r;
-  float* o = it.first ? a.part_o[it.own] + row * a.dv : a.cont_o + crow * a.dv;
-#pragma unroll
-  for (int k = 0; k < 2; ++k)
-    if (k < n && k * 128 + lane * 4 < a.dv) *reinterpret_cast<float4*>(o + k * 128 + lane * 4) = v[k];
-  if (lane == 0) {
+  if (write) {
     if (it.first) {
       a.part_ml[it.own][row] = ml;
       a.part_next[it.own][row] = attn_next((blockIdx.x + 1) * kRows + r, it.n_cont, kRows);
@@ -87,7 +83,11 @@ __device__ __forceinline__ void fma_put(const AttnArgs& a, const AttnPart& it, i
       a.cont_ml[crow] = ml;
     }
   }
+  return it.first ? a.part_o[it.own] + row * a.dv : a.cont_o + crow * a.dv;
 }
+// Row r of an item lies in slot r / 8 of warp r % 8's eight: neighbours for the
+// lanes of a warp, and few rows are spread over all warps.
+__device__ __forceinline__ int slot_of(int r) { return (r & (kWarps - 1)) * kPer + (r >> 3); }
 
 // four elements of a row in shared memory
 template <typename T>
@@ -115,7 +115,7 @@ struct FmaLayout {
     kv = 0;
     q = 2 * stage;
     w = q + kRows * qp * 4;
-    rows = w + kRows * kKeys * 4;
+    rows = w + kRows * kWeightPitch * 4;
     bytes = rows + 2 * kKeys * 8;
   }
 };
@@ -256,7 +256,8 @@ __device__ __forceinline__ bool few_rows(const AttnArgs& a, const AttnPart& it, 
         o.x += u.x * f, o.y += u.y * f, o.z += u.z * f, o.w += u.w * f;
       }
     }
-    fma_put(a, it, warp, lane, make_float2(top, sum), &o, 1);
+    float* dst = fma_put(a, it, warp, make_float2(top, sum), lane == 0);
+    if (lane * 4 < a.dv) *reinterpret_cast<float4*>(dst + lane * 4) = o;
   }
   return bad;
 }
@@ -268,7 +269,7 @@ __global__ void __launch_bounds__(kThreads, 2) prefix_attention_fma_kernel(const
   float* sq = reinterpret_cast<float*>(smem + ly.q);
   int64_t* s_row = reinterpret_cast<int64_t*>(smem + ly.rows);  // [2][kKeys] pool row of a key, -1: zeros, -2: none
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  float* sw = reinterpret_cast<float*>(smem + ly.w) + warp * (kPer * kKeys);  // the warp's weights
+  float* sw = reinterpret_cast<float*>(smem + ly.w) + warp * (kPer * kWeightPitch);  // the warp's weights
   const T* Q = static_cast<const T*>(a.Q);
   const int kvr = a.d / Vec<T>::N, vvr = a.dv / Vec<T>::N, vpr = kvr + vvr;
 
@@ -340,31 +341,41 @@ __global__ void __launch_bounds__(kThreads, 2) prefix_attention_fma_kernel(const
       Vec<T>::get(__ldg(reinterpret_cast<const uint4*>(Q + tok * a.q_st + hq * a.q_sh) + v), f);
 #pragma unroll
       for (int x = 0; x < Vec<T>::N; x += 4)
-        *reinterpret_cast<float4*>(sq + r * ly.qp + v * Vec<T>::N + x) = make_float4(f[x], f[x + 1], f[x + 2], f[x + 3]);
+        *reinterpret_cast<float4*>(sq + slot_of(r) * ly.qp + v * Vec<T>::N + x) = make_float4(f[x], f[x + 1], f[x + 2], f[x + 3]);
     }
     if (it.rows <= 4 && s_line.few) {
       __syncthreads();
       float* sj = reinterpret_cast<float*>(smem);  // the stages' place
-      bad |= it.rows == 1   ? few_rows<T, 1>(a, it, sq, ly.qp, sj)
-             : it.rows == 2 ? few_rows<T, 2>(a, it, sq, ly.qp, sj)
-                            : few_rows<T, 4>(a, it, sq, ly.qp, sj);
+      bad |= it.rows == 1   ? few_rows<T, 1>(a, it, sq, slot_of(1) * ly.qp, sj)
+             : it.rows == 2 ? few_rows<T, 2>(a, it, sq, slot_of(1) * ly.qp, sj)
+                            : few_rows<T, 4>(a, it, sq, slot_of(1) * ly.qp, sj);
       continue;
     }
     find_rows(it.t0);
     find_rows(it.t0 + 1);
     __syncthreads();
     fetch(it.t0);
-    float m[kPer], l[kPer];
-    float4 acc[kPer][2];
+    // NR: rows of a lane (0: one row a warp, whose keys its lanes share out); Q: runs
+    // of 32 columns of a lane's values
+    auto run = [&](auto nr, auto nq) {
+      constexpr bool ONE = decltype(nr)::value == 0;
+      constexpr int NR = ONE ? 1 : decltype(nr)::value, Q32 = decltype(nq)::value, NK = ONE ? 1 : 4;
+      // scores: rows ry, ry + 4 of the warp's, keys kx, kx + 8 .. (ONE: key `lane`)
+      const int ry = lane >> 3, kx = lane & 7, key = ONE ? lane : kx;
+      constexpr int kOver = ONE ? 16 : 4;  // a row's lanes: 32 or 8
+      float m[NR], l[NR];
+      float4 acc[NR][Q32];
+      const float* q[NR];
+      int row[NR];
 #pragma unroll
-    for (int i = 0; i < kPer; ++i) {
-      m[i] = -INFINITY, l[i] = 0.f;
-      acc[i][0] = acc[i][1] = make_float4(0, 0, 0, 0);
-    }
-
-    // NR: rows of the warp (its last ones repeat where the item has fewer)
-    auto run = [&](auto nr) {
-      constexpr int NR = decltype(nr)::value;
+      for (int u = 0; u < NR; ++u) {
+        m[u] = -INFINITY, l[u] = 0.f;
+        // (rows behind the item's last repeat it)
+        row[u] = ONE ? warp : warp + kWarps * (ry + 4 * u);
+        q[u] = sq + slot_of(min(row[u], it.rows - 1)) * ly.qp;
+#pragma unroll
+        for (int c = 0; c < Q32; ++c) acc[u][c] = make_float4(0, 0, 0, 0);
+      }
 #pragma unroll 1
       for (int t = it.t0; t < it.t1; ++t) {
         if (t + 1 < it.t1) {
@@ -379,72 +390,98 @@ __global__ void __launch_bounds__(kThreads, 2) prefix_attention_fma_kernel(const
         const uint8_t* sv = sk + kKeys * ly.kp;
         const int key0 = t * kKeys, n = min(kKeys, it.len - key0);
         if (warp < it.rows) {
-          // scores: key `lane`, the warp's rows
-          float x[NR];
-          const float* q[NR];
+          float x[NR][NK];
 #pragma unroll
-          for (int i = 0; i < NR; ++i) x[i] = 0.f, q[i] = sq + min(warp + i * kWarps, it.rows - 1) * ly.qp;
-          const uint8_t* kr = sk + lane * ly.kp;
+          for (int u = 0; u < NR; ++u)
+#pragma unroll
+            for (int k = 0; k < NK; ++k) x[u][k] = 0.f;
+          const uint8_t* kr = sk + key * ly.kp;
 #pragma unroll 2
           for (int v = 0; v < kvr; ++v) {
-            float f[Vec<T>::N];
-            Vec<T>::get(*reinterpret_cast<const uint4*>(kr + v * 16), f);
+            float f[NK][Vec<T>::N];
 #pragma unroll
-            for (int i = 0; i < NR; ++i)
+            for (int k = 0; k < NK; ++k) Vec<T>::get(*reinterpret_cast<const uint4*>(kr + k * 8 * ly.kp + v * 16), f[k]);
 #pragma unroll
-              for (int c = 0; c < Vec<T>::N; c += 4) {
-                const float4 u = *reinterpret_cast<const float4*>(q[i] + v * Vec<T>::N + c);
-                x[i] = fmaf(f[c], u.x, x[i]), x[i] = fmaf(f[c + 1], u.y, x[i]);
-                x[i] = fmaf(f[c + 2], u.z, x[i]), x[i] = fmaf(f[c + 3], u.w, x[i]);
+            for (int c = 0; c < Vec<T>::N; c += 4)
+#pragma unroll
+              for (int u = 0; u < NR; ++u) {
+                const float4 y = *reinterpret_cast<const float4*>(q[u] + v * Vec<T>::N + c);
+#pragma unroll
+                for (int k = 0; k < NK; ++k) {
+                  x[u][k] = fmaf(f[k][c], y.x, x[u][k]), x[u][k] = fmaf(f[k][c + 1], y.y, x[u][k]);
+                  x[u][k] = fmaf(f[k][c + 2], y.z, x[u][k]), x[u][k] = fmaf(f[k][c + 3], y.w, x[u][k]);
+                }
               }
           }
-          // keys that a row sees, running maximum and sum
+          // keys that a row sees, running maximum and sum over its lanes
           int see[NR];
 #pragma unroll
-          for (int i = 0; i < NR; ++i) {
-            const int r = min(warp + i * kWarps, it.rows - 1);
-            see[i] = it.own ? min(n, it.see0 + (it.row0 + r) / a.G + 1 - key0) : n;
-            const float s = lane < see[i] ? x[i] * a.scale_log2 : -INFINITY;
-            float top = s;
+          for (int u = 0; u < NR; ++u) {
+            see[u] = it.own ? min(n, it.see0 + (it.row0 + min(row[u], it.rows - 1)) / a.G + 1 - key0) : n;
+            float top = -INFINITY;
 #pragma unroll
-            for (int o = 16; o >= 1; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-            const float now = fmaxf(m[i], top);
+            for (int k = 0; k < NK; ++k) {
+              x[u][k] = key + 8 * k < see[u] ? x[u][k] * a.scale_log2 : -INFINITY;
+              top = fmaxf(top, x[u][k]);
+            }
+#pragma unroll
+            for (int o = kOver; o >= 1; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+            const float now = fmaxf(m[u], top);
             const float base = now == -INFINITY ? 0.f : now;  // nothing seen yet: weights 0, and no inf - inf
-            const float p = exp2f(s - base), al = exp2f(m[i] - base);
-            float sum = p;
+            const float al = exp2f(m[u] - base);
+            float sum = 0.f;
 #pragma unroll
-            for (int o = 16; o >= 1; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-            m[i] = now;
-            l[i] = l[i] * al + sum;
+            for (int k = 0; k < NK; ++k) {
+              const float p = exp2f(x[u][k] - base);
+              sum += p;
+              sw[(ONE ? 0 : (ry + 4 * u) * kWeightPitch) + key + 8 * k] = p;
+            }
 #pragma unroll
-            for (int k = 0; k < 2; ++k)
-              acc[i][k].x *= al, acc[i][k].y *= al, acc[i][k].z *= al, acc[i][k].w *= al;
-            sw[i * kKeys + lane] = p;
+            for (int o = kOver; o >= 1; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+            m[u] = now;
+            l[u] = l[u] * al + sum;
+#pragma unroll
+            for (int c = 0; c < Q32; ++c)
+              acc[u][c].x *= al, acc[u][c].y *= al, acc[u][c].z *= al, acc[u][c].w *= al;
           }
           __syncwarp();
-          // values, four columns a lane (and four more beyond 128); a key beyond a
-          // row's own has weight 0, but 0 * (inf or NaN) is NaN, so it is left out
+          // values, four of every 32 columns a lane; a key beyond a row's own has
+          // weight 0, but 0 * (inf or NaN) is NaN, so it is left out
           const bool ragged = it.own && key0 + n > it.see0 + it.row0 / a.G + 1;
           auto add = [&](auto guard) {
 #pragma unroll 1
             for (int j0 = 0; j0 < n; j0 += 4) {
+              if constexpr (ONE) {
+                // a key every eight lanes
+                const int j = j0 + ry;
+                if (j >= (decltype(guard)::value ? see[0] : n)) continue;
+                const float w = sw[j];
+#pragma unroll
+                for (int c = 0; c < Q32; ++c) {
+                  if (c * 32 >= a.dv) break;
+                  const float4 v = four<T>(sv + j * ly.vp, c * 32 + kx * 4);
+                  acc[0][c].x = fmaf(w, v.x, acc[0][c].x), acc[0][c].y = fmaf(w, v.y, acc[0][c].y);
+                  acc[0][c].z = fmaf(w, v.z, acc[0][c].z), acc[0][c].w = fmaf(w, v.w, acc[0][c].w);
+                }
+                continue;
+              }
               float4 p[NR];
 #pragma unroll
-              for (int i = 0; i < NR; ++i) p[i] = *reinterpret_cast<const float4*>(sw + i * kKeys + j0);
+              for (int u = 0; u < NR; ++u)
+                p[u] = *reinterpret_cast<const float4*>(sw + (ry + 4 * u) * kWeightPitch + j0);
 #pragma unroll
-              for (int u = 0; u < 4; ++u) {
-                if (j0 + u >= n) break;
+              for (int y = 0; y < 4; ++y) {
+                if (j0 + y >= n) break;
 #pragma unroll
-                for (int k = 0; k < 2; ++k) {
-                  const int c = k * 128 + lane * 4;
-                  if (c >= a.dv) continue;
-                  const float4 v = four<T>(sv + (j0 + u) * ly.vp, c);
+                for (int c = 0; c < Q32; ++c) {
+                  if (c * 32 >= a.dv) break;  // (a lane's columns behind the last are not kept)
+                  const float4 v = four<T>(sv + (j0 + y) * ly.vp, c * 32 + kx * 4);
 #pragma unroll
-                  for (int i = 0; i < NR; ++i) {
-                    if (decltype(guard)::value && j0 + u >= see[i]) continue;
-                    const float w = u == 0 ? p[i].x : u == 1 ? p[i].y : u == 2 ? p[i].z : p[i].w;
-                    acc[i][k].x = fmaf(w, v.x, acc[i][k].x), acc[i][k].y = fmaf(w, v.y, acc[i][k].y);
-                    acc[i][k].z = fmaf(w, v.z, acc[i][k].z), acc[i][k].w = fmaf(w, v.w, acc[i][k].w);
+                  for (int u = 0; u < NR; ++u) {
+                    if (decltype(guard)::value && j0 + y >= see[u]) continue;
+                    const float w = y == 0 ? p[u].x : y == 1 ? p[u].y : y == 2 ? p[u].z : p[u].w;
+                    acc[u][c].x = fmaf(w, v.x, acc[u][c].x), acc[u][c].y = fmaf(w, v.y, acc[u][c].y);
+                    acc[u][c].z = fmaf(w, v.z, acc[u][c].z), acc[u][c].w = fmaf(w, v.w, acc[u][c].w);
                   }
                 }
               }
@@ -452,21 +489,38 @@ __global__ void __launch_bounds__(kThreads, 2) prefix_attention_fma_kernel(const
           };
           if (ragged) add(IC<1>{});
           else add(IC<0>{});
+          __syncwarp();  // the weights may be written again
         }
         __syncthreads();  // the stage may be filled again, and the next rows are known
       }
-    };
-    if (it.rows <= kWarps) run(IC<1>{});
-    else if (it.rows <= 2 * kWarps) run(IC<2>{});
-    else run(IC<4>{});
-
-    // partial results: the row's own place, or this CTA's continuation buffer
+      if constexpr (ONE) {
 #pragma unroll
-    for (int i = 0; i < kPer; ++i) {
-      const int r = warp + i * kWarps;
-      if (r >= it.rows) break;
-      fma_put(a, it, r, lane, make_float2(m[i], l[i]), acc[i], 2);
-    }
+        for (int c = 0; c < Q32; ++c)
+#pragma unroll
+          for (int o = 8; o <= 16; o <<= 1) {
+            acc[0][c].x += __shfl_xor_sync(0xffffffffu, acc[0][c].x, o);
+            acc[0][c].y += __shfl_xor_sync(0xffffffffu, acc[0][c].y, o);
+            acc[0][c].z += __shfl_xor_sync(0xffffffffu, acc[0][c].z, o);
+            acc[0][c].w += __shfl_xor_sync(0xffffffffu, acc[0][c].w, o);
+          }
+      }
+      // partial results: the row's own place, or this CTA's continuation buffer
+#pragma unroll
+      for (int u = 0; u < NR; ++u) {
+        if (row[u] >= it.rows || (ONE && ry > 0)) continue;
+        float* dst = fma_put(a, it, row[u], make_float2(m[u], l[u]), kx == 0);
+#pragma unroll
+        for (int c = 0; c < Q32; ++c)
+          if (c * 32 + kx * 4 < a.dv) *reinterpret_cast<float4*>(dst + c * 32 + kx * 4) = acc[u][c];
+      }
+    };
+    auto rows = [&](auto nq) {
+      if (it.rows <= kWarps) run(IC<0>{}, nq);
+      else if (it.rows <= 4 * kWarps) run(IC<1>{}, nq);
+      else run(IC<2>{}, nq);
+    };
+    if (a.dv <= 128) rows(IC<4>{});
+    else rows(IC<8>{});
   }
   if (bad) atomicExch(&g_attn_fma_error, (unsigned)GFST_ERR_ARG);
 }
