@@ -3,21 +3,28 @@
 // the 32-bit memory, whose products the tensor cores would round, and the
 // shapes the tensor-core kernel does not tile.
 //
-// One CTA walks its share of the items (prefix_attention.cuh), 32 query rows
+// One CTA walks its share of the items (prefix_attention.cuh), up to 64 query rows
 // against 32-key tiles.  Keys and values arrive by cp.async in the pools' own
-// type, the next tile under this one's arithmetic.  Warp w has rows w, w + 8,
-// w + 16, w + 24 to itself: a lane scores one key against its rows, the warp
-// reduces maximum and sum by shuffles, leaves the weights in its own corner of
-// shared memory and then adds value rows, four columns a lane -- no barrier but
-// the tile's two.  What bounds it: shared-memory reads, 8 wavefronts for 16 warp
-// FMAs of the scores.
+// type, the next tile under this one's arithmetic.  Warp w has rows w, w + 8, ..
+// to itself: a lane scores up to two of them against four keys (items of up to
+// eight rows: one row against one key), eight lanes reduce a row's maximum and sum
+// by shuffles, the weights go to the warp's own corner of shared memory, and then
+// value rows are added, four of every 32 columns a lane -- no barrier but the
+// tile's two.  What bounds it: the latency of shared-memory reads with 16 warps on
+// an SM (registers allow no more), 3.4 wavefronts each for 16 or 32 products.
 //
 // Items of up to four rows (a decode step's) would leave warps idle and wait for
-// each tile: they go key by key instead, straight from memory.  Eight lanes have
-// a key, 16 bytes of every 128 each; a warp four keys of the 32-key tile.  Every
-// group of eight lanes keeps its own maximum, sum and values over its keys and
-// all are joined when the part ends, so the loop has no barrier at all and the
-// bytes of K and V bound it.
+// each tile: they go key by key instead.  Eight lanes have a key, 16 bytes of
+// every 128 each; a warp four keys of the 32-key tile.  A lane copies the pieces
+// that it reads itself, two tiles ahead, so that it waits for its own copies alone.
+// Every group of eight lanes keeps its own maximum, sum and values over its keys
+// and all are joined when the part ends, so the loop has no barrier at all.
+//
+// Measured, 32-bit, d = 128: 16 one-token requests of up to 8000 tokens (8 heads x
+// 4) 110 us, 2.95 TB/s; prompt pieces of 200 to 600 tokens (4 heads x 2) 499 us, 17
+// TFLOP/s; d = 64, 64 requests behind 4000 tokens (4 x 4) 90 us, 12 TFLOP/s.
+// Keys read straight into registers: 144 us for the first, 1.3 us less for the
+// smallest call.
 #include <cuda_fp16.h>
 
 #include "prefix_attention.cuh"
@@ -34,9 +41,10 @@ constexpr int kThreads = 256;
 constexpr int kWarps = kThreads / 32;
 constexpr int kPer = kRows / kWarps;  // rows of a warp
 constexpr int kWeightPitch = kKeys + 4;  // floats of a row of weights
-// A 32-key tile of up to four rows is memory bound, one of 32 rows took seven
-// times as long; an item's fixed cost is about four of the first (queries in,
-// partials out).
+// A 32-key tile of 64 rows counts eight of one of up to four rows, an item four
+// (queries in, partials out).  12 or 16 for a tile of 64 rows, and costs of 2 to 10
+// for an item, were slower over the range (decode 115-135 us for 110, prompt pieces
+// 484-514 for 499).
 using Cut = AttnCutAll<kRows, kKeys, 4, 8>;
 
 template <typename T>
@@ -120,11 +128,13 @@ struct FmaLayout {
   }
 };
 
-// Up to NR rows, key by key (see above); d and dv up to 128.  sj: shared memory
-// for the warps' sets, NR rows of dv + 4 floats each.  Returns whether a table
-// entry outside the pool was met.
+// Up to NR rows, key by key (see above); d and dv up to 128; qp: from one row's
+// queries to the next.  smem: two stages, and when the part is done the warps'
+// sets, NR rows of dv + 4 floats each.  Returns whether a table entry outside the
+// pool was met.
 template <typename T, int NR>
-__device__ __forceinline__ bool few_rows(const AttnArgs& a, const AttnPart& it, const float* sq, int qp, float* sj) {
+__device__ __forceinline__ bool few_rows(const AttnArgs& a, const AttnPart& it, const float* sq, int qp,
+                                         const FmaLayout& ly, uint8_t* smem) {
   constexpr int N = Vec<T>::N, S = 16 / N;            // elements and 16-byte pieces of a lane
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, grp = lane >> 3, piece = lane & 7;
   const int kvr = a.d / N, vvr = a.dv / N;
@@ -147,33 +157,47 @@ __device__ __forceinline__ bool few_rows(const AttnArgs& a, const AttnPart& it, 
 #pragma unroll
     for (int c = 0; c < 16; ++c) acc[i][c] = 0.f;
   }
-  int64_t row = row_of(it.t0);
+  // two tiles ahead: a lane copies what it will read itself, so it only waits for
+  // its own copies
+  uint8_t* sk = smem + (warp * 4 + grp) * ly.kp + piece * 16;
+  uint8_t* sv = smem + kKeys * ly.kp + (warp * 4 + grp) * ly.vp + piece * 16;
+  auto fetch = [&](int t) {
+    const int64_t row = row_of(t);
+    if (row != -2) {
+      const int64_t at = max(row, (int64_t)0);
+      const int bytes = row >= 0 ? 16 : 0;  // a table entry outside the pool: zeros
+#pragma unroll
+      for (int kv = 0; kv < 2; ++kv) {
+        const uint8_t* src = kv ? reinterpret_cast<const uint8_t*>(static_cast<const T*>(a.pool_V) + at * a.dv)
+                                : reinterpret_cast<const uint8_t*>(static_cast<const T*>(a.pool_K) + at * a.d);
+        const uint32_t dst = (uint32_t)__cvta_generic_to_shared((kv ? sv : sk) + (t & 1) * ly.stage);
+#pragma unroll
+        for (int s = 0; s < S; ++s)
+          if (s * 8 + piece < (kv ? vvr : kvr))
+            asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst + s * 128),
+                         "l"(src + (s * 8 + piece) * 16), "r"(bytes)
+                         : "memory");
+      }
+    }
+    asm volatile("cp.async.commit_group;" ::: "memory");
+  };
+  fetch(it.t0);
+  fetch(it.t0 + 1);
 #pragma unroll 1
   for (int t = it.t0; t < it.t1; ++t) {
-    uint4 k[S], v[S];
-    const uint4* kp = reinterpret_cast<const uint4*>(static_cast<const T*>(a.pool_K) + row * a.d);
-    const uint4* vp = reinterpret_cast<const uint4*>(static_cast<const T*>(a.pool_V) + row * a.dv);
-#pragma unroll
-    for (int s = 0; s < S; ++s) {
-      const int x = s * 8 + piece;
-      k[s] = row >= 0 && x < kvr ? __ldg(kp + x) : make_uint4(0, 0, 0, 0);
-    }
-#pragma unroll
-    for (int s = 0; s < S; ++s) {
-      const int x = s * 8 + piece;
-      v[s] = row >= 0 && x < vvr ? __ldg(vp + x) : make_uint4(0, 0, 0, 0);
-    }
+    asm volatile("cp.async.wait_group 1;" ::: "memory");
     const int p0 = t * kKeys + warp * 4 + grp;
-    const bool key = row != -2;
-    row = row_of(t + 1);
+    const bool key = p0 < it.len;
+    const uint8_t* ks = sk + (t & 1) * ly.stage;
+    const uint8_t* vs = sv + (t & 1) * ly.stage;
     float x[NR];
 #pragma unroll
     for (int i = 0; i < NR; ++i) x[i] = 0.f;
 #pragma unroll
     for (int s = 0; s < S; ++s) {
-      float f[N];
-      Vec<T>::get(k[s], f);
       if (s * 8 + piece < kvr) {
+        float f[N];
+        Vec<T>::get(*reinterpret_cast<const uint4*>(ks + s * 128), f);
 #pragma unroll
         for (int i = 0; i < NR; ++i)
 #pragma unroll
@@ -184,6 +208,8 @@ __device__ __forceinline__ bool few_rows(const AttnArgs& a, const AttnPart& it, 
           }
       }
     }
+    float w[NR];
+    bool any = false;
 #pragma unroll
     for (int i = 0; i < NR; ++i) {
 #pragma unroll
@@ -191,6 +217,7 @@ __device__ __forceinline__ bool few_rows(const AttnArgs& a, const AttnPart& it, 
       // a key that the row does not see is left out (its values may be inf or NaN)
       const bool seen = key && p0 < see[i];
       const float s = x[i] * a.scale_log2;
+      w[i] = -1.f;
       if (seen) {
         if (s > m[i]) {
           const float al = exp2f(m[i] - s);
@@ -200,18 +227,29 @@ __device__ __forceinline__ bool few_rows(const AttnArgs& a, const AttnPart& it, 
           for (int c = 0; c < 16; ++c) acc[i][c] *= al;
         }
         // only scores of -inf seen: weight 0
-        const float w = exp2f(s - (m[i] == -INFINITY ? 0.f : m[i]));
-        l[i] += w;
+        w[i] = exp2f(s - (m[i] == -INFINITY ? 0.f : m[i]));
+        l[i] += w[i];
+        any = true;
+      }
+    }
+    if (any) {
 #pragma unroll
-        for (int q = 0; q < S; ++q) {
-          float f[N];
-          Vec<T>::get(v[q], f);
+      for (int q = 0; q < S; ++q) {
+        if (q * 8 + piece >= vvr) continue;
+        float f[N];
+        Vec<T>::get(*reinterpret_cast<const uint4*>(vs + q * 128), f);
 #pragma unroll
-          for (int c = 0; c < N; ++c) acc[i][q * N + c] = fmaf(w, f[c], acc[i][q * N + c]);
+        for (int i = 0; i < NR; ++i) {
+          if (w[i] < 0.f) continue;
+#pragma unroll
+          for (int c = 0; c < N; ++c) acc[i][q * N + c] = fmaf(w[i], f[c], acc[i][q * N + c]);
         }
       }
     }
+    fetch(t + 2);  // into the stage just read
   }
+  __syncthreads();  // all warps are done with the stages
+  float* sj = reinterpret_cast<float*>(smem);
   // the warp's four groups, then the warps through shared memory
 #pragma unroll
   for (int i = 0; i < NR; ++i) {
@@ -345,10 +383,10 @@ __global__ void __launch_bounds__(kThreads, 2) prefix_attention_fma_kernel(const
     }
     if (it.rows <= 4 && s_line.few) {
       __syncthreads();
-      float* sj = reinterpret_cast<float*>(smem);  // the stages' place
-      bad |= it.rows == 1   ? few_rows<T, 1>(a, it, sq, slot_of(1) * ly.qp, sj)
-             : it.rows == 2 ? few_rows<T, 2>(a, it, sq, slot_of(1) * ly.qp, sj)
-                            : few_rows<T, 4>(a, it, sq, slot_of(1) * ly.qp, sj);
+      const int qp = slot_of(1) * ly.qp;
+      bad |= it.rows == 1   ? few_rows<T, 1>(a, it, sq, qp, ly, smem)
+             : it.rows == 2 ? few_rows<T, 2>(a, it, sq, qp, ly, smem)
+                            : few_rows<T, 4>(a, it, sq, qp, ly, smem);
       continue;
     }
     find_rows(it.t0);
