@@ -2,16 +2,28 @@
 // d = dv = 64 or 128, blocks that tile 128 keys (L a divisor of 128 from 8 up,
 // or a multiple of 128).
 //
-// A CTA (one per SM) runs two streams, each with a 128-row query tile:
-//   S = Q K^T     tcgen05.mma, both operands in shared memory, S in TMEM
+// A CTA (one per SM) runs two streams, each with a 128-row query tile, over units
+// of 64 keys (half of a 128-key stage):
+//   S = Q K^T     tcgen05.mma, both operands in shared memory, S in one of two TMEM
+//                 buffers, so that the next unit's scores are there in time
 //   P = 2^(c S - m) by four warps, one row per thread, rounded to the pools'
 //                 type and stored back to TMEM over S
 //   O += P V      tcgen05.mma, P from TMEM, V from shared memory (keys along
 //                 the contraction: V is the MN-major operand), O in TMEM
-// While one stream's rows are exponentiated, the other's products run.  Per
-// 128 x 128 tile at d = 128 the products take 1024 tensor cycles and the 16,384
-// exponentials 1024 cycles of the SM's special-function units: with many rows
-// the two bound the kernel together; with few rows the bytes of K and V do.
+// While one stream's rows are exponentiated, the other's products run.  For a unit
+// of both streams at d = 128 the products take 1230 tensor cycles (S 384: its
+// operands come from shared memory at 128 bytes a cycle; O 230) and the 16,384
+// exponentials 1024 cycles of the SM's special-function units; a unit takes 1930,
+// because a thread's loads, maximum, exponentials, sums and stores follow one
+// another and there is room for two such warps on a quarter of the SM.
+//
+// Measured, bf16, d = 128: 512 one-token requests behind 32,768 tokens (4 heads x
+// 8) 345 us, 800 TFLOP/s; prompt pieces of 12 requests behind 4096 tokens (8 x 4)
+// 925 us with the merge, 790 TFLOP/s; 16 requests of 4096 to 32,767 tokens 141 us,
+// 5.9 TB/s; 64 requests behind 8192 tokens 47 us.  Tried and slower: two threads a
+// row, each with half of the keys, that exchange maxima (the same for the document,
+// 7 % slower for prompts); a polynomial in place of some exponentials; tiles
+// prefetched into L2.
 //
 // Two kinds of work (prefix_attention.cuh), each cut evenly over the CTAs:
 //   pairs   items of more than 128 rows: both streams take the same K and V
