@@ -57,14 +57,16 @@ def _no_grad(what: str, *tensors: torch.Tensor) -> None:
 
 def _cuda(what: str, *tensors: torch.Tensor | None) -> int:
     """Index of the CUDA device that holds every given tensor; raises as nat.require_cuda does."""
-    first = tensors[0]
-    if isinstance(first, torch.Tensor) and first.is_cuda:
-        index = first.get_device()
-        for t in tensors:
-            if t is not None and not (isinstance(t, torch.Tensor) and t.is_cuda and t.get_device() == index):
-                break
-        else:
-            return index
+    try:
+        index = tensors[0].get_device()  # -1: not on a GPU
+        if index >= 0:
+            for t in tensors:
+                if t is not None and t.get_device() != index:
+                    break
+            else:
+                return index
+    except AttributeError:  # no tensor
+        pass
     return nat.require_cuda(*tensors, what=what).index
 
 
@@ -73,7 +75,7 @@ def _call(index: int, name: str, *args) -> None:
     fn = _ENTRY.get(name)
     if fn is None:
         fn = _ENTRY[name] = getattr(nat.load(), name)
-    stream = torch.cuda.current_stream(index).cuda_stream
+    stream = torch._C._cuda_getCurrentRawStream(index)  # current_stream(index).cuda_stream, without its 1.2 us
     if torch.cuda.current_device() == index:
         status = fn(*args, stream)
     else:
@@ -181,11 +183,12 @@ def block_tables(lens: torch.Tensor, new_lens: torch.Tensor, tables: torch.Tenso
 
 
 def _check_pools(what: str, pool_K: torch.Tensor, pool_V: torch.Tensor) -> tuple:
-    if pool_K.ndim != 4 or pool_V.ndim != 4 or pool_K.shape[:3] != pool_V.shape[:3]:
+    k, v = pool_K.shape, pool_V.shape
+    if len(k) != 4 or len(v) != 4 or k[0] != v[0] or k[1] != v[1] or k[2] != v[2]:
         raise ValueError(f"{what} expects pool_K [n_blocks, heads, L, d] and pool_V [n_blocks, heads, L, dv]")
     if not (pool_K.is_contiguous() and pool_V.is_contiguous()):
         raise ValueError(f"{what}: pools must be contiguous")
-    return (*pool_K.shape, pool_V.shape[3])
+    return (*k, v[3])
 
 
 def paged_append(K: torch.Tensor, V: torch.Tensor, pool_K: torch.Tensor, pool_V: torch.Tensor,
