@@ -19,7 +19,7 @@
 //
 // Measured, bf16, d = 128: 512 one-token requests behind 32,768 tokens (4 heads x
 // 8) 345 us, 800 TFLOP/s; prompt pieces of 12 requests behind 4096 tokens (8 x 4)
-// 925 us with the merge, 790 TFLOP/s; 16 requests of 4096 to 32,767 tokens 141 us,
+// 868 us with the merge, 840 TFLOP/s; 16 requests of 4096 to 32,767 tokens 141 us,
 // 5.9 TB/s; 64 requests behind 8192 tokens 47 us.  Tried and slower: two threads a
 // row, each with half of the keys, that exchange maxima (the same for the document,
 // 7 % slower for prompts); a polynomial in place of some exponentials; tiles
@@ -74,10 +74,12 @@ constexpr int kJoinRows = 16;                         // rows of joining copies 
 constexpr int kStageBytes = 2 * kJoinRows * 128 * 4;  // a stream's rows of joining copies (copies_of)
 
 // Costs in units of about 500 cycles of a CTA, from measured parts: a 256-row
-// tile takes about 4200 cycles and its item 16,000 more (queries in, first
-// scores, partials out); of the rest two streams run at once, so a tile of 3400
-// counts 1700 and an item's 8000 count 4000.
-using Pairs = AttnCutPairs<kHalf, kKeys, 30, 8>;
+// tile takes about 4200 cycles; of the rest two streams run at once, so a tile of
+// 3400 counts 1700 and an item's 8000 (queries in, first scores, partials out)
+// count 4000.  A pair's item alone would count 16,000, but 48 units spread the work
+// better: with 30, prompt pieces took 929 us for 868; with 60, drafted tokens 45.5
+// for 41.6; from 22 to 60 the other cases are within 2 %.
+using Pairs = AttnCutPairs<kHalf, kKeys, 48, 8>;
 using Rest = AttnCutRest<kHalf, kKeys, 8, 3>;
 
 template <int D>
