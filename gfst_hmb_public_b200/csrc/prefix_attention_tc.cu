@@ -32,8 +32,9 @@
 //           own stages, so two items are in flight on an SM
 //
 // Warps: 0-3 and 4-7 softmax of stream 0 and 1 (warp w reads TMEM lanes 32 (w %
-// 4) ..); 8, 9 the streams' producers (work list, queries by cp.async, K and V by
-// TMA, one box per block and 64 columns); 10, 11 their MMA issuers.
+// 4) ..); 8, 9 the streams' producers (work list, K and V by TMA, one box per block
+// and 64 columns, queries by cp.async but for the first part's, which the softmax
+// warps fetch); 10, 11 their MMA issuers.
 //
 // The maximum is followed lazily: m only moves when a row's new maximum exceeds
 // it by more than 8 (in log2), so O in TMEM is rescaled a few times per row and
