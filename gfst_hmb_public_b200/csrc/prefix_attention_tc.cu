@@ -560,9 +560,11 @@ struct Softmax {
       if (write) a.cont_ml[crow0 + r_] = ml;
       return a.cont_o + (crow0 + r_) * D;
     };
-    if (C > 1 && live) c.ml[copy][r] = make_float2(m, l);  // read behind the next meeting
     if (!wait.warp(&c.pv_done[(n_unit - 1) & 1], ((n_unit - 1) >> 1) & 1)) return false;
     tc_fence_after();
+    // only here: that product waited for this part's weights of all four warps, which
+    // by then were done with the last part's references (read behind the next meeting)
+    if (C > 1 && live) c.ml[copy][r] = make_float2(m, l);
     if constexpr (C == 1) {
       if (warp_live) {
         // 32 columns of the warp's 32 rows at a time through shared memory, so that
@@ -592,7 +594,8 @@ struct Softmax {
     } else {
       // both copies through shared memory, 16 rows at a time; the four warps join
       // them at the larger reference, a row of D values a warp.  (The next part
-      // writes the stage and c.ml behind products that wait for all four warps.)
+      // writes the stage and c.ml behind its last product, which waits for all four
+      // warps' weights.)
       constexpr int P = D / 4;                           // 16-byte pieces of a row
       float4* st = reinterpret_cast<float4*>(smem + TC::STAGE_OFF + j * kStageBytes);
 #pragma unroll 1
