@@ -80,7 +80,10 @@ __global__ void __launch_bounds__(kMergeThreads) prefix_attention_merge_kernel(c
   }
   const int tok = (int)row / heads;
   const bool live = tok < attn_tokens(a) && tok >= a.cu[0], prefix = live && attn_prefix_len(a) > 0;
-  if (!live && !a.fill_tail) return;
+  if (!live && !a.fill_tail) {  // the caller's rows of out stay, the log-sum-exp is of nothing
+    if (a.lse != nullptr && lane == 0) a.lse[row] = -INFINITY;
+    return;
+  }
   const bool has[2] = {prefix && !merge_empty(ml[0]), live && !merge_empty(ml[1])};
   MergeRow<V> x;
 #pragma unroll

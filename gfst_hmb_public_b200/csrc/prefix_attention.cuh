@@ -53,7 +53,7 @@ struct AttnArgs {
   float scale_log2;        // scale * log2(e)
   void* out;
   float* lse;              // or null
-  int fill_tail;           // tokens behind the last request: 1 = write 0 / -inf, 0 = leave
+  int fill_tail;           // out of tokens behind the last request: 1 = write 0, 0 = leave (lse: -inf)
   // partial results
   float* part_o[2];        // [n_tokens * H * G, dv]: prefix, own
   float2* part_ml[2];      // (m, l)

@@ -235,7 +235,7 @@ def prefix_attention(Q: torch.Tensor, pool_K: torch.Tensor, pool_V: torch.Tensor
     Returns (out [n, heads * group, dv], lse float32 [n, heads * group] or
     None).  A token that sees nothing gets zeros and -inf.  Tokens behind
     cu_new[B] (a padded batch) get the same; with ``out`` given (contiguous,
-    Q's dtype) their rows of it stay as they were.  A table entry outside the
+    Q's dtype) their rows of it stay as they were, and lse is -inf.  A table entry outside the
     pool within a request's length reads as zero keys and values and is
     reported by ``_native.check_device_errors``."""
     what = "prefix_attention"

@@ -653,8 +653,8 @@ GFST_API int gfst_paged_append(const void* K, int64_t k_stride_t, int64_t k_stri
  * out: [n_tokens, n_kv_heads * group, dv] dense; pools as gfst_paged_append;
  * tables: rows table_stride apart, width entries; prefix_len: [1] on the
  * device (prefix_width == 0: no prefix, both may be NULL); cu_new[0] == 0,
- * ascending.  Tokens behind cu_new[n_requests] get zeros and -inf when
- * fill_tail != 0 and are left as they were otherwise.  FP32 softmax statistics
+ * ascending.  Tokens behind cu_new[n_requests] get zeros and -inf; with
+ * fill_tail == 0 their rows of out are left as they were.  FP32 softmax statistics
  * and sums, one rounding of out; 16-bit weights p on the tensor cores are
  * rounded to the pools' type.  Lengths beyond the tables' positions are cut to
  * them; a table entry outside [0, n_blocks) reads as zero keys and values and

@@ -4,9 +4,16 @@ import numpy as np
 import pytest
 import torch
 
-from test_gpu_paged import BF16, FP16, Setup
+from gfst_hmb_public_b200 import paged
+from test_gpu_paged import BF16, F32, FP16, Setup, _dev
 
 pytestmark = pytest.mark.gpu
+
+
+def _soil(dev, floats):
+    """Leave numbers where the next allocation of that size begins."""
+    held = [torch.full((floats,), 7.0, device=dev) for _ in range(4)]
+    del held
 
 
 @pytest.mark.parametrize("dtype, d, G", [(BF16, 128, 1), (FP16, 64, 1), (BF16, 64, 2), (FP16, 128, 2)])
@@ -21,3 +28,25 @@ def test_many_one_tile_parts_of_few_rows_in_a_row(cuda_device, dtype, d, G):
     for _ in range(5):
         again, lse2 = s.run()
         assert torch.equal(out, again) and torch.equal(lse, lse2)
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+def test_log_sum_exp_of_padding_beside_a_given_out(cuda_device, dtype):
+    # ``out`` keeps its padding rows, the log-sum-exp is -inf there all the same
+    s = Setup(cuda_device, dtype, [30, 7], [2, 1], 40, 2, 2, 64, 16, seed=2)
+    Q = torch.cat([s.Q, torch.full((4, 4, 64), float("nan"), dtype=dtype, device=cuda_device)])
+    want, want_lse = s.run()
+    mine = torch.full((7, 4, 64), 5.0, dtype=dtype, device=cuda_device)
+    _soil(cuda_device, 7 * 4)
+    got, lse = s.run(Q=Q, out=mine)
+    assert got is mine and torch.equal(mine[:3], want) and (mine[3:] == 5.0).all()
+    assert torch.equal(lse[:3], want_lse) and torch.isneginf(lse[3:]).all()
+
+
+def test_log_sum_exp_of_a_short_step_beside_a_given_out(cuda_device):
+    mem = paged.PagedMemory(2, 16, 1, 64, max_requests=2, max_blocks=4, device=cuda_device)
+    t = mem.extend(_dev([40, 1], cuda_device), 41)
+    mine = torch.full((41, 2, 64), 5.0, dtype=BF16, device=cuda_device)
+    _soil(cuda_device, 41 * 2)
+    _, lse = mem.attend(torch.ones((41, 2, 64), dtype=BF16, device=cuda_device), t, out=mine, return_lse=True)
+    assert int(t.n_short) == 2 and (mine == 5.0).all() and torch.isneginf(lse).all()
