@@ -29,6 +29,7 @@ namespace {
 
 constexpr int kMaxRequests = 16384;  // three prefix sums of the step in one CTA's shared memory
 constexpr int kTablesMaxThreads = 1024;
+constexpr int kTablesStatic = 1024;  // at least the kernel's own shared memory (its warps' sums)
 
 struct TablesArgs {
   const int32_t* lens;
@@ -91,6 +92,7 @@ __global__ void __launch_bounds__(kTablesMaxThreads) block_tables_kernel(const T
   int32_t* s_back = s_first + a.B;  // [B] rank of its first returned block
   __shared__ int64_t w_add[33], w_want[33];  // by warp, then exclusive sums and the total
   __shared__ int w_grow[33], w_back[33];
+  static_assert(sizeof(w_add) + sizeof(w_want) + sizeof(w_grow) + sizeof(w_back) <= kTablesStatic, "shared memory");
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, n_warps = blockDim.x >> 5;
 
   const int head = min(max(a.free_state[0], 0), a.F - 1);
@@ -391,7 +393,7 @@ extern "C" int gfst_block_tables(const int32_t* lens, const int32_t* new_lens, c
   const int64_t wave = (int64_t)sms * (threads < kTablesMaxThreads ? 2 : 1);
   const int grid = (int)(want < wave ? want : wave);
   const size_t smem = ((size_t)3 * n_requests + 1) * 4;
-  if (smem > 48 * 1024) {
+  if (smem + kTablesStatic > 48 * 1024) {  // without leave, a launch has 48 KB of both together
     const cudaError_t e = cudaFuncSetAttribute(block_tables_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                                (kMaxRequests * 3 + 1) * 4);
     GFST_REQUIRE(e == cudaSuccess, GFST_ERR_DEVICE, "cudaFuncSetAttribute: %s", cudaGetErrorString(e));

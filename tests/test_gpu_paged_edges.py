@@ -1,5 +1,9 @@
 """Paged block memory on the GPU: calls at the edges of what its documentation
 allows.  Tolerances as in test_gpu_paged.py (``Setup.check``)."""
+import subprocess
+import sys
+from pathlib import Path
+
 import numpy as np
 import pytest
 import torch
@@ -8,6 +12,8 @@ from gfst_hmb_public_b200 import paged
 from test_gpu_paged import BF16, F32, FP16, Setup, _dev
 
 pytestmark = pytest.mark.gpu
+
+REPO = Path(__file__).resolve().parents[1]
 
 
 def _soil(dev, floats):
@@ -50,3 +56,16 @@ def test_log_sum_exp_of_a_short_step_beside_a_given_out(cuda_device):
     _soil(cuda_device, 41 * 2)
     _, lse = mem.attend(torch.ones((41, 2, 64), dtype=BF16, device=cuda_device), t, out=mine, return_lse=True)
     assert int(t.n_short) == 2 and (mine == 5.0).all() and torch.isneginf(lse).all()
+
+
+@pytest.mark.parametrize("B", [4029, 4030, 4095, 4096])
+def test_block_tables_around_48_kb_of_sums(cuda_device, B):
+    # in a process of its own: a larger call would have asked for the shared memory
+    code = (f"import sys; sys.path[:0] = {[str(REPO), str(REPO / 'tests')]!r}\n"
+            "import numpy as np, torch\n"
+            "from test_gpu_paged import _check_tables, _table_inputs\n"
+            f"inputs = _table_inputs(np.random.default_rng({B}), {B}, 5, 16, 60, 9, 0.1, 3)\n"
+            "for in_place in (False, True):\n"
+            "    _check_tables(torch.device('cuda:0'), inputs, 16, int(np.maximum(inputs[1], 0).sum()), in_place)\n")
+    run = subprocess.run([sys.executable, "-c", code], cwd=REPO, capture_output=True, text=True, timeout=300)
+    assert run.returncode == 0, run.stderr[-2000:]
