@@ -641,8 +641,8 @@ GFST_API int gfst_paged_append(const void* K, int64_t k_stride_t, int64_t k_stri
                                int n_heads, int d, int dv, int dtype, cudaStream_t stream);
 
 /* ---- paged memory: attention behind a shared prefix -------------------------
- * For token t, the i-th of the n_b = cu_new[b+1] - cu_new[b] new tokens of
- * request b, and query head hq = h * group + g (h in [0, n_kv_heads)):
+ * For token t < n_tokens, the i-th of the n_b = cu_new[b+1] - cu_new[b] new tokens
+ * of request b, and query head hq = h * group + g (h in [0, n_kv_heads)):
  *   out[t, hq] = sum_j p_j v_j / sum_j p_j,  p_j = exp(scale * q . k_j),
  *   lse[t, hq] = log(sum_j p_j)  (natural logarithm; lse may be NULL)
  * over the prefix_len positions of the prefix (blocks prefix_table[0 ..]) and

@@ -69,3 +69,13 @@ def test_block_tables_around_48_kb_of_sums(cuda_device, B):
             "    _check_tables(torch.device('cuda:0'), inputs, 16, int(np.maximum(inputs[1], 0).sum()), in_place)\n")
     run = subprocess.run([sys.executable, "-c", code], cwd=REPO, capture_output=True, text=True, timeout=300)
     assert run.returncode == 0, run.stderr[-2000:]
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("rows", [1, 5, 20, 47])
+def test_fewer_packed_rows_than_new_tokens(cuda_device, dtype, rows):
+    # the offsets count tokens whose queries are not there: the others see what they would see beside them
+    s = Setup(cuda_device, dtype, [90, 200], [8, 40], 33, 2, 4, 64, 16, seed=21)
+    out, lse = s.run(Q=s.Q[:rows])
+    assert out.shape[0] == rows
+    s.check(out, lse, slice(0, rows))
