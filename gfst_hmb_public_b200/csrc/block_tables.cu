@@ -17,8 +17,9 @@
 // the sums itself (the lengths stay in L2 and a scan of 4096 requests is four
 // loads and one block scan), then fills its share of the table entries and of
 // the slots, each found by its own arithmetic -- no CTA waits for another.  A
-// step in place that wants more blocks than there are leaves everything as it
-// was (every CTA knows it from the sums), so that it can be taken again.
+// step in place that wants more blocks than there are, or has more tokens than
+// slots to fill, leaves everything as it was (every CTA knows it from the sums), so
+// that it can be taken again.
 // What bounds it: launch and scan latency for a decode batch (256 requests of up
 // to 512 blocks: 5 us); for thousands of requests the table rows written, 4 B per
 // entry (4096 x 1024 entries and 0.8 M tokens: 16 us for 25 MB).
@@ -157,11 +158,15 @@ __global__ void __launch_bounds__(kTablesMaxThreads) block_tables_kernel(const T
   __syncthreads();
 
   const int taken = min(t_grow, count);
-  const int32_t lacking = clamp32((int64_t)(t_grow - taken) + t_want);
+  const bool in_place = a.tables == a.tables_out;
+  // in place, tokens that the slot map has no room for are lacking as well: they
+  // would count as held and never be written
+  const int64_t unheld = in_place ? max(t_add - a.n_tokens, (int64_t)0) : 0;
+  const int32_t lacking = clamp32((int64_t)(t_grow - taken) + t_want + unheld);
   const int64_t stride = (int64_t)gridDim.x * blockDim.x;
   const int64_t first = (int64_t)blockIdx.x * blockDim.x + tid;
 
-  if (lacking > 0 && a.tables == a.tables_out) {
+  if (lacking > 0 && in_place) {
     // a step in place that cannot be had: lengths, tables and ring stay, no token has a slot
     if (blockIdx.x == 0) {
       for (int b = tid; b <= a.B; b += blockDim.x) a.cu_new[b] = 0;

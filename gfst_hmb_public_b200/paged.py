@@ -138,7 +138,8 @@ def block_tables(lens: torch.Tensor, new_lens: torch.Tensor, tables: torch.Tenso
 
     A step that wants more blocks than there are has n_short > 0 and is not to
     be used; in place (``tables_out`` is ``tables``) it changes nothing, and no
-    token of it has a slot."""
+    token of it has a slot.  So does a step in place with more new tokens than
+    ``n_tokens``: n_short counts them too."""
     what = "block_tables"
     index = _cuda(what, lens, new_lens, tables, free_ring, free_state, tables_out)
     if tables.ndim != 2 or free_ring.ndim != 1:
@@ -325,10 +326,12 @@ class PagedMemory:
     def extend(self, new_lens: torch.Tensor, n_tokens: int) -> BlockTables:
         """Take and return blocks for one step; updates the memory's tables,
         lengths and free ring in place and returns the step (whose ``tables`` and
-        ``lens`` are the memory's own).  ``n_short`` of the step says how many
-        blocks the pool was short of; read it when the host waits anyway.  A step
-        with n_short > 0 did nothing: no request grew or ended, its tokens have no
-        slots and attend to nothing.  End a request and take it again."""
+        ``lens`` are the memory's own).  ``n_tokens`` is at least the sum of the
+        positive new_lens.  ``n_short`` of the step says how many blocks the pool,
+        and how many tokens ``n_tokens``, was short of; read it when the host waits
+        anyway.  A step with n_short > 0 did nothing: no request grew or ended, its
+        tokens have no slots and attend to nothing.  End a request (or pass more
+        tokens) and take it again."""
         t = block_tables(self.lens, new_lens, self.tables, self.free_ring, self.free_state,
                          block_len=self.block_len, n_tokens=n_tokens, tables_out=self.tables)
         self.lens.copy_(t.lens)

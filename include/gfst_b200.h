@@ -614,9 +614,12 @@ GFST_API int gfst_mpuc_recurrent_scan(const gfst_mpuc_weights* weights, int fast
  * free_ring (updated in place), n_short [1] = blocks that were wanted and not
  * had (ring empty, or beyond `width`): their table entries and slots are -1
  * and lens_out counts their tokens all the same, so a step with n_short > 0 is
- * not to be used.  In place (tables_out == tables) such a step changes nothing
- * instead: tables, ring, lens_out and free_state_out are as given, cu_new is 0
- * and every slot -1; it can be taken again once there is room.  lens_out and free_state_out must not alias the inputs.
+ * not to be used.  n_tokens is to be at least the sum of the positive new_lens;
+ * tokens behind it get no slot, but count in lens_out.  In place (tables_out ==
+ * tables) a step short of blocks or of n_tokens changes nothing instead: tables,
+ * ring, lens_out and free_state_out are as given, cu_new is 0, every slot -1, and
+ * n_short counts the tokens behind n_tokens too; it can be taken again once there
+ * is room.  lens_out and free_state_out must not alias the inputs.
  * All int32 on the device; nothing is read back.  Limits: n_requests <= 16384;
  * n_blocks * L, width * L and n_requests * width below 2^31.
  * No reference counterpart: its exact store holds one Python list of blocks

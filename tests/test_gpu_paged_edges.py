@@ -79,3 +79,22 @@ def test_fewer_packed_rows_than_new_tokens(cuda_device, dtype, rows):
     out, lse = s.run(Q=s.Q[:rows])
     assert out.shape[0] == rows
     s.check(out, lse, slice(0, rows))
+
+
+def test_step_in_place_with_fewer_rows_than_tokens_changes_nothing(cuda_device):
+    mem = paged.PagedMemory(12, 16, 1, 64, max_requests=3, max_blocks=5, device=cuda_device)
+    x = torch.randn((40, 1, 64), device=cuda_device).to(BF16)
+    mem.append(x, x, mem.extend(_dev([30, 10, 0], cuda_device), 40))
+    kept = (mem.tables, mem.lens, mem.free_ring, mem.free_state, mem.pool_K)
+    before = [t.clone() for t in kept]
+    new = _dev([3, -1, 18], cuda_device)
+    for n in (20, 3, 0):                                        # 21 tokens
+        t = mem.extend(new, n)
+        mem.append(x[:n], x[:n], t)
+        out, lse = mem.attend(torch.ones((n, 2, 64), dtype=BF16, device=cuda_device), t, return_lse=True)
+        assert int(t.n_short) == 21 - n
+        assert (t.cu_new == 0).all() and (t.slot_map == -1).all()
+        assert all(torch.equal(a, b) for a, b in zip(before, kept))
+        assert (out == 0).all() and torch.isneginf(lse).all()
+    t = mem.extend(new, 21)
+    assert int(t.n_short) == 0 and mem.lens.tolist() == [33, 0, 18]
