@@ -109,6 +109,7 @@ _SIGNATURES: dict[str, list] = {
         _c_void_p,
     ],
     "gfst_debug_bounded_wait": [_c_int64, _c_void_p],
+    "gfst_debug_attention_error": [_c_int, _c_int, _c_void_p],
     "gfst_exact_block_materialize": [_c_void_p, _c_int64, _c_int, _c_int64, _c_int64, _c_void_p, _c_void_p],
     "gfst_heev": [_c_void_p, _c_int64, _c_int, _c_int, _c_void_p, _c_void_p, _c_void_p, _c_void_p],
     "gfst_exact_block_score": [
@@ -195,8 +196,9 @@ def call(name: str, *args) -> None:
 
 def check_device_errors(clear: bool = True) -> None:
     """Raise RuntimeError when a kernel recorded a device-side failure since
-    the last check: a bounded in-kernel wait that gave up (GFST_ERR_TIMEOUT) or
-    an eigensolver that did not converge (GFST_ERR_NUMERIC).  Synchronises the
+    the last check: a bounded in-kernel wait that gave up (GFST_ERR_TIMEOUT), an
+    eigensolver that did not converge (GFST_ERR_NUMERIC) or, where there is nothing
+    worse, a block table entry outside the pool (GFST_ERR_ARG).  Synchronises the
     current device first, so work enqueued on any stream before the call is
     covered; the recorded status is cleared unless ``clear`` is False.  Call it
     at a point where the host waits anyway (the end of a pass, before results

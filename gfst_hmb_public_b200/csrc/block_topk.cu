@@ -26,31 +26,30 @@ extern "C" int gfst_debug_bounded_wait(int64_t cycles, cudaStream_t stream) {
   return gfst::launch_bounded_wait_probe((long long)cycles, stream);
 }
 
+extern "C" int gfst_debug_attention_error(int tensor_cores, int status, cudaStream_t stream) {
+  GFST_REQUIRE(status == GFST_ERR_ARG || status == GFST_ERR_ALIGN || status == GFST_ERR_TIMEOUT, GFST_ERR_ARG,
+               "status %d is none that an attention kernel records", status);
+  return tensor_cores ? gfst::launch_attn_tc_error(status, stream) : gfst::launch_attn_fma_error(status, stream);
+}
+
 extern "C" int gfst_check_device_errors(int clear) {
   // every stream of the current device, the library's non-blocking ones included
   const cudaError_t se = cudaDeviceSynchronize();
   GFST_REQUIRE(se == cudaSuccess, GFST_ERR_DEVICE, "cudaDeviceSynchronize: %s", cudaGetErrorString(se));
+  // the first word that holds a failure; a bad table entry, read as zeros, only
+  // where no word does
   unsigned int v = 0, w = 0;
-  int st = gfst::read_device_error(clear, &v);
-  if (st != GFST_OK) return st;
-  st = gfst::read_readout_error(clear, &w);
-  if (st != GFST_OK) return st;
-  v = v != 0 ? v : w;
-  st = gfst::read_commit_error(clear, &w);
-  if (st != GFST_OK) return st;
-  v = v != 0 ? v : w;
-  st = gfst::read_score_error(clear, &w);
-  if (st != GFST_OK) return st;
-  v = v != 0 ? v : w;
-  st = gfst::read_scan_error(clear, &w);
-  if (st != GFST_OK) return st;
-  v = v != 0 ? v : w;
-  st = gfst::read_attn_fma_error(clear, &w);
-  if (st != GFST_OK) return st;
-  v = v != 0 ? v : w;
-  st = gfst::read_attn_tc_error(clear, &w);
-  if (st != GFST_OK) return st;
-  v = v != 0 ? v : w;
+  for (auto* read : {gfst::read_device_error, gfst::read_readout_error, gfst::read_commit_error,
+                     gfst::read_score_error, gfst::read_scan_error, gfst::read_attn_fma_error,
+                     gfst::read_attn_tc_error}) {
+    const int st = read(clear, &w);
+    if (st != GFST_OK) return st;
+    if (v == 0 || (v == GFST_ERR_ARG && w != 0)) v = w;
+  }
+  if (v == GFST_ERR_ALIGN) {
+    gfst::set_last_error("a kernel found its shared memory misaligned (device error word %u)", v);
+    return (int)v;
+  }
   if (v == GFST_ERR_ARG) {
     gfst::set_last_error("a block table entry outside the pool was read (device error word %u)", v);
     return (int)v;

@@ -99,6 +99,8 @@ int read_score_error(int clear, unsigned int* value);    // block_score.cu
 int read_scan_error(int clear, unsigned int* value);     // mpuc_scan.cu
 int read_attn_fma_error(int clear, unsigned int* value); // prefix_attention_fma.cu
 int read_attn_tc_error(int clear, unsigned int* value);  // prefix_attention_tc.cu
+int launch_attn_fma_error(int status, cudaStream_t stream);  // prefix_attention_fma.cu
+int launch_attn_tc_error(int status, cudaStream_t stream);   // prefix_attention_tc.cu
 int launch_bounded_wait_probe(long long budget, cudaStream_t stream);  // block_topk_tc.cu
 
 int block_topk_simt(const void* Q, const void* Ksum, int64_t S, int Nq, int NB, int NBs, int d, int k, int dtype,

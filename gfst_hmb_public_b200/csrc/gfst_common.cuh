@@ -30,8 +30,9 @@ inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 
 // ---------------------------------------------------------------------------
 // sticky device error words
 // ---------------------------------------------------------------------------
-// One word per translation unit: kernels record a status with atomicExch; the
-// host reads it (and clears it when asked) in one atomic step through a
+// One word per translation unit: kernels record a status with atomicExch (where
+// they record several, with atomicMax: GFST_ERR_ARG, the least, never hides a wait
+// that gave up); the host reads it (and clears it when asked) in one atomic step through a
 // one-thread kernel on the legacy default stream, whose result lands in a
 // snapshot word that the following cudaMemcpyFromSymbol reads.  Callers
 // synchronise the device first (gfst_check_device_errors does), so the word

@@ -38,6 +38,9 @@ GFST_DEFINE_ERROR_WORD(g_attn_fma_error, read_attn_fma_error, "attention")
 
 namespace {
 
+// a status recorded as the kernel records it
+__global__ void attn_fma_error_kernel(int status) { atomicMax(&g_attn_fma_error, (unsigned)status); }
+
 constexpr int kRows = kAttnFmaRows;   // 64
 constexpr int kKeys = 32;
 constexpr int kThreads = 256;
@@ -563,7 +566,7 @@ __global__ void __launch_bounds__(kThreads, 2) prefix_attention_fma_kernel(const
     if (a.dv <= 128) rows(IC<4>{});
     else rows(IC<8>{});
   }
-  if (bad) atomicExch(&g_attn_fma_error, (unsigned)GFST_ERR_ARG);
+  if (bad) atomicMax(&g_attn_fma_error, (unsigned)GFST_ERR_ARG);
 }
 
 template <typename T>
@@ -579,6 +582,11 @@ int launch(const AttnArgs& a, int sms, cudaStream_t stream) {
 }
 
 }  // namespace
+
+int launch_attn_fma_error(int status, cudaStream_t stream) {
+  attn_fma_error_kernel<<<1, 1, 0, stream>>>(status);
+  return check_launch("attn_fma_error_kernel");
+}
 
 int launch_prefix_attention_fma(const AttnArgs& a, int dtype, int sms, cudaStream_t stream) {
   if (dtype == GFST_F32) return launch<float>(a, sms, stream);

@@ -62,6 +62,9 @@ GFST_DEFINE_ERROR_WORD(g_attn_tc_error, read_attn_tc_error, "attention")
 
 namespace {
 
+// a status recorded as the kernel records it
+__global__ void attn_tc_error_kernel(int status) { atomicMax(&g_attn_tc_error, (unsigned)status); }
+
 constexpr int kHalf = kAttnTcHalf;  // rows of a stream's tile
 constexpr int kKeys = 128;          // keys of a tile (a stage)
 constexpr int kUnit = 64;           // keys of a score buffer
@@ -648,7 +651,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   Ctrl* ctl = reinterpret_cast<Ctrl*>(smem + TC::CTRL_OFF);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   if ((smem_u32(smem) & 1023u) != 0) {  // cannot be: no other shared memory
-    if (threadIdx.x == 0) atomicExch(&g_attn_tc_error, (unsigned)GFST_ERR_ALIGN);
+    if (threadIdx.x == 0) atomicMax(&g_attn_tc_error, (unsigned)GFST_ERR_ALIGN);
     return;
   }
 
@@ -827,7 +830,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       mbar_arrive(&c.item_full[slot]);
     }
     asm volatile("cp.async.wait_all;" ::: "memory");
-    if (bad) atomicExch(&g_attn_tc_error, (unsigned)GFST_ERR_ARG);
+    if (bad) atomicMax(&g_attn_tc_error, (unsigned)GFST_ERR_ARG);
   } else {
     // ------------------------------------------------------------------ MMA
     // the whole warp walks the loop on warp-uniform values (descriptors then come
@@ -955,7 +958,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     tc_fence_after();
     tmem_dealloc(tmem, kTmemCols);
   }
-  if (threadIdx.x == 0 && ctl->abort) atomicExch(&g_attn_tc_error, (unsigned)GFST_ERR_TIMEOUT);
+  if (threadIdx.x == 0 && ctl->abort) atomicMax(&g_attn_tc_error, (unsigned)GFST_ERR_TIMEOUT);
 }
 
 template <int D, bool F16>
@@ -985,6 +988,11 @@ bool prefix_attention_tc_takes(const AttnArgs& a, int dtype) {
   return (dtype == GFST_BF16 || dtype == GFST_F16) && a.d == a.dv && (a.d == 64 || a.d == 128) &&
          ((a.L >= 8 && kKeys % a.L == 0) || a.L % kKeys == 0) && a.n_blocks * a.H * a.L < (1LL << 31) - kKeys &&
          a.scale_log2 > 0.f;  // the row maximum is taken before scaling
+}
+
+int launch_attn_tc_error(int status, cudaStream_t stream) {
+  attn_tc_error_kernel<<<1, 1, 0, stream>>>(status);
+  return check_launch("attn_tc_error_kernel");
 }
 
 int launch_prefix_attention_tc(const AttnArgs& a, int dtype, int sms, cudaStream_t stream) {

@@ -420,7 +420,9 @@ GFST_API int gfst_topk_merge(const float* scores, const int32_t* idx, int64_t ro
  * pipeline) bound every wait; a wait that gives up records GFST_ERR_TIMEOUT in
  * a sticky per-device word and the kernel returns without hanging.  This call
  * synchronises with the current device's work, returns GFST_OK or the
- * recorded status, and clears the word when `clear` is non-zero.            */
+ * recorded status, and clears the words when `clear` is non-zero.  Where several
+ * were recorded, GFST_ERR_ARG (a block table entry outside the pool, read as
+ * zeros) is returned only if there is nothing else.                          */
 GFST_API int gfst_check_device_errors(int clear);
 
 /* ---- failure-path probe ------------------------------------------------------
@@ -431,6 +433,10 @@ GFST_API int gfst_check_device_errors(int clear);
  * context usable.  For testing the failure path without a fault; no
  * counterpart in the reference.                                              */
 GFST_API int gfst_debug_bounded_wait(int64_t cycles, cudaStream_t stream);
+/* Records `status` (GFST_ERR_ARG, GFST_ERR_ALIGN or GFST_ERR_TIMEOUT) as the
+ * shared-prefix attention kernel on the tensor cores (or, with tensor_cores ==
+ * 0, on the FP32 units) would, for testing which of several is reported.     */
+GFST_API int gfst_debug_attention_error(int tensor_cores, int status, cudaStream_t stream);
 
 /* ---- exact-token readout ------------------------------------------------------
  * For every stream s and query q, over the tokens of the k blocks top_idx[s,q,:]

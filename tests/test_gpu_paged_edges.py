@@ -8,6 +8,7 @@ import numpy as np
 import pytest
 import torch
 
+from gfst_hmb_public_b200 import _native as nat
 from gfst_hmb_public_b200 import paged
 from test_gpu_paged import BF16, F32, FP16, Setup, _dev
 
@@ -98,3 +99,36 @@ def test_step_in_place_with_fewer_rows_than_tokens_changes_nothing(cuda_device):
         assert (out == 0).all() and torch.isneginf(lse).all()
     t = mem.extend(new, 21)
     assert int(t.n_short) == 0 and mem.lens.tolist() == [33, 0, 18]
+
+
+ARG, ALIGN, TIMEOUT = 1, 3, 6
+
+
+@pytest.mark.parametrize("recorded, reported", [
+    ([(1, TIMEOUT), (1, ARG)], TIMEOUT), ([(1, ARG), (1, TIMEOUT)], TIMEOUT), ([(0, ARG), (1, TIMEOUT)], TIMEOUT),
+    ([(0, ARG), (1, ARG)], ARG), ([(0, ARG)], ARG), ([(1, ARG)], ARG), ([(1, ALIGN), (1, ARG), (0, ARG)], ALIGN),
+    ([(1, TIMEOUT), (0, ARG), (1, ALIGN)], TIMEOUT),
+])
+def test_a_bad_table_entry_hides_nothing(cuda_device, recorded, reported):
+    lib, stream = nat.load(), torch.cuda.current_stream(cuda_device).cuda_stream
+    nat.check_device_errors()
+    for tensor_cores, status in recorded:
+        assert lib.gfst_debug_attention_error(tensor_cores, status, stream) == 0
+    assert lib.gfst_check_device_errors(0) == reported
+    text = {ARG: "table entry", ALIGN: "shared memory misaligned", TIMEOUT: "bounded wait"}[reported]
+    with pytest.raises(RuntimeError, match=text):
+        nat.check_device_errors()
+    nat.check_device_errors()
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+def test_a_bad_table_entry_behind_a_wait_that_gave_up(cuda_device, dtype):
+    # the same by the kernels themselves: a launch that meets a bad entry after the status of another one
+    s = Setup(cuda_device, dtype, [50], [1], 0, 1, 2, 64, 16, seed=12)
+    s.tables[0, 1] = -1
+    stream = torch.cuda.current_stream(cuda_device).cuda_stream
+    assert nat.load().gfst_debug_attention_error(int(dtype == BF16), TIMEOUT, stream) == 0
+    s.run()
+    with pytest.raises(RuntimeError, match="bounded wait"):
+        nat.check_device_errors()
+    nat.check_device_errors()

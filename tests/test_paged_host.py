@@ -158,3 +158,8 @@ def test_oracle_attention_against_a_dense_softmax(seed):
             assert np.isclose(lse[t, h], s.max() + np.log(w.sum()))
             assert np.allclose(mean_abs[t, h], w @ np.abs(np.stack(vals)) / w.sum())
     assert (out[5] == 0).all() and np.isneginf(lse[5]).all()
+
+
+@pytest.mark.parametrize("status", [0, 2, 7, 8, -1])
+def test_debug_attention_error_refuses_other_statuses(status):
+    assert nat.load().gfst_debug_attention_error(1, status, None) == 1
