@@ -28,7 +28,7 @@
 namespace gfst {
 
 // sticky GFST_ERR_NUMERIC report of the eigen commit
-GFST_DEFINE_ERROR_WORD(g_commit_error, read_commit_error, "commit")
+GFST_DEFINE_ERROR_WORD(g_commit_error, take_commit_error, "commit")
 
 namespace {
 

@@ -22,7 +22,7 @@
 namespace gfst {
 
 // sticky GFST_ERR_TIMEOUT report of the tensor-core block-score kernel
-GFST_DEFINE_ERROR_WORD(g_score_error, read_score_error, "block score")
+GFST_DEFINE_ERROR_WORD(g_score_error, take_score_error, "block score")
 
 namespace {
 

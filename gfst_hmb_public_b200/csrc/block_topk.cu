@@ -1,5 +1,20 @@
 // C-ABI entry of the coarse block retrieval (score + top-k).
+#include <mutex>
+
 #include "block_topk.cuh"
+
+namespace gfst {
+namespace {
+
+using TakeError = int (*)(int, unsigned int*);
+constexpr TakeError kErrorWords[] = {take_device_error, take_readout_error,  take_commit_error, take_score_error,
+                                     take_scan_error,   take_attn_fma_error, take_attn_tc_error};
+constexpr int kNumErrorWords = sizeof(kErrorWords) / sizeof(kErrorWords[0]);
+__device__ unsigned int g_error_words[kNumErrorWords];  // as the last check took them
+std::mutex g_error_mutex;                               // one check at a time
+
+}  // namespace
+}  // namespace gfst
 
 extern "C" int gfst_block_topk(const void* Q, const void* Ksum, int64_t n_streams, int n_queries, int n_blocks,
                                int n_blocks_stride, int d, int k, int dtype, float* top_scores, int32_t* top_idx,
@@ -36,16 +51,22 @@ extern "C" int gfst_check_device_errors(int clear) {
   // every stream of the current device, the library's non-blocking ones included
   const cudaError_t se = cudaDeviceSynchronize();
   GFST_REQUIRE(se == cudaSuccess, GFST_ERR_DEVICE, "cudaDeviceSynchronize: %s", cudaGetErrorString(se));
+  // All words by one copy: a copy a word took 14 us each.
+  std::lock_guard<std::mutex> lock(gfst::g_error_mutex);
+  void* at = nullptr;
+  cudaError_t e = cudaGetSymbolAddress(&at, gfst::g_error_words);
+  for (int i = 0; e == cudaSuccess && i < gfst::kNumErrorWords; ++i) {
+    const int st = gfst::kErrorWords[i](clear, static_cast<unsigned int*>(at) + i);
+    if (st != GFST_OK) return st;
+  }
+  unsigned int words[gfst::kNumErrorWords];
+  if (e == cudaSuccess) e = cudaMemcpyFromSymbol(words, gfst::g_error_words, sizeof(words));
+  GFST_REQUIRE(e == cudaSuccess, GFST_ERR_DEVICE, "reading the device error words: %s", cudaGetErrorString(e));
   // the first word that holds a failure; a bad table entry, read as zeros, only
   // where no word does
-  unsigned int v = 0, w = 0;
-  for (auto* read : {gfst::read_device_error, gfst::read_readout_error, gfst::read_commit_error,
-                     gfst::read_score_error, gfst::read_scan_error, gfst::read_attn_fma_error,
-                     gfst::read_attn_tc_error}) {
-    const int st = read(clear, &w);
-    if (st != GFST_OK) return st;
+  unsigned int v = 0;
+  for (const unsigned int w : words)
     if (v == 0 || (v == GFST_ERR_ARG && w != 0)) v = w;
-  }
   if (v == GFST_ERR_ALIGN) {
     gfst::set_last_error("a kernel found its shared memory misaligned (device error word %u)", v);
     return (int)v;

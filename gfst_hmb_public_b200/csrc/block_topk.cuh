@@ -92,13 +92,13 @@ struct TopK {
 
 int block_topk_tc(const void* Q, const void* Ksum, int64_t S, int Nq, int NB, int NBs, int d, int k, float* ts,
                   int32_t* ti, cudaStream_t stream);
-int read_device_error(int clear, unsigned int* value);
-int read_readout_error(int clear, unsigned int* value);  // exact_readout.cu
-int read_commit_error(int clear, unsigned int* value);   // block_commit_eig.cu
-int read_score_error(int clear, unsigned int* value);    // block_score.cu
-int read_scan_error(int clear, unsigned int* value);     // mpuc_scan.cu
-int read_attn_fma_error(int clear, unsigned int* value); // prefix_attention_fma.cu
-int read_attn_tc_error(int clear, unsigned int* value);  // prefix_attention_tc.cu
+int take_device_error(int clear, unsigned int* to);
+int take_readout_error(int clear, unsigned int* to);  // exact_readout.cu
+int take_commit_error(int clear, unsigned int* to);   // block_commit_eig.cu
+int take_score_error(int clear, unsigned int* to);    // block_score.cu
+int take_scan_error(int clear, unsigned int* to);     // mpuc_scan.cu
+int take_attn_fma_error(int clear, unsigned int* to); // prefix_attention_fma.cu
+int take_attn_tc_error(int clear, unsigned int* to);  // prefix_attention_tc.cu
 int launch_attn_fma_error(int status, cudaStream_t stream);  // prefix_attention_fma.cu
 int launch_attn_tc_error(int status, cudaStream_t stream);   // prefix_attention_tc.cu
 int launch_bounded_wait_probe(long long budget, cudaStream_t stream);  // block_topk_tc.cu

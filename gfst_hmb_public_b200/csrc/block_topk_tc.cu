@@ -26,7 +26,7 @@
 namespace gfst {
 
 // sticky GFST_ERR_TIMEOUT report of the tensor-core retrieval and the wait probe
-GFST_DEFINE_ERROR_WORD(g_device_error, read_device_error, "retrieval")
+GFST_DEFINE_ERROR_WORD(g_device_error, take_device_error, "retrieval")
 
 namespace {
 

@@ -24,7 +24,7 @@
 namespace gfst {
 
 // sticky GFST_ERR_TIMEOUT report of the pipelined readout's bounded waits
-GFST_DEFINE_ERROR_WORD(g_readout_error, read_readout_error, "readout")
+GFST_DEFINE_ERROR_WORD(g_readout_error, take_readout_error, "readout")
 
 namespace {
 

@@ -39,7 +39,7 @@
 
 namespace gfst {
 
-GFST_DEFINE_ERROR_WORD(g_scan_error, read_scan_error, "recurrent scan")
+GFST_DEFINE_ERROR_WORD(g_scan_error, take_scan_error, "recurrent scan")
 
 namespace {
 

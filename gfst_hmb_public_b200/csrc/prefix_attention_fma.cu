@@ -34,7 +34,7 @@
 
 namespace gfst {
 
-GFST_DEFINE_ERROR_WORD(g_attn_fma_error, read_attn_fma_error, "attention")
+GFST_DEFINE_ERROR_WORD(g_attn_fma_error, take_attn_fma_error, "attention")
 
 namespace {
 

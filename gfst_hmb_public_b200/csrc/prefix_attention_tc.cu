@@ -58,7 +58,7 @@
 
 namespace gfst {
 
-GFST_DEFINE_ERROR_WORD(g_attn_tc_error, read_attn_tc_error, "attention")
+GFST_DEFINE_ERROR_WORD(g_attn_tc_error, take_attn_tc_error, "attention")
 
 namespace {
 
