@@ -18,7 +18,8 @@ Layout: pool_K [n_blocks, heads, L, d], pool_V [n_blocks, heads, L, dv]; a block
 of one head is one contiguous L x d slab, as in ``memory.BlockMemory``.  Slot
 ``block * L + offset`` names a token's place in the pool.
 
-Serving operators: nothing here records gradients.  The reference
+Serving operators: nothing here records gradients, and tensors that ask for
+them (or carry forward-mode tangents) are refused.  The reference
 (pkhairkh/gfst-hmb-public) keeps one Python list of blocks per sample
 (src/gfst_hmb_mpuc/state.py:651-815) and has no shared prefix.
 """
@@ -30,6 +31,7 @@ import math
 from typing import NamedTuple
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _native as nat
 
@@ -48,11 +50,15 @@ def _dtype_code(what: str, *tensors: torch.Tensor) -> int:
     return _DTYPES[dtype]
 
 
-def _no_grad(what: str, *tensors: torch.Tensor) -> None:
+def _no_grad(what: str, *tensors: torch.Tensor | None) -> None:
     if torch.is_grad_enabled():
         for t in tensors:
-            if t.requires_grad:
+            if t is not None and t.requires_grad:
                 raise RuntimeError(f"{what} has no backward pass; call it under torch.no_grad()")
+    if forward_ad._current_level >= 0 and torch._C._is_fwd_grad_enabled():
+        for t in tensors:
+            if t is not None and forward_ad.unpack_dual(t).tangent is not None:
+                raise RuntimeError(f"{what} has no forward-mode derivative; pass tensors without tangents")
 
 
 def _cuda(what: str, *tensors: torch.Tensor | None) -> int:
@@ -266,7 +272,7 @@ def prefix_attention(Q: torch.Tensor, pool_K: torch.Tensor, pool_V: torch.Tensor
             prefix_len = _int32(what, "prefix_len", prefix_len, (1,))
         p_table, p_len = prefix_table.data_ptr(), prefix_len.data_ptr()
     code = _dtype_code(what, Q, pool_K, pool_V)
-    _no_grad(what, Q, pool_K, pool_V)
+    _no_grad(what, Q, pool_K, pool_V, out)
     scale = 1.0 / math.sqrt(d) if scale is None else float(scale)
     if not math.isfinite(scale):
         raise ValueError(f"prefix_attention: scale {scale} is not finite")

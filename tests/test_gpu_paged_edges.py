@@ -132,3 +132,25 @@ def test_a_bad_table_entry_behind_a_wait_that_gave_up(cuda_device, dtype):
     with pytest.raises(RuntimeError, match="bounded wait"):
         nat.check_device_errors()
     nat.check_device_errors()
+
+
+def test_tangents_and_a_differentiable_out_are_refused(cuda_device):
+    s = Setup(cuda_device, BF16, [30, 7], [2, 1], 40, 2, 2, 64, 16, seed=2)
+    out = torch.zeros((3, 4, 64), dtype=BF16, device=cuda_device)
+    with pytest.raises(RuntimeError, match="backward"):
+        s.run(out=out.clone().requires_grad_())
+    K = torch.ones((2, 2, 64), dtype=BF16, device=cuda_device)
+    slots, before = _dev([0, 1], cuda_device), s.pool_K.clone()
+    with torch.autograd.forward_ad.dual_level():
+        dual = torch.autograd.forward_ad.make_dual
+        with pytest.raises(RuntimeError, match="forward-mode"):
+            s.run(Q=dual(s.Q, s.Q))
+        with pytest.raises(RuntimeError, match="forward-mode"):
+            s.run(out=dual(out, out))
+        with pytest.raises(RuntimeError, match="forward-mode"):
+            paged.paged_append(dual(K, K), K, s.pool_K, s.pool_V, slots)
+    assert torch.equal(s.pool_K.nan_to_num(), before.nan_to_num())
+    with pytest.raises(RuntimeError):                           # transforms hand over no memory
+        torch.func.jvp(lambda q: s.run(Q=q)[0], (s.Q,), (s.Q,))
+    with pytest.raises(RuntimeError):
+        torch.func.vmap(lambda q: s.run(Q=q)[0])(torch.stack([s.Q, s.Q]))

@@ -163,3 +163,22 @@ def test_oracle_attention_against_a_dense_softmax(seed):
 @pytest.mark.parametrize("status", [0, 2, 7, 8, -1])
 def test_debug_attention_error_refuses_other_statuses(status):
     assert nat.load().gfst_debug_attention_error(1, status, None) == 1
+
+
+def test_gradients_of_either_mode_are_refused():
+    # the operators' own check, which asks no device
+    x, y = torch.ones(3), torch.ones(3, requires_grad=True)
+    paged._no_grad("op", x, None)
+    with pytest.raises(RuntimeError, match="backward"):
+        paged._no_grad("op", x, y)
+    with torch.no_grad():
+        paged._no_grad("op", x, y)
+    with torch.autograd.forward_ad.dual_level():
+        dual = torch.autograd.forward_ad.make_dual(x, x)
+        paged._no_grad("op", x)
+        with pytest.raises(RuntimeError, match="forward-mode"):
+            paged._no_grad("op", x, dual)
+        with torch.no_grad(), pytest.raises(RuntimeError, match="forward-mode"):
+            paged._no_grad("op", dual)
+        with torch.inference_mode():
+            paged._no_grad("op", dual)
