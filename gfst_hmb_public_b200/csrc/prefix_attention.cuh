@@ -70,17 +70,16 @@ __device__ __forceinline__ int attn_prefix_len(const AttnArgs& a) {
 
 struct AttnRequest {
   int tok0, n;   // first token, tokens (those that Q has rows for)
-  int len;       // own positions
-  int see0;      // token i sees positions < see0 + i + 1
+  int len;       // own positions that they see between them: token i sees those < len - n + i + 1
 };
 __device__ __forceinline__ AttnRequest attn_request(const AttnArgs& a, int b) {
   AttnRequest r;
   r.tok0 = min(max(a.cu[b], 0), a.n_tokens);
   const int end = max(a.cu[b + 1], r.tok0);
   r.n = min(end, a.n_tokens) - r.tok0;
-  r.len = (int)min((int64_t)max(a.lens[b], 0), (int64_t)a.width * a.L);
-  // from all new tokens, Q may have fewer rows; -n: none of those sees a position
-  r.see0 = max(r.len - (end - r.tok0), -r.n);
+  // Q may have fewer rows than there are new tokens: the positions of those behind
+  // them are seen by none
+  r.len = max((int)min((int64_t)max(a.lens[b], 0), (int64_t)a.width * a.L) - (end - r.tok0 - r.n), 0);
   return r;
 }
 
@@ -153,7 +152,7 @@ struct AttnLine {
   __device__ static __forceinline__ int tiles(int len) { return max(1, (len + C::KT - 1) / C::KT); }
   // positions that the rows up to `last_row` of a request see between them
   __device__ static __forceinline__ int see(const AttnRequest& r, int last_row, int G) {
-    return min(r.len, max(0, r.see0 + last_row / G + 1));
+    return min(r.len, max(0, r.len - r.n + last_row / G + 1));
   }
   __device__ static __forceinline__ int own_tiles(const AttnRequest& r, int m, int G) {
     const int R = r.n * G;
@@ -378,7 +377,7 @@ struct AttnWalk {
         it.b = b;
         it.tok0 = req.tok0;
         it.len = ln.see(req, it.row0 + it.rows - 1, a.G);
-        it.see0 = req.see0;
+        it.see0 = req.len - req.n;
         nt = ln.tiles(it.len);
       }
       // tile j begins at cost position base + j * w
