@@ -83,22 +83,44 @@ struct Vec<__half> {
   }
 };
 // Where a row's partial result goes: its own place, or this CTA's continuation
-// buffer; writes its (m, l) if told to.
-__device__ __forceinline__ float* fma_put(const AttnArgs& a, const AttnPart& it, int r, float2 ml, bool write) {
-  int tok, hq;
-  attn_row(a, it, r, tok, hq);
-  const int64_t row = (int64_t)tok * (a.H * a.G) + hq;
-  const int64_t crow = (int64_t)blockIdx.x * kRows + r;
-  if (write) {
-    if (it.first) {
-      a.part_ml[it.own][row] = ml;
-      a.part_next[it.own][row] = attn_next((blockIdx.x + 1) * kRows + r, it.n_cont, kRows);
-    } else {
-      a.cont_ml[crow] = ml;
+// buffer.  Called by a warp's lanes that hold the row, `write` for one of them,
+// which writes (m, l).  A later piece is joined to what is there: the lanes read
+// the (m, l) of before, which `write` changes only when all have, and their
+// columns' values, which they wrote themselves.
+struct FmaPut {
+  float* o;
+  float keep, f;  // factors of the values there and of the new ones
+  __device__ __forceinline__ FmaPut(const AttnArgs& a, const AttnPart& it, int r, float2 ml, bool live, bool write) {
+    int tok, hq;
+    attn_row(a, it, live ? r : 0, tok, hq);
+    const int64_t row = (int64_t)tok * (a.H * a.G) + hq;
+    const int64_t crow = (int64_t)blockIdx.x * kRows + r;
+    float2* at = it.first ? a.part_ml[it.own] + row : a.cont_ml + crow;
+    o = it.first ? a.part_o[it.own] + row * a.dv : a.cont_o + crow * a.dv;
+    keep = 0.f, f = 1.f;
+    if (it.again) {
+      if (live) {
+        const AttnJoin j(*at, ml);
+        ml = j.ml, keep = j.fa, f = j.fb;
+      }
+      __syncwarp();
+    }
+    if (live && write) {
+      *at = ml;
+      if (it.first) a.part_next[it.own][row] = attn_next((blockIdx.x + 1) * kRows + r, it.n_cont, kRows);
     }
   }
-  return it.first ? a.part_o[it.own] + row * a.dv : a.cont_o + crow * a.dv;
-}
+  // four columns
+  __device__ __forceinline__ void store(const AttnPart& it, int c, float4 v) const {
+    float4* to = reinterpret_cast<float4*>(o + c);
+    if (it.again) {
+      const float4 u = *to;
+      v = make_float4(fmaf(u.x, keep, v.x * f), fmaf(u.y, keep, v.y * f), fmaf(u.z, keep, v.z * f),
+                      fmaf(u.w, keep, v.w * f));
+    }
+    *to = v;
+  }
+};
 // Row r of an item lies in slot r / 8 of warp r % 8's eight: neighbours for the
 // lanes of a warp, and few rows are spread over all warps.
 __device__ __forceinline__ int slot_of(int r) { return (r & (kWarps - 1)) * kPer + (r >> 3); }
@@ -300,8 +322,8 @@ __device__ __forceinline__ bool few_rows(const AttnArgs& a, const AttnPart& it, 
         o.x += u.x * f, o.y += u.y * f, o.z += u.z * f, o.w += u.w * f;
       }
     }
-    float* dst = fma_put(a, it, warp, make_float2(top, sum), lane == 0);
-    if (lane * 4 < a.dv) *reinterpret_cast<float4*>(dst + lane * 4) = o;
+    const FmaPut put(a, it, warp, make_float2(top, sum), true, lane == 0);
+    if (lane * 4 < a.dv) put.store(it, lane * 4, o);
   }
   return bad;
 }
@@ -551,11 +573,11 @@ __global__ void __launch_bounds__(kThreads, 2) prefix_attention_fma_kernel(const
       // partial results: the row's own place, or this CTA's continuation buffer
 #pragma unroll
       for (int u = 0; u < NR; ++u) {
-        if (row[u] >= it.rows || (ONE && ry > 0)) continue;
-        float* dst = fma_put(a, it, row[u], make_float2(m[u], l[u]), kx == 0);
+        const bool mine = row[u] < it.rows && !(ONE && ry > 0);
+        const FmaPut put(a, s_it, row[u], make_float2(m[u], l[u]), mine, kx == 0);  // (s_it: no registers in the loop)
 #pragma unroll
         for (int c = 0; c < Q32; ++c)
-          if (c * 32 + kx * 4 < a.dv) *reinterpret_cast<float4*>(dst + c * 32 + kx * 4) = acc[u][c];
+          if (mine && c * 32 + kx * 4 < a.dv) put.store(s_it, c * 32 + kx * 4, acc[u][c]);
       }
     };
     auto rows = [&](auto nq) {

@@ -563,6 +563,19 @@ struct Softmax {
       if (write) a.cont_ml[crow0 + r_] = ml;
       return a.cont_o + (crow0 + r_) * D;
     };
+    // A later piece: what is there of a row, all lanes' own writes, joined with the
+    // new (m, l); `ml` becomes the joined one.
+    auto join = [&](int r_, float2& ml) -> AttnJoin {
+      int tok, hq;
+      attn_row(a, it, r_, tok, hq);
+      const AttnJoin j(it.first ? a.part_ml[it.own][(int64_t)tok * (a.H * a.G) + hq] : a.cont_ml[crow0 + r_], ml);
+      ml = j.ml;
+      return j;
+    };
+    auto joined = [](float4 u, float keep, float4 v, float f) {
+      return make_float4(fmaf(u.x, keep, v.x * f), fmaf(u.y, keep, v.y * f), fmaf(u.z, keep, v.z * f),
+                         fmaf(u.w, keep, v.w * f));
+    };
     if (!wait.warp(&c.pv_done[(n_unit - 1) & 1], ((n_unit - 1) >> 1) & 1)) return false;
     tc_fence_after();
     // only here: that product waited for this part's weights of all four warps, which
@@ -573,7 +586,13 @@ struct Softmax {
         // 32 columns of the warp's 32 rows at a time through shared memory, so that
         // a store writes whole 128-byte lines (four rows) and not 32 sectors
         float4* st = reinterpret_cast<float4*>(smem + TC::STAGE_OFF + j * kStageBytes) + quad * (32 * 8);
-        float* dst = live ? put(r, make_float2(m, l), true) : nullptr;
+        float2 ml = make_float2(m, l);
+        float keep = 0.f, f = 1.f;
+        if (it.again && live) {
+          const AttnJoin jn = join(r, ml);
+          keep = jn.fa, f = jn.fb;
+        }
+        float* dst = live ? put(r, ml, true) : nullptr;
 #pragma unroll 1
         for (int i = 0; i < D; i += 32) {
           float o[32];
@@ -584,13 +603,27 @@ struct Softmax {
           for (int k = 0; k < 8; ++k)
             st[lane * 8 + (k ^ (lane & 7))] = make_float4(o[4 * k], o[4 * k + 1], o[4 * k + 2], o[4 * k + 3]);
           __syncwarp();
+          auto row_to = [&](int row) {
+            float* to = reinterpret_cast<float*>(
+                __shfl_sync(0xffffffffu, reinterpret_cast<unsigned long long>(dst), row));
+            return to == nullptr ? nullptr : reinterpret_cast<float4*>(to + i + (lane & 7) * 4);
+          };
+          if (it.again) {  // (apart: drafted tokens took 44.4 us for 42.3 with it in the loop below)
+#pragma unroll 1
+            for (int k = 0; k < 8; ++k) {
+              const int row = k * 4 + (lane >> 3);
+              const float k0 = __shfl_sync(0xffffffffu, keep, row), f0 = __shfl_sync(0xffffffffu, f, row);
+              float4* to = row_to(row);
+              if (to != nullptr) *to = joined(*to, k0, st[row * 8 + ((lane & 7) ^ (row & 7))], f0);
+            }
+            continue;
+          }
 #pragma unroll
           for (int k = 0; k < 8; ++k) {
             const int row = k * 4 + (lane >> 3);
-            float* to = reinterpret_cast<float*>(
-                __shfl_sync(0xffffffffu, reinterpret_cast<unsigned long long>(dst), row));
+            float4* to = row_to(row);
             const float4 v = st[row * 8 + ((lane & 7) ^ (row & 7))];
-            if (to != nullptr) *reinterpret_cast<float4*>(to + i + (lane & 7) * 4) = v;
+            if (to != nullptr) *to = v;
           }
         }
       }
@@ -627,12 +660,23 @@ struct Softmax {
           const float mx = fmaxf(v0.x, v1.x);
           // equal references (both empty: -inf) need no exponential
           const float f0 = v0.x == mx ? 1.f : ex2(v0.x - mx), f1 = v1.x == mx ? 1.f : ex2(v1.x - mx);
-          float* dst = put(r0 + x, make_float2(mx, fmaf(v0.y, f0, v1.y * f1)), lane == 0);
-          if (lane < P) {
-            const float4 u = st[x * P + (lane ^ (x & 7))], w = st[(kJoinRows + x) * P + (lane ^ (x & 7))];
-            *reinterpret_cast<float4*>(dst + lane * 4) =
-                make_float4(fmaf(u.x, f0, w.x * f1), fmaf(u.y, f0, w.y * f1), fmaf(u.z, f0, w.z * f1), fmaf(u.w, f0, w.w * f1));
+          float2 ml = make_float2(mx, fmaf(v0.y, f0, v1.y * f1));
+          if (it.again) {
+            const AttnJoin jn = join(r0 + x, ml);
+            __syncwarp();  // all lanes have read what lane 0 writes
+            float* dst = put(r0 + x, ml, lane == 0);
+            if (lane < P) {
+              float4* to = reinterpret_cast<float4*>(dst + lane * 4);
+              *to = joined(*to, jn.fa,
+                           joined(st[x * P + (lane ^ (x & 7))], f0, st[(kJoinRows + x) * P + (lane ^ (x & 7))], f1),
+                           jn.fb);
+            }
+            continue;
           }
+          float* dst = put(r0 + x, ml, lane == 0);
+          if (lane < P)
+            *reinterpret_cast<float4*>(dst + lane * 4) =
+                joined(st[x * P + (lane ^ (x & 7))], f0, st[(kJoinRows + x) * P + (lane ^ (x & 7))], f1);
         }
       }
     }

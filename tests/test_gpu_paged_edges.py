@@ -154,3 +154,97 @@ def test_tangents_and_a_differentiable_out_are_refused(cuda_device):
         torch.func.jvp(lambda q: s.run(Q=q)[0], (s.Q,), (s.Q,))
     with pytest.raises(RuntimeError):
         torch.func.vmap(lambda q: s.run(Q=q)[0])(torch.stack([s.Q, s.Q]))
+
+
+# ---------------------------------------------------------------------------
+# long lengths: a table that lists a few blocks again and again
+# ---------------------------------------------------------------------------
+class Repeated:
+    """Keys and values of ``cycle`` positions, which a long table repeats.  The
+    oracle weighs each of them by how often a row sees it."""
+
+    def __init__(self, dev, dtype, H, G, n, d, L, blocks, dv=None, positive=False, seed=0):
+        g = torch.Generator(device=dev).manual_seed(seed)
+        dv = d if dv is None else dv
+        self.pool_K = torch.randn((blocks, H, L, d), generator=g, device=dev).to(dtype)
+        self.pool_V = torch.randn((blocks, H, L, dv), generator=g, device=dev)
+        self.pool_V = (self.pool_V.abs() if positive else self.pool_V).to(dtype)
+        self.Q = torch.randn((n, H * G, d), generator=g, device=dev).to(dtype)
+        self.dev, self.dtype, self.G, self.L, self.blocks, self.scale = dev, dtype, G, L, blocks, d ** -0.5
+
+    def table(self, length):
+        t = torch.arange(-(-length // self.L), dtype=torch.int32, device=self.dev) % self.blocks
+        return t.to(torch.int32)
+
+    def run(self, prefix, own):
+        """All queries are the last tokens of one request of ``own`` positions."""
+        n, i32 = self.Q.shape[0], dict(dtype=torch.int32, device=self.dev)
+        tables = self.table(max(own, 1))[None]
+        return paged.prefix_attention(self.Q, self.pool_K, self.pool_V, tables, torch.tensor([own], **i32),
+                                      torch.tensor([0, n], **i32), prefix_table=self.table(max(prefix, 1)),
+                                      prefix_len=torch.tensor([prefix], **i32), return_lse=True)
+
+    def check(self, out, lse, prefix, own, heads):
+        """Tolerances as in test_gpu_paged.py, with pieces of at most m = 65,536
+        keys, j of them: numerator's sums m 2^-23 (the tensor cores cut off where
+        FP32 rounds), denominator's m 2^-24, and j 2^-24 for their joining."""
+        n, G, L = self.Q.shape[0], self.G, self.L
+        cycle, u = self.blocks * L, torch.finfo(self.dtype).eps / 2
+        at = np.arange(cycle)
+        times = lambda length: np.maximum(0, (length - 1 - at) // cycle + 1)  # noqa: E731
+        for h in heads:
+            k = self.pool_K[:, h].double().cpu().numpy().reshape(cycle, -1)
+            v = self.pool_V[:, h].double().cpu().numpy().reshape(cycle, -1)
+            for t in range(n):
+                count = times(prefix) + times(max(0, own - n + t + 1))
+                q = self.Q[t, h * G:(h + 1) * G].double().cpu().numpy()
+                s = q @ k.T * self.scale
+                m = s.max(1, keepdims=True)
+                p = np.exp(s - m) * count
+                l = p.sum(1, keepdims=True)
+                want, A, z = p @ v / l, p @ np.abs(v) / l, m[:, 0] + np.log(l[:, 0])
+                top = self.scale * (np.abs(q) @ np.abs(k).T).max(1)
+                e, most = 2.0 ** -24, min(65536, max(prefix, own))
+                sums = 3 * most * e + (prefix + own) / 65536 * e
+                err_s = (q.shape[1] + 8) * e * top
+                per = (0 if self.dtype == F32 else u) + 2 * err_s + sums + 2.0 ** -20
+                got = out[t, h * G:(h + 1) * G].double().cpu().numpy()
+                assert (np.abs(got - want) <= u * np.abs(want) + per[:, None] * A).all()
+                got = lse[t, h * G:(h + 1) * G].double().cpu().numpy()
+                assert (np.abs(got - z) <= err_s + sums + 2.0 ** -20 + 2 * e * np.abs(z)).all()
+
+
+@pytest.mark.parametrize("dtype, G, n, d, dv", [
+    (BF16, 1, 1, 64, 64), (FP16, 8, 3, 128, 128), (BF16, 8, 5, 64, 64), (BF16, 8, 32, 64, 64),     # tensor cores
+    (F32, 1, 1, 64, 64), (F32, 3, 1, 64, 64), (F32, 6, 1, 64, 64), (F32, 8, 3, 64, 64), (F32, 16, 4, 64, 64),
+    (BF16, 2, 1, 80, 48), (F32, 2, 1, 136, 136),                                                    # FP32 units
+])
+@pytest.mark.parametrize("where", ["prefix", "own"])
+def test_parts_in_pieces(cuda_device, dtype, G, n, d, dv, where):
+    # as many heads as workers: a part is a whole item, of three pieces and a bit
+    s = Repeated(cuda_device, dtype, 300, G, n, d, 128, 4, dv=dv, seed=G + n)
+    prefix, own = (200_001, 40) if where == "prefix" else (0, 200_001)
+    out, lse = s.run(prefix, own)
+    s.check(out, lse, prefix, own, (0, 150, 299))
+    again, lse2 = s.run(prefix, own)
+    assert torch.equal(out, again) and torch.equal(lse, lse2)
+
+
+@pytest.mark.parametrize("dtype", [BF16, FP16])
+def test_long_sums_of_one_sign(cuda_device, dtype):
+    # in one go, the tensor cores' sums of 8 M positive terms come out 4 % too small
+    s = Repeated(cuda_device, dtype, 300, 1, 1, 64, 128, 8, positive=True, seed=3)
+    out, lse = s.run(1 << 23, 0)
+    s.check(out, lse, 1 << 23, 0, (0, 299))
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("where", ["prefix", "own"])
+def test_positions_up_to_the_last(cuda_device, dtype, where):
+    # the most positions that a table can hold: 2^31 - 1024
+    s = Repeated(cuda_device, dtype, 1, 4, 1, 64, 1024, 2, seed=4)
+    most = (1 << 31) - 1024
+    prefix, own = (most, 1) if where == "prefix" else (0, most)
+    out, lse = s.run(prefix, own)
+    s.check(out, lse, prefix, own, (0,))
+    nat.check_device_errors()
