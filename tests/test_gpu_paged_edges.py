@@ -248,3 +248,20 @@ def test_positions_up_to_the_last(cuda_device, dtype, where):
     out, lse = s.run(prefix, own)
     s.check(out, lse, prefix, own, (0,))
     nat.check_device_errors()
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+def test_odd_offsets_leave_sound_rows_right(cuda_device, dtype):
+    s = Setup(cuda_device, dtype, [20, 33, 5], [2, 1, 1], 40, 1, 2, 64, 16, seed=14)
+    tables, lens = s.np_tables, s.np_lens
+    # token 0 is request 0's first, tokens 2 and 3 are request 2's last of three; both claim token 1
+    s.cu = _dev([0, 2, 1, 4], cuda_device)
+    out, lse = s.run()
+    for b, cu, rows in ((0, [0, 2], [0]), (2, [1, 4], [2, 3])):
+        s.np_tables, s.np_lens, s.np_cu = tables[b:b + 1], lens[b:b + 1], np.array(cu)
+        s.check(out, lse, rows)
+    # no token is anyone's
+    for cu in ([3, 2, 1, 0], [2 ** 31 - 1] * 4, [-1, -1, -1, -1]):
+        s.cu = _dev(cu, cuda_device)
+        out, lse = s.run()
+        assert (out == 0).all() and torch.isneginf(lse).all()
