@@ -191,7 +191,7 @@ def block_tables(lens: torch.Tensor, new_lens: torch.Tensor, tables: torch.Tenso
 
 def _check_pools(what: str, pool_K: torch.Tensor, pool_V: torch.Tensor) -> tuple:
     k, v = pool_K.shape, pool_V.shape
-    if len(k) != 4 or len(v) != 4 or k[0] != v[0] or k[1] != v[1] or k[2] != v[2]:
+    if len(k) != 4 or len(v) != 4 or k[0] != v[0] or k[1] != v[1] or k[2] != v[2] or k[1] == 0:
         raise ValueError(f"{what} expects pool_K [n_blocks, heads, L, d] and pool_V [n_blocks, heads, L, dv]")
     if not (pool_K.is_contiguous() and pool_V.is_contiguous()):
         raise ValueError(f"{what}: pools must be contiguous")

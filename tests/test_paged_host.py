@@ -182,3 +182,9 @@ def test_gradients_of_either_mode_are_refused():
             paged._no_grad("op", dual)
         with torch.inference_mode():
             paged._no_grad("op", dual)
+
+
+def test_pools_without_heads_are_refused():
+    pool, x = torch.zeros((4, 0, 16, 64)), torch.zeros((2, 2, 64))
+    with pytest.raises(ValueError, match="heads"):
+        paged._check_pools("prefix_attention", pool, pool)
