@@ -9,7 +9,8 @@
 // are loaded at once, before it is known which of them are needed: one memory
 // latency a warp instead of four in a chain (which took 217 us).  One row a warp:
 // two or four, with their loads together, were slower from 16 rows (11.7 and 13.0
-// us a call for 11.2) to those (934 and 979 for 931).
+// us for attention and merge together, 11.2 with one) to those (934 and 979 us, 931
+// with one, before later steps that are not the merge's).
 #include <cuda_fp16.h>
 
 #include <cmath>

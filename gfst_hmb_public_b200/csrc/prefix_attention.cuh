@@ -6,8 +6,8 @@
 //     o = sum_j p_j v_j / sum_j p_j,   p_j = exp(scale q . k_j)
 // over the prefix_len positions of the shared prefix and the positions
 // j <= len_b - n_b + i of the request's own blocks (n_b new tokens, the last of
-// its len_b).  Softmax splits over disjoint key sets: with m the running
-// maximum of a set (in units of log2), l = sum 2^(s - m) and o unnormalised,
+// its len_b).  Softmax splits over disjoint key sets (the online softmax of Milakov
+// and Gimelshein, 2018): with m the running maximum of a set (in units of log2), l = sum 2^(s - m) and o unnormalised,
 // sets join as m* = max m, l* = sum l 2^(m - m*), o* = sum o 2^(m - m*).
 //
 // Items.  A prefix item is MR rows of ALL queries of one KV head (row = token

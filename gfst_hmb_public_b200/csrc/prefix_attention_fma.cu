@@ -20,9 +20,11 @@
 // Every group of eight lanes keeps its own maximum, sum and values over its keys
 // and all are joined when the part ends, so the loop has no barrier at all.
 //
-// Measured, 32-bit, d = 128: 16 one-token requests of up to 8000 tokens (8 heads x
-// 4) 110 us, 2.95 TB/s; prompt pieces of 200 to 600 tokens (4 heads x 2) 499 us, 17
-// TFLOP/s; d = 64, 64 requests behind 4000 tokens (4 x 4) 90 us, 12 TFLOP/s.
+// Measured (device time with the merge), 32-bit, d = 128: 16 one-token requests of
+// up to 8000 tokens (8 heads x 4) 113 us, 2.9 TB/s; prompt pieces of 200 to 600
+// tokens (4 heads x 2) 497 us, 17 TFLOP/s; d = 64, 64 requests behind 4000 tokens (4
+// x 4) 91 us, 12 TFLOP/s.  (The compiler's choice of registers at the cap of 128
+// moves these by up to 3 %.)
 // Keys read straight into registers: 144 us for the first, 1.3 us less for the
 // smallest call.  Without the way of few rows: 216 us for the first; without one
 // row a warp, 32 requests of 500 to 3000 tokens with eight query heads a key head:

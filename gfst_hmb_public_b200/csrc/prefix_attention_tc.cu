@@ -17,10 +17,12 @@
 // because a thread's loads, maximum, exponentials, sums and stores follow one
 // another and there is room for two such warps on a quarter of the SM.
 //
-// Measured, bf16, d = 128: 512 one-token requests behind 32,768 tokens (4 heads x
-// 8) 345 us, 800 TFLOP/s; prompt pieces of 12 requests behind 4096 tokens (8 x 4)
-// 868 us with the merge, 840 TFLOP/s; 16 requests of 4096 to 32,767 tokens 141 us,
-// 5.9 TB/s; 64 requests behind 8192 tokens 47 us.  Tried and slower: two threads a
+// Measured, bf16, d = 128, device time with the merge (graph replays, SMs near 1.9
+// GHz; calls one after another under the power limit in brackets): 512 one-token
+// requests behind 32,768 tokens (4 heads x 8) 344 us, 800 TFLOP/s (377 us); prompt
+// pieces of 12 requests behind 4096 tokens (8 x 4) 876 us, 837 TFLOP/s (965 us); 16
+// requests of 4096 to 32,767 tokens 142 us, 5.8 TB/s (162 us); 64 requests behind
+// 8192 tokens 47 us (49 us).  Tried and slower: two threads a
 // row, each with half of the keys, that exchange maxima (the same for the document,
 // 7 % slower for prompts); a polynomial in place of some exponentials; tiles
 // prefetched into L2.
@@ -132,6 +134,12 @@ __device__ __forceinline__ float ex2(float x) {
   return y;
 }
 
+// Weights take the pools' 16-bit type: both operands of a product have one, and V
+// is read as it lies in the pool.  Half a step of a weight (bf16 2^-8, fp16 2^-11)
+// beside half a step of the output: against 64 bits the outputs are off by 2.3e-3
+// (fp16 2.9e-4) where 32-bit weights would leave 1.7e-3 (2.1e-4).  Weights in two
+// 16-bit parts would double the second product; 32-bit pools round none.  The sums
+// l are of the weights before this rounding.
 template <bool F16>
 __device__ __forceinline__ uint32_t pack2(float lo, float hi) {
   uint32_t r;

@@ -205,7 +205,8 @@ def paged_append(K: torch.Tensor, V: torch.Tensor, pool_K: torch.Tensor, pool_V:
     with a negative slot (padding, or a block that was not had) are left out, and
     so is a slot outside the pool; nothing else of the pools changes.  The slots
     that are written must be distinct, as ``block_tables`` gives them.  K and V
-    may be strided views (a fused projection's output) with 16-byte rows."""
+    may be strided views (a fused projection's output) with 16-byte rows, but not
+    of the pools themselves."""
     what = "paged_append"
     index = _cuda(what, K, V, pool_K, pool_V, slot_map)
     n_blocks, H, L, d, dv = _check_pools(what, pool_K, pool_V)
@@ -244,7 +245,10 @@ def prefix_attention(Q: torch.Tensor, pool_K: torch.Tensor, pool_V: torch.Tensor
     cu_new[B] (a padded batch) get the same; with ``out`` given (contiguous,
     Q's dtype) their rows of it stay as they were, and lse is -inf.  A table entry outside the
     pool within a request's length reads as zero keys and values and is
-    reported by ``_native.check_device_errors``."""
+    reported by ``_native.check_device_errors``.  Keys and values that no token
+    sees may hold anything; one that is not finite and is seen makes columns of
+    the row inf or NaN.  Each call takes a workspace of 8 (dv + 4) bytes per row
+    of ``out`` and 42 MB (dv 128) from the caching allocator."""
     what = "prefix_attention"
     index = _cuda(what, Q, pool_K, pool_V, tables, lens, cu_new, prefix_table, prefix_len, out)
     n_blocks, H, L, d, dv = _check_pools(what, pool_K, pool_V)
@@ -301,6 +305,8 @@ class PagedMemory:
 
     A step: ``step = mem.extend(new_lens, n_tokens)``; then for every layer
     ``mem.append(K, V, step, layer)`` and ``mem.attend(Q, step, layer=layer)``.
+    A step's tables and lengths are the memory's own: it is over with the next
+    ``extend``, ``share``, ``unshare`` or ``reset``.
     Lengths and tables stay on the GPU; shapes depend on ``n_tokens`` alone, so a
     step can be captured in a CUDA graph and replayed with new ``new_lens`` in
     the same tensor (tokens behind the last request are padding)."""

@@ -667,9 +667,12 @@ GFST_API int gfst_paged_append(const void* K, int64_t k_stride_t, int64_t k_stri
  * and sums, one rounding of out; 16-bit weights p on the tensor cores are
  * rounded to the pools' type.  Lengths beyond the tables' positions are cut to
  * them; a table entry outside [0, n_blocks) reads as zero keys and values and
- * records GFST_ERR_ARG for gfst_check_device_errors().
+ * records GFST_ERR_ARG for gfst_check_device_errors().  A key or value that is
+ * not finite and that a row sees makes columns of the row inf or NaN.
  * workspace: gfst_prefix_attention_workspace_bytes bytes, 256-byte aligned,
- * one per concurrent call.  Limits: d, dv <= 256, rows and pointers multiples
+ * one per concurrent call: 8 (dv + 4) bytes per row (n_tokens * n_kv_heads *
+ * group of them), and 82k (dv > 128: 20k) rows of 4 (dv + 2) bytes for work
+ * split over CTAs (42 MB at dv = 128).  Limits: d, dv <= 256, rows and pointers multiples
  * of 16 bytes, n_requests <= 65536, n_tokens * heads below 2^31.
  * No reference counterpart: the reference attends per sample through torch.  */
 GFST_API int gfst_prefix_attention_workspace_bytes(int64_t n_tokens, int n_kv_heads, int group, int dv,
