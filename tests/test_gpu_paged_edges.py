@@ -265,3 +265,50 @@ def test_odd_offsets_leave_sound_rows_right(cuda_device, dtype):
         s.cu = _dev(cu, cuda_device)
         out, lse = s.run()
         assert (out == 0).all() and torch.isneginf(lse).all()
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+def test_most_requests_on_one_table_row(cuda_device, dtype):
+    # 65,536 requests, every third idle, all of whose rows of the tables are the same one (stride 0)
+    s = Repeated(cuda_device, dtype, 1, 2, 1, 64, 16, 3, seed=6)
+    B, i32 = 65536, dict(dtype=torch.int32, device=cuda_device)
+    lens = (torch.arange(B, device=cuda_device) % 41).to(torch.int32)
+    new = ((torch.arange(B, device=cuda_device) % 3 > 0) & (lens > 0)).to(torch.int32)
+    cu = torch.cat([torch.zeros(1, **i32), torch.cumsum(new, 0).to(torch.int32)])
+    n = int(cu[-1])
+    g = torch.Generator(device=cuda_device).manual_seed(7)
+    Q = torch.randn((n, 2, 64), generator=g, device=cuda_device).to(dtype)
+    out, lse = paged.prefix_attention(Q, s.pool_K, s.pool_V, s.table(48)[None].expand(B, 3), lens, cu, return_lse=True)
+    k = s.pool_K[:, 0].double().reshape(48, 64)
+    v = s.pool_V[:, 0].double().reshape(48, 64)
+    score = Q.double() @ k.T * s.scale
+    seen = torch.arange(48, device=cuda_device) < lens[new > 0][:, None]
+    score = score.masked_fill(~seen[:, None], float("-inf"))
+    p = torch.softmax(score, -1)
+    want, A = p @ v, p @ v.abs()
+    u, e = torch.finfo(dtype).eps / 2, 2.0 ** -24
+    top = s.scale * (Q.double().abs() @ k.abs().T).amax(-1)
+    per = (0 if dtype == F32 else u) + 2 * (64 + 8) * e * top + 2 * (48 * e + 2.0 ** -21)
+    assert ((out.double() - want).abs() <= u * want.abs() + per[..., None] * A).all()
+    z = torch.logsumexp(score, -1)
+    assert ((lse.double() - z).abs() <= (64 + 8) * e * top + 48 * e + 2.0 ** -21 + 2 * e * z.abs()).all()
+
+
+def test_block_tables_of_one_very_long_request(cuda_device):
+    # 2^26 new tokens and a million blocks of one request, beside a short one
+    L, n = 64, (1 << 26) + 5
+    F = n // L + 4
+    i32 = dict(dtype=torch.int32, device=cuda_device)
+    ring = torch.arange(F, **i32).flip(0).contiguous()
+    tables = torch.full((2, n // L + 2), -1, **i32)
+    t = paged.block_tables(torch.zeros(2, **i32), _dev([n, 3], cuda_device), tables, ring, _dev([7, F], cuda_device),
+                           block_len=L, n_tokens=n + 3)
+    held = n // L + 1
+    taken = ring[(torch.arange(held + 1, device=cuda_device) + 7) % F]
+    assert torch.equal(t.tables[0, :held], taken[:held]) and (t.tables[0, held:] == -1).all()
+    assert t.tables[1, 0] == taken[held] and (t.tables[1, 1:] == -1).all()
+    p = torch.arange(n, device=cuda_device)
+    assert torch.equal(t.slot_map[:n].long(), taken[p // L].long() * L + p % L)
+    assert t.slot_map[n:].tolist() == [int(taken[held]) * L + i for i in range(3)]
+    assert t.lens.tolist() == [n, 3] and t.cu_new.tolist() == [0, n, n + 3] and int(t.n_short) == 0
+    assert t.free_state.tolist() == [(7 + held + 1) % F, F - held - 1]
